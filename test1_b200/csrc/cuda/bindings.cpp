@@ -28,6 +28,17 @@ std::vector<torch::Tensor> linear_cross_entropy(torch::Tensor x, torch::Tensor w
                                                 int64_t ignore_index);
 std::vector<torch::Tensor> cross_entropy_fwd_bwd(torch::Tensor logits, torch::Tensor targets,
                                                  int64_t ignore_index, double grad_scale);
+std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets,
+                                              int64_t ignore_index, double temperature);
+void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, torch::Tensor targets,
+                        torch::Tensor lse, torch::Tensor dx, torch::Tensor dw, int64_t ignore_index,
+                        double temperature);
+std::vector<torch::Tensor> preference_loss(torch::Tensor logp, c10::optional<torch::Tensor> ref,
+                                           torch::Tensor targets, int64_t S, double beta, int64_t kind,
+                                           double smoothing, bool average, int64_t ignore_index);
+std::vector<torch::Tensor> policy_loss(torch::Tensor logp, torch::Tensor old, c10::optional<torch::Tensor> ref,
+                                       torch::Tensor advantages, torch::Tensor targets, int64_t S, double clip_low,
+                                       double clip_high, double kl_coef, bool per_sequence, int64_t ignore_index);
 void gemm_bf16(torch::Tensor A, torch::Tensor B, torch::Tensor C, bool a_mn, bool b_mn,
                c10::optional<torch::Tensor> R);
 int64_t gemm_check_error(bool reset);
@@ -68,6 +79,7 @@ void multi_tensor_adam(int64_t chunk_size, torch::Tensor noop_flag,
                        double weight_decay);
 // per-translation-unit bounds words (bounds.cuh); always 0 outside
 // bounds-checked builds
+unsigned long long bounds_word_answer_loss(bool);
 unsigned long long bounds_word_attention(bool);
 unsigned long long bounds_word_attention_tc(bool);
 unsigned long long bounds_word_attention_fwd2(bool);
@@ -78,6 +90,7 @@ unsigned long long bounds_word_fused_adam(bool);
 unsigned long long bounds_word_fused_ag_gemm(bool);
 unsigned long long bounds_word_fused_comm(bool);
 unsigned long long bounds_word_gemm(bool);
+unsigned long long bounds_word_logprob(bool);
 unsigned long long bounds_word_noalloc_rmsnorm(bool);
 }  // namespace t1
 
@@ -87,6 +100,7 @@ unsigned long long bounds_word_noalloc_rmsnorm(bool);
 static std::vector<std::tuple<std::string, int64_t, int64_t>> bounds_errors(bool reset) {
   using Reader = unsigned long long (*)(bool);
   static const std::pair<const char*, Reader> readers[] = {
+      {"answer_loss.cu", &t1::bounds_word_answer_loss},
       {"attention.cu", &t1::bounds_word_attention},
       {"attention_tc.cu", &t1::bounds_word_attention_tc},
       {"attention_fwd2.cu", &t1::bounds_word_attention_fwd2},
@@ -97,6 +111,7 @@ static std::vector<std::tuple<std::string, int64_t, int64_t>> bounds_errors(bool
       {"fused_ag_gemm.cu", &t1::bounds_word_fused_ag_gemm},
       {"fused_comm.cu", &t1::bounds_word_fused_comm},
       {"gemm.cu", &t1::bounds_word_gemm},
+      {"logprob.cu", &t1::bounds_word_logprob},
       {"noalloc_rmsnorm.cu", &t1::bounds_word_noalloc_rmsnorm},
   };
   std::vector<std::tuple<std::string, int64_t, int64_t>> out;
@@ -136,6 +151,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cross_entropy_fwd_bwd", &t1::cross_entropy_fwd_bwd);
   m.def("linear_cross_entropy", &t1::linear_cross_entropy,
         "chunked lm_head GEMM + cross-entropy forward/backward: (loss, count); writes dx and dW");
+  m.def("linear_logprob_fwd", &t1::linear_logprob_fwd,
+        "log-probabilities of the targets under the output layer: (logp [T], lse [T])");
+  m.def("linear_logprob_bwd", &t1::linear_logprob_bwd, "gradients of linear_logprob_fwd: writes dx and dW");
+  m.def("preference_loss", &t1::preference_loss, "paired log-ratio loss: (loss, dlogp [T], rewards [B])");
+  m.def("policy_loss", &t1::policy_loss, "clipped policy loss with a KL term: (loss, dlogp [T], stats [2])");
   m.def("gemm_bf16", &t1::gemm_bf16, pybind11::arg("A"), pybind11::arg("B"), pybind11::arg("C"),
         pybind11::arg("a_mn"), pybind11::arg("b_mn"), pybind11::arg("R") = pybind11::none());
   m.def("gemm_check_error", &t1::gemm_check_error, pybind11::arg("reset") = false);

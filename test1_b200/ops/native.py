@@ -179,3 +179,29 @@ def cross_entropy_fwd_bwd(logits, targets, ignore_index=-100, grad_scale=None):
     loss, count = _c().cross_entropy_fwd_bwd(logits, targets, int(ignore_index),
                                              -1.0 if grad_scale is None else float(grad_scale))
     return loss.reshape(()), logits, count
+
+
+# ------------------------------------- log-probabilities of the output layer
+def linear_logprob_fwd(x, w, targets, ignore_index=-100, temperature=1.0):
+    logp, lse = _c().linear_logprob_fwd(x, w, targets, int(ignore_index), float(temperature))
+    return logp, lse
+
+
+def linear_logprob_bwd(dlogp, x, w, targets, lse, dx, dw, ignore_index=-100, temperature=1.0):
+    _c().linear_logprob_bwd(dlogp, x, w, targets, lse, dx, dw, int(ignore_index), float(temperature))
+
+
+# ------------------------------------------- losses on those log-probabilities
+def preference_loss_fwd_bwd(logp, ref_logp, targets, seq_len, beta, kind, label_smoothing, average, ignore_index):
+    loss, dlogp, rewards = _c().preference_loss(logp, ref_logp, targets, int(seq_len), float(beta),
+                                                _ref.PREFERENCE_KINDS.index(kind), float(label_smoothing),
+                                                bool(average), int(ignore_index))
+    return loss, dlogp, rewards
+
+
+def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, clip_low, clip_high, kl_coef,
+                        reduction, ignore_index):
+    loss, dlogp, stats = _c().policy_loss(logp, old_logp, ref_logp, advantages, targets, int(seq_len),
+                                          float(clip_low), float(clip_high), float(kl_coef),
+                                          reduction == "sequence", int(ignore_index))
+    return loss, dlogp, stats

@@ -275,6 +275,108 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     return total / max(n_valid, 1), n_valid
 
 
+# --------------------------------- log-probabilities of the output layer
+
+
+def _answer_rows(targets: torch.Tensor, vocab: int, ignore_index: int) -> torch.Tensor:
+    return (targets != ignore_index) & (targets >= 0) & (targets < vocab)
+
+
+def linear_logprob_fwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                       temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """log softmax(x w^T / temperature)[t, targets[t]] and the row's
+    log-sum-exp (fp32), 0 where the target is ignored."""
+    if not temperature > 0:
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    valid = _answer_rows(targets, w.shape[0], ignore_index)
+    logits = (x.float() @ w.float().t()) / temperature
+    top = logits.max(dim=-1).values
+    log_sum = torch.logsumexp(logits - top[:, None], dim=-1)
+    picked = logits.gather(1, torch.where(valid, targets, 0)[:, None])[:, 0]
+    zero = torch.zeros_like(top)
+    return torch.where(valid, (picked - top) - log_sum, zero), torch.where(valid, top + log_sum, zero)
+
+
+def linear_logprob_bwd(dlogp: torch.Tensor, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
+                       lse: torch.Tensor, dx: torch.Tensor, dw: torch.Tensor, ignore_index: int = -100,
+                       temperature: float = 1.0) -> None:
+    """Writes dx and dw from dlogp and the forward's lse (fp32 arithmetic,
+    rounded once)."""
+    valid = _answer_rows(targets, w.shape[0], ignore_index)
+    rows = valid.nonzero()[:, 0]
+    xf, wf = x[rows].float(), w.float()
+    d = -torch.exp(xf @ wf.t() / temperature - lse[rows, None])
+    d[torch.arange(len(rows), device=d.device), targets[rows]] += 1.0
+    d *= dlogp[rows, None].float() / temperature
+    dx.zero_()
+    dx[rows] = (d @ wf).to(dx.dtype)
+    dw.copy_(d.t() @ xf)
+
+
+# ------------------------------------------- losses on those log-probabilities
+
+PREFERENCE_KINDS = ("sigmoid", "hinge", "ipo")
+
+
+def preference_loss_fwd_bwd(logp, ref_logp, targets, seq_len, beta=0.1, kind="sigmoid", label_smoothing=0.0,
+                            average=False, ignore_index=-100):
+    """Returns (loss, dloss/dlogp [T], rewards [T / seq_len]); the formulas are
+    at ``ops.preference_loss_fwd_bwd``."""
+    valid = (targets != ignore_index).view(-1, seq_len)
+    P = valid.shape[0] // 2
+    ratio = logp.float() if ref_logp is None else logp.float() - ref_logp.float()
+    r = torch.where(valid, ratio.view(-1, seq_len), 0.0).sum(1)
+    n = valid.sum(1)
+    per = 1.0 / n.clamp_min(1).float() if average else torch.ones_like(r)
+    r = r * per
+    m = r[:P] - r[P:]
+    live = (n[:P] + n[P:]) > 0
+    z = beta * m
+    if kind == "sigmoid":
+        e = label_smoothing
+        loss = -(1 - e) * F.logsigmoid(z) - e * F.logsigmoid(-z)
+        dm = beta * (e * torch.sigmoid(z) - (1 - e) * torch.sigmoid(-z))
+    elif kind == "hinge":
+        loss, dm = (1 - z).clamp_min(0), torch.where(z < 1, -beta, 0.0)
+    else:
+        loss, dm = (m - 0.5 / beta) ** 2, 2 * (m - 0.5 / beta)
+    pairs = live.sum().clamp_min(1)
+    dm = torch.where(live, dm, 0.0) / pairs
+    d = torch.cat([dm, -dm]) * per
+    dlogp = torch.where(valid, d[:, None], 0.0).reshape(-1)
+    return torch.where(live, loss, 0.0).sum() / pairs, dlogp, beta * r
+
+
+def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, clip_low=0.2, clip_high=0.2,
+                        kl_coef=0.0, reduction="token", ignore_index=-100):
+    """Returns (loss, dloss/dlogp [T], [mean KL, clipped share]); the formulas
+    are at ``ops.policy_loss_fwd_bwd``.  A token is clipped when its log ratio
+    lies past log(1 +- clip) on the side its advantage pushes to."""
+    valid = (targets != ignore_index).view(-1, seq_len)
+    a = advantages.float().view(valid.shape[0], -1)
+    d = (logp.float() - old_logp.float()).view_as(valid)
+    rho = torch.exp(d)
+    over, under = d > math.log1p(clip_high), d < math.log1p(-clip_low)
+    clipped = valid & (((a > 0) & over) | ((a < 0) & under))
+    loss = -a * torch.where(clipped, torch.where(over, 1 + clip_high, 1 - clip_low), rho)
+    grad = torch.where(clipped, 0.0, -a * rho)
+    kl = torch.zeros_like(d)
+    if ref_logp is not None:
+        e = (ref_logp.float() - logp.float()).view_as(valid)
+        kl = torch.expm1(e) - e
+        loss = loss + kl_coef * kl
+        grad = grad - kl_coef * torch.expm1(e)
+    n = valid.sum(1)
+    tokens = n.sum().clamp_min(1).float()
+    if reduction == "token":
+        weight = (1.0 / tokens).expand(len(n))
+    else:
+        weight = 1.0 / (n.clamp_min(1).float() * (n > 0).sum().clamp_min(1).float())
+    loss = (torch.where(valid, loss, 0.0).sum(1) * weight).sum()
+    stats = torch.stack([torch.where(valid, kl, 0.0).sum(), clipped.sum().float()]) / tokens
+    return loss, torch.where(valid, grad * weight[:, None], 0.0).reshape(-1), stats
+
+
 # ------------------------------------------------ fused-layout entry points
 # The model keeps q/k/v as column blocks of one [T, (Hq + 2 Hkv) * D] buffer
 # and gate/up as the two halves of one [T, 2 I] buffer; these wrappers state
