@@ -7,10 +7,11 @@
 // pairs (cta_group::2), 256 x 256 tiles, 128B-swizzled TMA loads into a
 // 6-stage ring, one elected thread issuing the MMAs, fp32 accumulators
 // double-buffered in TMEM, 4 epilogue warps per CTA that work on one
-// accumulator while the other fills.  Units of work are (k range, tile):
-// `splits` > 1 cuts the reduction into ranges whose results are separate
-// fp32 planes (kRowsF32 only), so that few tiles still fill the GPU and the
-// planes are added in a fixed order afterwards.
+// accumulator while the other fills.  The rows are those that the packing
+// kernel of logprob.cu kept, so their number is read on the GPU.  Units of
+// work are (k range, tile): `splits` > 1 cuts the reduction into ranges whose
+// results are separate fp32 planes (kRowsF32 only), so that few tiles still
+// fill the GPU and the planes are added in a fixed order afterwards.
 #pragma once
 
 #include "gemm_core.cuh"
@@ -32,22 +33,43 @@ static_assert(V_SMEM_BYTES <= 232448, "exceeds 227 KB of shared memory");
 
 enum Mode : int { kLse = 0, kSoftmaxGrad = 1, kRowsF32 = 2, kWeightGrad = 3 };
 
+// What the packing of the batch's rows found out on the GPU.
+struct RowsMeta {
+  int rows;    // rows that take part
+  int splits;  // ranges of k that the rows' product (kRowsF32) is cut into
+};
+
 struct VocabParams {
-  int M, N;              // rows and columns of the product
-  int tiles_m, tiles_n;
-  int k_blocks;          // of BK = 64
-  int splits;            // ranges of k
-  int plane_rows;        // kRowsF32: rows between two ranges' planes (a multiple of TILE)
+  const RowsMeta* meta;  // its rows are M, or in kWeightGrad the reduction's length
+  int M, N;              // rows and columns of the product (M: kWeightGrad only)
+  int k_blocks;          // of BK = 64 (not in kWeightGrad)
+  int ld_part;           // kLse: rows of a column block in `part`
   int accumulate;        // kRowsF32: add to what the plane holds
   float scale;           // 1 / temperature
   int col0;              // vocabulary index of column 0
-  const int64_t* targets;  // [M] vocabulary index, or anything outside the vocabulary: no target
-  float2* part;          // kLse: [tiles_n][M] (largest logit, sum of exp(logit - largest)) of a column block
+  const int* targets;    // [M] vocabulary index
+  float2* part;          // kLse: [tiles_n][ld_part] (largest logit, sum of exp(logit - largest)) of a column block
   float* target_logit;   // kLse: [M], unscaled
   const float* lse;      // kSoftmaxGrad: [M]
-  const float* drow;     // kSoftmaxGrad: [M] upstream gradient; rows at 0 give 0
   int* err;
 };
+
+// The product's extents, known once the packing has run.
+struct Extents {
+  int M, tiles_m, tiles_n, k_blocks, splits;
+};
+
+template <int MODE>
+__device__ __forceinline__ Extents extents(const VocabParams& p) {
+  const int rows = p.meta->rows;
+  Extents e;
+  e.M = MODE == kWeightGrad ? p.M : rows;
+  e.tiles_m = (e.M + TILE - 1) / TILE;
+  e.tiles_n = (p.N + TILE - 1) / TILE;
+  e.k_blocks = MODE == kWeightGrad ? (rows + BK - 1) / BK : p.k_blocks;
+  e.splits = MODE == kRowsF32 ? p.meta->splits : 1;
+  return e;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -57,13 +79,13 @@ __device__ __forceinline__ float ex2(float x) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ void vocab_unit(const VocabParams& p, int u, int& mb, int& nb, int& kb0, int& kb1,
+__device__ __forceinline__ void vocab_unit(const Extents& e, int u, int& mb, int& nb, int& kb0, int& kb1,
                                            int& split) {
-  const int tiles = p.tiles_m * p.tiles_n;
+  const int tiles = e.tiles_m * e.tiles_n;
   split = u / tiles;
-  raster(u % tiles, p.tiles_m, p.tiles_n, mb, nb);
-  kb0 = static_cast<int>(static_cast<long>(split) * p.k_blocks / p.splits);
-  kb1 = static_cast<int>(static_cast<long>(split + 1) * p.k_blocks / p.splits);
+  raster(u % tiles, e.tiles_m, e.tiles_n, mb, nb);
+  kb0 = static_cast<int>(static_cast<long>(split) * e.k_blocks / e.splits);
+  kb1 = static_cast<int>(static_cast<long>(split + 1) * e.k_blocks / e.splits);
 }
 
 template <bool A_MN, bool B_MN, int MODE>
@@ -116,7 +138,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   cluster_sync();  // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int num_units = p.tiles_m * p.tiles_n * p.splits;
+  const Extents e = extents<MODE>(p);
+  const int num_units = e.tiles_m * e.tiles_n * e.splits;
 
   if (warp == 0) {
     // ------------------------------------------------------ TMA producer
@@ -125,7 +148,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       uint32_t phase = 0;
       for (int u = cluster; u < num_units && !*abort_flag; u += nclusters) {
         int mb, nb, kb0, kb1, split;
-        vocab_unit(p, u, mb, nb, kb0, kb1, split);
+        vocab_unit(e, u, mb, nb, kb0, kb1, split);
         const int row_a = mb * TILE + static_cast<int>(crank) * HALF;
         const int row_b = nb * TILE + static_cast<int>(crank) * HALF;
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -167,7 +190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       int local = 0;
       for (int u = cluster; u < num_units && !*abort_flag; u += nclusters, ++local) {
         int mb, nb, kb0, kb1, split;
-        vocab_unit(p, u, mb, nb, kb0, kb1, split);
+        vocab_unit(e, u, mb, nb, kb0, kb1, split);
         const int acc = local & 1;
         const uint32_t acc_phase = (local >> 1) & 1;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1)) {
@@ -216,7 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     int local = 0;
     for (int u = cluster; u < num_units; u += nclusters, ++local) {
       int mb, nb, kb0, kb1, split;
-      vocab_unit(p, u, mb, nb, kb0, kb1, split);
+      vocab_unit(e, u, mb, nb, kb0, kb1, split);
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
       // one lane waits and the warp follows it, so the warp never diverges
@@ -234,7 +257,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       tc_fence_after();
       const int row0 = mb * TILE + static_cast<int>(crank) * HALF + q * 32;
       const int row = row0 + lane;
-      const bool row_ok = row < p.M;
+      const bool row_ok = row < e.M;
       const int tcol0 = nb * TILE;                       // first column of the tile
       const int cols = min(TILE, p.N - tcol0);           // columns of the tile that exist
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * TILE;
@@ -244,8 +267,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         // accumulator's own units: (logit - largest) is exact near the
         // largest, which is where the sum comes from.
         const float k2 = p.scale * kLog2e;
-        const int64_t t = row_ok ? p.targets[row] - p.col0 - tcol0 : -1;
-        const int tcol = (t >= 0 && t < cols) ? static_cast<int>(t) : -1;
+        const int t = row_ok ? p.targets[row] - tcol0 : -1;
+        const int tcol = t < cols ? t : -1;
         float m = -INFINITY, s = 0.f;
 #pragma unroll 1
         for (int c = 0; c < TILE; c += 32) {
@@ -266,17 +289,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) s += ex2((__uint_as_float(r[j]) - ref) * k2);
           m = mn;
-          if (static_cast<unsigned>(tcol - c) < 32u) {
-            float v = 0.f;
+          if (tcol >= c && tcol < c + 32) {
+            if (!T1_OOB(row, p.ld_part)) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v = tcol - c == j ? __uint_as_float(r[j]) : v;
-            if (!T1_OOB(row, p.M)) p.target_logit[row] = v;
+              for (int j = 0; j < 32; ++j)
+                if (tcol - c == j) p.target_logit[row] = __uint_as_float(r[j]);
+            }
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
-        if (row_ok && !T1_OOB(nb, p.tiles_n)) p.part[static_cast<size_t>(nb) * p.M + row] = make_float2(m, s);
+        if (row_ok && !T1_OOB(row, p.ld_part)) p.part[static_cast<size_t>(nb) * p.ld_part + row] = make_float2(m, s);
         continue;
       }
 
@@ -285,7 +309,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 #pragma unroll 1
         for (int c = 0; c < TILE; c += 32) {
           uint8_t* buf = wbuf + bi * EPI_BUF;
-          const bool live = c < cols && row0 < p.M;  // uniform over the warp
+          const bool live = c < cols && row0 < e.M;  // uniform over the warp
           if (lane == 0) bulk_wait_group_read<1>();
           __syncwarp();
           uint32_t r[32];
@@ -297,6 +321,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
             if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
           }
           if (!live) continue;
+          if (kb0 == kb1) {  // a range of no columns
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = 0;
+          }
           uint8_t* rowp = buf + lane * 128;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -305,7 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            const int prow = split * p.plane_rows + row0;
+            const int prow = split * e.tiles_m * TILE + row0;
             if (p.accumulate) tma_reduce_add_2d(&tma_c, buf, tcol0 + c, prow);
             else tma_store_2d(&tma_c, buf, tcol0 + c, prow);
             bulk_commit_group();
@@ -318,20 +346,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       // bf16 results (kSoftmaxGrad, kWeightGrad) through 32 x 64 slabs
       float lse2 = 0.f;
       int tcol = -1;
-      bool dead = true;  // a row without a gradient is 0 whatever its logits are
       const float k2 = p.scale * kLog2e;
       if (MODE == kSoftmaxGrad && row_ok) {
-        const int64_t t = p.targets[row] - p.col0;
-        if (p.drow[row] != 0.f) {
-          dead = false;
-          lse2 = p.lse[row] * kLog2e;
-          if (t >= tcol0 && t < tcol0 + cols) tcol = static_cast<int>(t - tcol0);
-        }
+        lse2 = p.lse[row] * kLog2e;
+        const int t = p.targets[row] - p.col0 - tcol0;
+        tcol = t < cols ? t : -1;
       }
+      // u's rows are a reduction's length in kWeightGrad: its last block of
+      // BK has to be there, with zeros past the last row
+      const int m_end = MODE == kSoftmaxGrad ? (e.M + BK - 1) / BK * BK : e.M;
 #pragma unroll 1
       for (int c = 0; c < TILE; c += 64) {
         uint8_t* buf = wbuf + bi * EPI_BUF;
-        const bool live = c < cols && row0 < p.M;
+        const bool live = c < cols && row0 < m_end;
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
         uint32_t r[2][32];
@@ -352,8 +379,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           for (int k = 0; k < 8; ++k) {
             f[k] = __uint_as_float(r[j >> 2][(j & 3) * 8 + k]);
             if (MODE == kSoftmaxGrad) {
-              f[k] = dead ? 0.f : -ex2(fmaf(f[k], k2, -lse2));
+              f[k] = row_ok ? -ex2(fmaf(f[k], k2, -lse2)) : 0.f;
               if (tcol == c + 8 * j + k) f[k] += 1.f;
+            } else if (kb0 == kb1) {  // a sum over no rows
+              f[k] = 0.f;
             }
           }
           uint4 ov;
