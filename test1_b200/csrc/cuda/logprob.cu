@@ -20,17 +20,19 @@ using vocab::VocabParams;
 using vocab::kLog2e;
 using vocab::ex2;
 
-// How many ranges the rows' product u W is cut into (tiles of 256 x 256 on
-// `clusters` CTA pairs): the smallest estimate of waves x (k blocks of a
-// range + start and drain of a tile) + the planes' traffic, in units of a k
-// block (0.13 us of tensor time; a tile's plane written and read back is
-// 0.5 MB, 0.08 us of the GPU's bandwidth).
-__host__ __device__ inline int pick_splits(int tiles, int k_blocks, int clusters) {
+// How many ranges of the vocabulary dx's product is cut into, so that its
+// `tiles` long units and the D dW tiles fill `clusters` evenly: the smallest
+// estimate of the time of the busiest cluster plus the planes' traffic, in
+// units of a k block (0.27 us; a tile's plane written and read back is 0.5 MB,
+// 0.08 us of the GPU's bandwidth).
+__host__ __device__ inline int pick_splits(int64_t tiles, int k_blocks, int64_t dw_tiles, int tiles_t, int clusters) {
   int best = 1;
   int64_t least = INT64_MAX;  // whole numbers: host and device must agree
-  for (int s = 1; s <= 32 && (s == 1 || k_blocks >= 16 * s); ++s) {
-    const int64_t waves = (static_cast<int64_t>(tiles) * s + clusters - 1) / clusters;
-    const int64_t cost = 10 * waves * ((k_blocks + s - 1) / s + 12) + 6ll * s * tiles;
+  for (int s = 1; s <= 32 && (s == 1 || k_blocks >= 8 * s); ++s) {
+    const int64_t ux = vocab::dx_unit_cost(k_blocks, s), uw = vocab::dw_unit_cost(tiles_t);
+    const int64_t even = (tiles * s * ux + dw_tiles * uw + clusters - 1) / clusters + uw;
+    const int64_t longest = (tiles * s + clusters - 1) / clusters * ux;
+    const int64_t cost = 10 * (even > longest ? even : longest) + (s > 1 ? 3 * s * tiles : 0);
     if (cost < least) {
       least = cost;
       best = s;
@@ -46,17 +48,18 @@ struct PackParams {
   int64_t ignore, V;
   int T, H;
   int per_block;         // tokens of a block
+  int per_slice;         // 8-column vectors of a block
   float scale;
   const float* dlogp;    // null in the forward
   const float* lse;      // with dlogp
-  int k_blocks, tiles_n, clusters;  // of the rows' product, with dlogp
+  int k_blocks, tiles_n, tiles_h, clusters;  // of the products with u, with dlogp
   vocab::RowsMeta* meta;
   int* index;            // [T] the packed row's token
-  int* target;           // [T]
+  int64_t* target;       // [T]
   float* g;              // [T] dlogp / tau, with dlogp
   float* lse_packed;     // with dlogp
-  bf16* xp;              // [T + 64, H] the rows of x
-  bf16* gxp;             // [T + 64, H] g x, with dlogp
+  bf16* xp;              // [T, H] the rows of x
+  bf16* gxp;             // [T rounded up to 64, H] g x, with dlogp
   float *zero0, *zero1;  // forward: logp and lse, 0 for the tokens left out
   bf16* dx;              // backward: likewise
 };
@@ -66,9 +69,10 @@ constexpr int kPackThreads = 256;
 // Packs the rows that take part: tokens with a target and, in the backward,
 // with a gradient (a clipped token's is exactly 0, and so is all it adds).
 // Prompts and padding are often half of a batch, and every product below
-// shrinks by them.  Each block counts the rows before its own tokens itself:
-// T / 2 targets out of L2 on average instead of a scan in a launch of its
-// own.  Rows keep their order, so sums over rows do not depend on timing.
+// shrinks by them.  A block takes some tokens and some columns; it counts the
+// rows before its own tokens itself: T / 2 targets out of L2 on average
+// instead of a scan in a launch of its own.  Rows keep their order, so sums
+// over rows do not depend on timing.
 //
 // In the backward also g x, rounded to bf16 for the tensor cores: a relative
 // error of 2^-9 at most per element of x, independent from element to
@@ -79,13 +83,17 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
   __shared__ int counts[kPackThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kWarps = kPackThreads / 32;
+  vocab::launch_dependents();
+  vocab::wait_previous();
   const int t0 = blockIdx.x * p.per_block, t1 = min(p.T, t0 + p.per_block);
+  const bool first_slice = blockIdx.y == 0;
   auto takes_part = [&](int t) {
     const int64_t v = p.targets[t];
     const bool valid = v != p.ignore && v >= 0 && v < p.V;
     return BWD ? valid && p.dlogp[t] != 0.f : valid;
   };
   int n = 0;
+#pragma unroll 4
   for (int t = threadIdx.x; t < t0; t += kPackThreads) n += takes_part(t);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
@@ -95,6 +103,7 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
   for (int w = 0; w < kWarps; ++w) pos += counts[w];
 
   const int nvec = p.H >> 3;
+  const int i0 = blockIdx.y * p.per_slice, i1 = min(nvec, i0 + p.per_slice);
   for (int base = t0; base < t1; base += 32) {
     const bool mine = base + lane < t1 && takes_part(base + lane);
     const unsigned mask = __ballot_sync(0xffffffffu, mine);
@@ -102,9 +111,9 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
     for (int j = warp; j < 32 && base + j < t1; j += kWarps) {
       const int t = base + j;
       if (!(mask >> j & 1)) {
-        if (!BWD && lane == 0) p.zero0[t] = p.zero1[t] = 0.f;
+        if (!BWD && lane == 0 && first_slice) p.zero0[t] = p.zero1[t] = 0.f;
         if (BWD)
-          for (int i = lane; i < nvec; i += 32)
+          for (int i = i0 + lane; i < i1; i += 32)
             reinterpret_cast<uint4*>(p.dx + static_cast<size_t>(t) * p.H)[i] = make_uint4(0, 0, 0, 0);
         continue;
       }
@@ -112,23 +121,29 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
       if (T1_OOB(at, p.T)) continue;
       float gr = 0.f;
       if (BWD) gr = p.dlogp[t] * p.scale;
-      if (lane == 0) {
+      if (lane == 0 && first_slice) {
         p.index[at] = t;
-        p.target[at] = static_cast<int>(p.targets[t]);
+        p.target[at] = p.targets[t];
         if (BWD) {
           p.g[at] = gr;
           p.lse_packed[at] = p.lse[t];
         }
       }
       const bf16* src = p.x + static_cast<size_t>(t) * p.ldx;
-      for (int i = lane; i < nvec; i += 32) {
+#pragma unroll 4
+      for (int i = i0 + lane; i < i1; i += 32) {
         const size_t dst = static_cast<size_t>(at) * p.H + 8 * i;
-        *reinterpret_cast<uint4*>(p.xp + dst) = *reinterpret_cast<const uint4*>(src + 8 * i);
+        const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(src + 8 * i));
+        *reinterpret_cast<uint4*>(p.xp + dst) = raw;
         if (BWD) {
           float v[8];
-          load8(src + 8 * i, v);
+          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] *= gr;
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __bfloat1622float2(h[k]);
+            v[2 * k] = f.x * gr;
+            v[2 * k + 1] = f.y * gr;
+          }
           store8(p.gxp + dst, v);
         }
       }
@@ -137,39 +152,42 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
   }
   if (t1 != p.T) return;
   // the last block knows how many there are
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && first_slice) {
     p.meta->rows = pos;
-    if (BWD) p.meta->splits = pick_splits((pos + vocab::TILE - 1) / vocab::TILE * p.tiles_n, p.k_blocks, p.clusters);
+    const int tiles_t = (pos + vocab::TILE - 1) / vocab::TILE;
+    if (BWD)
+      p.meta->splits = pick_splits(static_cast<int64_t>(tiles_t) * p.tiles_h, p.k_blocks,
+                                   static_cast<int64_t>(p.tiles_n) * p.tiles_h, tiles_t, p.clusters);
   }
   if (BWD) {  // dW's reduction runs over whole blocks of BK rows
     const int end = (pos + gemm::BK - 1) / gemm::BK * gemm::BK;
-    for (int i = threadIdx.x; i < (end - pos) * nvec; i += kPackThreads)
-      reinterpret_cast<uint4*>(p.gxp + static_cast<size_t>(pos) * p.H)[i] = make_uint4(0, 0, 0, 0);
+    for (int r = pos + warp; r < end; r += kWarps)
+      for (int i = i0 + lane; i < i1; i += 32)
+        reinterpret_cast<uint4*>(p.gxp + static_cast<size_t>(r) * p.H)[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
 // Joins the column blocks' (largest, sum) of 32 rows: lanes are rows (a
 // block's entries of neighbouring rows are neighbours in memory), warps
-// share the column blocks.
-constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(32 * kJoinWarps)
-    logprob_join_kernel(const float2* __restrict__ part, const float* __restrict__ target_logit,
-                        const vocab::RowsMeta* __restrict__ meta, const int* __restrict__ index, int T, int blocks,
-                        float scale, float* __restrict__ logp, float* __restrict__ lse) {
+// share the column blocks.  `meta` and `index` are null for rows that were
+// not packed.
+constexpr int kJoinWarps = 32;
+__global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const VocabParams p, int blocks) {
   __shared__ float sm[kJoinWarps][32], ss[kJoinWarps][32];
+  vocab::launch_dependents();
+  vocab::wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
-  if (blockIdx.x * 32 >= meta->rows) return;  // uniform over the block
-  const bool in = row < meta->rows;
-  const float k2 = scale * kLog2e;
+  const int rows = p.meta != nullptr ? p.meta->rows : p.rows;
+  if (static_cast<int>(blockIdx.x) * 32 >= rows) return;  // uniform over the block
+  const bool in = row < rows && !T1_OOB(row, p.ld_part);
+  const float k2 = p.scale * kLog2e;
   float m = -INFINITY, s = 0.f;
   if (in) {
+#pragma unroll 4
     for (int b = warp; b < blocks; b += kJoinWarps) {
-      const float2 v = part[static_cast<size_t>(b) * T + row];
-      const float mn = fmaxf(m, v.x);
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      s = s * ex2((m - ref) * k2) + v.y * ex2((v.x - ref) * k2);
-      m = mn;
+      const float2 v = p.part[static_cast<size_t>(b) * p.ld_part + row];
+      vocab::lse_join(m, s, v.x, v.y, k2);
     }
   }
   sm[warp][lane] = m;
@@ -180,49 +198,41 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   const float ref = m == -INFINITY ? 0.f : m;
   s = 0.f;
   for (int w = 0; w < kJoinWarps; ++w) s += ss[w][lane] * ex2((sm[w][lane] - ref) * k2);
-  const float log_s = logf(s);
-  const int t = index[row];
-  if (T1_OOB(t, T)) return;
-  // (target - largest) first: exact where the target is likely
-  logp[t] = (target_logit[row] - ref) * scale - log_s;
-  lse[t] = ref * scale + log_s;
-}
-
-// dx[t, :] = g[t] * (sum of the fp32 planes), in plane order, for the packed
-// rows (the packing wrote the others' zeros).
-__global__ void __launch_bounds__(128)
-    logprob_dx_kernel(const float* __restrict__ planes, const vocab::RowsMeta* __restrict__ meta, long ldp,
-                      const int* __restrict__ index, const float* __restrict__ g, int T, int H,
-                      bf16* __restrict__ dx) {
-  const int rows = meta->rows, splits = meta->splits;
-  const size_t stride = static_cast<size_t>((rows + vocab::TILE - 1) / vocab::TILE * vocab::TILE) * ldp;
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float gr = g[row];
-    const int t = index[row];
-    if (T1_OOB(t, T)) continue;
-    for (int i = threadIdx.x; i < H / 8; i += blockDim.x) {
-      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      for (int s = 0; s < splits; ++s) {
-        const float4* p = reinterpret_cast<const float4*>(planes + s * stride + static_cast<size_t>(row) * ldp + 8 * i);
-        const float4 a = p[0], b = p[1];
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= gr;
-      store8(dx + static_cast<size_t>(t) * H + 8 * i, v);
-    }
-  }
+  const int t = p.index != nullptr ? p.index[row] : row;
+  const int64_t v = p.targets[row];
+  vocab::write_logp(m, s, p.target_logit[row], v != p.ignore && v >= 0 && v < p.V, p.scale, p.logp + t, p.lse_out + t);
 }
 
 // ================================================================ host side
 T1_BOUNDS_READER(logprob)
 
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// A launch whose prologue may overlap the end of the stream's previous
+// kernel (every kernel here waits for it before it touches memory).
+template <class... P, class... A>
+static void launch_after(const char* what, void (*kern)(P...), dim3 grid, int threads, size_t smem, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream();
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+  TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e));
+  count_launch();
+}
+
 // `units`: the most units of work that the launch can have.
-template <bool A_MN, bool B_MN, int MODE>
-static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, VocabParams& p,
-                         int64_t units) {
-  auto kern = vocab::vocab_kernel<A_MN, B_MN, MODE>;
+template <int JOB>
+static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta2, const CUtensorMap& tb2,
+                         const CUtensorMap& tc, VocabParams& p, int64_t units) {
+  auto kern = vocab::vocab_kernel<JOB>;
   static bool configured = false;
   if (!configured) {
     T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, vocab::V_SMEM_BYTES));
@@ -230,13 +240,22 @@ static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
   }
   p.err = gemm_error_word().data_ptr<int>();
   const int clusters = static_cast<int>(std::min<int64_t>(units, num_sms() / 2));
-  kern<<<2 * clusters, 192, vocab::V_SMEM_BYTES, stream()>>>(ta, tb, tc, p);
-  check_launch("linear_logprob");
-  count_launch();
+  launch_after("linear_logprob", kern, dim3(2 * clusters), 192, vocab::V_SMEM_BYTES, ta, tb, ta2, tb2, tc, p);
 }
 
-static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+// Arrival counters, zero between launches (whoever arrives last clears its
+// counter); one set per (device, stream), so that concurrent calls never
+// share one.
+static int* tickets(int64_t n) {
+  static std::unordered_map<uint64_t, torch::Tensor> all;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t key = (static_cast<uint64_t>(dev) << 56) ^ reinterpret_cast<uint64_t>(stream());
+  torch::Tensor& t = all[key];
+  if (!t.defined() || t.numel() < n)
+    t = torch::zeros({std::max<int64_t>(4096, n)}, torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, dev));
+  return t.data_ptr<int>();
+}
 
 // A workspace cut into 256-byte aligned pieces.
 struct Pieces {
@@ -270,14 +289,27 @@ static void check_logprob(const torch::Tensor& x, const torch::Tensor& w, const 
 static int64_t row_ld(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 static void launch_pack(PackParams& p) {
-  // a few blocks per SM, and no more than 32 tokens each where T allows it
-  p.per_block = static_cast<int>(std::max<int64_t>(8, ceil_div(p.T, 4 * num_sms())));
-  const int blocks = static_cast<int>(ceil_div(p.T, p.per_block));
-  if (p.dlogp != nullptr) logprob_pack_kernel<true><<<blocks, kPackThreads, 0, stream()>>>(p);
-  else logprob_pack_kernel<false><<<blocks, kPackThreads, 0, stream()>>>(p);
-  check_launch("logprob_pack");
-  count_launch();
+  // about four blocks per SM: 8 to 32 tokens each and, when these are few,
+  // slices of the columns (64 vectors at least, two per lane)
+  p.per_block = static_cast<int>(std::min<int64_t>(32, std::max<int64_t>(8, ceil_div(p.T, 4 * num_sms()))));
+  const int64_t groups = ceil_div(p.T, p.per_block);
+  const int64_t slices = std::max<int64_t>(1, std::min(ceil_div(p.H / 8, 64), 4 * num_sms() / groups));
+  p.per_slice = static_cast<int>(ceil_div(p.H / 8, slices));
+  const dim3 grid(groups, ceil_div(p.H / 8, p.per_slice));
+  if (p.dlogp != nullptr) launch_after("logprob_pack", logprob_pack_kernel<true>, grid, kPackThreads, 0, p);
+  else launch_after("logprob_pack", logprob_pack_kernel<false>, grid, kPackThreads, 0, p);
 }
+
+// Whether the forward packs its rows first.  Below 256 tokens there is one
+// row of tiles whatever is left out, and a product of less than about 30 us
+// gains less from losing half of its rows than the packing costs (6 us).
+static bool packs(int64_t T, int64_t H, int64_t V) {
+  return T > vocab::TILE && static_cast<double>(T) * H * V > 2e10;
+}
+
+// Column blocks up to which the last of them joins the rows' sums itself: a
+// launch of its own costs about as much as 32 dependent reads.
+constexpr int kJoinBlocks = 32;
 
 // Returns (logp [T], lse [T]), fp32.
 std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets,
@@ -289,53 +321,60 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   auto logp = torch::empty({T}, f32), lse = torch::empty({T}, f32);
   if (T == 0) return {logp, lse};
   auto tg = targets.contiguous();
-  const int64_t blocks = ceil_div(V, vocab::TILE);
+  const int64_t blocks = ceil_div(V, vocab::TILE), tiles_t = ceil_div(T, vocab::TILE);
+  const bool pack = packs(T, H, V);
   Pieces ws;
-  const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(4 * T),
-                o_logit = ws.take(4 * T), o_part = ws.take(8 * blocks * T), o_x = ws.take(2 * T * H);
+  const int64_t o_logit = ws.take(4 * T), o_part = ws.take(8 * blocks * T);
+  const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(8 * T);
+  const int64_t o_x = ws.take(pack ? 2 * T * H : 0);
   auto buf = torch::empty({ws.used}, x.options().dtype(torch::kUInt8));
   uint8_t* base = buf.data_ptr<uint8_t>();
-  const float scale = static_cast<float>(1.0 / temperature);
-
-  PackParams k{};
-  k.x = (const bf16*)x.data_ptr();
-  k.ldx = row_ld(x);
-  k.targets = tg.data_ptr<int64_t>();
-  k.ignore = ignore_index;
-  k.V = V;
-  k.T = T;
-  k.H = H;
-  k.meta = reinterpret_cast<vocab::RowsMeta*>(base + o_meta);
-  k.index = reinterpret_cast<int*>(base + o_index);
-  k.target = reinterpret_cast<int*>(base + o_target);
-  k.xp = reinterpret_cast<bf16*>(base + o_x);
-  k.zero0 = logp.data_ptr<float>();
-  k.zero1 = lse.data_ptr<float>();
-  launch_pack(k);
 
   VocabParams p{};
-  p.meta = k.meta;
+  p.rows = static_cast<int>(T);
   p.N = static_cast<int>(V);
-  p.k_blocks = static_cast<int>(ceil_div(H, gemm::BK));
+  p.H = static_cast<int>(H);
+  p.scale = static_cast<float>(1.0 / temperature);
+  p.targets = tg.data_ptr<int64_t>();
+  p.ignore = ignore_index;
+  p.V = V;
   p.ld_part = static_cast<int>(T);
-  p.scale = scale;
-  p.targets = k.target;
   p.part = reinterpret_cast<float2*>(base + o_part);
   p.target_logit = reinterpret_cast<float*>(base + o_logit);
-  CUtensorMap ta = make_map_any(k.xp, false, H, T, H, vocab::HALF);
+  p.logp = logp.data_ptr<float>();
+  p.lse_out = lse.data_ptr<float>();
+  p.join = blocks <= kJoinBlocks;
+  if (p.join) p.tickets = tickets(tiles_t * 8);
+  if (pack) {
+    PackParams k{};
+    k.x = (const bf16*)x.data_ptr();
+    k.ldx = row_ld(x);
+    k.targets = p.targets;
+    k.ignore = ignore_index;
+    k.V = V;
+    k.T = T;
+    k.H = H;
+    k.meta = reinterpret_cast<vocab::RowsMeta*>(base + o_meta);
+    k.index = reinterpret_cast<int*>(base + o_index);
+    k.target = reinterpret_cast<int64_t*>(base + o_target);
+    k.xp = reinterpret_cast<bf16*>(base + o_x);
+    k.zero0 = p.logp;
+    k.zero1 = p.lse_out;
+    launch_pack(k);
+    p.meta = k.meta;
+    p.index = k.index;
+    p.targets = k.target;
+  }
+  CUtensorMap ta = make_map_any(pack ? base + o_x : x.data_ptr(), false, H, T, pack ? H : row_ld(x), vocab::HALF);
   CUtensorMap tb = make_map_any(w.data_ptr(), false, H, V, row_ld(w), vocab::HALF);
-  launch_vocab<false, false, vocab::kLse>(ta, tb, ta, p, ceil_div(T, vocab::TILE) * blocks);
-  logprob_join_kernel<<<ceil_div(T, 32), 32 * kJoinWarps, 0, stream()>>>(p.part, p.target_logit, k.meta, k.index, T,
-                                                                       blocks, scale, logp.data_ptr<float>(),
-                                                                       lse.data_ptr<float>());
-  check_launch("logprob_join");
-  count_launch();
+  launch_vocab<vocab::kLse>(ta, tb, ta, tb, ta, p, tiles_t * blocks);
+  if (!p.join) launch_after("logprob_join", logprob_join_kernel, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, blocks);
   return {logp, lse};
 }
 
 // The softmax gradient u exists for as many vocabulary columns at a time as
 // fit this many bytes; dW's rows of those columns are then final, and dx
-// gathers the chunks' products in fp32.
+// gathers the pieces' products in fp32.
 constexpr int64_t kGradBufferBytes = 1ll << 30;
 
 // Writes dx [T, H] and dw [V, H].
@@ -361,25 +400,27 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     return;
   }
   auto tg = targets.contiguous(), up = dlogp.contiguous(), ls = lse.contiguous();
-  const float scale = static_cast<float>(1.0 / temperature);
   const int clusters = num_sms() / 2;
-  const int64_t tiles_t = ceil_div(T, vocab::TILE), tiles_h = ceil_div(H, vocab::TILE), k_h = ceil_div(H, gemm::BK);
+  const int64_t tiles_t = ceil_div(T, vocab::TILE), tiles_h = ceil_div(H, vocab::TILE);
 
   const int64_t most = std::max<int64_t>(vocab::TILE, kGradBufferBytes / (2 * T) / vocab::TILE * vocab::TILE);
-  const int64_t chunks = ceil_div(V, most);
-  const int64_t width = std::min(V, round_up(ceil_div(V, chunks), vocab::TILE));
+  const int64_t pieces = ceil_div(V, most);
+  const int64_t width = std::min(V, round_up(ceil_div(V, pieces), vocab::TILE));
   const int64_t ldu = round_up(width, 8), u_rows = round_up(T, gemm::BK), k_v = ceil_div(width, gemm::BK);
-  // the planes of the most rows that the split rule can ask for
-  int64_t plane_rows = 0, most_units = 0;
+  const int64_t tiles_v = ceil_div(width, vocab::TILE);
+  // the most planes and units that the split rule can ask for, over the
+  // numbers of rows that the packing may leave
+  int64_t planes = 0, most_units = 0;
   for (int64_t m = 1; m <= tiles_t; ++m) {
-    const int64_t s = pick_splits(m * tiles_h, k_v, clusters);
-    plane_rows = std::max(plane_rows, s * m * vocab::TILE);
-    most_units = std::max(most_units, s * m * tiles_h);
+    const int64_t n = m * tiles_h * pick_splits(m * tiles_h, k_v, tiles_v * tiles_h, m, clusters);
+    most_units = std::max(most_units, n);
+    if (pieces > 1 || n > m * tiles_h) planes = std::max(planes, n);
   }
   Pieces ws;
-  const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(4 * T),
+  const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(8 * T),
                 o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_x = ws.take(2 * T * H),
-                o_gx = ws.take(2 * u_rows * H), o_planes = ws.take(4 * plane_rows * H), o_u = ws.take(2 * u_rows * ldu);
+                o_gx = ws.take(2 * u_rows * H), o_planes = ws.take(4 * 8 * vocab::PLANE_BLOCK * planes),
+                o_u = ws.take(2 * u_rows * ldu);
   auto buf = torch::empty({ws.used}, x.options().dtype(torch::kUInt8));
   uint8_t* base = buf.data_ptr<uint8_t>();
 
@@ -391,15 +432,16 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   k.V = V;
   k.T = T;
   k.H = H;
-  k.scale = scale;
+  k.scale = static_cast<float>(1.0 / temperature);
   k.dlogp = up.data_ptr<float>();
   k.lse = ls.data_ptr<float>();
   k.k_blocks = k_v;
-  k.tiles_n = tiles_h;
+  k.tiles_n = tiles_v;
+  k.tiles_h = tiles_h;
   k.clusters = clusters;
   k.meta = reinterpret_cast<vocab::RowsMeta*>(base + o_meta);
   k.index = reinterpret_cast<int*>(base + o_index);
-  k.target = reinterpret_cast<int*>(base + o_target);
+  k.target = reinterpret_cast<int64_t*>(base + o_target);
   k.g = reinterpret_cast<float*>(base + o_g);
   k.lse_packed = reinterpret_cast<float*>(base + o_lse);
   k.xp = reinterpret_cast<bf16*>(base + o_x);
@@ -407,42 +449,36 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   k.dx = (bf16*)dx.data_ptr();
   launch_pack(k);
 
+  VocabParams p{};
+  p.meta = k.meta;
+  p.H = static_cast<int>(H);
+  p.scale = k.scale;
+  p.index = k.index;
+  p.targets = k.target;
+  p.tickets = tickets(tiles_t * tiles_h * 8);
+  p.lse = k.lse_packed;
+  p.g = k.g;
+  p.dx = k.dx;
+  p.planes = reinterpret_cast<float*>(base + o_planes);
   bf16* u = reinterpret_cast<bf16*>(base + o_u);
-  float* planes = reinterpret_cast<float*>(base + o_planes);
   CUtensorMap tx = make_map_any(k.xp, false, H, T, H, vocab::HALF);
-  CUtensorMap tgx = make_map_any(k.gxp, false, H, u_rows, H, 64);
-  CUtensorMap tpl = make_map_any(planes, true, H, plane_rows, H, 32);
+  CUtensorMap tgx = make_map_any(k.gxp, false, H, u_rows, H, gemm::BK);
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int64_t n = std::min(width, V - v0);
     const bf16* wp = (const bf16*)w.data_ptr() + v0 * row_ld(w);
-    VocabParams p{};
-    p.meta = k.meta;
-    // u = onehot - softmax
-    p.N = n;
-    p.k_blocks = k_h;
-    p.scale = scale;
-    p.col0 = v0;
-    p.targets = k.target;
-    p.lse = k.lse_packed;
-    launch_vocab<false, false, vocab::kSoftmaxGrad>(tx, make_map_any(wp, false, H, n, row_ld(w), vocab::HALF),
-                                                    make_map_any(u, false, n, u_rows, ldu, 32), p,
-                                                    tiles_t * ceil_div(n, vocab::TILE));
-    // dx's sums: u W
-    p.N = H;
-    p.k_blocks = ceil_div(n, gemm::BK);
-    p.accumulate = v0 > 0;
-    launch_vocab<false, true, vocab::kRowsF32>(make_map_any(u, false, n, T, ldu, vocab::HALF),
-                                               make_map_any(wp, false, H, n, row_ld(w), 64), tpl, p, most_units);
-    // dW: u^T (g x)
-    p.M = n;
-    launch_vocab<true, true, vocab::kWeightGrad>(make_map_any(u, false, n, u_rows, ldu, 64), tgx,
-                                                 make_map_any((bf16*)dw.data_ptr() + v0 * H, false, H, n, H, 32), p,
-                                                 ceil_div(n, vocab::TILE) * tiles_h);
+    p.N = static_cast<int>(n);
+    p.col0 = static_cast<int>(v0);
+    p.first = v0 == 0;
+    p.last = v0 + width >= V;
+    const CUtensorMap tw = make_map_any(wp, false, H, n, row_ld(w), vocab::HALF);
+    const CUtensorMap twc = make_map_any(wp, false, H, n, row_ld(w), gemm::BK);
+    const CUtensorMap tu = make_map_any(u, false, n, u_rows, ldu, vocab::HALF);
+    const CUtensorMap tuc = make_map_any(u, false, n, u_rows, ldu, gemm::BK);
+    const CUtensorMap tus = make_map_any(u, false, n, u_rows, ldu, 32);
+    const CUtensorMap tdw = make_map_any((bf16*)dw.data_ptr() + v0 * H, false, H, n, H, 32);
+    launch_vocab<vocab::kSoftmaxGrad>(tx, tw, tx, tw, tus, p, tiles_t * ceil_div(n, vocab::TILE));
+    launch_vocab<vocab::kGrads>(tu, twc, tuc, tgx, tdw, p, most_units + ceil_div(n, vocab::TILE) * tiles_h);
   }
-  logprob_dx_kernel<<<std::min<int64_t>(T, 16 * num_sms()), 128, 0, stream()>>>(planes, k.meta, H, k.index, k.g, T, H,
-                                                                               (bf16*)dx.data_ptr());
-  check_launch("logprob_dx");
-  count_launch();
 }
 
 }  // namespace t1

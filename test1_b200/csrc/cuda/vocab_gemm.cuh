@@ -1,17 +1,22 @@
 // tcgen05 products of the output layer whose [T, V] result is consumed on
-// the spot: the logits x W^T reduced to a log-sum-exp per row (kLse), the
-// logits turned into their softmax gradient (kSoftmaxGrad), and the two
-// products with that gradient (kRowsF32: rows of dx, kWeightGrad: dW).
+// the spot.  One kernel, three jobs:
+//   kLse          logits x W^T, reduced to (largest, sum of exponentials) per
+//                 row and 256-column block, and the target's logit;
+//   kSoftmaxGrad  the same logits turned into u = onehot - softmax (bf16);
+//   kGrads        both products with u in one launch: rows of dx = g (u W) and
+//                 dW = u^T (g x).
 //
-// The main loop is that of gemm_pair.cuh without its stream-K tail: CTA
-// pairs (cta_group::2), 256 x 256 tiles, 128B-swizzled TMA loads into a
-// 6-stage ring, one elected thread issuing the MMAs, fp32 accumulators
-// double-buffered in TMEM, 4 epilogue warps per CTA that work on one
-// accumulator while the other fills.  The rows are those that the packing
-// kernel of logprob.cu kept, so their number is read on the GPU.  Units of
-// work are (k range, tile): `splits` > 1 cuts the reduction into ranges whose
-// results are separate fp32 planes (kRowsF32 only), so that few tiles still
-// fill the GPU and the planes are added in a fixed order afterwards.
+// The main loop is that of gemm_pair.cuh: CTA pairs (cta_group::2), 256 x 256
+// tiles, 128B-swizzled TMA loads into a 6-stage ring, one elected thread
+// issuing the MMAs, fp32 accumulators double-buffered in TMEM, 4 epilogue
+// warps per CTA that work on one accumulator while the other fills.  The
+// rows may be those that the packing kernel of logprob.cu kept, so their
+// number is read on the GPU.
+//
+// Work of a cluster: kLse and kSoftmaxGrad take tiles in turn.  kGrads has
+// units of two lengths, dx tiles (over a range of the vocabulary) and dW
+// tiles (over the rows); the long ones are dealt out first and the clusters
+// that got one less take short ones meanwhile (grad_unit).
 #pragma once
 
 #include "gemm_core.cuh"
@@ -31,45 +36,45 @@ constexpr int EPI_BYTES = 4 /*warps*/ * 2 * EPI_BUF;
 constexpr int V_SMEM_BYTES = VSTAGES * V_STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 static_assert(V_SMEM_BYTES <= 232448, "exceeds 227 KB of shared memory");
 
-enum Mode : int { kLse = 0, kSoftmaxGrad = 1, kRowsF32 = 2, kWeightGrad = 3 };
+enum Job : int { kLse = 0, kSoftmaxGrad = 1, kGrads = 2 };
 
 // What the packing of the batch's rows found out on the GPU.
 struct RowsMeta {
   int rows;    // rows that take part
-  int splits;  // ranges of k that the rows' product (kRowsF32) is cut into
+  int splits;  // ranges of the vocabulary that dx's product is cut into
 };
+
+// Row distances and offsets of one 32-row x 256-column block of fp32 sums:
+// [column / 4][row][4], so that a warp (a lane per row) moves 512
+// consecutive bytes at a time.
+constexpr int PLANE_BLOCK = 32 * TILE;
 
 struct VocabParams {
-  const RowsMeta* meta;  // its rows are M, or in kWeightGrad the reduction's length
-  int M, N;              // rows and columns of the product (M: kWeightGrad only)
-  int k_blocks;          // of BK = 64 (not in kWeightGrad)
-  int ld_part;           // kLse: rows of a column block in `part`
-  int accumulate;        // kRowsF32: add to what the plane holds
-  float scale;           // 1 / temperature
-  int col0;              // vocabulary index of column 0
-  const int* targets;    // [M] vocabulary index
-  float2* part;          // kLse: [tiles_n][ld_part] (largest logit, sum of exp(logit - largest)) of a column block
-  float* target_logit;   // kLse: [M], unscaled
-  const float* lse;      // kSoftmaxGrad: [M]
+  const RowsMeta* meta;    // null: `rows` and `splits` as given here
+  int rows, splits;
+  int N;                   // vocabulary columns of this launch
+  int H;
+  float scale;             // 1 / temperature
+  int col0;                // vocabulary index of column 0
+  const int* index;        // [rows] token of a packed row; null: the row itself
+  const int64_t* targets;  // [rows] vocabulary index
+  int* tickets;            // zero between launches: arrivals per 32 rows (kLse) or per 32 x 256 block of dx (kGrads)
+  // kLse
+  int64_t ignore, V;
+  int ld_part;
+  float2* part;            // [column block][ld_part]
+  float* target_logit;     // [rows], unscaled
+  int join;                // the last block of a row group joins its rows
+  float *logp, *lse_out;   // with join
+  // kSoftmaxGrad
+  const float* lse;        // [rows]
+  // kGrads
+  const float* g;          // [rows]
+  bf16* dx;                // [T, H]
+  float* planes;           // [tile][split][8] blocks of PLANE_BLOCK
+  int first, last;         // first / last piece of the vocabulary
   int* err;
 };
-
-// The product's extents, known once the packing has run.
-struct Extents {
-  int M, tiles_m, tiles_n, k_blocks, splits;
-};
-
-template <int MODE>
-__device__ __forceinline__ Extents extents(const VocabParams& p) {
-  const int rows = p.meta->rows;
-  Extents e;
-  e.M = MODE == kWeightGrad ? p.M : rows;
-  e.tiles_m = (e.M + TILE - 1) / TILE;
-  e.tiles_n = (p.N + TILE - 1) / TILE;
-  e.k_blocks = MODE == kWeightGrad ? (rows + BK - 1) / BK : p.k_blocks;
-  e.splits = MODE == kRowsF32 ? p.meta->splits : 1;
-  return e;
-}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -79,18 +84,108 @@ __device__ __forceinline__ float ex2(float x) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ void vocab_unit(const Extents& e, int u, int& mb, int& nb, int& kb0, int& kb1,
-                                           int& split) {
-  const int tiles = e.tiles_m * e.tiles_n;
-  split = u / tiles;
-  raster(u % tiles, e.tiles_m, e.tiles_n, mb, nb);
-  kb0 = static_cast<int>(static_cast<long>(split) * e.k_blocks / e.splits);
-  kb1 = static_cast<int>(static_cast<long>(split + 1) * e.k_blocks / e.splits);
+// Programmatic launch: the next kernel of the stream may start its prologue,
+// and this one touches nothing of the previous kernel's before it has ended.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Running (largest m, sum s of exp((v - m) / tau)); k2 = log2(e) / tau.
+__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2, float k2) {
+  const float mn = fmaxf(m, m2);
+  const float ref = mn == -INFINITY ? 0.f : mn;
+  s = s * ex2((m - ref) * k2) + s2 * ex2((m2 - ref) * k2);
+  m = mn;
 }
 
-template <bool A_MN, bool B_MN, int MODE>
+// log-probability and log-sum-exp of a row.  (target - largest) first: exact
+// where the target is likely.
+__device__ __forceinline__ void write_logp(const float m, const float s, const float target, const bool valid,
+                                           const float scale, float* logp, float* lse) {
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float log_s = logf(s);
+  *logp = valid ? (target - ref) * scale - log_s : 0.f;
+  *lse = valid ? ref * scale + log_s : 0.f;
+}
+
+// ---------------------------------------------------------- units of work
+// Time of a unit in k blocks of 64 (0.27 us of tensor time for a pair): dx
+// tiles pay about 12 for start, drain and planes; a dW tile cannot be faster
+// than its 128 KB leave (about 9).
+__host__ __device__ inline int dx_unit_cost(int k_blocks, int splits) { return k_blocks / splits + 12; }
+__host__ __device__ inline int dw_unit_cost(int tiles_t) {
+  const int k = tiles_t * (TILE / BK);
+  return k > 9 ? k : 9;
+}
+
+struct Shape {
+  int rows, tiles_t, tiles_n, tiles_h, k_h, k_n, k_rows, splits;
+};
+
+__device__ __forceinline__ Shape shape_of(const VocabParams& p, bool splits) {
+  Shape e;
+  e.rows = p.meta != nullptr ? p.meta->rows : p.rows;
+  e.splits = !splits ? 1 : p.meta != nullptr ? p.meta->splits : p.splits;
+  e.tiles_t = (e.rows + TILE - 1) / TILE;
+  e.tiles_n = (p.N + TILE - 1) / TILE;
+  e.tiles_h = (p.H + TILE - 1) / TILE;
+  e.k_h = (p.H + BK - 1) / BK;
+  e.k_n = (p.N + BK - 1) / BK;
+  e.k_rows = (e.rows + BK - 1) / BK;
+  return e;
+}
+
+struct Unit {
+  int mb, nb, kb0, kb1;
+  int split;  // kGrads: range of the vocabulary, or -1 for a dW tile
+};
+
+// The i-th unit of cluster c out of C; false when there is none.
+template <int JOB>
+__device__ __forceinline__ bool get_unit(const Shape& e, int i, int c, int C, Unit& u) {
+  if (JOB != kGrads) {
+    const int64_t t = c + static_cast<int64_t>(i) * C;
+    if (t >= static_cast<int64_t>(e.tiles_t) * e.tiles_n) return false;
+    raster(static_cast<int>(t), e.tiles_t, e.tiles_n, u.mb, u.nb);
+    u.kb0 = 0;
+    u.kb1 = e.k_h;
+    u.split = 0;
+    return true;
+  }
+  const int tiles = e.tiles_t * e.tiles_h, X = tiles * e.splits, D = e.tiles_n * e.tiles_h;
+  const int q = X / C, r = X % C;
+  const int mine = q + (c < r);
+  if (i < mine) {
+    const int x = c + i * C;
+    u.split = x / tiles;
+    raster(x % tiles, e.tiles_t, e.tiles_h, u.mb, u.nb);
+    u.kb0 = static_cast<int>(static_cast<int64_t>(u.split) * e.k_n / e.splits);
+    u.kb1 = static_cast<int>(static_cast<int64_t>(u.split + 1) * e.k_n / e.splits);
+    return true;
+  }
+  int j = i - mine;
+  // dW tiles that clusters r.. take while the first r work on one more dx tile
+  const int uw = dw_unit_cost(e.tiles_t);
+  const int rounds = r == 0 ? 0 : (dx_unit_cost(e.k_n, e.splits) + uw / 2) / uw;
+  const int early = static_cast<int>(min(static_cast<int64_t>(D), static_cast<int64_t>(rounds) * (C - r)));
+  const int before = c < r || early <= c - r ? 0 : (early - (c - r) + (C - r) - 1) / (C - r);
+  int64_t d;
+  if (j < before) d = static_cast<int64_t>(j) * (C - r) + (c - r);
+  else d = early + static_cast<int64_t>(j - before) * C + c;
+  if (d >= D) return false;
+  raster(static_cast<int>(d), e.tiles_n, e.tiles_h, u.mb, u.nb);
+  u.kb0 = 0;
+  u.kb1 = e.k_rows;
+  u.split = -1;
+  return true;
+}
+
+// Operands: kLse, kSoftmaxGrad: A = rows of x, B = W.  kGrads, dx: A = u, B =
+// W by columns; dW: A2 = u by columns, B2 = g x by columns.  tma_c: u
+// (kSoftmaxGrad) or dW (kGrads).
+template <int JOB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     vocab_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                 const __grid_constant__ CUtensorMap tma_a2, const __grid_constant__ CUtensorMap tma_b2,
                  const __grid_constant__ CUtensorMap tma_c, const VocabParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -112,6 +207,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   const int nclusters = gridDim.x >> 1;
   const ErrorSlot err{p.err};
 
+  launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < VSTAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -127,7 +223,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&tma_a);
     prefetch_tensormap(&tma_b);
-    if (MODE != kLse) prefetch_tensormap(&tma_c);
+    if (JOB != kLse) prefetch_tensormap(&tma_c);
+    if (JOB == kGrads) {
+      prefetch_tensormap(&tma_a2);
+      prefetch_tensormap(&tma_b2);
+    }
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, TMEM_COLS);
@@ -138,20 +238,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   cluster_sync();  // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const Extents e = extents<MODE>(p);
-  const int num_units = e.tiles_m * e.tiles_n * e.splits;
+  wait_previous();
+  const Shape e = shape_of(p, JOB == kGrads);
+  Unit u;
 
   if (warp == 0) {
     // ------------------------------------------------------ TMA producer
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      for (int u = cluster; u < num_units && !*abort_flag; u += nclusters) {
-        int mb, nb, kb0, kb1, split;
-        vocab_unit(e, u, mb, nb, kb0, kb1, split);
-        const int row_a = mb * TILE + static_cast<int>(crank) * HALF;
-        const int row_b = nb * TILE + static_cast<int>(crank) * HALF;
-        for (int kb = kb0; kb < kb1; ++kb) {
+      for (int i = 0; !*abort_flag && get_unit<JOB>(e, i, cluster, nclusters, u); ++i) {
+        const bool dw = JOB == kGrads && u.split < 0;
+        const int row_a = u.mb * TILE + static_cast<int>(crank) * HALF;
+        const int row_b = u.nb * TILE + static_cast<int>(crank) * HALF;
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1)) {
             err.set(121);
             *abort_flag = 1;
@@ -162,17 +262,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           uint8_t* a = sA + stage * V_A_BYTES;
           uint8_t* b = sB + stage * V_A_BYTES;
           const int k0 = kb * BK;
-          if (!A_MN) {
+          if (dw) {
+            tma_load_2d_pair(a, &tma_a2, lfull, row_a, k0);
+            tma_load_2d_pair(a + 8192, &tma_a2, lfull, row_a + 64, k0);
+            tma_load_2d_pair(b, &tma_b2, lfull, row_b, k0);
+            tma_load_2d_pair(b + 8192, &tma_b2, lfull, row_b + 64, k0);
+          } else {
             tma_load_2d_pair(a, &tma_a, lfull, k0, row_a);
-          } else {
-            tma_load_2d_pair(a, &tma_a, lfull, row_a, k0);
-            tma_load_2d_pair(a + 8192, &tma_a, lfull, row_a + 64, k0);
-          }
-          if (!B_MN) {
-            tma_load_2d_pair(b, &tma_b, lfull, k0, row_b);
-          } else {
-            tma_load_2d_pair(b, &tma_b, lfull, row_b, k0);
-            tma_load_2d_pair(b + 8192, &tma_b, lfull, row_b + 64, k0);
+            if (JOB == kGrads) {
+              tma_load_2d_pair(b, &tma_b, lfull, row_b, k0);
+              tma_load_2d_pair(b + 8192, &tma_b, lfull, row_b + 64, k0);
+            } else {
+              tma_load_2d_pair(b, &tma_b, lfull, k0, row_b);
+            }
           }
           if (++stage == VSTAGES) {
             stage = 0;
@@ -184,15 +286,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   } else if (warp == 1) {
     // ------------------------------------------- MMA issuer (leader only)
     if (lane == 0 && crank == 0) {
-      constexpr uint32_t IDESC = idesc_bf16_f32(TILE, TILE, A_MN, B_MN);
       int stage = 0;
       uint32_t phase = 0;
-      int local = 0;
-      for (int u = cluster; u < num_units && !*abort_flag; u += nclusters, ++local) {
-        int mb, nb, kb0, kb1, split;
-        vocab_unit(e, u, mb, nb, kb0, kb1, split);
-        const int acc = local & 1;
-        const uint32_t acc_phase = (local >> 1) & 1;
+      for (int i = 0; !*abort_flag && get_unit<JOB>(e, i, cluster, nclusters, u); ++i) {
+        const bool a_mn = JOB == kGrads && u.split < 0;
+        constexpr bool b_mn = JOB == kGrads;
+        const uint32_t idesc = a_mn ? idesc_bf16_f32(TILE, TILE, true, b_mn) : idesc_bf16_f32(TILE, TILE, false, b_mn);
+        const int acc = i & 1;
+        const uint32_t acc_phase = (i >> 1) & 1;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1)) {
           err.set(122);
           *abort_flag = 1;
@@ -201,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * TILE;
         bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait(&full[stage], phase)) {
             err.set(123);
             *abort_flag = 1;
@@ -213,11 +314,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           const uint32_t b_addr = smem_u32(sB + stage * V_A_BYTES);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t ad = A_MN ? smem_desc_sw128(a_addr + k * 2048, 8192, 1024)
+            const uint64_t ad = a_mn ? smem_desc_sw128(a_addr + k * 2048, 8192, 1024)
                                      : smem_desc_sw128(a_addr + k * 32, 16, 1024);
-            const uint64_t bd = B_MN ? smem_desc_sw128(b_addr + k * 2048, 8192, 1024)
+            const uint64_t bd = b_mn ? smem_desc_sw128(b_addr + k * 2048, 8192, 1024)
                                      : smem_desc_sw128(b_addr + k * 32, 16, 1024);
-            mma_bf16_pair(d_tmem, ad, bd, IDESC, (kb != kb0 || k != 0) ? 1u : 0u);
+            mma_bf16_pair(d_tmem, ad, bd, idesc, (kb != u.kb0 || k != 0) ? 1u : 0u);
           }
           mma_commit_pair(&empty[stage], 0x3);
           if (++stage == VSTAGES) {
@@ -235,13 +336,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     uint8_t* wbuf = sE + q * 2 * EPI_BUF;
     const uint32_t leader_tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
     const uint32_t leader_tempty1 = mapa_shared(smem_u32(&tempty[1]), 0);
+    const float k2 = p.scale * kLog2e;
     int bi = 0;
-    int local = 0;
-    for (int u = cluster; u < num_units; u += nclusters, ++local) {
-      int mb, nb, kb0, kb1, split;
-      vocab_unit(e, u, mb, nb, kb0, kb1, split);
-      const int acc = local & 1;
-      const uint32_t acc_phase = (local >> 1) & 1;
+    for (int i = 0; get_unit<JOB>(e, i, cluster, nclusters, u); ++i) {
+      const int acc = i & 1;
+      const uint32_t acc_phase = (i >> 1) & 1;
       // one lane waits and the warp follows it, so the warp never diverges
       // around the .sync.aligned TMEM loads below
       int ok = 0;
@@ -255,20 +354,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       }
       if (!__shfl_sync(0xffffffffu, ok, 0)) break;
       tc_fence_after();
-      const int row0 = mb * TILE + static_cast<int>(crank) * HALF + q * 32;
+      const int w8 = static_cast<int>(crank) * 4 + q;  // which 32 rows of the tile
+      const int row0 = u.mb * TILE + w8 * 32;
       const int row = row0 + lane;
-      const bool row_ok = row < e.M;
-      const int tcol0 = nb * TILE;                       // first column of the tile
-      const int cols = min(TILE, p.N - tcol0);           // columns of the tile that exist
+      const int tcol0 = u.nb * TILE;  // first column of the tile
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * TILE;
+      auto release = [&] {  // the accumulator's last read is done
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
+      };
 
-      if (MODE == kLse) {
+      if (JOB == kLse) {
         // A running (largest, sum) over the tile's columns, kept in the
         // accumulator's own units: (logit - largest) is exact near the
         // largest, which is where the sum comes from.
-        const float k2 = p.scale * kLog2e;
-        const int t = row_ok ? p.targets[row] - tcol0 : -1;
-        const int tcol = t < cols ? t : -1;
+        const bool row_ok = row < e.rows;
+        const int cols = min(TILE, p.N - tcol0);
+        const int64_t t = row_ok ? p.targets[row] - tcol0 : -1;
+        const int tcol = t >= 0 && t < cols ? static_cast<int>(t) : -1;
         float m = -INFINITY, s = 0.f;
 #pragma unroll 1
         for (int c = 0; c < TILE; c += 32) {
@@ -277,99 +381,171 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           tmem_ld_wait();
           if (c + 32 > cols) {  // columns past the vocabulary
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j >= cols) r[j] = __float_as_uint(-INFINITY);
+            for (int j = 0; j < 32; ++j) r[j] = c + j >= cols ? __float_as_uint(-INFINITY) : r[j];
           }
-          float mx = __uint_as_float(r[0]);
+          float mx[4];
 #pragma unroll
-          for (int j = 1; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(r[j]));
-          const float mn = fmaxf(m, mx);
+          for (int j = 0; j < 4; ++j) mx[j] = fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 4]));
+#pragma unroll
+          for (int j = 8; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(r[j]));
+          const float mn = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
           const float ref = mn == -INFINITY ? 0.f : mn;
-          s *= ex2((m - ref) * k2);
+          float a[4] = {s * ex2((m - ref) * k2), 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s += ex2((__uint_as_float(r[j]) - ref) * k2);
+          for (int j = 0; j < 32; ++j) a[j & 3] += ex2((__uint_as_float(r[j]) - ref) * k2);
+          s = (a[0] + a[1]) + (a[2] + a[3]);
           m = mn;
-          if (tcol >= c && tcol < c + 32) {
-            if (!T1_OOB(row, p.ld_part)) {
+          if (tcol >= c && tcol < c + 32 && !T1_OOB(row, p.ld_part)) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (tcol - c == j) p.target_logit[row] = __uint_as_float(r[j]);
+            for (int j = 0; j < 32; ++j)
+              if (tcol - c == j) p.target_logit[row] = __uint_as_float(r[j]);
+          }
+        }
+        release();
+        if (row_ok && !T1_OOB(row, p.ld_part)) __stcg(&p.part[static_cast<size_t>(u.nb) * p.ld_part + row], make_float2(m, s));
+        if (!p.join) continue;
+        // the last of the row group's column blocks joins them all, in order
+        __threadfence();
+        __syncwarp();
+        int last = 0;
+        if (lane == 0) last = atomicAdd(&p.tickets[u.mb * 8 + w8], 1) == e.tiles_n - 1;
+        if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+        __threadfence();
+        if (lane == 0) p.tickets[u.mb * 8 + w8] = 0;
+        if (!row_ok) continue;
+        m = -INFINITY;
+        s = 0.f;
+#pragma unroll 4
+        for (int b = 0; b < e.tiles_n; ++b) {
+          const float2 v = __ldcg(&p.part[static_cast<size_t>(b) * p.ld_part + row]);
+          lse_join(m, s, v.x, v.y, k2);
+        }
+        const int at = p.index != nullptr ? p.index[row] : row;
+        const int64_t target = p.targets[row];
+        write_logp(m, s, __ldcg(&p.target_logit[row]), target != p.ignore && target >= 0 && target < p.V, p.scale,
+                   p.logp + at, p.lse_out + at);
+        continue;
+      }
+
+      if (JOB == kGrads && u.split >= 0) {
+        // dx: these columns' sums, in fp32 until all of the vocabulary is in
+        const bool live = row0 < e.rows;
+        const int tile = u.mb * e.tiles_h + u.nb;
+        const size_t tile_block = (static_cast<size_t>(tile) * e.splits) * 8 + w8;
+        float4* plane = reinterpret_cast<float4*>(p.planes + (tile_block + static_cast<size_t>(u.split) * 8) * PLANE_BLOCK);
+        const float gr = row < e.rows ? p.g[row] : 0.f;
+        const int at = row < e.rows && p.index != nullptr ? p.index[row] : row;
+        const bool direct = e.splits == 1 && p.last;  // no other range, no later piece
+        // 64 columns of dx: g x sums, rounded once, to whole 128-byte lines
+        // of the rows' tokens
+        auto store64 = [&](const float* f, int c) {
+          uint8_t* rowp = wbuf + lane * 128;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint4 ov;
+            __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&ov);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) oh[k] = __floats2bfloat162_rn(f[8 * j + 2 * k] * gr, f[8 * j + 2 * k + 1] * gr);
+            if (gr == 0.f) ov = make_uint4(0, 0, 0, 0);  // whatever W holds
+            *reinterpret_cast<uint4*>(rowp + ((j ^ (lane & 7)) << 4)) = ov;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int rr = it * 4 + (lane >> 3), j = lane & 7;
+            const int64_t t = __shfl_sync(0xffffffffu, at, rr);
+            const uint4 v = *reinterpret_cast<const uint4*>(wbuf + rr * 128 + ((j ^ (rr & 7)) << 4));
+            const int col = tcol0 + c + 8 * j;
+            if (row0 + rr < e.rows && col < p.H) *reinterpret_cast<uint4*>(p.dx + t * p.H + col) = v;
+          }
+          __syncwarp();
+        };
+        if (lane == 0) bulk_wait_group_read<0>();  // stores of an earlier dW tile have read the slab
+        __syncwarp();
+#pragma unroll 1
+        for (int c = 0; c < TILE; c += 64) {
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32(taddr + c, r[0]);
+          tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
+          tmem_ld_wait();
+          if (c + 64 == TILE) release();
+          if (!live) continue;
+          float f[64];
+#pragma unroll
+          for (int j = 0; j < 64; ++j) f[j] = u.kb0 == u.kb1 ? 0.f : __uint_as_float(r[j >> 5][j & 31]);
+          if (!p.first) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float4 v = __ldcg(plane + (c / 4 + j) * 32 + lane);
+              f[4 * j] += v.x;
+              f[4 * j + 1] += v.y;
+              f[4 * j + 2] += v.z;
+              f[4 * j + 3] += v.w;
             }
           }
+          if (direct) {
+            store64(f, c);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              __stcg(plane + (c / 4 + j) * 32 + lane, make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]));
+          }
         }
-        tc_fence_before();
+        if (direct || !p.last || !live) continue;
+        // the last range to finish adds the planes, in their order
+        __threadfence();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
-        if (row_ok && !T1_OOB(row, p.ld_part)) p.part[static_cast<size_t>(nb) * p.ld_part + row] = make_float2(m, s);
-        continue;
-      }
-
-      if (MODE == kRowsF32) {
-        // fp32 rows through 32 x 32 slabs (128-byte rows)
+        int last = 0;
+        if (lane == 0) last = atomicAdd(&p.tickets[tile * 8 + w8], 1) == e.splits - 1;
+        if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+        __threadfence();
+        if (lane == 0) p.tickets[tile * 8 + w8] = 0;
+        const float4* planes = reinterpret_cast<const float4*>(p.planes + tile_block * PLANE_BLOCK);
 #pragma unroll 1
-        for (int c = 0; c < TILE; c += 32) {
-          uint8_t* buf = wbuf + bi * EPI_BUF;
-          const bool live = c < cols && row0 < e.M;  // uniform over the warp
-          if (lane == 0) bulk_wait_group_read<1>();
-          __syncwarp();
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(taddr + c, r);
-          tmem_ld_wait();
-          if (c + 32 == TILE) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
-          }
-          if (!live) continue;
-          if (kb0 == kb1) {  // a range of no columns
+        for (int c = 0; c < TILE; c += 64) {
+          float f[64];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = 0;
-          }
-          uint8_t* rowp = buf + lane * 128;
+          for (int j = 0; j < 64; ++j) f[j] = 0.f;
+          for (int s = 0; s < e.splits; ++s) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(rowp + ((j ^ (lane & 7)) << 4)) =
-                make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            const int prow = split * e.tiles_m * TILE + row0;
-            if (p.accumulate) tma_reduce_add_2d(&tma_c, buf, tcol0 + c, prow);
-            else tma_store_2d(&tma_c, buf, tcol0 + c, prow);
-            bulk_commit_group();
+            for (int j = 0; j < 16; ++j) {
+              const float4 v = __ldcg(planes + static_cast<size_t>(s) * (8 * PLANE_BLOCK / 4) + (c / 4 + j) * 32 + lane);
+              f[4 * j] += v.x;
+              f[4 * j + 1] += v.y;
+              f[4 * j + 2] += v.z;
+              f[4 * j + 3] += v.w;
+            }
           }
-          bi ^= 1;
+          store64(f, c);
         }
         continue;
       }
 
-      // bf16 results (kSoftmaxGrad, kWeightGrad) through 32 x 64 slabs
+      // bf16 results (u, dW) through 32 x 64 slabs
+      const bool row_ok = row < e.rows;
+      const int cols = min(TILE, (JOB == kSoftmaxGrad ? p.N : p.H) - tcol0);
+      // u's rows are a reduction's length in kGrads: its last block of BK has
+      // to be there, with zeros past the last row
+      const int m_end = JOB == kSoftmaxGrad ? e.k_rows * BK : p.N;
       float lse2 = 0.f;
       int tcol = -1;
-      const float k2 = p.scale * kLog2e;
-      if (MODE == kSoftmaxGrad && row_ok) {
+      if (JOB == kSoftmaxGrad && row_ok) {
         lse2 = p.lse[row] * kLog2e;
-        const int t = p.targets[row] - p.col0 - tcol0;
-        tcol = t < cols ? t : -1;
+        const int64_t t = p.targets[row] - p.col0 - tcol0;
+        tcol = t >= 0 && t < cols ? static_cast<int>(t) : -1;
       }
-      // u's rows are a reduction's length in kWeightGrad: its last block of
-      // BK has to be there, with zeros past the last row
-      const int m_end = MODE == kSoftmaxGrad ? (e.M + BK - 1) / BK * BK : e.M;
 #pragma unroll 1
       for (int c = 0; c < TILE; c += 64) {
         uint8_t* buf = wbuf + bi * EPI_BUF;
-        const bool live = c < cols && row0 < m_end;
+        const bool live = c < cols && row0 < m_end;  // uniform over the warp
+        // the store issued from this buffer two slabs ago has read it
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
         uint32_t r[2][32];
         tmem_ld_32x32b_x32(taddr + c, r[0]);
         tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
         tmem_ld_wait();
-        if (c + 64 == TILE) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
-        }
+        if (c + 64 == TILE) release();
         if (!live) continue;
         uint8_t* rowp = buf + lane * 128;
 #pragma unroll
@@ -378,10 +554,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             f[k] = __uint_as_float(r[j >> 2][(j & 3) * 8 + k]);
-            if (MODE == kSoftmaxGrad) {
+            if (JOB == kSoftmaxGrad) {
               f[k] = row_ok ? -ex2(fmaf(f[k], k2, -lse2)) : 0.f;
               if (tcol == c + 8 * j + k) f[k] += 1.f;
-            } else if (kb0 == kb1) {  // a sum over no rows
+            } else if (u.kb0 == u.kb1) {  // a sum over no rows
               f[k] = 0.f;
             }
           }
