@@ -203,6 +203,222 @@ __global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const Voc
   vocab::write_logp(m, s, p.target_logit[row], v != p.ignore && v >= 0 && v < p.V, p.scale, p.logp + t, p.lse_out + t);
 }
 
+// -------------------------------------------------------------- few rows
+// At most 16 tokens (a decoding step's, a short answer's): all that counts is
+// reading W once.  A block takes 16 rows of W at a time; its 16 warps share
+// the columns, read W straight into mma fragments (a thread's 16 bytes are
+// the four k's that two m16n8k16 steps give it: the order of a sum is free, so
+// no shuffling and no shared memory for W) and keep x in shared memory.  The
+// next rows' loads are in flight while a block adds up its warps' parts.
+// tcgen05 tiles would spend 256 rows of tensor time on them and read x
+// through TMA boxes that are mostly padding (T=1 at V=128256, H=4096: 260 us
+// against 177 us here, 5.9 TB/s).
+struct FewParams {
+  const bf16* x;
+  long ldx;
+  const bf16* w;
+  long ldw;
+  const int64_t* targets;
+  int64_t ignore;
+  int T, H, V;
+  float scale;
+  int* ticket;
+  // forward
+  float2* part;          // [block][16]
+  float* target_logit;   // [16]
+  float *logp, *lse_out;
+  // backward: u, g and g x
+  const float *dlogp, *lse;
+  bf16* u;               // [T, ldu]
+  long ldu;
+  float* g;
+  bf16* gx;              // [T, H]
+};
+
+constexpr int kFewThreads = 512;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kFewRows = 16;    // rows of W per step
+constexpr int kFewLoads = 8;    // blocks of 32 columns that a warp has in flight
+
+// Distance of two tokens' columns in shared memory: 64 bytes past a multiple
+// of 128, so that the 8 threads of a 16-byte read's phase (2 tokens x 4)
+// touch every bank once.
+__host__ __device__ inline int few_pitch(int H) { return (2 * H + 127) / 128 * 128 + 64; }
+inline size_t few_smem(int tokens8, int H) {
+  return static_cast<size_t>(tokens8) * few_pitch(H) + 2 * kFewWarps * kFewRows * tokens8 * sizeof(float);
+}
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int NT, bool BWD>
+__global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewParams p) {
+  constexpr int TOK = 8 * NT;
+  constexpr int CELLS = kFewRows * TOK;  // a step's logits, one per thread of the first CELLS
+  extern __shared__ __align__(16) uint8_t few_raw[];
+  uint8_t* xs = few_raw;
+  const int pitch = few_pitch(p.H);
+  float* red = reinterpret_cast<float*>(few_raw + TOK * pitch);
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  vocab::launch_dependents();
+  vocab::wait_previous();
+
+  const int blocks32 = (p.H + 31) / 32;                       // of columns
+  const int kb_lo = warp * blocks32 / kFewWarps, kb_hi = (warp + 1) * blocks32 / kFewWarps;
+  const int per_warp = (blocks32 + kFewWarps - 1) / kFewWarps;
+  const int chunks = (per_warp + kFewLoads - 1) / kFewLoads;  // the same for every warp
+  const int groups = (p.V + kFewRows - 1) / kFewRows;
+  const int steps = (groups - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) * chunks;
+
+  uint4 wa[kFewLoads], wb[kFewLoads];
+  auto load = [&](int step) {
+    const int group = blockIdx.x + step / chunks * gridDim.x;
+    const int ra = min(p.V - 1, group * kFewRows + g), rb = min(p.V - 1, group * kFewRows + g + 8);
+    const bf16* pa = p.w + static_cast<size_t>(ra) * p.ldw;
+    const bf16* pb = p.w + static_cast<size_t>(rb) * p.ldw;
+#pragma unroll
+    for (int i = 0; i < kFewLoads; ++i) {
+      const int kb = kb_lo + step % chunks * kFewLoads + i, k = kb * 32 + c * 8;
+      const bool in = kb < kb_hi && k < p.H;
+      wa[i] = in ? ld_stream(pa + k) : make_uint4(0, 0, 0, 0);
+      wb[i] = in ? ld_stream(pb + k) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  if (steps > 0) load(0);
+
+  // x to shared memory, zeros past its columns and tokens
+  const int vecs = (pitch - 64) / 16;
+  for (int i = tid; i < TOK * vecs; i += kFewThreads) {
+    const int t = i / vecs, v = i % vecs;
+    uint4 val = make_uint4(0, 0, 0, 0);
+    if (t < p.T && 8 * v < p.H) val = *reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(t) * p.ldx + 8 * v);
+    *reinterpret_cast<uint4*>(xs + t * pitch + 16 * v) = val;
+  }
+  // what this thread's cell (row of the step, token) needs to know
+  const int token = tid % TOK, wrow = tid / TOK;
+  const bool cell = tid < CELLS && token < p.T;
+  const int64_t target = cell ? p.targets[token] : -1;
+  const bool valid = cell && target != p.ignore && target >= 0 && target < p.V;
+  const float k2 = p.scale * kLog2e;
+  float lse2 = 0.f, gr = 0.f;
+  if (BWD && valid) {
+    lse2 = p.lse[token] * kLog2e;
+    gr = p.dlogp[token] * p.scale;
+  }
+  if (BWD && blockIdx.x == 0 && cell && wrow == 0) p.g[token] = gr;
+  __syncthreads();
+  if (BWD) {  // g x, a share of it per block
+    for (int64_t i = blockIdx.x * kFewThreads + tid; i < static_cast<int64_t>(p.T) * (p.H / 8); i += static_cast<int64_t>(gridDim.x) * kFewThreads) {
+      const int t = static_cast<int>(i / (p.H / 8)), v = static_cast<int>(i % (p.H / 8));
+      const int64_t tt = p.targets[t];
+      const float s = tt != p.ignore && tt >= 0 && tt < p.V ? p.dlogp[t] * p.scale : 0.f;
+      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (s != 0.f) {
+        load8(reinterpret_cast<const bf16*>(xs + t * pitch + 16 * v), f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] *= s;
+      }
+      store8(p.gx + static_cast<size_t>(t) * p.H + 8 * v, f);
+    }
+  }
+
+  float m = -INFINITY, s = 0.f;
+  float acc[NT][4] = {};
+  int buf = 0;
+  for (int step = 0; step < steps; ++step) {
+    const int chunk = step % chunks;
+#pragma unroll
+    for (int i = 0; i < kFewLoads; ++i) {
+      const int kb = kb_lo + chunk * kFewLoads + i;
+      if (kb >= kb_hi) break;  // uniform over the warp
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint4 xv = *reinterpret_cast<const uint4*>(xs + (n * 8 + g) * pitch + kb * 64 + c * 16);
+        mma_16816(acc[n], wa[i].x, wb[i].x, wa[i].y, wb[i].y, xv.x, xv.y);
+        mma_16816(acc[n], wa[i].z, wb[i].z, wa[i].w, wb[i].w, xv.z, xv.w);
+      }
+    }
+    if (step + 1 < steps) load(step + 1);
+    if (chunk + 1 < chunks) continue;
+    // the warps' parts of 16 x TOK logits
+    float* mine = red + (buf * kFewWarps + warp) * CELLS;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      *reinterpret_cast<float2*>(mine + g * TOK + n * 8 + 2 * c) = make_float2(acc[n][0], acc[n][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * TOK + n * 8 + 2 * c) = make_float2(acc[n][2], acc[n][3]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
+    }
+    __syncthreads();  // two buffers: the next step's parts go to the other
+    const int v = (static_cast<int>(blockIdx.x) + step / chunks * static_cast<int>(gridDim.x)) * kFewRows + wrow;
+    if (cell && v < p.V) {
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) l += red[(buf * kFewWarps + w) * CELLS + tid];
+      if (BWD) {
+        float uv = gr != 0.f ? -ex2(fmaf(l, k2, -lse2)) : 0.f;
+        if (gr != 0.f && v == target) uv += 1.f;
+        p.u[token * p.ldu + v] = __float2bfloat16_rn(uv);
+      } else {
+        vocab::lse_join(m, s, l, 1.f, k2);
+        if (v == target) __stcg(&p.target_logit[token], l);
+      }
+    }
+    buf ^= 1;
+  }
+  if (BWD) return;
+
+  // this block's (largest, sum) per token, then all blocks' by the last one
+  float2* cells = reinterpret_cast<float2*>(red);
+  __syncthreads();
+  if (tid < CELLS) cells[tid] = make_float2(m, s);
+  __syncthreads();
+  if (tid < TOK) {
+    for (int r = 1; r < kFewRows; ++r) vocab::lse_join(m, s, cells[r * TOK + tid].x, cells[r * TOK + tid].y, k2);
+    __stcg(&p.part[blockIdx.x * 16 + tid], make_float2(m, s));
+  }
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  if (tid == 0) *p.ticket = 0;
+  if (warp >= p.T) return;  // a warp per token
+  m = -INFINITY;
+  s = 0.f;
+  for (int b = lane; b < static_cast<int>(gridDim.x); b += 32) {
+    const float2 v = __ldcg(&p.part[b * 16 + warp]);
+    vocab::lse_join(m, s, v.x, v.y, k2);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    vocab::lse_join(m, s, m2, s2, k2);
+  }
+  if (lane == 0) {
+    const int64_t t = p.targets[warp];
+    vocab::write_logp(m, s, __ldcg(&p.target_logit[warp]), t != p.ignore && t >= 0 && t < p.V, p.scale, p.logp + warp,
+                      p.lse_out + warp);
+  }
+}
+
 // ================================================================ host side
 T1_BOUNDS_READER(logprob)
 
@@ -300,6 +516,40 @@ static void launch_pack(PackParams& p) {
   else launch_after("logprob_pack", logprob_pack_kernel<false>, grid, kPackThreads, 0, p);
 }
 
+// Whether a batch takes the few-rows kernel: x has to fit in shared memory.
+constexpr size_t kFewSmem = 200 * 1024;
+static bool few_rows(int64_t T, int64_t H) { return T <= 16 && few_smem(T <= 8 ? 8 : 16, H) <= kFewSmem; }
+
+static int few_grid(int64_t V) { return static_cast<int>(std::min<int64_t>(ceil_div(V, kFewRows), num_sms())); }
+
+static FewParams few_params(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets, int64_t ignore,
+                            double temperature) {
+  FewParams p{};
+  p.x = (const bf16*)x.data_ptr();
+  p.ldx = row_ld(x);
+  p.w = (const bf16*)w.data_ptr();
+  p.ldw = row_ld(w);
+  p.targets = targets.data_ptr<int64_t>();
+  p.ignore = ignore;
+  p.T = x.size(0);
+  p.H = x.size(1);
+  p.V = w.size(0);
+  p.scale = static_cast<float>(1.0 / temperature);
+  return p;
+}
+
+template <bool BWD>
+static void launch_few(const FewParams& p) {
+  const int tokens8 = p.T <= 8 ? 8 : 16;
+  auto kern = tokens8 == 8 ? logprob_few_kernel<1, BWD> : logprob_few_kernel<2, BWD>;
+  static bool configured[2] = {false, false};
+  if (!configured[tokens8 / 8 - 1]) {
+    T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    configured[tokens8 / 8 - 1] = true;
+  }
+  launch_after("logprob_few", kern, dim3(few_grid(p.V)), kFewThreads, few_smem(tokens8, p.H), p);
+}
+
 // Whether the forward packs its rows first.  Below 256 tokens there is one
 // row of tiles whatever is left out, and a product of less than about 30 us
 // gains less from losing half of its rows than the packing costs (6 us).
@@ -321,6 +571,18 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   auto logp = torch::empty({T}, f32), lse = torch::empty({T}, f32);
   if (T == 0) return {logp, lse};
   auto tg = targets.contiguous();
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 && row_ld(w) % 8 == 0, "w must have 16-byte aligned rows");
+  if (few_rows(T, H)) {
+    FewParams p = few_params(x, w, tg, ignore_index, temperature);
+    auto ws = torch::empty({32 * few_grid(V) + 16}, f32);
+    p.part = reinterpret_cast<float2*>(ws.data_ptr<float>());
+    p.target_logit = ws.data_ptr<float>() + 32 * few_grid(V);
+    p.ticket = tickets(1);
+    p.logp = logp.data_ptr<float>();
+    p.lse_out = lse.data_ptr<float>();
+    launch_few<false>(p);
+    return {logp, lse};
+  }
   const int64_t blocks = ceil_div(V, vocab::TILE), tiles_t = ceil_div(T, vocab::TILE);
   const bool pack = packs(T, H, V);
   Pieces ws;
@@ -394,6 +656,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   TORCH_CHECK(dlogp.device() == x.device() && lse.device() == x.device() && dx.device() == x.device() &&
                   dw.device() == x.device(), "operands must be on one device");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(dx.data_ptr()) % 16 == 0, "dx must be 16-byte aligned");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 && row_ld(w) % 8 == 0, "w must have 16-byte aligned rows");
   const c10::cuda::CUDAGuard guard(x.device());
   if (T == 0) {
     dw.zero_();
@@ -406,7 +669,10 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   const int64_t most = std::max<int64_t>(vocab::TILE, kGradBufferBytes / (2 * T) / vocab::TILE * vocab::TILE);
   const int64_t pieces = ceil_div(V, most);
   const int64_t width = std::min(V, round_up(ceil_div(V, pieces), vocab::TILE));
-  const int64_t ldu = round_up(width, 8), u_rows = round_up(T, gemm::BK), k_v = ceil_div(width, gemm::BK);
+  const bool few = few_rows(T, H) && pieces == 1;
+  // with few rows nothing is packed: u and g x have T rows, and TMA reads
+  // zeros past them
+  const int64_t ldu = round_up(width, 8), u_rows = few ? T : round_up(T, gemm::BK), k_v = ceil_div(width, gemm::BK);
   const int64_t tiles_v = ceil_div(width, vocab::TILE);
   // the most planes and units that the split rule can ask for, over the
   // numbers of rows that the packing may leave
@@ -423,6 +689,34 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
                 o_u = ws.take(2 * u_rows * ldu);
   auto buf = torch::empty({ws.used}, x.options().dtype(torch::kUInt8));
   uint8_t* base = buf.data_ptr<uint8_t>();
+
+  VocabParams p{};
+  p.H = static_cast<int>(H);
+  p.tickets = tickets(tiles_t * tiles_h * 8);
+  p.g = reinterpret_cast<float*>(base + o_g);
+  p.dx = (bf16*)dx.data_ptr();
+  p.planes = reinterpret_cast<float*>(base + o_planes);
+  bf16 *u = reinterpret_cast<bf16*>(base + o_u), *gx = reinterpret_cast<bf16*>(base + o_gx);
+  const CUtensorMap tgx = make_map_any(gx, false, H, u_rows, H, gemm::BK);
+  if (few) {
+    FewParams f = few_params(x, w, tg, ignore_index, temperature);
+    f.dlogp = up.data_ptr<float>();
+    f.lse = ls.data_ptr<float>();
+    f.u = u;
+    f.ldu = ldu;
+    f.g = reinterpret_cast<float*>(base + o_g);
+    f.gx = gx;
+    launch_few<true>(f);
+    p.rows = static_cast<int>(T);
+    p.splits = pick_splits(tiles_h, k_v, tiles_v * tiles_h, 1, clusters);
+    p.N = static_cast<int>(V);
+    p.first = p.last = 1;
+    launch_vocab<vocab::kGrads>(make_map_any(u, false, V, T, ldu, vocab::HALF),
+                                make_map_any(w.data_ptr(), false, H, V, row_ld(w), gemm::BK),
+                                make_map_any(u, false, V, T, ldu, gemm::BK), tgx,
+                                make_map_any(dw.data_ptr(), false, H, V, H, 32), p, most_units + tiles_v * tiles_h);
+    return;
+  }
 
   PackParams k{};
   k.x = (const bf16*)x.data_ptr();
@@ -445,24 +739,16 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   k.g = reinterpret_cast<float*>(base + o_g);
   k.lse_packed = reinterpret_cast<float*>(base + o_lse);
   k.xp = reinterpret_cast<bf16*>(base + o_x);
-  k.gxp = reinterpret_cast<bf16*>(base + o_gx);
-  k.dx = (bf16*)dx.data_ptr();
+  k.gxp = gx;
+  k.dx = p.dx;
   launch_pack(k);
 
-  VocabParams p{};
   p.meta = k.meta;
-  p.H = static_cast<int>(H);
   p.scale = k.scale;
   p.index = k.index;
   p.targets = k.target;
-  p.tickets = tickets(tiles_t * tiles_h * 8);
   p.lse = k.lse_packed;
-  p.g = k.g;
-  p.dx = k.dx;
-  p.planes = reinterpret_cast<float*>(base + o_planes);
-  bf16* u = reinterpret_cast<bf16*>(base + o_u);
-  CUtensorMap tx = make_map_any(k.xp, false, H, T, H, vocab::HALF);
-  CUtensorMap tgx = make_map_any(k.gxp, false, H, u_rows, H, gemm::BK);
+  const CUtensorMap tx = make_map_any(k.xp, false, H, T, H, vocab::HALF);
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int64_t n = std::min(width, V - v0);
     const bf16* wp = (const bf16*)w.data_ptr() + v0 * row_ld(w);
