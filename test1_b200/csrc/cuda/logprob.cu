@@ -11,6 +11,10 @@
 // gives logp = lse = 0 and no gradient, whatever its hidden state holds.
 #include "vocab_gemm.cuh"
 
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+
+#include <unordered_map>
+
 namespace t1 {
 
 CUtensorMap make_map_any(const void* ptr, bool f32, int64_t inner, int64_t outer, int64_t ld, int box_outer);
@@ -461,16 +465,16 @@ static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
 
 // Arrival counters, zero between launches (whoever arrives last clears its
 // counter); one set per (device, stream), so that concurrent calls never
-// share one.
-static int* tickets(int64_t n) {
+// share one.  A captured graph has a set of its own, for the same reason.
+torch::Tensor arrival_counters(int64_t n) {
   static std::unordered_map<uint64_t, torch::Tensor> all;
   int dev = 0;
   cudaGetDevice(&dev);
-  const uint64_t key = (static_cast<uint64_t>(dev) << 56) ^ reinterpret_cast<uint64_t>(stream());
-  torch::Tensor& t = all[key];
-  if (!t.defined() || t.numel() < n)
-    t = torch::zeros({std::max<int64_t>(4096, n)}, torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, dev));
-  return t.data_ptr<int>();
+  const auto opts = torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, dev);
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return torch::zeros({n}, opts);
+  torch::Tensor& t = all[(static_cast<uint64_t>(dev) << 56) ^ reinterpret_cast<uint64_t>(stream())];
+  if (!t.defined() || t.numel() < n) t = torch::zeros({std::max<int64_t>(4096, n)}, opts);
+  return t;
 }
 
 // A workspace cut into 256-byte aligned pieces.
@@ -577,7 +581,8 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
     auto ws = torch::empty({32 * few_grid(V) + 16}, f32);
     p.part = reinterpret_cast<float2*>(ws.data_ptr<float>());
     p.target_logit = ws.data_ptr<float>() + 32 * few_grid(V);
-    p.ticket = tickets(1);
+    const torch::Tensor counters = arrival_counters(1);
+    p.ticket = counters.data_ptr<int>();
     p.logp = logp.data_ptr<float>();
     p.lse_out = lse.data_ptr<float>();
     launch_few<false>(p);
@@ -606,7 +611,11 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   p.logp = logp.data_ptr<float>();
   p.lse_out = lse.data_ptr<float>();
   p.join = blocks <= kJoinBlocks;
-  if (p.join) p.tickets = tickets(tiles_t * 8);
+  torch::Tensor counters;
+  if (p.join) {
+    counters = arrival_counters(tiles_t * 8);
+    p.tickets = counters.data_ptr<int>();
+  }
   if (pack) {
     PackParams k{};
     k.x = (const bf16*)x.data_ptr();
@@ -692,7 +701,8 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
 
   VocabParams p{};
   p.H = static_cast<int>(H);
-  p.tickets = tickets(tiles_t * tiles_h * 8);
+  const torch::Tensor counters = arrival_counters(tiles_t * tiles_h * 8);
+  p.tickets = counters.data_ptr<int>();
   p.g = reinterpret_cast<float*>(base + o_g);
   p.dx = (bf16*)dx.data_ptr();
   p.planes = reinterpret_cast<float*>(base + o_planes);
