@@ -13,13 +13,13 @@
 //      several units have a mean of their own)
 //   C  per token: the gradient, and the policy loss's own sums
 //   D  the policy loss's totals
-// Up to kClusterTokens a single launch runs them all, a cluster of 1 to 8
-// blocks whose barrier stands between the phases: such a call is launches and
-// latency, and every launch saved is 4 us of the host's time.  A larger batch
-// is bound by its bytes and takes a launch per phase over all SMs (D: the
-// last block of C).  A unit belongs to a warp or, for sequences shorter than
-// 32 tokens, to the fewest lanes that hold one.  Sums are carried in fp64 and
-// joined in a fixed order: two runs give the same bits.
+// One launch runs them all, with a barrier of the whole grid between the
+// phases: a launch costs 4 us of the host's time, a barrier about 1.5 us of the
+// GPU's.  All blocks are on the GPU together (a cooperative launch of at most
+// two blocks per SM); a batch that one block handles as fast has no barrier at
+// all.  A unit belongs to a warp or, for sequences shorter than 32 tokens, to
+// the fewest lanes that hold one.  Sums are carried in fp64 and joined in a
+// fixed order: two runs give the same bits.
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -31,9 +31,9 @@
 namespace t1 {
 
 torch::Tensor arrival_counters(int64_t n);
+torch::Tensor& gemm_error_word();
 
 enum PreferenceKind : int { kSigmoid = 0, kHinge = 1, kIpo = 2 };
-enum Phase : int { kA = 1, kB = 2, kC = 4, kD = 8 };
 
 struct LossParams {
   const float *logp, *ref, *old, *adv;
@@ -43,8 +43,11 @@ struct LossParams {
   int S;
   int unit, chunks;        // tokens of a unit, units of a sequence
   int lanes;               // lanes of a unit: 32, or the power of two >= S
-  int phases;              // of this launch
-  int parts;               // entries of `totals` when C starts
+  int vectors;             // 16-byte vectors of tokens
+  int lengths_phase;       // policy: phase B takes place
+  int* arrivals;           // the barrier's counter, zero between launches
+  int* err;
+  uint8_t* answer;         // [T] phase A's finding, an eighth of the targets to read again
   double2* units;          // [B * chunks] (sum of log ratios, answer tokens)
   double2* totals;         // [block] preference: (loss, pairs); policy: (answer tokens, sequences that have one)
   float *loss, *dlogp;
@@ -58,25 +61,38 @@ struct LossParams {
   float lo, hi, edge_lo, edge_hi, kl_coef;
   int* lengths;            // [B] answer tokens, with phase B
   double* sums;            // [block of C][3] loss, KL, clipped
-  int* ticket;             // arrivals of C's blocks, zero between launches
   float* stats;            // [2]
 };
 
 constexpr int kLossThreads = 512;
 constexpr int kLossWarps = kLossThreads / 32;
+constexpr int kLossPerSm = 2;  // blocks of an SM
 constexpr int kAhead = 4;  // tokens of a lane whose loads are issued together
 
-// Block-wide sum in fp64, every thread gets it.
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {
+// Sum over a warp's lanes, every lane gets it.
+__device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double t = 0;
+  return v;
+}
+
+struct Sums {
+  double v[3];
+};
+
+// Block-wide sums in fp64; the first warp gets them.
+template <int N>
+__device__ __forceinline__ Sums block_sums(Sums s, Sums* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int w = 0; w < kLossWarps; ++w) t += red[w];
-  return t;
+  for (int k = 0; k < N; ++k) s.v[k] = warp_sum_f64(s.v[k]);
+  __syncthreads();
+  if (lane == 0) red[warp] = s;
+  __syncthreads();
+  if (warp != 0) return s;
+#pragma unroll
+  for (int k = 0; k < N; ++k) s.v[k] = warp_sum_f64(lane < kLossWarps ? red[lane].v[k] : 0.0);
+  return s;
 }
 
 // Sum over the `by` neighbouring lanes that share v's subject.
@@ -96,24 +112,28 @@ __device__ __forceinline__ double2 join_units(const LossParams& p, int64_t b, in
   return make_double2(group_sum(t.x, by), group_sum(t.y, by));
 }
 
-__device__ __forceinline__ double2 join_totals(const LossParams& p, double* red) {
-  double2 t = make_double2(0, 0);
-  for (int i = threadIdx.x; i < p.parts; i += kLossThreads) {
+// The blocks' totals added up, for every thread.
+__device__ __forceinline__ double2 join_totals(const LossParams& p, Sums* red) {
+  Sums s{{0, 0, 0}};
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kLossThreads) {
     const double2 v = __ldcg(&p.totals[i]);
-    t.x += v.x;
-    t.y += v.y;
+    s.v[0] += v.x;
+    s.v[1] += v.y;
   }
-  return make_double2(block_sum_f64(t.x, red), block_sum_f64(t.y, red));
+  s = block_sums<2>(s, red);
+  __syncthreads();
+  if (threadIdx.x == 0) red[0] = s;
+  __syncthreads();
+  return make_double2(red[0].v[0], red[0].v[1]);
 }
 
-__device__ __forceinline__ void write_totals(const LossParams& p, double x, double y, double* red) {
-  x = block_sum_f64(x, red);
-  y = block_sum_f64(y, red);
-  if (threadIdx.x == 0) __stcg(&p.totals[blockIdx.x], make_double2(x, y));
+__device__ __forceinline__ void write_totals(const LossParams& p, double x, double y, Sums* red) {
+  const Sums s = block_sums<2>(Sums{{x, y, 0}}, red);
+  if (threadIdx.x == 0) __stcg(&p.totals[blockIdx.x], make_double2(s.v[0], s.v[1]));
 }
 
-// The warps' walk over units: body(unit, sequence, first token, past the last
-// token, lane of the unit), with all lanes of a warp in step; unit is -1 for
+// The warps' walk over units: body(unit, sequence, first token, tokens, lane
+// of the unit), with all lanes of a warp in step; unit is -1 and tokens 0 for
 // lanes that have none in a warp's last round.
 template <class F>
 __device__ __forceinline__ void for_units(const LossParams& p, F body) {
@@ -121,38 +141,115 @@ __device__ __forceinline__ void for_units(const LossParams& p, F body) {
   const int64_t count = p.B * p.chunks, step = static_cast<int64_t>(gridDim.x) * kLossWarps * per_warp;
   for (int64_t u0 = (static_cast<int64_t>(blockIdx.x) * kLossWarps + (threadIdx.x >> 5)) * per_warp; u0 < count; u0 += step) {
     const int64_t u = u0 + in_warp / p.lanes;
-    const int64_t b = u < count ? u / p.chunks : 0;
-    const int s0 = u < count ? static_cast<int>(u - b * p.chunks) * p.unit : 0;
-    body(u < count ? u : -1, b, b * p.S + s0, u < count ? b * p.S + min(p.S, s0 + p.unit) : s0, in_warp & (p.lanes - 1));
+    if (u < count) {
+      const int64_t b = u / p.chunks;
+      const int s0 = static_cast<int>(u - b * p.chunks) * p.unit;
+      body(u, b, b * p.S + s0, min(p.unit, p.S - s0), in_warp & (p.lanes - 1));
+    } else {
+      body(-1, 0, 0, 0, in_warp & (p.lanes - 1));
+    }
+  }
+}
+
+// Four tokens of a lane, loaded and stored together.  STEP 1: neighbours in
+// 16-byte vectors (sequences and units of a multiple of 4 tokens, aligned
+// tensors); 32 and 0: a token per lane and round, the other lanes' between
+// them (0: `lanes` of them), past the unit's end skipped unless `full`.
+template <int STEP>
+struct Four {
+  int first, step, len;
+  bool full;
+  __device__ bool in(int k) const { return STEP == 1 || full || first + k * step < len; }
+  __device__ int at(int k) const { return first + k * (STEP > 0 ? STEP : step); }
+  __device__ void load(const float* p, float (&v)[kAhead], float other) const {
+    if (STEP == 1) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(p + first));
+      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) v[k] = in(k) ? __ldg(p + at(k)) : other;
+    }
+  }
+  __device__ void load(const int64_t* p, int64_t (&v)[kAhead], int64_t other) const {
+    if (STEP == 1) {
+      const longlong2 f = __ldg(reinterpret_cast<const longlong2*>(p + first));
+      const longlong2 g = __ldg(reinterpret_cast<const longlong2*>(p + first + 2));
+      v[0] = f.x; v[1] = f.y; v[2] = g.x; v[3] = g.y;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) v[k] = in(k) ? __ldg(p + at(k)) : other;
+    }
+  }
+  __device__ void load(const uint8_t* p, bool (&v)[kAhead]) const {
+    if (STEP == 1) {
+      const uchar4 f = *reinterpret_cast<const uchar4*>(p + first);
+      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) v[k] = in(k) ? p[at(k)] : 0;
+    }
+  }
+  __device__ void store(uint8_t* p, const bool (&v)[kAhead]) const {
+    if (STEP == 1) {
+      *reinterpret_cast<uchar4*>(p + first) = make_uchar4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (in(k)) p[at(k)] = v[k];
+    }
+  }
+  __device__ void store(float* p, const float (&v)[kAhead]) const {
+    if (STEP == 1) {
+      *reinterpret_cast<float4*>(p + first) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (in(k)) p[at(k)] = v[k];
+    }
+  }
+};
+static_assert(kAhead == 4, "Four");
+
+// Calls body with each four of the lane's tokens of a unit.
+template <class F>
+__device__ __forceinline__ void for_fours(const LossParams& p, int len, int lane, F body) {
+  if (p.vectors) {
+    for (int s = 4 * lane; s < len; s += 4 * 32) body(Four<1>{s, 1, len, true});
+  } else if (p.lanes == 32) {
+    int s = lane;
+    for (; s - lane + 32 * kAhead <= len; s += 32 * kAhead) body(Four<32>{s, 32, len, true});
+    if (s < len) body(Four<32>{s, 32, len, false});
+  } else {
+    for (int s = lane; s < len; s += kAhead * p.lanes) body(Four<0>{s, p.lanes, len, false});
   }
 }
 
 // ------------------------------------------------------------------ phase A
 template <bool POLICY>
-__device__ __forceinline__ void count_phase(const LossParams& p, double* red) {
+__device__ __forceinline__ void count_phase(const LossParams& p, Sums* red) {
   double tokens = 0, live = 0;
-  for_units(p, [&](int64_t u, int64_t, int64_t i0, int64_t i1, int lane) {
+  for_units(p, [&](int64_t u, int64_t, int64_t i0, int len, int lane) {
     double sum = 0;
     int n = 0;
-    if (u < 0) i1 = i0;
-    for (int64_t i = i0 + lane; i < i1; i += kAhead * p.lanes) {
+    const int64_t* targets = p.targets + i0;
+    const float *logp = p.logp + i0, *ref = p.ref + i0;
+    uint8_t* answer = p.answer + i0;
+    for_fours(p, len, lane, [&](const auto& four) {
+      int64_t t[kAhead];
+      float v[kAhead] = {}, r[kAhead] = {}, part = 0.f;
       bool ok[kAhead];
-      float v[kAhead], r[kAhead];
+      four.load(targets, t, p.ignore);
+      if (!POLICY) four.load(logp, v, 0.f);
+      if (!POLICY && p.ref != nullptr) four.load(ref, r, 0.f);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        const int64_t at = i + k * p.lanes;
-        ok[k] = at < i1 && p.targets[at] != p.ignore;
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int64_t at = i + k * p.lanes;
+        ok[k] = t[k] != p.ignore;
         n += ok[k];
-        v[k] = !POLICY && ok[k] ? p.logp[at] : 0.f;
-        r[k] = !POLICY && ok[k] && p.ref != nullptr ? p.ref[at] : 0.f;
+        if (!POLICY) part += ok[k] ? v[k] - r[k] : 0.f;
       }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) sum += v[k] - r[k];
-    }
+      four.store(answer, ok);
+      sum += part;
+    });
     const double cnt = group_sum(n, p.lanes);
     if (!POLICY) sum = group_sum(sum, p.lanes);
     if (u >= 0 && lane == 0) {
@@ -165,7 +262,7 @@ __device__ __forceinline__ void count_phase(const LossParams& p, double* red) {
 }
 
 // ------------------------------------------------------------------ phase B
-__device__ __forceinline__ void pairs_phase(const LossParams& p, double* red) {
+__device__ __forceinline__ void pairs_phase(const LossParams& p, Sums* red) {
   const int64_t P = p.B / 2;
   // a thread for a pair of few units, a warp for one of many
   const int by = p.chunks <= 4 ? 1 : 32, lane = threadIdx.x & (by - 1);
@@ -203,7 +300,7 @@ __device__ __forceinline__ void pairs_phase(const LossParams& p, double* red) {
   write_totals(p, loss, live, red);
 }
 
-__device__ __forceinline__ void lengths_phase(const LossParams& p, double* red) {
+__device__ __forceinline__ void lengths_phase(const LossParams& p, Sums* red) {
   const int lane = threadIdx.x & 31;
   double tokens = 0, live = 0;
   for (int64_t b = static_cast<int64_t>(blockIdx.x) * kLossWarps + (threadIdx.x >> 5); b < p.B; b += static_cast<int64_t>(gridDim.x) * kLossWarps) {
@@ -217,145 +314,169 @@ __device__ __forceinline__ void lengths_phase(const LossParams& p, double* red) 
 }
 
 // ------------------------------------------------------------------ phase C
-__device__ __forceinline__ void preference_grad_phase(const LossParams& p, double* red) {
+__device__ __forceinline__ void preference_grad_phase(const LossParams& p, Sums* red) {
   const double2 total = join_totals(p, red);
   const double pairs = fmax(1.0, total.y);
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.loss = static_cast<float>(total.x / pairs);
-  for_units(p, [&](int64_t u, int64_t b, int64_t i0, int64_t i1, int lane) {
+  for_units(p, [&](int64_t u, int64_t b, int64_t i0, int len, int lane) {
     if (u < 0) return;
     const float d = static_cast<float>(__ldcg(&p.coef[b]) / pairs);
-    for (int64_t i = i0 + lane; i < i1; i += kAhead * p.lanes) {
+    const uint8_t* answer = p.answer + i0;
+    float* dlogp = p.dlogp + i0;
+    for_fours(p, len, lane, [&](const auto& four) {
       bool ok[kAhead];
+      float g[kAhead];
+      four.load(answer, ok);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int64_t at = i + k * p.lanes;
-        ok[k] = at < i1 && p.targets[at] != p.ignore;
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (i + k * p.lanes < i1) p.dlogp[i + k * p.lanes] = ok[k] ? d : 0.f;
-    }
+      for (int k = 0; k < kAhead; ++k) g[k] = ok[k] ? d : 0.f;
+      four.store(dlogp, g);
+    });
   });
 }
 
-__device__ __forceinline__ void policy_grad_phase(const LossParams& p, double* red) {
+// exp(e) - 1 - e: its series up to e^7 for small e, where the difference would
+// keep no digit (the first term left out is below 2^-25 of the sum).
+__device__ __forceinline__ float kl_term(float e) {
+  float s = fmaf(e, 1.f / 5040, 1.f / 720);
+  s = fmaf(e, s, 1.f / 120);
+  s = fmaf(e, s, 1.f / 24);
+  s = fmaf(e, s, 1.f / 6);
+  s = fmaf(e, s, 0.5f);
+  return fabsf(e) < 0.25f ? s * e * e : (__expf(e) - 1.f) - e;
+}
+
+__device__ __forceinline__ void policy_grad_phase(const LossParams& p, Sums* red) {
   const double2 total = join_totals(p, red);
   const double tokens = fmax(1.0, total.x), live = fmax(1.0, total.y);
+  const float token_weight = static_cast<float>(1 / tokens);
   double loss = 0, kls = 0;
   int cut = 0;
-  for_units(p, [&](int64_t u, int64_t b, int64_t i0, int64_t i1, int lane) {
+  for_units(p, [&](int64_t u, int64_t b, int64_t i0, int len, int lane) {
     if (u < 0) return;
-    float w = static_cast<float>(1 / tokens);
+    float w = token_weight;
     if (p.per_sequence) {
       const double n = p.chunks == 1 ? __ldcg(&p.units[u]).y : static_cast<double>(__ldcg(&p.lengths[b]));
       w = static_cast<float>(1 / (fmax(1.0, n) * live));
     }
     const float seq_adv = p.adv_per_token ? 0.f : p.adv[b];
     double unit_loss = 0;
-    for (int64_t i = i0 + lane; i < i1; i += kAhead * p.lanes) {
+    const float *logp = p.logp + i0, *old = p.old + i0, *ref = p.ref + i0, *adv = p.adv + i0;
+    const uint8_t* answer = p.answer + i0;
+    float* dlogp = p.dlogp + i0;
+    for_fours(p, len, lane, [&](const auto& four) {
       bool ok[kAhead];
-      float lp[kAhead], od[kAhead], rf[kAhead], a[kAhead];
+      float lp[kAhead], od[kAhead], rf[kAhead], a[kAhead] = {seq_adv, seq_adv, seq_adv, seq_adv}, part = 0.f, kl_part = 0.f;
+      four.load(answer, ok);
+      four.load(logp, lp, 0.f);
+      four.load(old, od, 0.f);
+      if (p.ref != nullptr) four.load(ref, rf, 0.f);
+      if (p.adv_per_token) four.load(adv, a, 0.f);
+      float g[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        const int64_t at = i + k * p.lanes;
-        ok[k] = at < i1 && p.targets[at] != p.ignore;
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int64_t at = i + k * p.lanes;
-        lp[k] = ok[k] ? p.logp[at] : 0.f;
-        od[k] = ok[k] ? p.old[at] : 0.f;
-        rf[k] = ok[k] && p.ref != nullptr ? p.ref[at] : 0.f;
-        a[k] = ok[k] && p.adv_per_token ? p.adv[at] : seq_adv;
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (i + k * p.lanes >= i1) continue;
-        float g = 0.f;
-        if (ok[k]) {
-          // clipped where the log ratio is past log(1 +- clip): the same
-          // token whatever exp's rounding does at the edge
-          const float d = lp[k] - od[k], rho = expf(d);
-          const bool over = d > p.hi, under = d < p.lo;
-          const bool clipped = (a[k] > 0.f && over) || (a[k] < 0.f && under);
-          float l = -a[k] * (clipped ? (over ? p.edge_hi : p.edge_lo) : rho);
-          g = clipped ? 0.f : -a[k] * rho;
-          if (p.ref != nullptr) {
-            const float e = rf[k] - lp[k], x = expm1f(e), kl = x - e;
-            l += p.kl_coef * kl;
-            g -= p.kl_coef * x;
-            kls += kl;
-          }
-          g *= w;
-          unit_loss += l;
-          cut += clipped;
+        // clipped where the log ratio is past log(1 +- clip): the same token
+        // whatever exp's rounding does at the edge
+        const float d = lp[k] - od[k], rho = __expf(d);
+        const bool over = d > p.hi, under = d < p.lo;
+        const bool clipped = (a[k] > 0.f && over) || (a[k] < 0.f && under);
+        float l = -a[k] * (clipped ? (over ? p.edge_hi : p.edge_lo) : rho);
+        g[k] = clipped ? 0.f : -a[k] * rho;
+        if (p.ref != nullptr) {
+          const float e = rf[k] - lp[k], kl = kl_term(e);
+          l += p.kl_coef * kl;
+          g[k] -= p.kl_coef * (kl + e);  // exp(e) - 1
+          kl_part += ok[k] ? kl : 0.f;
         }
-        p.dlogp[i + k * p.lanes] = g;
+        part += ok[k] ? l : 0.f;
+        cut += ok[k] && clipped;
+        g[k] = ok[k] ? g[k] * w : 0.f;
       }
-    }
+      four.store(dlogp, g);
+      unit_loss += part;
+      kls += kl_part;
+    });
     loss += unit_loss * w;
   });
-  loss = block_sum_f64(loss, red);
-  kls = block_sum_f64(kls, red);
-  const double cuts = block_sum_f64(cut, red);
-  if (threadIdx.x < 3) __stcg(&p.sums[3 * blockIdx.x + threadIdx.x], threadIdx.x == 0 ? loss : threadIdx.x == 1 ? kls : cuts);
+  const Sums s = block_sums<3>(Sums{{loss, kls, static_cast<double>(cut)}}, red);
+  if (threadIdx.x == 0)
+    for (int k = 0; k < 3; ++k) __stcg(&p.sums[3 * blockIdx.x + k], s.v[k]);
 }
 
 // ------------------------------------------------------------------ phase D
-__device__ __forceinline__ void policy_total_phase(const LossParams& p, double* red) {
+__device__ __forceinline__ void policy_total_phase(const LossParams& p, Sums* red) {
   const double tokens = fmax(1.0, join_totals(p, red).x);
-  double v[3] = {0, 0, 0};
-  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kLossThreads)
+  if (threadIdx.x >= 32) return;
+  Sums s{{0, 0, 0}};
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += 32)
 #pragma unroll
-    for (int k = 0; k < 3; ++k) v[k] += __ldcg(&p.sums[3 * i + k]);
+    for (int k = 0; k < 3; ++k) s.v[k] += __ldcg(&p.sums[3 * i + k]);
 #pragma unroll
-  for (int k = 0; k < 3; ++k) v[k] = block_sum_f64(v[k], red);
+  for (int k = 0; k < 3; ++k) s.v[k] = warp_sum_f64(s.v[k]);
   if (threadIdx.x == 0) {
-    *p.loss = static_cast<float>(v[0]);
-    p.stats[0] = static_cast<float>(v[1] / tokens);
-    p.stats[1] = static_cast<float>(v[2] / tokens);
+    *p.loss = static_cast<float>(s.v[0]);
+    p.stats[0] = static_cast<float>(s.v[1] / tokens);
+    p.stats[1] = static_cast<float>(s.v[2] / tokens);
   }
 }
 
+// Waits until every block of the grid has arrived for the `nth` time.  False
+// (and an error code) if that takes longer than any launch can.
+__device__ __forceinline__ bool grid_barrier(const LossParams& p, int nth) {
+  __shared__ int ok;
+  __syncthreads();
+  if (gridDim.x == 1) return true;
+  if (threadIdx.x == 0) {
+    const int all = nth * static_cast<int>(gridDim.x);
+    __threadfence();
+    atomicAdd(p.arrivals, 1);
+    ok = 1;
+    const uint64_t t0 = sm100::globaltimer_ns();
+    int v, n = 0;
+    while (true) {
+      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.arrivals) : "memory");
+      if (v >= all) break;
+      if ((++n & 255) == 0 && sm100::globaltimer_ns() - t0 > sm100::kWaitLimitNs) {
+        sm100::ErrorSlot{p.err}.set(131);
+        ok = 0;
+        break;
+      }
+    }
+    __threadfence();
+  }
+  __syncthreads();
+  return ok;
+}
+
 template <bool POLICY>
-__global__ void __launch_bounds__(kLossThreads, 2) answer_loss_kernel(const LossParams p) {
-  __shared__ double red[kLossWarps];
+__global__ void __launch_bounds__(kLossThreads, kLossPerSm) answer_loss_kernel(const LossParams p) {
+  __shared__ Sums red[kLossWarps];
   __shared__ int last;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (p.phases & kA) count_phase<POLICY>(p, red);
-  if (p.phases & kB) {
-    if (p.phases & kA) sm100::cluster_sync();
+  int barriers = 0;
+  count_phase<POLICY>(p, red);
+  if (!grid_barrier(p, ++barriers)) return;
+  if (!POLICY || p.lengths_phase) {
     if (POLICY) lengths_phase(p, red);
     else pairs_phase(p, red);
+    if (!grid_barrier(p, ++barriers)) return;
   }
-  if (p.phases & kC) {
-    if (p.phases & kA) sm100::cluster_sync();
-    if (POLICY) policy_grad_phase(p, red);
-    else preference_grad_phase(p, red);
-  }
-  if (!POLICY || !(p.phases & kD)) return;
-  if (p.phases & kA) {
-    sm100::cluster_sync();
-    if (blockIdx.x == 0) policy_total_phase(p, red);
-    return;
-  }
+  if (POLICY) policy_grad_phase(p, red);
+  else preference_grad_phase(p, red);
+  // the last block clears the counter, and adds up the policy loss's sums
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+  if (threadIdx.x == 0)
+    last = gridDim.x == 1 || atomicAdd(p.arrivals, 1) == (barriers + 1) * static_cast<int>(gridDim.x) - 1;
   __syncthreads();
   if (!last) return;
   __threadfence();
-  if (threadIdx.x == 0) *p.ticket = 0;
-  policy_total_phase(p, red);
+  if (threadIdx.x == 0 && gridDim.x > 1) *p.arrivals = 0;
+  if (POLICY) policy_total_phase(p, red);
 }
 
 // ================================================================ host side
 T1_BOUNDS_READER(answer_loss)
-
-// Tokens up to which one cluster does it all.  Eight SMs read about 1.5 TB/s:
-// at 256 K tokens (6 MB) that costs what the launches saved were worth.
-constexpr int64_t kClusterTokens = 256 * 1024;
 
 static void check_tokens(const torch::Tensor& t, int64_t T, const torch::Tensor& like, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), what, " must be on the device of logp");
@@ -374,30 +495,27 @@ static int64_t check_batch(const torch::Tensor& logp, const torch::Tensor& targe
   return logp.size(0) / S;
 }
 
-// The units of a batch, and how the phases' launches look.
+// Tokens up to which a single block works: what it loses against a full GPU
+// (16 tokens of a lane, about 4 us) is what the barriers and the cooperative
+// launch would cost.
+constexpr int64_t kBlockTokens = 8192;
+
+// The units of a batch and the blocks that share them.
 struct LossPlan {
-  int cluster;         // blocks of the single launch, 0: a launch per phase
-  int blocks, seq_blocks;  // of the launches over units, over sequences
-  int unit, chunks, lanes;
+  int blocks, unit, chunks, lanes;
 
   LossPlan(int64_t B, int64_t S) {
-    const int64_t T = B * S;
-    cluster = 0;
-    int64_t warps = 8 * num_sms() * kLossWarps;
-    if (T <= kClusterTokens) {
-      cluster = 1;
-      while (cluster < 8 && cluster * 4096 < T) cluster *= 2;
-      warps = cluster * kLossWarps;
-    }
+    const int64_t T = B * S, warps = T <= kBlockTokens ? kLossWarps : kLossPerSm * num_sms() * kLossWarps;
     lanes = 32;
     while (lanes > 1 && lanes / 2 >= S) lanes /= 2;
-    const int64_t even = (T + warps - 1) / warps;
-    unit = static_cast<int>(std::min<int64_t>(std::max<int64_t>((even + 127) / 128 * 128, 128), 2048));
-    if (unit > S) unit = static_cast<int>(S);
+    // as many units as there are warps, of equal lengths, but no shorter than
+    // one round of a lane's loads
+    chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(warps / B, (S + 32 * kAhead - 1) / (32 * kAhead))));
+    unit = static_cast<int>((S + chunks - 1) / chunks);
+    if (S % 4 == 0) unit = (unit + 3) / 4 * 4;
     chunks = static_cast<int>((S + unit - 1) / unit);
-    const int64_t per_block = kLossWarps * (32 / lanes), units = B * chunks;
-    blocks = cluster ? cluster : static_cast<int>(std::min<int64_t>((units + per_block - 1) / per_block, 4 * num_sms()));
-    seq_blocks = cluster ? cluster : static_cast<int>(std::min<int64_t>((B + kLossWarps - 1) / kLossWarps, num_sms()));
+    const int64_t per_block = kLossWarps * (32 / lanes);
+    blocks = T <= kBlockTokens ? 1 : static_cast<int>(std::min<int64_t>((B * chunks + per_block - 1) / per_block, kLossPerSm * num_sms()));
   }
 };
 
@@ -415,55 +533,49 @@ static torch::Tensor loss_workspace(int64_t bytes) {
   return t;
 }
 
-// Lays the phases' workspace out and launches `first` | ... | last.
+// Lays the phases' workspace out and launches.
 template <bool POLICY>
 static void launch_loss(LossParams& p, const LossPlan& plan) {
-  const int64_t units = p.B * plan.chunks, blocks = std::max(plan.blocks, plan.seq_blocks);
+  const int64_t units = p.B * plan.chunks;
   auto pad = [](int64_t n) { return (n + 255) / 256 * 256; };
-  const torch::Tensor held = loss_workspace(pad(16 * units) + pad(16 * blocks) + pad(24 * blocks) + pad(4 * p.B));
+  const torch::Tensor held =
+      loss_workspace(pad(16 * units) + pad(16 * plan.blocks) + pad(24 * plan.blocks) + pad(4 * p.B) + p.B * p.S);
   uint8_t* ws = held.data_ptr<uint8_t>();
   p.units = reinterpret_cast<double2*>(ws);
   p.totals = reinterpret_cast<double2*>(ws + pad(16 * units));
-  p.sums = reinterpret_cast<double*>(ws + pad(16 * units) + pad(16 * blocks));
-  uint8_t* per_seq = ws + pad(16 * units) + pad(16 * blocks) + pad(24 * blocks);
+  p.sums = reinterpret_cast<double*>(ws + pad(16 * units) + pad(16 * plan.blocks));
+  uint8_t* per_seq = ws + pad(16 * units) + pad(16 * plan.blocks) + pad(24 * plan.blocks);
   p.coef = reinterpret_cast<float*>(per_seq);
   p.lengths = reinterpret_cast<int*>(per_seq);
+  p.answer = per_seq + pad(4 * p.B);
   p.unit = plan.unit;
   p.chunks = plan.chunks;
   p.lanes = plan.lanes;
-  const bool b_phase = !POLICY || (p.per_sequence && plan.chunks > 1);
-  auto launch = [&](int phases, int blocks_, int cluster) {
-    p.phases = phases;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(blocks_);
-    cfg.blockDim = dim3(kLossThreads);
-    cfg.stream = stream();
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, answer_loss_kernel<POLICY>, static_cast<LossParams>(p));
-    TORCH_CHECK(e == cudaSuccess, "answer_loss launch failed: ", cudaGetErrorString(e));
-    count_launch();
-  };
-  if (plan.cluster) {
-    p.parts = plan.cluster;
-    launch(kA | (b_phase ? kB : 0) | kC | (POLICY ? kD : 0), plan.cluster, plan.cluster);
-    return;
+  auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  p.vectors = p.S % 4 == 0 && plan.lanes == 32 && aligned(p.targets) && aligned(p.logp) && aligned(p.old) &&
+              aligned(p.ref) && (!p.adv_per_token || aligned(p.adv));
+  p.lengths_phase = POLICY && p.per_sequence && plan.chunks > 1;
+  p.err = gemm_error_word().data_ptr<int>();
+  torch::Tensor arrivals;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(plan.blocks);
+  cfg.blockDim = dim3(kLossThreads);
+  cfg.stream = stream();
+  cudaLaunchAttribute attr;
+  if (plan.blocks > 1) {  // blocks that wait for one another
+    arrivals = arrival_counters(1);
+    p.arrivals = arrivals.data_ptr<int>();
+    attr.id = cudaLaunchAttributeCooperative;
+    attr.val.cooperative = 1;
+  } else {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
   }
-  torch::Tensor tickets;
-  if (POLICY) {
-    tickets = arrival_counters(1);
-    p.ticket = tickets.data_ptr<int>();
-  }
-  p.parts = b_phase ? plan.seq_blocks : plan.blocks;
-  launch(kA, plan.blocks, 1);
-  if (b_phase) launch(kB, plan.seq_blocks, 1);
-  launch(kC | (POLICY ? kD : 0), plan.blocks, 1);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, answer_loss_kernel<POLICY>, static_cast<LossParams>(p));
+  TORCH_CHECK(e == cudaSuccess, "answer_loss launch failed: ", cudaGetErrorString(e));
+  count_launch();
 }
 
 // Returns (loss [], dlogp [T], rewards [B]).
