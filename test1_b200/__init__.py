@@ -2,12 +2,14 @@
 
 Public API (same names as the SlideFSDP reference):
     SlideFSDPConfig, SlideFSDP, LayerAdam, SlidingCheckpoint
+and for training on preferences or sampled answers:
+    PreferenceObjective, PolicyObjective
 """
 from .config import SlideFSDPConfig
 from .optim.layer_adam import LayerAdam
 
 __all__ = ["SlideFSDPConfig", "SlideFSDP", "LayerAdam", "SlidingCheckpoint", "LlamaConfig",
-           "LlamaForCausalLM"]
+           "LlamaForCausalLM", "PreferenceObjective", "PolicyObjective"]
 __version__ = "0.1.0"
 
 
@@ -20,6 +22,10 @@ def __getattr__(name):
         from .sliding_checkpoint import SlidingCheckpoint
 
         return SlidingCheckpoint
+    if name in ("PreferenceObjective", "PolicyObjective"):
+        from . import objectives
+
+        return getattr(objectives, name)
     if name in ("LlamaConfig", "LlamaForCausalLM"):
         from .models import llama
 

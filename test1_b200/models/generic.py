@@ -102,6 +102,13 @@ class GenericEmbedding(nn.Module):
             torch.autograd.backward(out, dh)
 
 
+def _label_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: float) -> torch.Tensor:
+    """Log-probability of every target [T], 0 where it is -100."""
+    nll = torch.nn.functional.cross_entropy(logits.view(targets.numel(), -1) / temperature, targets,
+                                            ignore_index=-100, reduction="none")
+    return -nll
+
+
 class GenericOutputLayer(nn.Module):
     """Final norm + lm_head of any architecture; loss = mean token
     cross-entropy on shifted labels (ignore_index -100)."""
@@ -116,6 +123,11 @@ class GenericOutputLayer(nn.Module):
         _zero_grads(self)
         with torch.enable_grad():
             logits = self.lm_head(self.norm(x)).float()
+            if getattr(ctx, "objective", None) is not None:
+                logp = _label_logprobs(logits, ctx.targets, ctx.objective.temperature)
+                loss, dlogp = ctx.objective.loss_and_grad(logp.detach(), ctx.targets, ctx.seq_len)
+                logp.backward(dlogp)
+                return loss, x.grad
             loss = torch.nn.functional.cross_entropy(logits, ctx.targets, ignore_index=-100)
             loss.backward()
         return loss.detach(), x.grad
@@ -123,6 +135,10 @@ class GenericOutputLayer(nn.Module):
     def logits(self, h: torch.Tensor) -> torch.Tensor:
         with torch.no_grad():
             return self.lm_head(self.norm(h))
+
+    def logprobs(self, h: torch.Tensor, targets: torch.Tensor, temperature: float) -> torch.Tensor:
+        with torch.no_grad():
+            return _label_logprobs(self.logits(h).float(), targets, temperature)
 
 
 def causal_masks(config, batch: int, seq_len: int, hidden: int, position_ids, device, dtype) -> dict:

@@ -141,6 +141,7 @@ class StepContext:
     sin: torch.Tensor
     input_ids: Optional[torch.Tensor] = None  # [T] int64 on the device
     targets: Optional[torch.Tensor] = None    # [T] int64 (shifted labels)
+    objective: Optional[Any] = None           # objectives.ObjectiveStep; None: cross-entropy
 
     @property
     def tokens(self) -> int:

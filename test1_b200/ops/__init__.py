@@ -138,14 +138,7 @@ def preference_loss_fwd_bwd(logp, ref_logp, targets, seq_len, beta=0.1, kind="si
     _check_loss(logp, targets, seq_len)
     if (logp.shape[0] // seq_len) % 2:
         raise ValueError(f"a preference batch needs an even number of sequences, got {logp.shape[0] // seq_len}")
-    if kind not in PREFERENCE_KINDS:
-        raise ValueError(f"kind must be one of {PREFERENCE_KINDS}, got {kind!r}")
-    if not (0 < beta < float("inf")):
-        raise ValueError(f"beta must be positive, got {beta}")
-    if not 0.0 <= label_smoothing < 0.5:
-        raise ValueError(f"label_smoothing must lie in [0, 0.5), got {label_smoothing}")
-    if label_smoothing and kind != "sigmoid":
-        raise ValueError("label_smoothing goes with kind='sigmoid'")
+    check_preference(beta, kind, label_smoothing)
     return _impl(logp).preference_loss_fwd_bwd(logp, ref_logp, targets, seq_len, beta, kind, label_smoothing,
                                                average, ignore_index)
 
@@ -161,18 +154,33 @@ def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, 
     ref_logp may be None when kl_coef is 0.  Returns (loss [] fp32,
     dloss/dlogp [T], [mean KL term, share of clipped tokens])."""
     _check_loss(logp, targets, seq_len)
-    if not (0 <= clip_low < 1 and 0 <= clip_high < float("inf")):
-        raise ValueError(f"clip_low must lie in [0, 1) and clip_high in [0, inf), got {clip_low} and {clip_high}")
-    if reduction not in ("token", "sequence"):
-        raise ValueError(f"reduction must be 'token' or 'sequence', got {reduction!r}")
-    if not (0 <= kl_coef < float("inf")):
-        raise ValueError(f"kl_coef must not be negative, got {kl_coef}")
+    check_policy(clip_low, clip_high, kl_coef, reduction)
     if kl_coef and ref_logp is None:
         raise ValueError("a KL term (kl_coef > 0) needs ref_logp")
     if advantages.dim() != 1 or advantages.shape[0] not in (logp.shape[0], logp.shape[0] // seq_len):
         raise ValueError(f"advantages must be [T] or [T / seq_len], got {tuple(advantages.shape)}")
     return _impl(logp).policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, clip_low,
                                            clip_high, kl_coef, reduction, ignore_index)
+
+
+def check_preference(beta, kind, label_smoothing):
+    if kind not in PREFERENCE_KINDS:
+        raise ValueError(f"kind must be one of {PREFERENCE_KINDS}, got {kind!r}")
+    if not (0 < beta < float("inf")):
+        raise ValueError(f"beta must be positive, got {beta}")
+    if not 0.0 <= label_smoothing < 0.5:
+        raise ValueError(f"label_smoothing must lie in [0, 0.5), got {label_smoothing}")
+    if label_smoothing and kind != "sigmoid":
+        raise ValueError("label_smoothing goes with kind='sigmoid'")
+
+
+def check_policy(clip_low, clip_high, kl_coef, reduction):
+    if not (0 <= clip_low < 1 and 0 <= clip_high < float("inf")):
+        raise ValueError(f"clip_low must lie in [0, 1) and clip_high in [0, inf), got {clip_low} and {clip_high}")
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"reduction must be 'token' or 'sequence', got {reduction!r}")
+    if not (0 <= kl_coef < float("inf")):
+        raise ValueError(f"kl_coef must not be negative, got {kl_coef}")
 
 
 def _check_loss(logp, targets, seq_len):

@@ -54,6 +54,7 @@ from .models import generic
 from .models.llama import LlamaConfig, LlamaDecoderLayer, LlamaForCausalLM, make_context
 from .optim.layer_adam import LayerAdam
 from .parallel.comm import CpuReduceSlots, make_comm
+from .objectives import ObjectiveStep
 from .runtime.activations import ActivationStore
 from .runtime.device import Event, Stream
 from .runtime import host_memory
@@ -82,7 +83,9 @@ class OutputLayer(nn.Module):
     cross-entropy and both gradients run in chunks of that many tokens, so
     only a [chunk_tokens, V] logits buffer ever exists -- the role of
     Liger's fused linear cross-entropy in the reference
-    (slide_fsdp.py:86-98); 0 materialises the full [T, V] logits."""
+    (slide_fsdp.py:86-98); 0 materialises the full [T, V] logits.  A step
+    with an objective (``objectives.py``) takes the log-probabilities of the
+    labels instead, in either setting without logits."""
 
     def __init__(self, norm: nn.Module, lm_head: nn.Module, eps: float, chunk_tokens: int = 0):
         super().__init__()
@@ -102,7 +105,13 @@ class OutputLayer(nn.Module):
         w_n, w_lm = self.norm.weight.data, self.lm_head.weight.data
         x, rstd = ops.rmsnorm_fwd(h, w_n, self.eps)
         g_n, g_lm = self._grads()
-        if self.chunk_tokens > 0:
+        if getattr(ctx, "objective", None) is not None:
+            tau = ctx.objective.temperature
+            logp, lse = ops.linear_logprob_fwd(x, w_lm, ctx.targets, temperature=tau)
+            loss, dlogp = ctx.objective.loss_and_grad(logp, ctx.targets, ctx.seq_len)
+            dx = torch.empty_like(x)
+            ops.linear_logprob_bwd(dlogp, x, w_lm, ctx.targets, lse, dx, g_lm, temperature=tau)
+        elif self.chunk_tokens > 0:
             dx = torch.empty_like(x)
             loss, _ = ops.linear_cross_entropy(x, w_lm, ctx.targets, dx, g_lm, self.chunk_tokens)
         else:
@@ -119,6 +128,10 @@ class OutputLayer(nn.Module):
     def logits(self, h: torch.Tensor) -> torch.Tensor:
         x, _ = ops.rmsnorm_fwd(h, self.norm.weight.data, self.eps)
         return ops.linear_fwd(x, self.lm_head.weight.data)
+
+    def logprobs(self, h: torch.Tensor, targets: torch.Tensor, temperature: float) -> torch.Tensor:
+        x, _ = ops.rmsnorm_fwd(h, self.norm.weight.data, self.eps)
+        return ops.linear_logprob_fwd(x, self.lm_head.weight.data, targets, temperature=temperature)[0]
 
 
 def _convert_hf_llama(model: nn.Module) -> LlamaForCausalLM:
@@ -142,6 +155,7 @@ class SlideFSDP(nn.Module):
         self.config = config
         self.device = torch.device(config.device)
         self.init_times: Dict[str, float] = {}  # seconds per set-up phase
+        self.last_objective: Dict[str, torch.Tensor] = {}  # results of the last step's objective
         t_phase = [time.perf_counter()]
 
         def phase(name: str) -> None:
@@ -815,14 +829,38 @@ class SlideFSDP(nn.Module):
 
     # -------------------------------------------------------------- step
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
-                labels: Optional[torch.Tensor] = None, **kwargs) -> CausalLMOutputWithPast:
+                labels: Optional[torch.Tensor] = None, *, objective=None,
+                ref_logps: Optional[torch.Tensor] = None, old_logps: Optional[torch.Tensor] = None,
+                advantages: Optional[torch.Tensor] = None, **kwargs) -> CausalLMOutputWithPast:
+        """One training step with labels, logits without.  ``objective``
+        (``objectives.PreferenceObjective``, ``objectives.PolicyObjective``)
+        replaces the cross-entropy loss; the tensors after it are what it
+        takes, and ``last_objective`` holds its results."""
         if attention_mask is not None:
             self._check_mask(attention_mask)
         self._check_ids(input_ids, labels)
+        if objective is None and any(t is not None for t in (ref_logps, old_logps, advantages)):
+            raise ValueError("ref_logps, old_logps and advantages go with an objective")
         if labels is None:
+            if objective is not None:
+                raise ValueError("an objective needs labels")
             return CausalLMOutputWithPast(loss=None, logits=self._inference(input_ids))
-        loss = self._train_step(input_ids, labels)
+        step = None
+        if objective is not None:
+            step = ObjectiveStep.build(objective, *input_ids.shape, self.device, ref_logps=ref_logps,
+                                       old_logps=old_logps, advantages=advantages)
+        loss = self._train_step(input_ids, labels, step)
         return CausalLMOutputWithPast(loss=loss, logits=None)
+
+    @torch.no_grad()
+    def token_logprobs(self, input_ids: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
+        """Log-probabilities [B, S] (fp32) of the labels under the present
+        weights, forward only: entry [b, s] is that of labels[b, s + 1] given
+        input_ids[b, : s + 1], 0 where that label is -100 and in the last
+        column.  With the weights of a run's start they are an objective's
+        ``ref_logps``."""
+        self._check_ids(input_ids, labels)
+        return self._inference(input_ids, labels, temperature)
 
     def _check_ids(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor]) -> None:
         """Token ids and labels that arrive in host memory are range-checked
@@ -878,7 +916,8 @@ class SlideFSDP(nn.Module):
                 host.counter_wait_geq(self.counters, base + r, step, 0.05)
 
     @torch.no_grad()
-    def _train_step(self, input_ids: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+    def _train_step(self, input_ids: torch.Tensor, labels: torch.Tensor,
+                    objective: Optional[ObjectiveStep] = None) -> torch.Tensor:
         cfg = self.model_config
         dev = self.device
         step = self.completed_steps + 1
@@ -886,6 +925,7 @@ class SlideFSDP(nn.Module):
         if self.cpu_slots is not None:
             self.cpu_slots.step = step
         ctx = self._make_context(input_ids, labels)
+        ctx.objective = objective
         S = self.layer_states
         L = self.num_decoder_layers
         emb, out = S[0], S[L + 1]
@@ -955,6 +995,8 @@ class SlideFSDP(nn.Module):
         self._check_unit(out, "forward")
         with self.tracer.span("loss", L + 1):
             loss, dh = out.module.loss_and_grad(h, ctx)
+        if objective is not None:
+            self.last_objective = objective.results
         del h
         if L > 0:
             S[L].bind_device(with_grad=True)
@@ -1017,9 +1059,11 @@ class SlideFSDP(nn.Module):
             self.updates.submit(idx, None, lambda fn=fn, g=g: fn(g, coef))
 
     @torch.no_grad()
-    def _inference(self, input_ids: torch.Tensor) -> torch.Tensor:
-        """Forward only; returns logits [B, S, V]."""
-        ctx = self._make_context(input_ids, None)
+    def _inference(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
+                   temperature: float = 1.0) -> torch.Tensor:
+        """Forward only; returns logits [B, S, V], or with labels their
+        log-probabilities [B, S]."""
+        ctx = self._make_context(input_ids, labels)
         S = self.layer_states
         L = self.num_decoder_layers
         self._fetch(S[0], with_grad=False)
@@ -1034,11 +1078,13 @@ class SlideFSDP(nn.Module):
             self._wait_loaded(st)
             if i <= L:
                 h = st.module(h, ctx)
-            else:
+            elif labels is None:
                 h = st.module.logits(h)
+            else:
+                h = st.module.logprobs(h, ctx.targets, temperature)
             self._release(st, Event(self.device).record())
         B, T = input_ids.shape
-        return h.view(B, T, -1)
+        return h.view(B, T, -1) if labels is None else h.view(B, T)
 
     # ------------------------------------------------------------ control
     def wait_for_updates(self) -> None:
