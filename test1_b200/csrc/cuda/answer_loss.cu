@@ -13,13 +13,13 @@
 //      several units have a mean of their own)
 //   C  per token: the gradient, and the policy loss's own sums
 //   D  the policy loss's totals
-// One launch runs them all, with a barrier of the whole grid between the
-// phases: a launch costs 4 us of the host's time, a barrier about 1.5 us of the
-// GPU's.  All blocks are on the GPU together (a cooperative launch of at most
-// two blocks per SM); a batch that one block handles as fast has no barrier at
-// all.  A unit belongs to a warp or, for sequences shorter than 32 tokens, to
-// the fewest lanes that hold one.  Sums are carried in fp64 and joined in a
-// fixed order: two runs give the same bits.
+// One launch runs them all, with a barrier of its blocks between the phases:
+// a launch of each phase costs 4 us of the host's time.  Up to 32 K tokens the
+// blocks are one cluster, whose barrier is the hardware's; above that they are
+// a cooperative grid of at most two blocks per SM (5 us more to launch, 1.5
+// us a barrier).  A unit belongs to a warp or, for sequences shorter than 32
+// tokens, to the fewest lanes that hold one.  Sums are carried in fp64 and
+// joined in a fixed order: two runs give the same bits.
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -45,7 +45,7 @@ struct LossParams {
   int lanes;               // lanes of a unit: 32, or the power of two >= S
   int vectors;             // 16-byte vectors of tokens
   int lengths_phase;       // policy: phase B takes place
-  int* arrivals;           // the barrier's counter, zero between launches
+  int* arrivals;           // the grid barrier's counter, zero between launches; null: the blocks are one cluster
   int* err;
   uint8_t* answer;         // [T] phase A's finding, an eighth of the targets to read again
   double2* units;          // [B * chunks] (sum of log ratios, answer tokens)
@@ -334,6 +334,16 @@ __device__ __forceinline__ void preference_grad_phase(const LossParams& p, Sums*
   });
 }
 
+// A token's clipped term for one advantage: past log(1 +- clip) on the side
+// that the advantage pushes to, the loss is flat.  The log ratio decides, so
+// the same tokens are clipped whatever exp's rounding does at the edge.
+struct Clip {
+  float minus_a, sign, past, flat;
+  __device__ Clip(const LossParams& p, float a)
+      : minus_a(-a), sign(a > 0.f ? 1.f : -1.f), past(a > 0.f ? p.hi : a < 0.f ? -p.lo : INFINITY),
+        flat(-a * (a > 0.f ? p.edge_hi : p.edge_lo)) {}
+};
+
 // exp(e) - 1 - e: its series up to e^7 for small e, where the difference would
 // keep no digit (the first term left out is below 2^-25 of the sum).
 __device__ __forceinline__ float kl_term(float e) {
@@ -358,14 +368,14 @@ __device__ __forceinline__ void policy_grad_phase(const LossParams& p, Sums* red
       const double n = p.chunks == 1 ? __ldcg(&p.units[u]).y : static_cast<double>(__ldcg(&p.lengths[b]));
       w = static_cast<float>(1 / (fmax(1.0, n) * live));
     }
-    const float seq_adv = p.adv_per_token ? 0.f : p.adv[b];
+    Clip clip(p, p.adv_per_token ? 0.f : p.adv[b]);
     double unit_loss = 0;
     const float *logp = p.logp + i0, *old = p.old + i0, *ref = p.ref + i0, *adv = p.adv + i0;
     const uint8_t* answer = p.answer + i0;
     float* dlogp = p.dlogp + i0;
     for_fours(p, len, lane, [&](const auto& four) {
       bool ok[kAhead];
-      float lp[kAhead], od[kAhead], rf[kAhead], a[kAhead] = {seq_adv, seq_adv, seq_adv, seq_adv}, part = 0.f, kl_part = 0.f;
+      float lp[kAhead], od[kAhead], rf[kAhead], a[kAhead], part = 0.f, kl_part = 0.f;
       four.load(answer, ok);
       four.load(logp, lp, 0.f);
       four.load(old, od, 0.f);
@@ -374,20 +384,18 @@ __device__ __forceinline__ void policy_grad_phase(const LossParams& p, Sums* red
       float g[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        // clipped where the log ratio is past log(1 +- clip): the same token
-        // whatever exp's rounding does at the edge
-        const float d = lp[k] - od[k], rho = __expf(d);
-        const bool over = d > p.hi, under = d < p.lo;
-        const bool clipped = (a[k] > 0.f && over) || (a[k] < 0.f && under);
-        float l = -a[k] * (clipped ? (over ? p.edge_hi : p.edge_lo) : rho);
-        g[k] = clipped ? 0.f : -a[k] * rho;
+        if (p.adv_per_token) clip = Clip(p, a[k]);
+        const float d = lp[k] - od[k], grad = clip.minus_a * __expf(d);
+        const bool clipped = clip.sign * d > clip.past;
+        float l = clipped ? clip.flat : grad;
+        g[k] = clipped ? 0.f : grad;
         if (p.ref != nullptr) {
           const float e = rf[k] - lp[k], kl = kl_term(e);
-          l += p.kl_coef * kl;
-          g[k] -= p.kl_coef * (kl + e);  // exp(e) - 1
-          kl_part += ok[k] ? kl : 0.f;
+          l = fmaf(p.kl_coef, kl, l);
+          g[k] = fmaf(-p.kl_coef, kl + e, g[k]);  // exp(e) - 1
+          if (ok[k]) kl_part += kl;
         }
-        part += ok[k] ? l : 0.f;
+        if (ok[k]) part += l;
         cut += ok[k] && clipped;
         g[k] = ok[k] ? g[k] * w : 0.f;
       }
@@ -419,12 +427,15 @@ __device__ __forceinline__ void policy_total_phase(const LossParams& p, Sums* re
   }
 }
 
-// Waits until every block of the grid has arrived for the `nth` time.  False
-// (and an error code) if that takes longer than any launch can.
+// Waits until every block has arrived for the `nth` time.  False (and an error
+// code) if that takes longer than any launch can.
 __device__ __forceinline__ bool grid_barrier(const LossParams& p, int nth) {
   __shared__ int ok;
   __syncthreads();
-  if (gridDim.x == 1) return true;
+  if (p.arrivals == nullptr) {
+    if (gridDim.x > 1) sm100::cluster_sync();
+    return true;
+  }
   if (threadIdx.x == 0) {
     const int all = nth * static_cast<int>(gridDim.x);
     __threadfence();
@@ -463,15 +474,17 @@ __global__ void __launch_bounds__(kLossThreads, kLossPerSm) answer_loss_kernel(c
   }
   if (POLICY) policy_grad_phase(p, red);
   else preference_grad_phase(p, red);
-  // the last block clears the counter, and adds up the policy loss's sums
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0)
-    last = gridDim.x == 1 || atomicAdd(p.arrivals, 1) == (barriers + 1) * static_cast<int>(gridDim.x) - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  if (threadIdx.x == 0 && gridDim.x > 1) *p.arrivals = 0;
+  if (p.arrivals == nullptr) {
+    if (!POLICY || !grid_barrier(p, ++barriers) || blockIdx.x != 0) return;
+  } else {  // the last block to arrive clears the counter
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(p.arrivals, 1) == (barriers + 1) * static_cast<int>(gridDim.x) - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    if (threadIdx.x == 0) *p.arrivals = 0;
+  }
   if (POLICY) policy_total_phase(p, red);
 }
 
@@ -495,27 +508,35 @@ static int64_t check_batch(const torch::Tensor& logp, const torch::Tensor& targe
   return logp.size(0) / S;
 }
 
-// Tokens up to which a single block works: what it loses against a full GPU
-// (16 tokens of a lane, about 4 us) is what the barriers and the cooperative
-// launch would cost.
-constexpr int64_t kBlockTokens = 8192;
+// Tokens of a cluster's block (8 of a lane, two rounds of loads), and blocks of
+// the largest cluster that runs anywhere.
+constexpr int64_t kBlockTokens = 4096;
+constexpr int kLargestCluster = 8;
 
 // The units of a batch and the blocks that share them.
 struct LossPlan {
+  bool cluster;
   int blocks, unit, chunks, lanes;
 
   LossPlan(int64_t B, int64_t S) {
-    const int64_t T = B * S, warps = T <= kBlockTokens ? kLossWarps : kLossPerSm * num_sms() * kLossWarps;
+    const int64_t T = B * S;
+    int most = kLossPerSm * num_sms();
     lanes = 32;
     while (lanes > 1 && lanes / 2 >= S) lanes /= 2;
+    const int64_t per_block = kLossWarps * (32 / lanes);
+    // no more than two sequences in a row for a group of lanes, four in the
+    // largest cluster
+    cluster = T <= kBlockTokens * kLargestCluster && B <= 4 * per_block * kLargestCluster;
+    if (cluster)
+      for (most = 1; most < kLargestCluster && (most * kBlockTokens < T || most * 2 * per_block < B);) most *= 2;
+    const int64_t warps = static_cast<int64_t>(most) * kLossWarps;
     // as many units as there are warps, of equal lengths, but no shorter than
     // one round of a lane's loads
     chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(warps / B, (S + 32 * kAhead - 1) / (32 * kAhead))));
     unit = static_cast<int>((S + chunks - 1) / chunks);
     if (S % 4 == 0) unit = (unit + 3) / 4 * 4;
     chunks = static_cast<int>((S + unit - 1) / unit);
-    const int64_t per_block = kLossWarps * (32 / lanes);
-    blocks = T <= kBlockTokens ? 1 : static_cast<int>(std::min<int64_t>((B * chunks + per_block - 1) / per_block, kLossPerSm * num_sms()));
+    blocks = cluster ? most : static_cast<int>(std::min<int64_t>((B * chunks + per_block - 1) / per_block, most));
   }
 };
 
@@ -561,18 +582,22 @@ static void launch_loss(LossParams& p, const LossPlan& plan) {
   cfg.gridDim = dim3(plan.blocks);
   cfg.blockDim = dim3(kLossThreads);
   cfg.stream = stream();
-  cudaLaunchAttribute attr;
-  if (plan.blocks > 1) {  // blocks that wait for one another
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (plan.cluster) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = plan.blocks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  } else {  // blocks that wait for one another
     arrivals = arrival_counters(1);
     p.arrivals = arrivals.data_ptr<int>();
-    attr.id = cudaLaunchAttributeCooperative;
-    attr.val.cooperative = 1;
-  } else {
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cfg.numAttrs = 1;
   }
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, answer_loss_kernel<POLICY>, static_cast<LossParams>(p));
   TORCH_CHECK(e == cudaSuccess, "answer_loss launch failed: ", cudaGetErrorString(e));
   count_launch();

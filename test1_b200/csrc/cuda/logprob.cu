@@ -25,24 +25,36 @@ using vocab::kLog2e;
 using vocab::ex2;
 
 // How many ranges of the vocabulary dx's product is cut into, so that its
-// `tiles` long units and the D dW tiles fill `clusters` evenly: the smallest
+// `tiles` long units and the dW tiles fill `clusters` evenly: the smallest
 // estimate of the time of the busiest cluster plus the planes' traffic, in
-// units of a k block (0.27 us; a tile's plane written and read back is 0.5 MB,
-// 0.08 us of the GPU's bandwidth).
-__host__ __device__ inline int pick_splits(int64_t tiles, int k_blocks, int64_t dw_tiles, int tiles_t, int clusters) {
+// tenths of a k block (0.27 us; a tile's plane written and read back is 0.5
+// MB, 0.08 us of the GPU's bandwidth).
+constexpr int kMaxSplits = 32;
+__host__ __device__ inline int64_t splits_cost(int s, int tiles, int k_blocks, int dw_tiles, int tiles_t, int clusters) {
+  const int64_t ux = vocab::dx_unit_cost(k_blocks, s), uw = vocab::dw_unit_cost(tiles_t);
+  const int64_t units = static_cast<int64_t>(tiles) * s;
+  const int64_t even = units * ux + dw_tiles * uw + clusters * uw;  // x clusters, so that nothing is divided
+  const int64_t longest = (units < clusters ? 1 : units / clusters + (units % clusters != 0)) * ux * clusters;
+  return 10 * (even > longest ? even : longest) + (s > 1 ? 3 * units * clusters : 0);
+}
+// The smallest s of the least cost, on the host and by a warp (a lane per s:
+// one thread's 32 turns took 10 us).  Whole numbers: both find the same.
+__host__ __device__ inline bool splits_allowed(int s, int k_blocks) { return s == 1 || k_blocks >= 8 * s; }
+inline int pick_splits(int tiles, int k_blocks, int dw_tiles, int tiles_t, int clusters) {
   int best = 1;
-  int64_t least = INT64_MAX;  // whole numbers: host and device must agree
-  for (int s = 1; s <= 32 && (s == 1 || k_blocks >= 8 * s); ++s) {
-    const int64_t ux = vocab::dx_unit_cost(k_blocks, s), uw = vocab::dw_unit_cost(tiles_t);
-    const int64_t even = (tiles * s * ux + dw_tiles * uw + clusters - 1) / clusters + uw;
-    const int64_t longest = (tiles * s + clusters - 1) / clusters * ux;
-    const int64_t cost = 10 * (even > longest ? even : longest) + (s > 1 ? 3 * s * tiles : 0);
-    if (cost < least) {
-      least = cost;
+  for (int s = 2; s <= kMaxSplits && splits_allowed(s, k_blocks); ++s)
+    if (splits_cost(s, tiles, k_blocks, dw_tiles, tiles_t, clusters) <
+        splits_cost(best, tiles, k_blocks, dw_tiles, tiles_t, clusters))
       best = s;
-    }
-  }
   return best;
+}
+__device__ __forceinline__ int pick_splits_warp(int tiles, int k_blocks, int dw_tiles, int tiles_t, int clusters) {
+  const int s = static_cast<int>(threadIdx.x & 31) + 1;
+  const int64_t cost = splits_allowed(s, k_blocks) ? splits_cost(s, tiles, k_blocks, dw_tiles, tiles_t, clusters) : INT64_MAX;
+  int64_t least = cost;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) least = min(least, static_cast<int64_t>(__shfl_xor_sync(0xffffffffu, static_cast<long long>(least), o)));
+  return __ffs(__ballot_sync(0xffffffffu, cost == least));
 }
 
 struct PackParams {
@@ -156,12 +168,13 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
   }
   if (t1 != p.T) return;
   // the last block knows how many there are
-  if (threadIdx.x == 0 && first_slice) {
-    p.meta->rows = pos;
+  if (warp == 0 && first_slice) {
     const int tiles_t = (pos + vocab::TILE - 1) / vocab::TILE;
-    if (BWD)
-      p.meta->splits = pick_splits(static_cast<int64_t>(tiles_t) * p.tiles_h, p.k_blocks,
-                                   static_cast<int64_t>(p.tiles_n) * p.tiles_h, tiles_t, p.clusters);
+    const int splits = BWD ? pick_splits_warp(tiles_t * p.tiles_h, p.k_blocks, p.tiles_n * p.tiles_h, tiles_t, p.clusters) : 1;
+    if (lane == 0) {
+      p.meta->rows = pos;
+      p.meta->splits = splits;
+    }
   }
   if (BWD) {  // dW's reduction runs over whole blocks of BK rows
     const int end = (pos + gemm::BK - 1) / gemm::BK * gemm::BK;

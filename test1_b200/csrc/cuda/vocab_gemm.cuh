@@ -108,10 +108,10 @@ __device__ __forceinline__ void write_logp(const float m, const float s, const f
 }
 
 // ---------------------------------------------------------- units of work
-// Time of a unit in k blocks of 64 (0.27 us of tensor time for a pair): dx
-// tiles pay about 12 for start, drain and planes; a dW tile cannot be faster
-// than its 128 KB leave (about 9).
-__host__ __device__ inline int dx_unit_cost(int k_blocks, int splits) { return k_blocks / splits + 12; }
+// Time of a unit in k blocks of 64 (0.27 us of tensor time for a pair): a dx
+// tile pays about 12 for its start and drain, and 10 more for planes and
+// their join; a dW tile cannot be faster than its 128 KB leave (about 9).
+__host__ __device__ inline int dx_unit_cost(int k_blocks, int splits) { return k_blocks / splits + (splits > 1 ? 22 : 12); }
 __host__ __device__ inline int dw_unit_cost(int tiles_t) {
   const int k = tiles_t * (TILE / BK);
   return k > 9 ? k : 9;

@@ -163,3 +163,47 @@ def test_refusals(cuda_device):
                    (pol, dict(kl_coef=-1.0)), (pol, dict(kl_coef=0.1, ref_logp=None)), (pol, dict(advantages=adv[:3]))):
         with pytest.raises(ValueError):
             f(**bad)
+
+
+@pytest.mark.parametrize("B,S", [(4, 64), (40, 1024)])
+@pytest.mark.parametrize("offset", [0, 1, 2])
+def test_alignment(B, S, offset, cuda_device):
+    """Sequences that 16-byte vectors divide, in tensors that start on such a
+    boundary and in ones that do not."""
+    from test1_b200 import ops
+
+    targets, logp, old, ref, adv, adv_tok = _batch(B, S, seed=6)
+    shift = lambda v: torch.cat([v[:offset], v])[offset:]  # noqa: E731
+    t, lp, od, rf = shift(targets), shift(logp), shift(old), shift(ref)
+    assert offset == 0 or lp.data_ptr() % 16
+    got = ops.preference_loss_fwd_bwd(lp, rf, t, S)
+    for a, b in zip(got, oracle.preference(logp, ref, targets, S, 0.1, "sigmoid", 0.0, False)):
+        _close(a, b, float(b.abs().max()) + (0.1 * math.sqrt(S) if b.shape == (B,) else 0))
+    for a_in, per in ((adv, adv), (shift(adv_tok), adv_tok)):
+        got = ops.policy_loss_fwd_bwd(lp, od, rf, a_in, t, S, kl_coef=0.1)
+        want = oracle.policy(logp, old, ref, per, targets, S, 0.2, 0.2, 0.1, "token")
+        for a, b, size in zip(got, want, (4.0, None, 1.0)):
+            _close(a, b, size)
+
+
+def test_captured_in_a_graph(cuda_device):
+    """A graph of the operators, replayed on new values in its inputs; the
+    eager calls between leave it alone."""
+    from test1_b200 import ops
+
+    targets, logp, old, ref, adv, _ = _batch(40, 1024, seed=7, fill=0.0)
+    small = [v[:2048].clone() for v in (targets, logp, old, ref)]
+    f = lambda: ops.policy_loss_fwd_bwd(logp, old, ref, adv, targets, 1024, kl_coef=0.1) + \
+        ops.preference_loss_fwd_bwd(logp, ref, targets, 1024) + \
+        ops.preference_loss_fwd_bwd(small[1], small[3], small[0], 64)  # noqa: E731
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f()
+    for k in range(2):
+        logp.add_(0.01 * k)
+        want = f()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -234,3 +234,32 @@ def test_refusals(cuda_device):
         a = {**dict(up=up, lse=lse, dx=dx, dw=dw), **bad}
         with pytest.raises(RuntimeError):
             ops.linear_logprob_bwd(a["up"], x, w, t, a["lse"], a["dx"], a["dw"])
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_captured_in_a_graph(T, cuda_device):
+    """Forward and backward in one graph, replayed on other hidden states."""
+    from test1_b200 import ops
+
+    x, w, t, up = _inputs(T, 256, 5003)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+
+    def f():
+        logp, lse = ops.linear_logprob_fwd(x, w, t)
+        ops.linear_logprob_bwd(up, x, w, t, lse, dx, dw)
+        return logp, lse
+
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f()
+    for k in range(2):
+        x.mul_(1 - 0.25 * k)
+        want = f()
+        want_dx, want_dw = dx.clone(), dw.clone()
+        dx.zero_(), dw.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        assert torch.equal(dx, want_dx) and torch.equal(dw, want_dw)
