@@ -3,9 +3,13 @@
 //
 //   logit[t, v] = x[t, :] . W[v, :] / tau
 //   lse[t]      = log sum_v exp(logit[t, v]),  logp[t] = logit[t, target[t]] - lse[t]
-//   u[t, v]     = onehot(target[t])[v] - exp(logit[t, v] - lse[t])
-//   dx[t, :]    = (dlogp[t] / tau) sum_v u[t, v] W[v, :]
-//   dW[v, :]    = sum_t u[t, v] (dlogp[t] / tau) x[t, :]
+//   u[t, v]     = (dlogp[t] / tau) (onehot(target[t])[v] - exp(logit[t, v] - lse[t]))
+//   dx[t, :]    = sum_v u[t, v] W[v, :]
+//   dW[v, :]    = sum_t u[t, v] x[t, :]
+//
+// u is the one intermediate that is rounded: to bf16, for the tensor cores.
+// Its relative error of 2^-9 at most per element adds to the 2^-9 of the
+// results' own rounding; all sums are fp32.
 //
 // A token whose target is ignored (ignore_index, or outside the vocabulary)
 // gives logp = lse = 0 and no gradient, whatever its hidden state holds.
@@ -74,8 +78,7 @@ struct PackParams {
   int64_t* target;       // [T]
   float* g;              // [T] dlogp / tau, with dlogp
   float* lse_packed;     // with dlogp
-  bf16* xp;              // [T, H] the rows of x
-  bf16* gxp;             // [T rounded up to 64, H] g x, with dlogp
+  bf16* xp;              // [T, with dlogp rounded up to 64; H] the rows of x
   float *zero0, *zero1;  // forward: logp and lse, 0 for the tokens left out
   bf16* dx;              // backward: likewise
 };
@@ -89,11 +92,6 @@ constexpr int kPackThreads = 256;
 // rows before its own tokens itself: T / 2 targets out of L2 on average
 // instead of a scan in a launch of its own.  Rows keep their order, so sums
 // over rows do not depend on timing.
-//
-// In the backward also g x, rounded to bf16 for the tensor cores: a relative
-// error of 2^-9 at most per element of x, independent from element to
-// element.  (Scaling the other factor instead, u, would round the one large
-// entry of each row, whose error all of a row of dx and dW shares.)
 template <bool BWD>
 __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackParams p) {
   __shared__ int counts[kPackThreads / 32];
@@ -135,33 +133,19 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
       }
       const int at = pos + __popc(mask & ((1u << j) - 1));
       if (T1_OOB(at, p.T)) continue;
-      float gr = 0.f;
-      if (BWD) gr = p.dlogp[t] * p.scale;
       if (lane == 0 && first_slice) {
         p.index[at] = t;
         p.target[at] = p.targets[t];
         if (BWD) {
-          p.g[at] = gr;
+          p.g[at] = p.dlogp[t] * p.scale;
           p.lse_packed[at] = p.lse[t];
         }
       }
       const bf16* src = p.x + static_cast<size_t>(t) * p.ldx;
 #pragma unroll 4
       for (int i = i0 + lane; i < i1; i += 32) {
-        const size_t dst = static_cast<size_t>(at) * p.H + 8 * i;
-        const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(src + 8 * i));
-        *reinterpret_cast<uint4*>(p.xp + dst) = raw;
-        if (BWD) {
-          float v[8];
-          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = __bfloat1622float2(h[k]);
-            v[2 * k] = f.x * gr;
-            v[2 * k + 1] = f.y * gr;
-          }
-          store8(p.gxp + dst, v);
-        }
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(src + 8 * i));
+        *reinterpret_cast<uint4*>(p.xp + static_cast<size_t>(at) * p.H + 8 * i) = v;
       }
     }
     pos += __popc(mask);
@@ -180,7 +164,7 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
     const int end = (pos + gemm::BK - 1) / gemm::BK * gemm::BK;
     for (int r = pos + warp; r < end; r += kWarps)
       for (int i = i0 + lane; i < i1; i += 32)
-        reinterpret_cast<uint4*>(p.gxp + static_cast<size_t>(r) * p.H)[i] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(p.xp + static_cast<size_t>(r) * p.H)[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -244,12 +228,12 @@ struct FewParams {
   float2* part;          // [block][16]
   float* target_logit;   // [16]
   float *logp, *lse_out;
-  // backward: u, g and g x
+  // backward
   const float *dlogp, *lse;
   bf16* u;               // [T, ldu]
   long ldu;
-  float* g;
-  bf16* gx;              // [T, H]
+  float* g;              // [T] dlogp / tau
+  bf16* xz;              // [T, H] x, zeros for tokens without a gradient
 };
 
 constexpr int kFewThreads = 512;
@@ -340,18 +324,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   }
   if (BWD && blockIdx.x == 0 && cell && wrow == 0) p.g[token] = gr;
   __syncthreads();
-  if (BWD) {  // g x, a share of it per block
-    for (int64_t i = blockIdx.x * kFewThreads + tid; i < static_cast<int64_t>(p.T) * (p.H / 8); i += static_cast<int64_t>(gridDim.x) * kFewThreads) {
-      const int t = static_cast<int>(i / (p.H / 8)), v = static_cast<int>(i % (p.H / 8));
+  if (BWD) {  // a share of x per block
+    const int nvec = p.H / 8;
+    for (int i = blockIdx.x * kFewThreads + tid; i < p.T * nvec; i += gridDim.x * kFewThreads) {
+      const int t = i / nvec, v = i % nvec;
       const int64_t tt = p.targets[t];
-      const float s = tt != p.ignore && tt >= 0 && tt < p.V ? p.dlogp[t] * p.scale : 0.f;
-      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (s != 0.f) {
-        load8(reinterpret_cast<const bf16*>(xs + t * pitch + 16 * v), f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] *= s;
-      }
-      store8(p.gx + static_cast<size_t>(t) * p.H + 8 * v, f);
+      const bool live = tt != p.ignore && tt >= 0 && tt < p.V && p.dlogp[t] != 0.f;
+      *reinterpret_cast<uint4*>(p.xz + static_cast<size_t>(t) * p.H + 8 * v) =
+          live ? *reinterpret_cast<const uint4*>(xs + t * pitch + 16 * v) : make_uint4(0, 0, 0, 0);
     }
   }
 
@@ -389,8 +369,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) l += red[(buf * kFewWarps + w) * CELLS + tid];
       if (BWD) {
-        float uv = gr != 0.f ? -ex2(fmaf(l, k2, -lse2)) : 0.f;
-        if (gr != 0.f && v == target) uv += 1.f;
+        const float uv = gr != 0.f ? gr * ((v == target ? 1.f : 0.f) - ex2(fmaf(l, k2, -lse2))) : 0.f;
         p.u[token * p.ldu + v] = __float2bfloat16_rn(uv);
       } else {
         vocab::lse_join(m, s, l, 1.f, k2);
@@ -473,7 +452,7 @@ static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
   }
   p.err = gemm_error_word().data_ptr<int>();
   const int clusters = static_cast<int>(std::min<int64_t>(units, num_sms() / 2));
-  launch_after("linear_logprob", kern, dim3(2 * clusters), 192, vocab::V_SMEM_BYTES, ta, tb, ta2, tb2, tc, p);
+  launch_after("linear_logprob", kern, dim3(2 * clusters), 64 + 32 * vocab::kEpiWarps<JOB>, vocab::V_SMEM_BYTES, ta, tb, ta2, tb2, tc, p);
 }
 
 // Arrival counters, zero between launches (whoever arrives last clears its
@@ -574,8 +553,8 @@ static bool packs(int64_t T, int64_t H, int64_t V) {
   return T > vocab::TILE && static_cast<double>(T) * H * V > 2e10;
 }
 
-// Column blocks up to which the last of them joins the rows' sums itself: a
-// launch of its own costs about as much as 32 dependent reads.
+// Tiles of columns up to which the last of them joins the rows' sums itself: a
+// launch of its own costs about as much as the 64 reads of 32 tiles.
 constexpr int kJoinBlocks = 32;
 
 // Returns (logp [T], lse [T]), fp32.
@@ -604,7 +583,7 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   const int64_t blocks = ceil_div(V, vocab::TILE), tiles_t = ceil_div(T, vocab::TILE);
   const bool pack = packs(T, H, V);
   Pieces ws;
-  const int64_t o_logit = ws.take(4 * T), o_part = ws.take(8 * blocks * T);
+  const int64_t o_logit = ws.take(4 * T), o_part = ws.take(2 * 8 * blocks * T);
   const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(8 * T);
   const int64_t o_x = ws.take(pack ? 2 * T * H : 0);
   auto buf = torch::empty({ws.used}, x.options().dtype(torch::kUInt8));
@@ -652,7 +631,7 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   CUtensorMap ta = make_map_any(pack ? base + o_x : x.data_ptr(), false, H, T, pack ? H : row_ld(x), vocab::HALF);
   CUtensorMap tb = make_map_any(w.data_ptr(), false, H, V, row_ld(w), vocab::HALF);
   launch_vocab<vocab::kLse>(ta, tb, ta, tb, ta, p, tiles_t * blocks);
-  if (!p.join) launch_after("logprob_join", logprob_join_kernel, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, blocks);
+  if (!p.join) launch_after("logprob_join", logprob_join_kernel, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, 2 * blocks);
   return {logp, lse};
 }
 
@@ -692,8 +671,8 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   const int64_t pieces = ceil_div(V, most);
   const int64_t width = std::min(V, round_up(ceil_div(V, pieces), vocab::TILE));
   const bool few = few_rows(T, H) && pieces == 1;
-  // with few rows nothing is packed: u and g x have T rows, and TMA reads
-  // zeros past them
+  // with few rows nothing is packed: u and x have T rows, and TMA reads zeros
+  // past them
   const int64_t ldu = round_up(width, 8), u_rows = few ? T : round_up(T, gemm::BK), k_v = ceil_div(width, gemm::BK);
   const int64_t tiles_v = ceil_div(width, vocab::TILE);
   // the most planes and units that the split rule can ask for, over the
@@ -706,8 +685,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   }
   Pieces ws;
   const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(8 * T),
-                o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_x = ws.take(2 * T * H),
-                o_gx = ws.take(2 * u_rows * H), o_planes = ws.take(4 * 8 * vocab::PLANE_BLOCK * planes),
+                o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_x = ws.take(2 * u_rows * H), o_planes = ws.take(4 * 8 * vocab::PLANE_BLOCK * planes),
                 o_u = ws.take(2 * u_rows * ldu);
   auto buf = torch::empty({ws.used}, x.options().dtype(torch::kUInt8));
   uint8_t* base = buf.data_ptr<uint8_t>();
@@ -719,8 +697,8 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   p.g = reinterpret_cast<float*>(base + o_g);
   p.dx = (bf16*)dx.data_ptr();
   p.planes = reinterpret_cast<float*>(base + o_planes);
-  bf16 *u = reinterpret_cast<bf16*>(base + o_u), *gx = reinterpret_cast<bf16*>(base + o_gx);
-  const CUtensorMap tgx = make_map_any(gx, false, H, u_rows, H, gemm::BK);
+  bf16 *u = reinterpret_cast<bf16*>(base + o_u), *xp = reinterpret_cast<bf16*>(base + o_x);
+  const CUtensorMap txc = make_map_any(xp, false, H, u_rows, H, gemm::BK);
   if (few) {
     FewParams f = few_params(x, w, tg, ignore_index, temperature);
     f.dlogp = up.data_ptr<float>();
@@ -728,7 +706,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     f.u = u;
     f.ldu = ldu;
     f.g = reinterpret_cast<float*>(base + o_g);
-    f.gx = gx;
+    f.xz = xp;
     launch_few<true>(f);
     p.rows = static_cast<int>(T);
     p.splits = pick_splits(tiles_h, k_v, tiles_v * tiles_h, 1, clusters);
@@ -736,7 +714,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     p.first = p.last = 1;
     launch_vocab<vocab::kGrads>(make_map_any(u, false, V, T, ldu, vocab::HALF),
                                 make_map_any(w.data_ptr(), false, H, V, row_ld(w), gemm::BK),
-                                make_map_any(u, false, V, T, ldu, gemm::BK), tgx,
+                                make_map_any(u, false, V, T, ldu, gemm::BK), txc,
                                 make_map_any(dw.data_ptr(), false, H, V, H, 32), p, most_units + tiles_v * tiles_h);
     return;
   }
@@ -761,8 +739,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   k.target = reinterpret_cast<int64_t*>(base + o_target);
   k.g = reinterpret_cast<float*>(base + o_g);
   k.lse_packed = reinterpret_cast<float*>(base + o_lse);
-  k.xp = reinterpret_cast<bf16*>(base + o_x);
-  k.gxp = gx;
+  k.xp = xp;
   k.dx = p.dx;
   launch_pack(k);
 
@@ -771,7 +748,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   p.index = k.index;
   p.targets = k.target;
   p.lse = k.lse_packed;
-  const CUtensorMap tx = make_map_any(k.xp, false, H, T, H, vocab::HALF);
+  const CUtensorMap tx = make_map_any(xp, false, H, u_rows, H, vocab::HALF);
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int64_t n = std::min(width, V - v0);
     const bf16* wp = (const bf16*)w.data_ptr() + v0 * row_ld(w);
@@ -786,7 +763,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     const CUtensorMap tus = make_map_any(u, false, n, u_rows, ldu, 32);
     const CUtensorMap tdw = make_map_any((bf16*)dw.data_ptr() + v0 * H, false, H, n, H, 32);
     launch_vocab<vocab::kSoftmaxGrad>(tx, tw, tx, tw, tus, p, tiles_t * ceil_div(n, vocab::TILE));
-    launch_vocab<vocab::kGrads>(tu, twc, tuc, tgx, tdw, p, most_units + ceil_div(n, vocab::TILE) * tiles_h);
+    launch_vocab<vocab::kGrads>(tu, twc, tuc, txc, tdw, p, most_units + ceil_div(n, vocab::TILE) * tiles_h);
   }
 }
 

@@ -1,14 +1,14 @@
 // tcgen05 products of the output layer whose [T, V] result is consumed on
 // the spot.  One kernel, three jobs:
 //   kLse          logits x W^T, reduced to (largest, sum of exponentials) per
-//                 row and 256-column block, and the target's logit;
-//   kSoftmaxGrad  the same logits turned into u = onehot - softmax (bf16);
-//   kGrads        both products with u in one launch: rows of dx = g (u W) and
-//                 dW = u^T (g x).
+//                 row and 128-column block, and the target's logit;
+//   kSoftmaxGrad  the same logits turned into u = g (onehot - softmax), bf16;
+//   kGrads        both products with u in one launch: the rows of dx = u W, and
+//                 dW = u^T x.
 //
 // The main loop is that of gemm_pair.cuh: CTA pairs (cta_group::2), 256 x 256
 // tiles, 128B-swizzled TMA loads into a 6-stage ring, one elected thread
-// issuing the MMAs, fp32 accumulators double-buffered in TMEM, 4 epilogue
+// issuing the MMAs, fp32 accumulators double-buffered in TMEM, 4 or 8 epilogue
 // warps per CTA that work on one accumulator while the other fills.  The
 // rows may be those that the packing kernel of logprob.cu kept, so their
 // number is read on the GPU.
@@ -62,14 +62,14 @@ struct VocabParams {
   // kLse
   int64_t ignore, V;
   int ld_part;
-  float2* part;            // [column block][ld_part]
+  float2* part;            // [block of 128 columns][ld_part]
   float* target_logit;     // [rows], unscaled
   int join;                // the last block of a row group joins its rows
   float *logp, *lse_out;   // with join
   // kSoftmaxGrad
   const float* lse;        // [rows]
+  const float* g;          // [rows] dlogp / tau
   // kGrads
-  const float* g;          // [rows]
   bf16* dx;                // [T, H]
   float* planes;           // [tile][split][8] blocks of PLANE_BLOCK
   int first, last;         // first / last piece of the vocabulary
@@ -88,6 +88,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 // and this one touches nothing of the previous kernel's before it has ended.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Warps that read accumulators.  kLse keeps 128 columns of a row in a
+// thread's registers, so eight warps share a tile's 256.
+template <int JOB>
+constexpr int kEpiWarps = JOB == kLse ? 8 : 4;
+
+// The tensor cores drop what falls below the accumulator's last bit at every
+// step, which adds up: over 4096 products the logits lose 2e-6 of their size.
+// kLse, whose results are fp32, therefore starts a new accumulator after about
+// 24 k blocks (1536 products), in equal parts of k, and adds them up in
+// registers, rounded (kLseBlocks = 24: 6e-7, at 3 % more time).
+constexpr int kLseBlocks = 24;
 
 // Running (largest m, sum s of exp((v - m) / tau)); k2 = log2(e) / tau.
 __device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2, float k2) {
@@ -119,6 +131,7 @@ __host__ __device__ inline int dw_unit_cost(int tiles_t) {
 
 struct Shape {
   int rows, tiles_t, tiles_n, tiles_h, k_h, k_n, k_rows, splits;
+  int k_acc;  // kLse: k blocks of an accumulator
 };
 
 __device__ __forceinline__ Shape shape_of(const VocabParams& p, bool splits) {
@@ -131,6 +144,8 @@ __device__ __forceinline__ Shape shape_of(const VocabParams& p, bool splits) {
   e.k_h = (p.H + BK - 1) / BK;
   e.k_n = (p.N + BK - 1) / BK;
   e.k_rows = (e.rows + BK - 1) / BK;
+  const int accs = max(1, (e.k_h + kLseBlocks / 2) / kLseBlocks);
+  e.k_acc = (e.k_h + accs - 1) / accs;
   return e;
 }
 
@@ -180,10 +195,10 @@ __device__ __forceinline__ bool get_unit(const Shape& e, int i, int c, int C, Un
 }
 
 // Operands: kLse, kSoftmaxGrad: A = rows of x, B = W.  kGrads, dx: A = u, B =
-// W by columns; dW: A2 = u by columns, B2 = g x by columns.  tma_c: u
+// W by columns; dW: A2 = u by columns, B2 = x by columns.  tma_c: u
 // (kSoftmaxGrad) or dW (kGrads).
 template <int JOB>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpiWarps<JOB>, 1)
     vocab_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_a2, const __grid_constant__ CUtensorMap tma_b2,
                  const __grid_constant__ CUtensorMap tma_c, const VocabParams p) {
@@ -215,7 +230,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 8);  // 4 epilogue warps x 2 CTAs
+      mbar_init(&tempty[a], 2 * kEpiWarps<JOB>);  // of both CTAs
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -288,46 +303,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     if (lane == 0 && crank == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      for (int i = 0; !*abort_flag && get_unit<JOB>(e, i, cluster, nclusters, u); ++i) {
+      int filled = 0;  // accumulators handed over so far
+      bool ok = true;
+      for (int i = 0; ok && !*abort_flag && get_unit<JOB>(e, i, cluster, nclusters, u); ++i) {
         const bool a_mn = JOB == kGrads && u.split < 0;
         constexpr bool b_mn = JOB == kGrads;
         const uint32_t idesc = a_mn ? idesc_bf16_f32(TILE, TILE, true, b_mn) : idesc_bf16_f32(TILE, TILE, false, b_mn);
-        const int acc = i & 1;
-        const uint32_t acc_phase = (i >> 1) & 1;
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1)) {
-          err.set(122);
-          *abort_flag = 1;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * TILE;
-        bool ok = true;
-        for (int kb = u.kb0; kb < u.kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase)) {
-            err.set(123);
+        int kb = u.kb0;
+        do {  // once per accumulator
+          const int acc = filled & 1;
+          if (!mbar_wait(&tempty[acc], ((filled >> 1) & 1) ^ 1)) {
+            err.set(122);
             *abort_flag = 1;
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(sA + stage * V_A_BYTES);
-          const uint32_t b_addr = smem_u32(sB + stage * V_A_BYTES);
+          const uint32_t d_tmem = tmem_base + acc * TILE;
+          const int first = kb, end = JOB == kLse ? min(u.kb1, kb + e.k_acc) : u.kb1;
+          for (; kb < end; ++kb) {
+            if (!mbar_wait(&full[stage], phase)) {
+              err.set(123);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(sA + stage * V_A_BYTES);
+            const uint32_t b_addr = smem_u32(sB + stage * V_A_BYTES);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t ad = a_mn ? smem_desc_sw128(a_addr + k * 2048, 8192, 1024)
-                                     : smem_desc_sw128(a_addr + k * 32, 16, 1024);
-            const uint64_t bd = b_mn ? smem_desc_sw128(b_addr + k * 2048, 8192, 1024)
-                                     : smem_desc_sw128(b_addr + k * 32, 16, 1024);
-            mma_bf16_pair(d_tmem, ad, bd, idesc, (kb != u.kb0 || k != 0) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) {
+              const uint64_t ad = a_mn ? smem_desc_sw128(a_addr + k * 2048, 8192, 1024)
+                                       : smem_desc_sw128(a_addr + k * 32, 16, 1024);
+              const uint64_t bd = b_mn ? smem_desc_sw128(b_addr + k * 2048, 8192, 1024)
+                                       : smem_desc_sw128(b_addr + k * 32, 16, 1024);
+              mma_bf16_pair(d_tmem, ad, bd, idesc, (kb != first || k != 0) ? 1u : 0u);
+            }
+            mma_commit_pair(&empty[stage], 0x3);
+            if (++stage == VSTAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          mma_commit_pair(&empty[stage], 0x3);
-          if (++stage == VSTAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
-        if (!ok) break;
-        mma_commit_pair(&tfull[acc], 0x3);
+          if (!ok) break;
+          mma_commit_pair(&tfull[acc], 0x3);
+          ++filled;
+        } while (kb < u.kb1);
       }
     }
   } else {
@@ -338,77 +359,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     const uint32_t leader_tempty1 = mapa_shared(smem_u32(&tempty[1]), 0);
     const float k2 = p.scale * kLog2e;
     int bi = 0;
-    for (int i = 0; get_unit<JOB>(e, i, cluster, nclusters, u); ++i) {
-      const int acc = i & 1;
-      const uint32_t acc_phase = (i >> 1) & 1;
-      // one lane waits and the warp follows it, so the warp never diverges
-      // around the .sync.aligned TMEM loads below
+    int taken = 0;  // accumulators taken over so far
+    // One lane waits and the warp follows it, so the warp never diverges
+    // around the .sync.aligned TMEM loads that come after.
+    auto take = [&](int& acc) {
+      acc = taken & 1;
       int ok = 0;
       if (lane == 0) {
         ok = !*abort_flag;
-        if (ok && !mbar_wait(&tfull[acc], acc_phase)) {
+        if (ok && !mbar_wait(&tfull[acc], (taken >> 1) & 1)) {
           err.set(124);
           *abort_flag = 1;
           ok = 0;
         }
       }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      ++taken;
+      if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
       tc_fence_after();
-      const int w8 = static_cast<int>(crank) * 4 + q;  // which 32 rows of the tile
+      return true;
+    };
+    // The accumulator's last read is done.
+    auto release = [&](int acc) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
+    };
+    const uint32_t quarter = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+    const int w8 = static_cast<int>(crank) * 4 + q;  // which 32 rows of a tile
+    for (int i = 0; get_unit<JOB>(e, i, cluster, nclusters, u); ++i) {
       const int row0 = u.mb * TILE + w8 * 32;
       const int row = row0 + lane;
       const int tcol0 = u.nb * TILE;  // first column of the tile
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * TILE;
-      auto release = [&] {  // the accumulator's last read is done
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
-      };
+      int acc;
 
       if (JOB == kLse) {
-        // A running (largest, sum) over the tile's columns, kept in the
-        // accumulator's own units: (logit - largest) is exact near the
-        // largest, which is where the sum comes from.
-        const bool row_ok = row < e.rows;
-        const int cols = min(TILE, p.N - tcol0);
-        const int64_t t = row_ok ? p.targets[row] - tcol0 : -1;
-        const int tcol = t >= 0 && t < cols ? static_cast<int>(t) : -1;
-        float m = -INFINITY, s = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < TILE; c += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(taddr + c, r);
-          tmem_ld_wait();
-          if (c + 32 > cols) {  // columns past the vocabulary
+        // 128 columns of the row, the sum of the tile's accumulators
+        const int half = (warp - 2) >> 2;
+        float v[HALF];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = c + j >= cols ? __float_as_uint(-INFINITY) : r[j];
+        for (int j = 0; j < HALF; ++j) v[j] = 0.f;
+        bool ok = true;
+        for (int kb = u.kb0; kb < u.kb1; kb += e.k_acc) {
+          ok = take(acc);
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < HALF; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(quarter + acc * TILE + half * HALF + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[c + j] += __uint_as_float(r[j]);
           }
-          float mx[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mx[j] = fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 4]));
-#pragma unroll
-          for (int j = 8; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(r[j]));
-          const float mn = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          float a[4] = {s * ex2((m - ref) * k2), 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 32; ++j) a[j & 3] += ex2((__uint_as_float(r[j]) - ref) * k2);
-          s = (a[0] + a[1]) + (a[2] + a[3]);
-          m = mn;
-          if (tcol >= c && tcol < c + 32 && !T1_OOB(row, p.ld_part)) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (tcol - c == j) p.target_logit[row] = __uint_as_float(r[j]);
-          }
+          release(acc);
         }
-        release();
-        if (row_ok && !T1_OOB(row, p.ld_part)) __stcg(&p.part[static_cast<size_t>(u.nb) * p.ld_part + row], make_float2(m, s));
+        if (!ok) break;
+        // (largest, sum) in the accumulator's own units: (logit - largest) is
+        // exact near the largest, which is where the sum comes from
+        const bool row_ok = row < e.rows;
+        const int col0 = tcol0 + half * HALF, cols = p.N - col0;
+        if (cols < HALF) {  // columns past the vocabulary
+#pragma unroll
+          for (int j = 0; j < HALF; ++j) v[j] = j < cols ? v[j] : -INFINITY;
+        }
+        float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int j = 4; j < HALF; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+        float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float ref = m == -INFINITY ? 0.f : m;
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) a[j & 3] += ex2((v[j] - ref) * k2);
+        float s = (a[0] + a[1]) + (a[2] + a[3]);
+        const int64_t t = row_ok ? p.targets[row] - col0 : -1;
+        const bool mine = t >= 0 && t < min(cols, HALF) && !T1_OOB(row, p.ld_part);
+        if (__any_sync(0xffffffffu, mine)) {
+          float x = 0.f;
+#pragma unroll
+          for (int j = 0; j < HALF; ++j) x = static_cast<int>(t) == j ? v[j] : x;
+          if (mine) __stcg(&p.target_logit[row], x);
+        }
+        if (row_ok && !T1_OOB(row, p.ld_part))
+          __stcg(&p.part[static_cast<size_t>(2 * u.nb + half) * p.ld_part + row], make_float2(m, s));
         if (!p.join) continue;
         // the last of the row group's column blocks joins them all, in order
         __threadfence();
         __syncwarp();
         int last = 0;
-        if (lane == 0) last = atomicAdd(&p.tickets[u.mb * 8 + w8], 1) == e.tiles_n - 1;
+        if (lane == 0) last = atomicAdd(&p.tickets[u.mb * 8 + w8], 1) == 2 * e.tiles_n - 1;
         if (!__shfl_sync(0xffffffffu, last, 0)) continue;
         __threadfence();
         if (lane == 0) p.tickets[u.mb * 8 + w8] = 0;
@@ -416,9 +453,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         m = -INFINITY;
         s = 0.f;
 #pragma unroll 4
-        for (int b = 0; b < e.tiles_n; ++b) {
-          const float2 v = __ldcg(&p.part[static_cast<size_t>(b) * p.ld_part + row]);
-          lse_join(m, s, v.x, v.y, k2);
+        for (int b = 0; b < 2 * e.tiles_n; ++b) {
+          const float2 w = __ldcg(&p.part[static_cast<size_t>(b) * p.ld_part + row]);
+          lse_join(m, s, w.x, w.y, k2);
         }
         const int at = p.index != nullptr ? p.index[row] : row;
         const int64_t target = p.targets[row];
@@ -427,17 +464,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         continue;
       }
 
+      if (!take(acc)) break;
+      const uint32_t taddr = quarter + acc * TILE;
+
       if (JOB == kGrads && u.split >= 0) {
         // dx: these columns' sums, in fp32 until all of the vocabulary is in
         const bool live = row0 < e.rows;
         const int tile = u.mb * e.tiles_h + u.nb;
         const size_t tile_block = (static_cast<size_t>(tile) * e.splits) * 8 + w8;
         float4* plane = reinterpret_cast<float4*>(p.planes + (tile_block + static_cast<size_t>(u.split) * 8) * PLANE_BLOCK);
-        const float gr = row < e.rows ? p.g[row] : 0.f;
+        const bool dead = row < e.rows && p.g[row] == 0.f;  // its dx is 0, whatever W holds
         const int at = row < e.rows && p.index != nullptr ? p.index[row] : row;
         const bool direct = e.splits == 1 && p.last;  // no other range, no later piece
-        // 64 columns of dx: g x sums, rounded once, to whole 128-byte lines
-        // of the rows' tokens
+        // 64 columns of dx, rounded once, to whole 128-byte lines of the rows'
+        // tokens
         auto store64 = [&](const float* f, int c) {
           uint8_t* rowp = wbuf + lane * 128;
 #pragma unroll
@@ -445,8 +485,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
             uint4 ov;
             __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&ov);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) oh[k] = __floats2bfloat162_rn(f[8 * j + 2 * k] * gr, f[8 * j + 2 * k + 1] * gr);
-            if (gr == 0.f) ov = make_uint4(0, 0, 0, 0);  // whatever W holds
+            for (int k = 0; k < 4; ++k) oh[k] = __floats2bfloat162_rn(f[8 * j + 2 * k], f[8 * j + 2 * k + 1]);
+            if (dead) ov = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(rowp + ((j ^ (lane & 7)) << 4)) = ov;
           }
           __syncwarp();
@@ -468,7 +508,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           tmem_ld_32x32b_x32(taddr + c, r[0]);
           tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
           tmem_ld_wait();
-          if (c + 64 == TILE) release();
+          if (c + 64 == TILE) release(acc);
           if (!live) continue;
           float f[64];
 #pragma unroll
@@ -527,9 +567,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       // u's rows are a reduction's length in kGrads: its last block of BK has
       // to be there, with zeros past the last row
       const int m_end = JOB == kSoftmaxGrad ? e.k_rows * BK : p.N;
-      float lse2 = 0.f;
+      float lse2 = 0.f, gr = 0.f;
       int tcol = -1;
       if (JOB == kSoftmaxGrad && row_ok) {
+        gr = p.g[row];
         lse2 = p.lse[row] * kLog2e;
         const int64_t t = p.targets[row] - p.col0 - tcol0;
         tcol = t >= 0 && t < cols ? static_cast<int>(t) : -1;
@@ -545,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         tmem_ld_32x32b_x32(taddr + c, r[0]);
         tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
         tmem_ld_wait();
-        if (c + 64 == TILE) release();
+        if (c + 64 == TILE) release(acc);
         if (!live) continue;
         uint8_t* rowp = buf + lane * 128;
 #pragma unroll
@@ -555,8 +596,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           for (int k = 0; k < 8; ++k) {
             f[k] = __uint_as_float(r[j >> 2][(j & 3) * 8 + k]);
             if (JOB == kSoftmaxGrad) {
-              f[k] = row_ok ? -ex2(fmaf(f[k], k2, -lse2)) : 0.f;
-              if (tcol == c + 8 * j + k) f[k] += 1.f;
+              const float onehot = tcol == c + 8 * j + k ? 1.f : 0.f;
+              f[k] = row_ok ? gr * (onehot - ex2(fmaf(f[k], k2, -lse2))) : 0.f;
             } else if (u.kb0 == u.kb1) {  // a sum over no rows
               f[k] = 0.f;
             }
