@@ -133,7 +133,7 @@ def preference_loss_fwd_bwd(logp, ref_logp, targets, seq_len, beta=0.1, kind="si
       hinge    max(0, 1 - beta m)
       ipo      (m - 1 / (2 beta))^2
     averaged over the pairs that have an answer token (a pair of padding only
-    is left out).  Returns (loss [] fp32, dloss/dlogp [T], rewards
+    is left out); label_smoothing is the sigmoid loss's alone.  Returns (loss [] fp32, dloss/dlogp [T], rewards
     [T / seq_len] = beta r)."""
     _check_loss(logp, targets, seq_len)
     if (logp.shape[0] // seq_len) % 2:
@@ -170,8 +170,6 @@ def check_preference(beta, kind, label_smoothing):
         raise ValueError(f"beta must be positive, got {beta}")
     if not 0.0 <= label_smoothing < 0.5:
         raise ValueError(f"label_smoothing must lie in [0, 0.5), got {label_smoothing}")
-    if label_smoothing and kind != "sigmoid":
-        raise ValueError("label_smoothing goes with kind='sigmoid'")
 
 
 def check_policy(clip_low, clip_high, kl_coef, reduction):

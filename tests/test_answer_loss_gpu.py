@@ -42,7 +42,7 @@ SIZES = [(2, 1), (2, 7), (4, 33), (6, 255), (4, 4097), (2, 20001), (300, 5), (20
 @pytest.mark.parametrize("B,S", SIZES)
 @pytest.mark.parametrize("kind,smoothing,average,with_ref",
                          [("sigmoid", 0.0, False, True), ("sigmoid", 0.2, True, False), ("hinge", 0.0, True, True),
-                          ("ipo", 0.0, True, True)])
+                          ("ipo", 0.0, True, True), ("hinge", 0.1, False, True)])
 def test_preference(B, S, kind, smoothing, average, with_ref, cuda_device):
     from test1_b200 import ops
 
@@ -158,7 +158,7 @@ def test_refusals(cuda_device):
         with pytest.raises(RuntimeError):
             f(**bad)
     for f, bad in ((pref, dict(seq_len=7)), (pref, dict(seq_len=0)), (pref, dict(seq_len=32)), (pref, dict(beta=0.0)),
-                   (pref, dict(kind="other")), (pref, dict(label_smoothing=0.5)), (pref, dict(kind="ipo", label_smoothing=0.1)),
+                   (pref, dict(kind="other")), (pref, dict(label_smoothing=0.5)),
                    (pol, dict(clip_low=1.0)), (pol, dict(clip_high=-0.1)), (pol, dict(reduction="mean")),
                    (pol, dict(kl_coef=-1.0)), (pol, dict(kl_coef=0.1, ref_logp=None)), (pol, dict(advantages=adv[:3]))):
         with pytest.raises(ValueError):
