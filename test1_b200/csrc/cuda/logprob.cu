@@ -30,16 +30,17 @@ using vocab::ex2;
 
 // How many ranges of the vocabulary dx's product is cut into, so that its
 // `tiles` long units and the dW tiles fill `clusters` evenly: the smallest
-// estimate of the time of the busiest cluster plus the planes' traffic, in
-// tenths of a k block (0.27 us; a tile's plane written and read back is 0.5
-// MB, 0.08 us of the GPU's bandwidth).
+// estimate of the time of the busiest cluster plus the planes' traffic and
+// the launch that adds them, in tenths of a k block (0.27 us; a tile's plane
+// written and read back is 0.5 MB, 0.08 us of the GPU's bandwidth; the launch
+// costs about 3 us).
 constexpr int kMaxSplits = 32;
 __host__ __device__ inline int64_t splits_cost(int s, int tiles, int k_blocks, int dw_tiles, int tiles_t, int clusters) {
   const int64_t ux = vocab::dx_unit_cost(k_blocks, s), uw = vocab::dw_unit_cost(tiles_t);
   const int64_t units = static_cast<int64_t>(tiles) * s;
   const int64_t even = units * ux + dw_tiles * uw + clusters * uw;  // x clusters, so that nothing is divided
   const int64_t longest = (units < clusters ? 1 : units / clusters + (units % clusters != 0)) * ux * clusters;
-  return 10 * (even > longest ? even : longest) + (s > 1 ? 3 * units * clusters : 0);
+  return 10 * (even > longest ? even : longest) + (s > 1 ? (100 + 3 * units) * clusters : 0);
 }
 // The smallest s of the least cost, on the host and by a warp (a lane per s:
 // one thread's 32 turns took 10 us).  Whole numbers: both find the same.
@@ -202,6 +203,57 @@ __global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const Voc
   const int t = p.index != nullptr ? p.index[row] : row;
   const int64_t v = p.targets[row];
   vocab::write_logp(m, s, p.target_logit[row], v != p.ignore && v >= 0 && v < p.V, p.scale, p.logp + t, p.lse_out + t);
+}
+
+// dx from the planes of several ranges of the vocabulary, added in their
+// order: a block per 32 rows x 64 columns, a lane per row, a warp per four
+// columns (512 consecutive bytes of a plane), eight planes' loads in flight.
+// Adding them up in the product's own epilogue left it to one warp per 32
+// rows, one latency after the other (40 us for 32 planes; here 6).
+constexpr int kPlanesThreads = 512;
+__global__ void __launch_bounds__(kPlanesThreads) logprob_planes_kernel(const VocabParams p) {
+  __shared__ __align__(16) uint8_t slab[32 * 128];
+  vocab::launch_dependents();
+  vocab::wait_previous();
+  const vocab::Shape e = vocab::shape_of(p, true);
+  if (e.splits == 1) return;  // written by the product
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tile = blockIdx.x >> 3, w8 = blockIdx.x & 7;
+  const int mb = tile / e.tiles_h, nb = tile % e.tiles_h;
+  const int row0 = mb * vocab::TILE + w8 * 32, row = row0 + lane;
+  const int col0 = nb * vocab::TILE + blockIdx.y * 64;
+  if (row0 >= e.rows || col0 >= p.H) return;
+  const float4* plane = reinterpret_cast<const float4*>(p.planes + (static_cast<size_t>(tile) * e.splits * 8 + w8) * vocab::PLANE_BLOCK) +
+                        (blockIdx.y * 16 + warp) * 32 + lane;
+  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col0 + warp * 4 < p.H) {
+    for (int s0 = 0; s0 < e.splits; s0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[k] = s0 + k < e.splits ? __ldcg(plane + static_cast<size_t>(s0 + k) * (8 * vocab::PLANE_BLOCK / 4))
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        f.x += v[k].x;
+        f.y += v[k].y;
+        f.z += v[k].z;
+        f.w += v[k].w;
+      }
+    }
+  }
+  if (row < e.rows && p.g[row] == 0.f) f = make_float4(0.f, 0.f, 0.f, 0.f);  // whatever W holds
+  uint2 o;
+  __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&o);
+  oh[0] = __floats2bfloat162_rn(f.x, f.y);
+  oh[1] = __floats2bfloat162_rn(f.z, f.w);
+  *reinterpret_cast<uint2*>(slab + lane * 128 + (((warp >> 1) ^ (lane & 7)) << 4) + (warp & 1) * 8) = o;
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  const int rr = threadIdx.x >> 3, j = threadIdx.x & 7, col = col0 + 8 * j;
+  if (row0 + rr >= e.rows || col >= p.H) return;
+  const int64_t t = p.index != nullptr ? p.index[row0 + rr] : row0 + rr;
+  *reinterpret_cast<uint4*>(p.dx + t * p.H + col) = *reinterpret_cast<const uint4*>(slab + rr * 128 + ((j ^ (rr & 7)) << 4));
 }
 
 // -------------------------------------------------------------- few rows
@@ -452,7 +504,7 @@ static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
   }
   p.err = gemm_error_word().data_ptr<int>();
   const int clusters = static_cast<int>(std::min<int64_t>(units, num_sms() / 2));
-  launch_after("linear_logprob", kern, dim3(2 * clusters), 64 + 32 * vocab::kEpiWarps<JOB>, vocab::V_SMEM_BYTES, ta, tb, ta2, tb2, tc, p);
+  launch_after("linear_logprob", kern, dim3(2 * clusters), vocab::V_THREADS, vocab::V_SMEM_BYTES, ta, tb, ta2, tb2, tc, p);
 }
 
 // Arrival counters, zero between launches (whoever arrives last clears its
@@ -677,12 +729,14 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   const int64_t tiles_v = ceil_div(width, vocab::TILE);
   // the most planes and units that the split rule can ask for, over the
   // numbers of rows that the packing may leave
-  int64_t planes = 0, most_units = 0;
+  int64_t planes = 0, most_units = 0, split_tiles = 0;
   for (int64_t m = 1; m <= tiles_t; ++m) {
-    const int64_t n = m * tiles_h * pick_splits(m * tiles_h, k_v, tiles_v * tiles_h, m, clusters);
+    const int64_t tiles = m * tiles_h, n = tiles * pick_splits(tiles, k_v, tiles_v * tiles_h, m, clusters);
     most_units = std::max(most_units, n);
-    if (pieces > 1 || n > m * tiles_h) planes = std::max(planes, n);
+    if (pieces > 1 || n > tiles) planes = std::max(planes, n);
+    if (n > tiles) split_tiles = std::max(split_tiles, tiles);
   }
+  const bool may_split = split_tiles > 0;
   Pieces ws;
   const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(8 * T),
                 o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_x = ws.take(2 * u_rows * H), o_planes = ws.take(4 * 8 * vocab::PLANE_BLOCK * planes),
@@ -692,8 +746,6 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
 
   VocabParams p{};
   p.H = static_cast<int>(H);
-  const torch::Tensor counters = arrival_counters(tiles_t * tiles_h * 8);
-  p.tickets = counters.data_ptr<int>();
   p.g = reinterpret_cast<float*>(base + o_g);
   p.dx = (bf16*)dx.data_ptr();
   p.planes = reinterpret_cast<float*>(base + o_planes);
@@ -716,6 +768,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
                                 make_map_any(w.data_ptr(), false, H, V, row_ld(w), gemm::BK),
                                 make_map_any(u, false, V, T, ldu, gemm::BK), txc,
                                 make_map_any(dw.data_ptr(), false, H, V, H, 32), p, most_units + tiles_v * tiles_h);
+    if (p.splits > 1) launch_after("logprob_planes", logprob_planes_kernel, dim3(tiles_h * 8, 4), kPlanesThreads, 0, p);
     return;
   }
 
@@ -765,6 +818,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     launch_vocab<vocab::kSoftmaxGrad>(tx, tw, tx, tw, tus, p, tiles_t * ceil_div(n, vocab::TILE));
     launch_vocab<vocab::kGrads>(tu, twc, tuc, txc, tdw, p, most_units + ceil_div(n, vocab::TILE) * tiles_h);
   }
+  if (may_split) launch_after("logprob_planes", logprob_planes_kernel, dim3(split_tiles * 8, 4), kPlanesThreads, 0, p);
 }
 
 }  // namespace t1

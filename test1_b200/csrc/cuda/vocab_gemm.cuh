@@ -8,8 +8,10 @@
 //
 // The main loop is that of gemm_pair.cuh: CTA pairs (cta_group::2), 256 x 256
 // tiles, 128B-swizzled TMA loads into a 6-stage ring, one elected thread
-// issuing the MMAs, fp32 accumulators double-buffered in TMEM, 4 or 8 epilogue
-// warps per CTA that work on one accumulator while the other fills.  The
+// issuing the MMAs, fp32 accumulators double-buffered in TMEM, 8 epilogue warps
+// per CTA that work on one accumulator while the other fills (with 4, one per
+// SM partition, each waited for its own latencies: a u tile took 8 K cycles,
+// more than the 8 K of a mainloop at H = 1024).  The
 // rows may be those that the packing kernel of logprob.cu kept, so their
 // number is read on the GPU.
 //
@@ -31,8 +33,10 @@ constexpr int HALF = 128;   // a CTA's rows of A and of B
 constexpr int VSTAGES = 6;
 constexpr int V_A_BYTES = HALF * BK * 2;
 constexpr int V_STAGE_BYTES = 2 * V_A_BYTES;
-constexpr int EPI_BUF = 32 * 128;                // 32 rows x 128 bytes, 128B-swizzled
-constexpr int EPI_BYTES = 4 /*warps*/ * 2 * EPI_BUF;
+constexpr int EPI_WARPS = 8;                     // two per SM partition; a warp has 32 rows x 128 columns
+constexpr int EPI_BUF = 32 * 128;                // 32 rows x 128 bytes, 128B-swizzled, one per warp
+constexpr int EPI_BYTES = EPI_WARPS * EPI_BUF;
+constexpr int V_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int V_SMEM_BYTES = VSTAGES * V_STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 static_assert(V_SMEM_BYTES <= 232448, "exceeds 227 KB of shared memory");
 
@@ -58,7 +62,7 @@ struct VocabParams {
   int col0;                // vocabulary index of column 0
   const int* index;        // [rows] token of a packed row; null: the row itself
   const int64_t* targets;  // [rows] vocabulary index
-  int* tickets;            // zero between launches: arrivals per 32 rows (kLse) or per 32 x 256 block of dx (kGrads)
+  int* tickets;            // kLse: arrivals per 32 rows, zero between launches
   // kLse
   int64_t ignore, V;
   int ld_part;
@@ -89,11 +93,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Warps that read accumulators.  kLse keeps 128 columns of a row in a
-// thread's registers, so eight warps share a tile's 256.
-template <int JOB>
-constexpr int kEpiWarps = JOB == kLse ? 8 : 4;
-
 // The tensor cores drop what falls below the accumulator's last bit at every
 // step, which adds up: over 4096 products the logits lose 2e-6 of their size.
 // kLse, whose results are fp32, therefore starts a new accumulator after about
@@ -121,12 +120,12 @@ __device__ __forceinline__ void write_logp(const float m, const float s, const f
 
 // ---------------------------------------------------------- units of work
 // Time of a unit in k blocks of 64 (0.27 us of tensor time for a pair): a dx
-// tile pays about 12 for its start and drain, and 10 more for planes and
-// their join; a dW tile cannot be faster than its 128 KB leave (about 9).
-__host__ __device__ inline int dx_unit_cost(int k_blocks, int splits) { return k_blocks / splits + (splits > 1 ? 22 : 12); }
+// tile pays about 12 for its start and drain; a dW tile cannot be faster than
+// its 128 KB leave (about 6).
+__host__ __device__ inline int dx_unit_cost(int k_blocks, int splits) { return k_blocks / splits + 12; }
 __host__ __device__ inline int dw_unit_cost(int tiles_t) {
   const int k = tiles_t * (TILE / BK);
-  return k > 9 ? k : 9;
+  return k > 6 ? k : 6;
 }
 
 struct Shape {
@@ -198,7 +197,7 @@ __device__ __forceinline__ bool get_unit(const Shape& e, int i, int c, int C, Un
 // W by columns; dW: A2 = u by columns, B2 = x by columns.  tma_c: u
 // (kSoftmaxGrad) or dW (kGrads).
 template <int JOB>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpiWarps<JOB>, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
     vocab_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_a2, const __grid_constant__ CUtensorMap tma_b2,
                  const __grid_constant__ CUtensorMap tma_c, const VocabParams p) {
@@ -230,7 +229,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpiWarps<
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 2 * kEpiWarps<JOB>);  // of both CTAs
+      mbar_init(&tempty[a], 2 * EPI_WARPS);  // of both CTAs
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -354,11 +353,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpiWarps<
   } else {
     // ---------------------------------------------------------- epilogue
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    uint8_t* wbuf = sE + q * 2 * EPI_BUF;
+    const int half = (warp - 2) >> 2;  // which 128 columns of the tile
+    uint8_t* slab = sE + (warp - 2) * EPI_BUF;
     const uint32_t leader_tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
     const uint32_t leader_tempty1 = mapa_shared(smem_u32(&tempty[1]), 0);
     const float k2 = p.scale * kLog2e;
-    int bi = 0;
     int taken = 0;  // accumulators taken over so far
     // One lane waits and the warp follows it, so the warp never diverges
     // around the .sync.aligned TMEM loads that come after.
@@ -394,7 +393,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpiWarps<
 
       if (JOB == kLse) {
         // 128 columns of the row, the sum of the tile's accumulators
-        const int half = (warp - 2) >> 2;
         float v[HALF];
 #pragma unroll
         for (int j = 0; j < HALF; ++j) v[j] = 0.f;
@@ -465,105 +463,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpiWarps<
       }
 
       if (!take(acc)) break;
-      const uint32_t taddr = quarter + acc * TILE;
+      const int col0 = tcol0 + half * HALF;  // this warp's first column
+      const uint32_t taddr = quarter + acc * TILE + half * HALF;
+      uint8_t* rowp = slab + lane * 128;
+      // 32 columns of the row, rounded, to the slab's left or right half
+      auto to_slab = [&](const float (&f)[32], int right, bool zero) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint4 ov;
+          __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&ov);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) oh[k] = __floats2bfloat162_rn(f[8 * j + 2 * k], f[8 * j + 2 * k + 1]);
+          if (zero) ov = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(rowp + (((4 * right + j) ^ (lane & 7)) << 4)) = ov;
+        }
+      };
 
       if (JOB == kGrads && u.split >= 0) {
         // dx: these columns' sums, in fp32 until all of the vocabulary is in
         const bool live = row0 < e.rows;
-        const int tile = u.mb * e.tiles_h + u.nb;
-        const size_t tile_block = (static_cast<size_t>(tile) * e.splits) * 8 + w8;
-        float4* plane = reinterpret_cast<float4*>(p.planes + (tile_block + static_cast<size_t>(u.split) * 8) * PLANE_BLOCK);
+        const size_t block = (static_cast<size_t>(u.mb * e.tiles_h + u.nb) * e.splits + u.split) * 8 + w8;
+        float4* plane = reinterpret_cast<float4*>(p.planes + block * PLANE_BLOCK) + half * (HALF / 4) * 32 + lane;
         const bool dead = row < e.rows && p.g[row] == 0.f;  // its dx is 0, whatever W holds
         const int at = row < e.rows && p.index != nullptr ? p.index[row] : row;
         const bool direct = e.splits == 1 && p.last;  // no other range, no later piece
-        // 64 columns of dx, rounded once, to whole 128-byte lines of the rows'
-        // tokens
-        auto store64 = [&](const float* f, int c) {
-          uint8_t* rowp = wbuf + lane * 128;
+        if (lane == 0) bulk_wait_group_read<0>();  // stores of an earlier dW tile have read the slab
+        __syncwarp();
+#pragma unroll 1
+        for (int c = 0; c < HALF; c += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(taddr + c, r);
+          tmem_ld_wait();
+          if (c + 32 == HALF) release(acc);
+          if (!live || col0 + c >= p.H) continue;
+          float f[32];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint4 ov;
-            __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&ov);
+          for (int j = 0; j < 32; ++j) f[j] = u.kb0 == u.kb1 ? 0.f : __uint_as_float(r[j]);
+          if (!p.first) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) oh[k] = __floats2bfloat162_rn(f[8 * j + 2 * k], f[8 * j + 2 * k + 1]);
-            if (dead) ov = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(rowp + ((j ^ (lane & 7)) << 4)) = ov;
+            for (int j = 0; j < 8; ++j) {
+              const float4 v = __ldcg(plane + (c / 4 + j) * 32);
+              f[4 * j] += v.x;
+              f[4 * j + 1] += v.y;
+              f[4 * j + 2] += v.z;
+              f[4 * j + 3] += v.w;
+            }
           }
+          if (!direct) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              __stcg(plane + (c / 4 + j) * 32, make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]));
+            continue;
+          }
+          const int right = (c >> 5) & 1;
+          to_slab(f, right, dead);
+          if (!right && col0 + c + 32 < p.H) continue;
+          // whole 128-byte lines (as far as dx goes) of the rows' tokens
           __syncwarp();
 #pragma unroll
           for (int it = 0; it < 8; ++it) {
             const int rr = it * 4 + (lane >> 3), j = lane & 7;
             const int64_t t = __shfl_sync(0xffffffffu, at, rr);
-            const uint4 v = *reinterpret_cast<const uint4*>(wbuf + rr * 128 + ((j ^ (rr & 7)) << 4));
-            const int col = tcol0 + c + 8 * j;
-            if (row0 + rr < e.rows && col < p.H) *reinterpret_cast<uint4*>(p.dx + t * p.H + col) = v;
+            const uint4 v = *reinterpret_cast<const uint4*>(slab + rr * 128 + ((j ^ (rr & 7)) << 4));
+            const int col = col0 + (c & ~63) + 8 * j;
+            if (row0 + rr < e.rows && col < p.H && (right || j < 4)) *reinterpret_cast<uint4*>(p.dx + t * p.H + col) = v;
           }
           __syncwarp();
-        };
-        if (lane == 0) bulk_wait_group_read<0>();  // stores of an earlier dW tile have read the slab
-        __syncwarp();
-#pragma unroll 1
-        for (int c = 0; c < TILE; c += 64) {
-          uint32_t r[2][32];
-          tmem_ld_32x32b_x32(taddr + c, r[0]);
-          tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
-          tmem_ld_wait();
-          if (c + 64 == TILE) release(acc);
-          if (!live) continue;
-          float f[64];
-#pragma unroll
-          for (int j = 0; j < 64; ++j) f[j] = u.kb0 == u.kb1 ? 0.f : __uint_as_float(r[j >> 5][j & 31]);
-          if (!p.first) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float4 v = __ldcg(plane + (c / 4 + j) * 32 + lane);
-              f[4 * j] += v.x;
-              f[4 * j + 1] += v.y;
-              f[4 * j + 2] += v.z;
-              f[4 * j + 3] += v.w;
-            }
-          }
-          if (direct) {
-            store64(f, c);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              __stcg(plane + (c / 4 + j) * 32 + lane, make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]));
-          }
-        }
-        if (direct || !p.last || !live) continue;
-        // the last range to finish adds the planes, in their order
-        __threadfence();
-        __syncwarp();
-        int last = 0;
-        if (lane == 0) last = atomicAdd(&p.tickets[tile * 8 + w8], 1) == e.splits - 1;
-        if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-        __threadfence();
-        if (lane == 0) p.tickets[tile * 8 + w8] = 0;
-        const float4* planes = reinterpret_cast<const float4*>(p.planes + tile_block * PLANE_BLOCK);
-#pragma unroll 1
-        for (int c = 0; c < TILE; c += 64) {
-          float f[64];
-#pragma unroll
-          for (int j = 0; j < 64; ++j) f[j] = 0.f;
-          for (int s = 0; s < e.splits; ++s) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float4 v = __ldcg(planes + static_cast<size_t>(s) * (8 * PLANE_BLOCK / 4) + (c / 4 + j) * 32 + lane);
-              f[4 * j] += v.x;
-              f[4 * j + 1] += v.y;
-              f[4 * j + 2] += v.z;
-              f[4 * j + 3] += v.w;
-            }
-          }
-          store64(f, c);
         }
         continue;
       }
 
       // bf16 results (u, dW) through 32 x 64 slabs
       const bool row_ok = row < e.rows;
-      const int cols = min(TILE, (JOB == kSoftmaxGrad ? p.N : p.H) - tcol0);
+      const int width = JOB == kSoftmaxGrad ? p.N : p.H;
       // u's rows are a reduction's length in kGrads: its last block of BK has
       // to be there, with zeros past the last row
       const int m_end = JOB == kSoftmaxGrad ? e.k_rows * BK : p.N;
@@ -572,49 +544,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpiWarps<
       if (JOB == kSoftmaxGrad && row_ok) {
         gr = p.g[row];
         lse2 = p.lse[row] * kLog2e;
-        const int64_t t = p.targets[row] - p.col0 - tcol0;
-        tcol = t >= 0 && t < cols ? static_cast<int>(t) : -1;
+        const int64_t t = p.targets[row] - p.col0 - col0;
+        tcol = t >= 0 && t < HALF ? static_cast<int>(t) : -1;
       }
 #pragma unroll 1
-      for (int c = 0; c < TILE; c += 64) {
-        uint8_t* buf = wbuf + bi * EPI_BUF;
-        const bool live = c < cols && row0 < m_end;  // uniform over the warp
-        // the store issued from this buffer two slabs ago has read it
-        if (lane == 0) bulk_wait_group_read<1>();
-        __syncwarp();
+      for (int c = 0; c < HALF; c += 64) {
+        const bool live = col0 + c < width && row0 < m_end;  // uniform over the warp
         uint32_t r[2][32];
         tmem_ld_32x32b_x32(taddr + c, r[0]);
         tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
+        // the store issued from the slab before has read it
+        if (lane == 0) bulk_wait_group_read<0>();
+        __syncwarp();
         tmem_ld_wait();
-        if (c + 64 == TILE) release(acc);
+        if (c + 64 == HALF) release(acc);
         if (!live) continue;
-        uint8_t* rowp = buf + lane * 128;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float f[8];
+        for (int right = 0; right < 2; ++right) {
+          float f[32];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            f[k] = __uint_as_float(r[j >> 2][(j & 3) * 8 + k]);
-            if (JOB == kSoftmaxGrad) {
-              const float onehot = tcol == c + 8 * j + k ? 1.f : 0.f;
-              f[k] = row_ok ? gr * (onehot - ex2(fmaf(f[k], k2, -lse2))) : 0.f;
-            } else if (u.kb0 == u.kb1) {  // a sum over no rows
-              f[k] = 0.f;
-            }
+          for (int j = 0; j < 32; ++j) {
+            f[j] = __uint_as_float(r[right][j]);
+            if (JOB == kSoftmaxGrad) f[j] = -gr * ex2(fmaf(f[j], k2, -lse2));
           }
-          uint4 ov;
-          __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&ov);
+          if (JOB == kSoftmaxGrad && __any_sync(0xffffffffu, tcol >= c + 32 * right && tcol < c + 32 * right + 32)) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) oh[k] = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
-          *reinterpret_cast<uint4*>(rowp + ((j ^ (lane & 7)) << 4)) = ov;
+            for (int j = 0; j < 32; ++j) f[j] += tcol == c + 32 * right + j ? gr : 0.f;
+          }
+          // rows past the last, and sums over no rows, are 0
+          to_slab(f, right, JOB == kSoftmaxGrad ? !row_ok : u.kb0 == u.kb1);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_2d(&tma_c, buf, tcol0 + c, row0);
+          tma_store_2d(&tma_c, slab, col0 + c, row0);
           bulk_commit_group();
         }
-        bi ^= 1;
       }
     }
     // every store of this warp completed before the CTA may exit
