@@ -102,23 +102,21 @@ CUtensorMap make_map_f32(const void* ptr, int64_t inner, int64_t outer, int64_t 
   return m;
 }
 
-// 2-D tensor map, 128B swizzle, of any element type and extents: `inner`
-// contiguous elements per row (any number: columns past it read as zero and
-// are not stored), box = one 128-byte row x `box_outer` rows.
-CUtensorMap make_map_any(const void* ptr, bool f32, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
-  const int64_t es = f32 ? 4 : 2;
+// 2-D bf16 tensor map, 128B swizzle, of any extents: `inner` contiguous
+// elements per row (any number: columns past it read as zero and are not
+// stored), `outer` rows `ld` elements apart, box = 64 x box_outer.
+CUtensorMap make_map_any(const void* ptr, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
   TORCH_CHECK(reinterpret_cast<uintptr_t>(ptr) % 16 == 0, "TMA operand must be 16-byte aligned");
-  TORCH_CHECK((ld * es) % 16 == 0, "TMA operand rows must be multiples of 16 bytes apart");
+  TORCH_CHECK(ld % 8 == 0, "TMA operand rows must be a multiple of 8 elements apart");
   TORCH_CHECK(inner > 0 && outer > 0 && inner <= INT32_MAX && outer <= INT32_MAX, "TMA operand extents out of range");
   CUtensorMap m;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * es)};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_outer)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * 2)};
+  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_outer)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode_fn()(&m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                           const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with ", std::to_string(static_cast<int>(r)));
   return m;
 }

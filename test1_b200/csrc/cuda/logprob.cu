@@ -21,7 +21,7 @@
 
 namespace t1 {
 
-CUtensorMap make_map_any(const void* ptr, bool f32, int64_t inner, int64_t outer, int64_t ld, int box_outer);
+CUtensorMap make_map_any(const void* ptr, int64_t inner, int64_t outer, int64_t ld, int box_outer);
 torch::Tensor& gemm_error_word();
 
 using vocab::VocabParams;
@@ -531,6 +531,13 @@ struct Pieces {
   }
 };
 
+// Distance of two rows; a single row's own stride says nothing.
+static int64_t row_ld(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+static bool aligned_rows(const torch::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_ld(t) % 8 == 0;
+}
+
 static void check_logprob(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets,
                           double temperature) {
   T1_CHECK_INPUT(x, torch::kBFloat16);
@@ -544,13 +551,9 @@ static void check_logprob(const torch::Tensor& x, const torch::Tensor& w, const 
                   (w.size(0) < 2 || w.stride(0) >= w.size(1)), "x and w must be row-major");
   TORCH_CHECK(targets.dim() == 1 && targets.size(0) == x.size(0), "targets must have T entries");
   TORCH_CHECK(w.device() == x.device() && targets.device() == x.device(), "operands must be on one device");
-  const int64_t ldx = x.size(0) > 1 ? x.stride(0) : x.size(1);
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && ldx % 8 == 0, "x must have 16-byte aligned rows");
+  TORCH_CHECK(aligned_rows(x) && aligned_rows(w), "x and w must have 16-byte aligned rows");
   TORCH_CHECK(std::isfinite(temperature) && temperature > 0, "temperature must be positive");
 }
-
-// Distance of two rows; a single row's own stride says nothing.
-static int64_t row_ld(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 static void launch_pack(PackParams& p) {
   // about four blocks per SM: 8 to 32 tokens each and, when these are few,
@@ -619,7 +622,6 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   auto logp = torch::empty({T}, f32), lse = torch::empty({T}, f32);
   if (T == 0) return {logp, lse};
   auto tg = targets.contiguous();
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 && row_ld(w) % 8 == 0, "w must have 16-byte aligned rows");
   if (few_rows(T, H)) {
     FewParams p = few_params(x, w, tg, ignore_index, temperature);
     auto ws = torch::empty({32 * few_grid(V) + 16}, f32);
@@ -680,8 +682,8 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
     p.index = k.index;
     p.targets = k.target;
   }
-  CUtensorMap ta = make_map_any(pack ? base + o_x : x.data_ptr(), false, H, T, pack ? H : row_ld(x), vocab::HALF);
-  CUtensorMap tb = make_map_any(w.data_ptr(), false, H, V, row_ld(w), vocab::HALF);
+  CUtensorMap ta = make_map_any(pack ? base + o_x : x.data_ptr(), H, T, pack ? H : row_ld(x), vocab::HALF);
+  CUtensorMap tb = make_map_any(w.data_ptr(), H, V, row_ld(w), vocab::HALF);
   launch_vocab<vocab::kLse>(ta, tb, ta, tb, ta, p, tiles_t * blocks);
   if (!p.join) launch_after("logprob_join", logprob_join_kernel, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, 2 * blocks);
   return {logp, lse};
@@ -709,7 +711,6 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   TORCH_CHECK(dlogp.device() == x.device() && lse.device() == x.device() && dx.device() == x.device() &&
                   dw.device() == x.device(), "operands must be on one device");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(dx.data_ptr()) % 16 == 0, "dx must be 16-byte aligned");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 && row_ld(w) % 8 == 0, "w must have 16-byte aligned rows");
   const c10::cuda::CUDAGuard guard(x.device());
   if (T == 0) {
     dw.zero_();
@@ -750,7 +751,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   p.dx = (bf16*)dx.data_ptr();
   p.planes = reinterpret_cast<float*>(base + o_planes);
   bf16 *u = reinterpret_cast<bf16*>(base + o_u), *xp = reinterpret_cast<bf16*>(base + o_x);
-  const CUtensorMap txc = make_map_any(xp, false, H, u_rows, H, gemm::BK);
+  const CUtensorMap txc = make_map_any(xp, H, u_rows, H, gemm::BK);
   if (few) {
     FewParams f = few_params(x, w, tg, ignore_index, temperature);
     f.dlogp = up.data_ptr<float>();
@@ -764,10 +765,10 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     p.splits = pick_splits(tiles_h, k_v, tiles_v * tiles_h, 1, clusters);
     p.N = static_cast<int>(V);
     p.first = p.last = 1;
-    launch_vocab<vocab::kGrads>(make_map_any(u, false, V, T, ldu, vocab::HALF),
-                                make_map_any(w.data_ptr(), false, H, V, row_ld(w), gemm::BK),
-                                make_map_any(u, false, V, T, ldu, gemm::BK), txc,
-                                make_map_any(dw.data_ptr(), false, H, V, H, 32), p, most_units + tiles_v * tiles_h);
+    launch_vocab<vocab::kGrads>(make_map_any(u, V, T, ldu, vocab::HALF),
+                                make_map_any(w.data_ptr(), H, V, row_ld(w), gemm::BK),
+                                make_map_any(u, V, T, ldu, gemm::BK), txc,
+                                make_map_any(dw.data_ptr(), H, V, H, 32), p, most_units + tiles_v * tiles_h);
     if (p.splits > 1) launch_after("logprob_planes", logprob_planes_kernel, dim3(tiles_h * 8, 4), kPlanesThreads, 0, p);
     return;
   }
@@ -801,7 +802,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   p.index = k.index;
   p.targets = k.target;
   p.lse = k.lse_packed;
-  const CUtensorMap tx = make_map_any(xp, false, H, u_rows, H, vocab::HALF);
+  const CUtensorMap tx = make_map_any(xp, H, u_rows, H, vocab::HALF);
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int64_t n = std::min(width, V - v0);
     const bf16* wp = (const bf16*)w.data_ptr() + v0 * row_ld(w);
@@ -809,12 +810,12 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     p.col0 = static_cast<int>(v0);
     p.first = v0 == 0;
     p.last = v0 + width >= V;
-    const CUtensorMap tw = make_map_any(wp, false, H, n, row_ld(w), vocab::HALF);
-    const CUtensorMap twc = make_map_any(wp, false, H, n, row_ld(w), gemm::BK);
-    const CUtensorMap tu = make_map_any(u, false, n, u_rows, ldu, vocab::HALF);
-    const CUtensorMap tuc = make_map_any(u, false, n, u_rows, ldu, gemm::BK);
-    const CUtensorMap tus = make_map_any(u, false, n, u_rows, ldu, 32);
-    const CUtensorMap tdw = make_map_any((bf16*)dw.data_ptr() + v0 * H, false, H, n, H, 32);
+    const CUtensorMap tw = make_map_any(wp, H, n, row_ld(w), vocab::HALF);
+    const CUtensorMap twc = make_map_any(wp, H, n, row_ld(w), gemm::BK);
+    const CUtensorMap tu = make_map_any(u, n, u_rows, ldu, vocab::HALF);
+    const CUtensorMap tuc = make_map_any(u, n, u_rows, ldu, gemm::BK);
+    const CUtensorMap tus = make_map_any(u, n, u_rows, ldu, 32);
+    const CUtensorMap tdw = make_map_any((bf16*)dw.data_ptr() + v0 * H, H, n, H, 32);
     launch_vocab<vocab::kSoftmaxGrad>(tx, tw, tx, tw, tus, p, tiles_t * ceil_div(n, vocab::TILE));
     launch_vocab<vocab::kGrads>(tu, twc, tuc, txc, tdw, p, most_units + ceil_div(n, vocab::TILE) * tiles_h);
   }
