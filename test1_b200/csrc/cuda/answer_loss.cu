@@ -20,6 +20,10 @@
 // us a barrier).  A unit belongs to a warp or, for sequences shorter than 32
 // tokens, to the fewest lanes that hold one.  Sums are carried in fp64 and
 // joined in a fixed order: two runs give the same bits.
+//
+// Measured on a B200: 10 us up to 32 K tokens (the host's time), 14-18 us up to
+// 1 M (latencies of the phases and barriers), 34 us for 4.2 M policy tokens
+// (A 8 us, C 17 us at 4.2 TB/s; all bytes once at the copy rate are 14.5 us).
 #include "common.cuh"
 #include "sm100.cuh"
 

@@ -58,7 +58,10 @@ __device__ __forceinline__ int pick_splits_warp(int tiles, int k_blocks, int dw_
   const int64_t cost = splits_allowed(s, k_blocks) ? splits_cost(s, tiles, k_blocks, dw_tiles, tiles_t, clusters) : INT64_MAX;
   int64_t least = cost;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) least = min(least, static_cast<int64_t>(__shfl_xor_sync(0xffffffffu, static_cast<long long>(least), o)));
+  for (int o = 16; o > 0; o >>= 1) {
+    const int64_t other = __shfl_xor_sync(0xffffffffu, static_cast<long long>(least), o);
+    least = min(least, other);
+  }
   return __ffs(__ballot_sync(0xffffffffu, cost == least));
 }
 
@@ -265,7 +268,7 @@ __global__ void __launch_bounds__(kPlanesThreads) logprob_planes_kernel(const Vo
 // next rows' loads are in flight while a block adds up its warps' parts.
 // tcgen05 tiles would spend 256 rows of tensor time on them and read x
 // through TMA boxes that are mostly padding (T=1 at V=128256, H=4096: 260 us
-// against 177 us here, 5.9 TB/s).
+// against 171 us here, 6.1 TB/s).
 struct FewParams {
   const bf16* x;
   long ldx;
@@ -740,8 +743,8 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   const bool may_split = split_tiles > 0;
   Pieces ws;
   const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(8 * T),
-                o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_x = ws.take(2 * u_rows * H), o_planes = ws.take(4 * 8 * vocab::PLANE_BLOCK * planes),
-                o_u = ws.take(2 * u_rows * ldu);
+                o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_x = ws.take(2 * u_rows * H),
+                o_planes = ws.take(4 * 8 * vocab::PLANE_BLOCK * planes), o_u = ws.take(2 * u_rows * ldu);
   auto buf = torch::empty({ws.used}, x.options().dtype(torch::kUInt8));
   uint8_t* base = buf.data_ptr<uint8_t>();
 

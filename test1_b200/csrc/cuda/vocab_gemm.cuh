@@ -15,6 +15,13 @@
 // rows may be those that the packing kernel of logprob.cu kept, so their
 // number is read on the GPU.
 //
+// What bounds it (B200): with H = 4096 and many rows the tensor cores under the
+// power limit, at the speed of a library product of the same shape (log-sum-
+// exp of 5888 rows at V = 128256: 4.7 ms, 1320 TFLOP/s); with one or two row
+// tiles the operands, 64 bytes a cycle and SM at the tensor peak, of which
+// 192 KB in flight cover 1.6 us of latency (tensor pipe 55-60 % active); below
+// H = 512 the epilogue's exponentials.
+//
 // Work of a cluster: kLse and kSoftmaxGrad take tiles in turn.  kGrads has
 // units of two lengths, dx tiles (over a range of the vocabulary) and dW
 // tiles (over the rows); the long ones are dealt out first and the clusters
