@@ -261,8 +261,9 @@ __global__ void __launch_bounds__(kPlanesThreads) logprob_planes_kernel(const Vo
 
 // -------------------------------------------------------------- few rows
 // At most 16 tokens (a decoding step's, a short answer's): all that counts is
-// reading W once.  A block takes 16 rows of W at a time; its 16 warps share
-// the columns, read W straight into mma fragments (a thread's 16 bytes are
+// reading W once.  A group of warps takes 16 rows of W at a time and shares
+// their columns, as many warps as leave each about 256 columns (8 loads of 16
+// bytes per row in flight for a thread, 128 KB for an SM); they read W straight into mma fragments (a thread's 16 bytes are
 // the four k's that two m16n8k16 steps give it: the order of a sum is free, so
 // no shuffling and no shared memory for W) and keep x in shared memory.  The
 // next rows' loads are in flight while a block adds up its warps' parts.
@@ -277,6 +278,7 @@ struct FewParams {
   const int64_t* targets;
   int64_t ignore;
   int T, H, V;
+  int share;             // warps that share a group's columns, a power of two
   float scale;
   int* ticket;
   // forward
@@ -293,7 +295,7 @@ struct FewParams {
 
 constexpr int kFewThreads = 512;
 constexpr int kFewWarps = kFewThreads / 32;
-constexpr int kFewRows = 16;    // rows of W per step
+constexpr int kFewRows = 16;    // rows of W of a group
 constexpr int kFewLoads = 8;    // blocks of 32 columns that a warp has in flight
 
 // Distance of two tokens' columns in shared memory: 64 bytes past a multiple
@@ -324,7 +326,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 template <int NT, bool BWD>
 __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewParams p) {
   constexpr int TOK = 8 * NT;
-  constexpr int CELLS = kFewRows * TOK;  // a step's logits, one per thread of the first CELLS
+  constexpr int CELLS = kFewRows * TOK;  // a group's logits
   extern __shared__ __align__(16) uint8_t few_raw[];
   uint8_t* xs = few_raw;
   const int pitch = few_pitch(p.H);
@@ -335,16 +337,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   vocab::launch_dependents();
   vocab::wait_previous();
 
+  const int teams = kFewWarps / p.share, team = warp / p.share, part = warp % p.share;
   const int blocks32 = (p.H + 31) / 32;                       // of columns
-  const int kb_lo = warp * blocks32 / kFewWarps, kb_hi = (warp + 1) * blocks32 / kFewWarps;
-  const int per_warp = (blocks32 + kFewWarps - 1) / kFewWarps;
+  const int kb_lo = part * blocks32 / p.share, kb_hi = (part + 1) * blocks32 / p.share;
+  const int per_warp = (blocks32 + p.share - 1) / p.share;
   const int chunks = (per_warp + kFewLoads - 1) / kFewLoads;  // the same for every warp
-  const int groups = (p.V + kFewRows - 1) / kFewRows;
-  const int steps = (groups - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) * chunks;
+  const int rounds = (p.V + kFewRows * teams - 1) / (kFewRows * teams);  // of all blocks: a group per team
+  const int steps = (rounds - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) * chunks;
 
   uint4 wa[kFewLoads], wb[kFewLoads];
   auto load = [&](int step) {
-    const int group = blockIdx.x + step / chunks * gridDim.x;
+    const int group = (static_cast<int>(blockIdx.x) + step / chunks * static_cast<int>(gridDim.x)) * teams + team;
     const int ra = min(p.V - 1, group * kFewRows + g), rb = min(p.V - 1, group * kFewRows + g + 8);
     const bf16* pa = p.w + static_cast<size_t>(ra) * p.ldw;
     const bf16* pb = p.w + static_cast<size_t>(rb) * p.ldw;
@@ -366,9 +369,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
     if (t < p.T && 8 * v < p.H) val = *reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(t) * p.ldx + 8 * v);
     *reinterpret_cast<uint4*>(xs + t * pitch + 16 * v) = val;
   }
-  // what this thread's cell (row of the step, token) needs to know
-  const int token = tid % TOK, wrow = tid / TOK;
-  const bool cell = tid < CELLS && token < p.T;
+  // what this thread's cells need to know: all are of one token
+  const int token = tid % TOK;
+  const bool cell = tid < CELLS * teams && token < p.T;
   const int64_t target = cell ? p.targets[token] : -1;
   const bool valid = cell && target != p.ignore && target >= 0 && target < p.V;
   const float k2 = p.scale * kLog2e;
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
     lse2 = p.lse[token] * kLog2e;
     gr = p.dlogp[token] * p.scale;
   }
-  if (BWD && blockIdx.x == 0 && cell && wrow == 0) p.g[token] = gr;
+  if (BWD && blockIdx.x == 0 && cell && tid < TOK) p.g[token] = gr;
   __syncthreads();
   if (BWD) {  // a share of x per block
     const int nvec = p.H / 8;
@@ -418,11 +421,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
       for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
     }
     __syncthreads();  // two buffers: the next step's parts go to the other
-    const int v = (static_cast<int>(blockIdx.x) + step / chunks * static_cast<int>(gridDim.x)) * kFewRows + wrow;
-    if (cell && v < p.V) {
+    const int round = static_cast<int>(blockIdx.x) + step / chunks * static_cast<int>(gridDim.x);
+    for (int i = tid; cell && i < CELLS * teams; i += kFewThreads) {
+      const int of = i / CELLS, at = i % CELLS;
+      const int v = (round * teams + of) * kFewRows + at / TOK;
+      if (v >= p.V) continue;
       float l = 0.f;
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) l += red[(buf * kFewWarps + w) * CELLS + tid];
+      for (int w = 0; w < p.share; ++w) l += red[(buf * kFewWarps + of * p.share + w) * CELLS + at];
       if (BWD) {
         const float uv = gr != 0.f ? gr * ((v == target ? 1.f : 0.f) - ex2(fmaf(l, k2, -lse2))) : 0.f;
         p.u[token * p.ldu + v] = __float2bfloat16_rn(uv);
@@ -438,10 +443,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   // this block's (largest, sum) per token, then all blocks' by the last one
   float2* cells = reinterpret_cast<float2*>(red);
   __syncthreads();
-  if (tid < CELLS) cells[tid] = make_float2(m, s);
+  cells[tid] = make_float2(m, s);
   __syncthreads();
   if (tid < TOK) {
-    for (int r = 1; r < kFewRows; ++r) vocab::lse_join(m, s, cells[r * TOK + tid].x, cells[r * TOK + tid].y, k2);
+    for (int r = 1; r < min(kFewThreads, CELLS * teams) / TOK; ++r)
+      vocab::lse_join(m, s, cells[r * TOK + tid].x, cells[r * TOK + tid].y, k2);
     __stcg(&p.part[blockIdx.x * 16 + tid], make_float2(m, s));
   }
   __threadfence();
@@ -574,7 +580,15 @@ static void launch_pack(PackParams& p) {
 constexpr size_t kFewSmem = 200 * 1024;
 static bool few_rows(int64_t T, int64_t H) { return T <= 16 && few_smem(T <= 8 ? 8 : 16, H) <= kFewSmem; }
 
-static int few_grid(int64_t V) { return static_cast<int>(std::min<int64_t>(ceil_div(V, kFewRows), num_sms())); }
+static int few_share(int64_t H) {
+  int share = 1;
+  while (share < kFewWarps && share * kFewLoads * 32 < H) share *= 2;
+  return share;
+}
+
+static int few_grid(int64_t V, int64_t H) {
+  return static_cast<int>(std::min<int64_t>(ceil_div(V, kFewRows * (kFewWarps / few_share(H))), num_sms()));
+}
 
 static FewParams few_params(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets, int64_t ignore,
                             double temperature) {
@@ -588,6 +602,7 @@ static FewParams few_params(const torch::Tensor& x, const torch::Tensor& w, cons
   p.T = x.size(0);
   p.H = x.size(1);
   p.V = w.size(0);
+  p.share = few_share(p.H);
   p.scale = static_cast<float>(1.0 / temperature);
   return p;
 }
@@ -601,7 +616,7 @@ static void launch_few(const FewParams& p) {
     T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     configured[tokens8 / 8 - 1] = true;
   }
-  launch_after("logprob_few", kern, dim3(few_grid(p.V)), kFewThreads, few_smem(tokens8, p.H), p);
+  launch_after("logprob_few", kern, dim3(few_grid(p.V, p.H)), kFewThreads, few_smem(tokens8, p.H), p);
 }
 
 // Whether the forward packs its rows first.  Below 256 tokens there is one
@@ -627,9 +642,9 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   auto tg = targets.contiguous();
   if (few_rows(T, H)) {
     FewParams p = few_params(x, w, tg, ignore_index, temperature);
-    auto ws = torch::empty({32 * few_grid(V) + 16}, f32);
+    auto ws = torch::empty({32 * few_grid(V, H) + 16}, f32);
     p.part = reinterpret_cast<float2*>(ws.data_ptr<float>());
-    p.target_logit = ws.data_ptr<float>() + 32 * few_grid(V);
+    p.target_logit = ws.data_ptr<float>() + 32 * few_grid(V, H);
     const torch::Tensor counters = arrival_counters(1);
     p.ticket = counters.data_ptr<int>();
     p.logp = logp.data_ptr<float>();

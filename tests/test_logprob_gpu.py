@@ -18,7 +18,8 @@ pytestmark = pytest.mark.gpu
 SIZES = [(1, 64, 257), (2, 8, 5), (1, 256, 1), (33, 72, 255), (129, 264, 1000), (300, 520, 4097),
          (513, 256, 20011), (700, 1024, 2048), (257, 2048, 520),
          # few tokens: one or two column blocks of 8, x that fits in shared memory or not
-         (8, 1032, 5003), (9, 4096, 777), (16, 2056, 1500), (5, 8192, 600), (16, 8192, 300), (17, 4096, 300)]
+         (8, 1032, 5003), (9, 4096, 777), (16, 2056, 1500), (5, 8192, 600), (16, 8192, 300), (17, 4096, 300),
+         (3, 512, 40009), (16, 520, 4001)]
 GRAD_TOL = 4 * 2.0 ** -9
 
 
