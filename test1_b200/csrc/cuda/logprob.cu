@@ -9,7 +9,10 @@
 //
 // u is the one intermediate that is rounded: to bf16, for the tensor cores.
 // Its relative error of 2^-9 at most per element adds to the 2^-9 of the
-// results' own rounding; all sums are fp32.
+// results' own rounding; all sums are fp32.  Before that rounding u is as good
+// as its formula in fp32: 1 - exp(logit - lse) of a target that is nearly sure
+// is off by what fp32 holds of lse (2^-24 of it), which logits summed in the
+// forward's order do not add to.
 //
 // A token whose target is ignored (ignore_index, or outside the vocabulary)
 // gives logp = lse = 0 and no gradient, whatever its hidden state holds.
@@ -375,9 +378,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   const int64_t target = cell ? p.targets[token] : -1;
   const bool valid = cell && target != p.ignore && target >= 0 && target < p.V;
   const float k2 = p.scale * kLog2e;
-  float lse2 = 0.f, gr = 0.f;
+  float lse = 0.f, gr = 0.f;
   if (BWD && valid) {
-    lse2 = p.lse[token] * kLog2e;
+    lse = p.lse[token];
     gr = p.dlogp[token] * p.scale;
   }
   if (BWD && blockIdx.x == 0 && cell && tid < TOK) p.g[token] = gr;
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
       float l = 0.f;
       for (int w = 0; w < p.share; ++w) l += red[(buf * kFewWarps + of * p.share + w) * CELLS + at];
       if (BWD) {
-        const float uv = gr != 0.f ? gr * ((v == target ? 1.f : 0.f) - ex2(fmaf(l, k2, -lse2))) : 0.f;
+        const float uv = gr != 0.f ? gr * ((v == target ? 1.f : 0.f) - ex2(fmaf(l, p.scale, -lse) * kLog2e)) : 0.f;
         p.u[token * p.ldu + v] = __float2bfloat16_rn(uv);
       } else {
         vocab::lse_join(m, s, l, 1.f, k2);

@@ -102,10 +102,13 @@ __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.w
 
 // The tensor cores drop what falls below the accumulator's last bit at every
 // step, which adds up: over 4096 products the logits lose 2e-6 of their size.
-// kLse, whose results are fp32, therefore starts a new accumulator after about
-// 16 k blocks (1024 products), in equal parts of k, and adds them up in
-// registers, rounded: 4e-7, for 4 % more time at H = 4096.
-constexpr int kLseBlocks = 16;
+// The logits are therefore summed from accumulators of about 16 k blocks each
+// (equal parts of k, 1472 products at most), added up in registers, rounded:
+// 4e-7 at H = 4096, for 4 % more time.  kSoftmaxGrad sums them in the same
+// order as kLse: where a target is nearly sure, u is what exp(logit - lse)
+// leaves of 1, and an error of the logit that lse does not share is all of u
+// (one accumulator there put dx rows of targets with p = 0.999 off by a half).
+constexpr int kLogitBlocks = 16;
 
 // Running (largest m, sum s of exp((v - m) / tau)); k2 = log2(e) / tau.
 __device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2, float k2) {
@@ -137,7 +140,7 @@ __host__ __device__ inline int dw_unit_cost(int tiles_t) {
 
 struct Shape {
   int rows, tiles_t, tiles_n, tiles_h, k_h, k_n, k_rows, splits;
-  int k_acc;  // kLse: k blocks of an accumulator
+  int k_acc;  // k blocks of a logit's accumulator
 };
 
 __device__ __forceinline__ Shape shape_of(const VocabParams& p, bool splits) {
@@ -150,7 +153,7 @@ __device__ __forceinline__ Shape shape_of(const VocabParams& p, bool splits) {
   e.k_h = (p.H + BK - 1) / BK;
   e.k_n = (p.N + BK - 1) / BK;
   e.k_rows = (e.rows + BK - 1) / BK;
-  const int accs = max(1, (e.k_h + kLseBlocks / 2) / kLseBlocks);
+  const int accs = max(1, (e.k_h + kLogitBlocks / 2) / kLogitBlocks);
   e.k_acc = (e.k_h + accs - 1) / accs;
   return e;
 }
@@ -326,7 +329,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * TILE;
-          const int first = kb, end = JOB == kLse ? min(u.kb1, kb + e.k_acc) : u.kb1;
+          const int first = kb, end = JOB == kGrads ? u.kb1 : min(u.kb1, kb + e.k_acc);
           for (; kb < end; ++kb) {
             if (!mbar_wait(&full[stage], phase)) {
               err.set(123);
@@ -398,15 +401,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
       const int tcol0 = u.nb * TILE;  // first column of the tile
       int acc;
 
-      if (JOB == kLse) {
-        // 128 columns of the row, the sum of the tile's accumulators
-        float v[HALF];
+      // logits of 128 columns of the row, the sum of the tile's accumulators
+      auto take_logits = [&](float (&v)[HALF]) {
+        if (!take(acc)) return false;
+        uint32_t first[HALF / 32][32];
 #pragma unroll
-        for (int j = 0; j < HALF; ++j) v[j] = 0.f;
-        bool ok = true;
-        for (int kb = u.kb0; kb < u.kb1; kb += e.k_acc) {
-          ok = take(acc);
-          if (!ok) break;
+        for (int c = 0; c < HALF; c += 32) tmem_ld_32x32b_x32(quarter + acc * TILE + half * HALF + c, first[c / 32]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) v[j] = __uint_as_float(first[j / 32][j % 32]);
+        release(acc);
+        for (int kb = u.kb0 + e.k_acc; kb < u.kb1; kb += e.k_acc) {
+          if (!take(acc)) return false;
 #pragma unroll
           for (int c = 0; c < HALF; c += 32) {
             uint32_t r[32];
@@ -417,7 +423,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
           }
           release(acc);
         }
-        if (!ok) break;
+        return true;
+      };
+
+      if (JOB == kLse) {
+        float v[HALF];
+        if (!take_logits(v)) break;
         // (largest, sum) in the accumulator's own units: (logit - largest) is
         // exact near the largest, which is where the sum comes from
         const bool row_ok = row < e.rows;
@@ -469,9 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         continue;
       }
 
-      if (!take(acc)) break;
       const int col0 = tcol0 + half * HALF;  // this warp's first column
-      const uint32_t taddr = quarter + acc * TILE + half * HALF;
       uint8_t* rowp = slab + lane * 128;
       // 32 columns of the row, rounded, to the slab's left or right half
       auto to_slab = [&](const float (&f)[32], int right, bool zero) {
@@ -486,7 +495,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         }
       };
 
-      if (JOB == kGrads && u.split >= 0) {
+      // a 32 x 64 slab to the columns c.. of the result, by TMA
+      auto store_slab = [&](int c) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tma_c, slab, col0 + c, row0);
+          bulk_commit_group();
+        }
+      };
+
+      if (JOB == kSoftmaxGrad) {
+        // u, zeros in the rows past the last that complete kGrads' last block
+        // of BK rows (a reduction's length there)
+        float v[HALF];
+        if (!take_logits(v)) break;
+        if (row0 >= e.k_rows * BK) continue;  // uniform over the warp
+        const bool row_ok = row < e.rows;
+        float lse = 0.f, gr = 0.f;
+        int tcol = -1;
+        if (row_ok) {
+          gr = p.g[row];
+          lse = p.lse[row];
+          const int64_t t = p.targets[row] - p.col0 - col0;
+          tcol = t >= 0 && t < HALF ? static_cast<int>(t) : -1;
+        }
+#pragma unroll
+        for (int c = 0; c < HALF; c += 64) {
+          if (col0 + c >= p.N) break;
+          // the store issued from the slab before has read it
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int right = 0; right < 2; ++right) {
+            float f[32];
+            // logit - lse is rounded once, near 0 where the target is sure
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = -gr * ex2(fmaf(v[c + 32 * right + j], p.scale, -lse) * kLog2e);
+            if (__any_sync(0xffffffffu, tcol >= c + 32 * right && tcol < c + 32 * right + 32)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] += tcol == c + 32 * right + j ? gr : 0.f;
+            }
+            to_slab(f, right, !row_ok);
+          }
+          store_slab(c);
+        }
+        continue;
+      }
+
+      if (!take(acc)) break;
+      const uint32_t taddr = quarter + acc * TILE + half * HALF;
+      if (u.split >= 0) {
         // dx: these columns' sums, in fp32 until all of the vocabulary is in
         const bool live = row0 < e.rows;
         const size_t block = (static_cast<size_t>(u.mb * e.tiles_h + u.nb) * e.splits + u.split) * 8 + w8;
@@ -540,23 +599,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         continue;
       }
 
-      // bf16 results (u, dW) through 32 x 64 slabs
-      const bool row_ok = row < e.rows;
-      const int width = JOB == kSoftmaxGrad ? p.N : p.H;
-      // u's rows are a reduction's length in kGrads: its last block of BK has
-      // to be there, with zeros past the last row
-      const int m_end = JOB == kSoftmaxGrad ? e.k_rows * BK : p.N;
-      float lse2 = 0.f, gr = 0.f;
-      int tcol = -1;
-      if (JOB == kSoftmaxGrad && row_ok) {
-        gr = p.g[row];
-        lse2 = p.lse[row] * kLog2e;
-        const int64_t t = p.targets[row] - p.col0 - col0;
-        tcol = t >= 0 && t < HALF ? static_cast<int>(t) : -1;
-      }
+      // dW through 32 x 64 slabs
 #pragma unroll 1
       for (int c = 0; c < HALF; c += 64) {
-        const bool live = col0 + c < width && row0 < m_end;  // uniform over the warp
         uint32_t r[2][32];
         tmem_ld_32x32b_x32(taddr + c, r[0]);
         tmem_ld_32x32b_x32(taddr + c + 32, r[1]);
@@ -565,28 +610,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         __syncwarp();
         tmem_ld_wait();
         if (c + 64 == HALF) release(acc);
-        if (!live) continue;
+        if (col0 + c >= p.H || row0 >= p.N) continue;  // uniform over the warp
 #pragma unroll
         for (int right = 0; right < 2; ++right) {
           float f[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            f[j] = __uint_as_float(r[right][j]);
-            if (JOB == kSoftmaxGrad) f[j] = -gr * ex2(fmaf(f[j], k2, -lse2));
-          }
-          if (JOB == kSoftmaxGrad && __any_sync(0xffffffffu, tcol >= c + 32 * right && tcol < c + 32 * right + 32)) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] += tcol == c + 32 * right + j ? gr : 0.f;
-          }
-          // rows past the last, and sums over no rows, are 0
-          to_slab(f, right, JOB == kSoftmaxGrad ? !row_ok : u.kb0 == u.kb1);
+          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[right][j]);
+          to_slab(f, right, u.kb0 == u.kb1);  // a sum over no rows is 0
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&tma_c, slab, col0 + c, row0);
-          bulk_commit_group();
-        }
+        store_slab(c);
       }
     }
     // every store of this warp completed before the CTA may exit
