@@ -24,17 +24,18 @@
 // Measured on a B200: 10 us up to 32 K tokens (the host's time), 14-18 us up to
 // 1 M (latencies of the phases and barriers), 34 us for 4.2 M policy tokens
 // (A 8 us, C 17 us at 4.2 TB/s; all bytes once at the copy rate are 14.5 us).
+#include "arrivals.cuh"
 #include "common.cuh"
 #include "sm100.cuh"
 
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 
+#include <optional>
 #include <string>
 #include <unordered_map>
 
 namespace t1 {
 
-torch::Tensor arrival_counters(int64_t n);
 torch::Tensor& gemm_error_word();
 
 enum PreferenceKind : int { kSigmoid = 0, kHinge = 1, kIpo = 2 };
@@ -49,7 +50,7 @@ struct LossParams {
   int lanes;               // lanes of a unit: 32, or the power of two >= S
   int vectors;             // 16-byte vectors of tokens
   int lengths_phase;       // policy: phase B takes place
-  int* arrivals;           // the grid barrier's counter, zero between launches; null: the blocks are one cluster
+  Arrivals arrivals;       // the grid barrier's counter; none: the blocks are one cluster
   int* err;
   uint8_t* answer;         // [T] phase A's finding, an eighth of the targets to read again
   double2* units;          // [B * chunks] (sum of log ratios, answer tokens)
@@ -436,19 +437,19 @@ __device__ __forceinline__ void policy_total_phase(const LossParams& p, Sums* re
 __device__ __forceinline__ bool grid_barrier(const LossParams& p, int nth) {
   __shared__ int ok;
   __syncthreads();
-  if (p.arrivals == nullptr) {
+  if (p.arrivals.use == nullptr) {
     if (gridDim.x > 1) sm100::cluster_sync();
     return true;
   }
   if (threadIdx.x == 0) {
     const int all = nth * static_cast<int>(gridDim.x);
     __threadfence();
-    atomicAdd(p.arrivals, 1);
+    atomicAdd(p.arrivals.use, 1);
     ok = 1;
     const uint64_t t0 = sm100::globaltimer_ns();
     int v, n = 0;
     while (true) {
-      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.arrivals) : "memory");
+      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.arrivals.use) : "memory");
       if (v >= all) break;
       if ((++n & 255) == 0 && sm100::globaltimer_ns() - t0 > sm100::kWaitLimitNs) {
         sm100::ErrorSlot{p.err}.set(131);
@@ -468,6 +469,7 @@ __global__ void __launch_bounds__(kLossThreads, kLossPerSm) answer_loss_kernel(c
   __shared__ int last;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  clear_arrivals(p.arrivals);
   int barriers = 0;
   count_phase<POLICY>(p, red);
   if (!grid_barrier(p, ++barriers)) return;
@@ -478,18 +480,18 @@ __global__ void __launch_bounds__(kLossThreads, kLossPerSm) answer_loss_kernel(c
   }
   if (POLICY) policy_grad_phase(p, red);
   else preference_grad_phase(p, red);
-  if (p.arrivals == nullptr) {
-    if (!POLICY || !grid_barrier(p, ++barriers) || blockIdx.x != 0) return;
-  } else {  // the last block to arrive clears the counter
+  if (!POLICY) return;
+  if (p.arrivals.use == nullptr) {
+    if (!grid_barrier(p, ++barriers) || blockIdx.x != 0) return;
+  } else {  // the last block to arrive
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(p.arrivals, 1) == (barriers + 1) * static_cast<int>(gridDim.x) - 1;
+    if (threadIdx.x == 0) last = atomicAdd(p.arrivals.use, 1) == (barriers + 1) * static_cast<int>(gridDim.x) - 1;
     __syncthreads();
     if (!last) return;
     __threadfence();
-    if (threadIdx.x == 0) *p.arrivals = 0;
   }
-  if (POLICY) policy_total_phase(p, red);
+  policy_total_phase(p, red);
 }
 
 // ================================================================ host side
@@ -581,7 +583,7 @@ static void launch_loss(LossParams& p, const LossPlan& plan) {
               aligned(p.ref) && (!p.adv_per_token || aligned(p.adv));
   p.lengths_phase = POLICY && p.per_sequence && plan.chunks > 1;
   p.err = gemm_error_word().data_ptr<int>();
-  torch::Tensor arrivals;
+  std::optional<ArrivalCounters> counters;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(plan.blocks);
   cfg.blockDim = dim3(kLossThreads);
@@ -596,14 +598,15 @@ static void launch_loss(LossParams& p, const LossPlan& plan) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   } else {  // blocks that wait for one another
-    arrivals = arrival_counters(1);
-    p.arrivals = arrivals.data_ptr<int>();
+    counters.emplace(1);
+    p.arrivals = counters->arrivals;
     attr[0].id = cudaLaunchAttributeCooperative;
     attr[0].val.cooperative = 1;
     cfg.numAttrs = 1;
   }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, answer_loss_kernel<POLICY>, static_cast<LossParams>(p));
   TORCH_CHECK(e == cudaSuccess, "answer_loss launch failed: ", cudaGetErrorString(e));
+  if (counters) counters->launched();
   count_launch();
 }
 

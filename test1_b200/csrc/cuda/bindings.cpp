@@ -30,6 +30,7 @@ std::vector<torch::Tensor> cross_entropy_fwd_bwd(torch::Tensor logits, torch::Te
                                                  int64_t ignore_index, double grad_scale);
 std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets,
                                               int64_t ignore_index, double temperature);
+void fill_last_arrivals(int64_t value);
 void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, torch::Tensor targets,
                         torch::Tensor lse, torch::Tensor dx, torch::Tensor dw, int64_t ignore_index,
                         double temperature);
@@ -154,6 +155,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_logprob_fwd", &t1::linear_logprob_fwd,
         "log-probabilities of the targets under the output layer: (logp [T], lse [T])");
   m.def("linear_logprob_bwd", &t1::linear_logprob_bwd, "gradients of linear_logprob_fwd: writes dx and dW");
+  m.def("fill_last_arrivals", &t1::fill_last_arrivals,
+        "leaves the arrival counters as an expired wait does (for tests of what follows one)");
   m.def("preference_loss", &t1::preference_loss, "paired log-ratio loss: (loss, dlogp [T], rewards [B])");
   m.def("policy_loss", &t1::policy_loss, "clipped policy loss with a KL term: (loss, dlogp [T], stats [2])");
   m.def("gemm_bf16", &t1::gemm_bf16, pybind11::arg("A"), pybind11::arg("B"), pybind11::arg("C"),

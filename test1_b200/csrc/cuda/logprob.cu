@@ -20,6 +20,7 @@
 
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 
+#include <optional>
 #include <unordered_map>
 
 namespace t1 {
@@ -283,8 +284,8 @@ struct FewParams {
   int T, H, V;
   int share;             // warps that share a group's columns, a power of two
   float scale;
-  int* ticket;
   // forward
+  Arrivals ticket;       // of the blocks
   float2* part;          // [block][16]
   float* target_logit;   // [16]
   float *logp, *lse_out;
@@ -339,6 +340,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   const int g = lane >> 2, c = lane & 3;
   vocab::launch_dependents();
   vocab::wait_previous();
+  if (!BWD) clear_arrivals(p.ticket);
 
   const int teams = kFewWarps / p.share, team = warp / p.share, part = warp % p.share;
   const int blocks32 = (p.H + 31) / 32;                       // of columns
@@ -455,11 +457,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   }
   __threadfence();
   __syncthreads();
-  if (tid == 0) last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+  if (tid == 0) last = atomicAdd(p.ticket.use, 1) == static_cast<int>(gridDim.x) - 1;
   __syncthreads();
   if (!last) return;
   __threadfence();
-  if (tid == 0) *p.ticket = 0;
   if (warp >= p.T) return;  // a warp per token
   m = -INFINITY;
   s = 0.f;
@@ -519,18 +520,41 @@ static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
   launch_after("linear_logprob", kern, dim3(2 * clusters), vocab::V_THREADS, vocab::V_SMEM_BYTES, ta, tb, ta2, tb2, tc, p);
 }
 
-// Arrival counters, zero between launches (whoever arrives last clears its
-// counter); one set per (device, stream), so that concurrent calls never
-// share one.  A captured graph has a set of its own, for the same reason.
-torch::Tensor arrival_counters(int64_t n) {
-  static std::unordered_map<uint64_t, torch::Tensor> all;
+static torch::TensorOptions counter_options() {
   int dev = 0;
   cudaGetDevice(&dev);
-  const auto opts = torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, dev);
-  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return torch::zeros({n}, opts);
-  torch::Tensor& t = all[(static_cast<uint64_t>(dev) << 56) ^ reinterpret_cast<uint64_t>(stream())];
-  if (!t.defined() || t.numel() < n) t = torch::zeros({std::max<int64_t>(4096, n)}, opts);
-  return t;
+  return torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, dev);
+}
+
+// The current stream's.
+static ArrivalSets& arrival_sets() {
+  static std::unordered_map<uint64_t, ArrivalSets> all;
+  return all[(static_cast<uint64_t>(counter_options().device().index()) << 56) ^ reinterpret_cast<uint64_t>(stream())];
+}
+
+ArrivalCounters::ArrivalCounters(int64_t n) : n_(n) {
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
+    held_ = torch::zeros({n}, counter_options());
+    arrivals.use = held_.data_ptr<int>();
+    return;
+  }
+  ArrivalSets& s = arrival_sets();
+  if (s.capacity < n) {
+    s.capacity = std::max<int64_t>(4096, n);
+    s.counters = torch::zeros({2 * s.capacity}, counter_options());
+    s.used = 0;
+  }
+  arrivals.use = s.counters.data_ptr<int>() + s.next * s.capacity;
+  arrivals.clear = s.counters.data_ptr<int>() + (1 - s.next) * s.capacity;
+  arrivals.clear_n = static_cast<int>(s.used);
+  sets_ = &s;
+}
+
+// Leaves the counters of the current stream's last launch at `value`, as a
+// launch whose wait expired does.
+void fill_last_arrivals(int64_t value) {
+  ArrivalSets& s = arrival_sets();
+  if (s.used > 0) s.counters.narrow(0, (1 - s.next) * s.capacity, s.used).fill_(value);
 }
 
 // A workspace cut into 256-byte aligned pieces.
@@ -648,11 +672,12 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
     auto ws = torch::empty({32 * few_grid(V, H) + 16}, f32);
     p.part = reinterpret_cast<float2*>(ws.data_ptr<float>());
     p.target_logit = ws.data_ptr<float>() + 32 * few_grid(V, H);
-    const torch::Tensor counters = arrival_counters(1);
-    p.ticket = counters.data_ptr<int>();
+    ArrivalCounters counters(1);
+    p.ticket = counters.arrivals;
     p.logp = logp.data_ptr<float>();
     p.lse_out = lse.data_ptr<float>();
     launch_few<false>(p);
+    counters.launched();
     return {logp, lse};
   }
   const int64_t blocks = ceil_div(V, vocab::TILE), tiles_t = ceil_div(T, vocab::TILE);
@@ -678,10 +703,10 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   p.logp = logp.data_ptr<float>();
   p.lse_out = lse.data_ptr<float>();
   p.join = blocks <= kJoinBlocks;
-  torch::Tensor counters;
+  std::optional<ArrivalCounters> counters;
   if (p.join) {
-    counters = arrival_counters(tiles_t * 8);
-    p.tickets = counters.data_ptr<int>();
+    counters.emplace(tiles_t * 8);
+    p.tickets = counters->arrivals;
   }
   if (pack) {
     PackParams k{};
@@ -706,7 +731,8 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   CUtensorMap ta = make_map_any(pack ? base + o_x : x.data_ptr(), H, T, pack ? H : row_ld(x), vocab::HALF);
   CUtensorMap tb = make_map_any(w.data_ptr(), H, V, row_ld(w), vocab::HALF);
   launch_vocab<vocab::kLse>(ta, tb, ta, tb, ta, p, tiles_t * blocks);
-  if (!p.join) launch_after("logprob_join", logprob_join_kernel, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, 2 * blocks);
+  if (p.join) counters->launched();
+  else launch_after("logprob_join", logprob_join_kernel, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, 2 * blocks);
   return {logp, lse};
 }
 

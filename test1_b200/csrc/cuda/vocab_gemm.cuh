@@ -28,6 +28,7 @@
 // that got one less take short ones meanwhile (grad_unit).
 #pragma once
 
+#include "arrivals.cuh"
 #include "gemm_core.cuh"
 
 namespace t1 {
@@ -69,7 +70,7 @@ struct VocabParams {
   int col0;                // vocabulary index of column 0
   const int* index;        // [rows] token of a packed row; null: the row itself
   const int64_t* targets;  // [rows] vocabulary index
-  int* tickets;            // kLse: arrivals per 32 rows, zero between launches
+  Arrivals tickets;        // kLse with join: arrivals per 32 rows
   // kLse
   int64_t ignore, V;
   int ld_part;
@@ -263,6 +264,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   wait_previous();
+  if (JOB == kLse) clear_arrivals(p.tickets);
   const Shape e = shape_of(p, JOB == kGrads);
   Unit u;
 
@@ -461,10 +463,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         __threadfence();
         __syncwarp();
         int last = 0;
-        if (lane == 0) last = atomicAdd(&p.tickets[u.mb * 8 + w8], 1) == 2 * e.tiles_n - 1;
+        if (lane == 0) last = atomicAdd(&p.tickets.use[u.mb * 8 + w8], 1) == 2 * e.tiles_n - 1;
         if (!__shfl_sync(0xffffffffu, last, 0)) continue;
         __threadfence();
-        if (lane == 0) p.tickets[u.mb * 8 + w8] = 0;
         if (!row_ok) continue;
         m = -INFINITY;
         s = 0.f;
