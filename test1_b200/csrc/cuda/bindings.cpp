@@ -43,6 +43,7 @@ std::vector<torch::Tensor> policy_loss(torch::Tensor logp, torch::Tensor old, c1
 void gemm_bf16(torch::Tensor A, torch::Tensor B, torch::Tensor C, bool a_mn, bool b_mn,
                c10::optional<torch::Tensor> R);
 int64_t gemm_check_error(bool reset);
+torch::Tensor& gemm_error_word();
 void gemm_set_mode(int64_t mode);
 void gemm_set_streamk(bool on);
 void fused_set_peer_wait(double seconds);
@@ -161,6 +162,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("policy_loss", &t1::policy_loss, "clipped policy loss with a KL term: (loss, dlogp [T], stats [2])");
   m.def("gemm_bf16", &t1::gemm_bf16, pybind11::arg("A"), pybind11::arg("B"), pybind11::arg("C"),
         pybind11::arg("a_mn"), pybind11::arg("b_mn"), pybind11::arg("R") = pybind11::none());
+  m.def("gemm_error_word", [] { return t1::gemm_error_word(); },
+        "the current device's error word [1] of this thread's launches");
   m.def("gemm_check_error", &t1::gemm_check_error, pybind11::arg("reset") = false);
   m.def("gemm_set_mode", &t1::gemm_set_mode, "0: single-CTA tiles, 1: CTA-pair (cta_group::2) tiles");
   m.def("fused_set_peer_wait", &t1::fused_set_peer_wait,

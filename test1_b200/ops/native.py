@@ -124,6 +124,12 @@ def gemm_error(reset: bool = False) -> int:
     return int(_c().gemm_check_error(reset))
 
 
+def error_word() -> torch.Tensor:
+    """The device word that a kernel whose bounded wait expired writes its code
+    to (0: none did)."""
+    return _c().gemm_error_word()
+
+
 # --------------------------------------------------------------------- RoPE
 def rope_qkv_(qkv, n_q, n_kv, head_dim, cos, sin, seq_len, inverse=False):
     _c().rope_qkv(qkv, n_q, n_kv, head_dim, cos, sin, seq_len, inverse)

@@ -167,6 +167,8 @@ class SlideFSDP(nn.Module):
         self.rank = dist.get_rank() if dist.is_initialized() else 0
         self.world_size = dist.get_world_size() if dist.is_initialized() else 1
         self.is_cuda = self.device.type == "cuda"
+        self._kernel_error = torch.zeros(1, dtype=torch.int32, pin_memory=self.is_cuda)
+        self._kernel_error_read: Optional[Event] = None
         local_ranks = int(os.environ.get("LOCAL_WORLD_SIZE", str(self.world_size)) or self.world_size)
         if self.world_size > 1 and local_ranks < self.world_size:
             # the master weights and the update counters live in one node's
@@ -915,12 +917,34 @@ class SlideFSDP(nn.Module):
                                        f"(it stalled or died); rank {self.rank} stops before the step")
                 host.counter_wait_geq(self.counters, base + r, step, 0.05)
 
+    def _read_kernel_errors(self, objective=None) -> None:
+        """Bring the kernels' error word to the host behind the work launched
+        so far; ``_check_kernels`` looks at it once it is there."""
+        if self.is_cuda and (not self.generic or objective is not None):
+            from .ops import native
+
+            self._kernel_error.copy_(native.error_word(), non_blocking=True)
+            self._kernel_error_read = Event(self.device).record()
+
+    def _check_kernels(self, wait: bool = False) -> None:
+        """Raise if a kernel of an earlier step or forward pass gave up a
+        bounded wait: its results, and all that came of them, are unfinished."""
+        if self._kernel_error_read is None:
+            return
+        if wait:
+            self._kernel_error_read.synchronize()
+        code = int(self._kernel_error[0])
+        if code:
+            raise RuntimeError(f"a kernel's bounded wait expired (error {code}): the results of the last step or "
+                               f"forward pass, and the weights updated with them, are not to be used")
+
     @torch.no_grad()
     def _train_step(self, input_ids: torch.Tensor, labels: torch.Tensor,
                     objective: Optional[ObjectiveStep] = None) -> torch.Tensor:
         cfg = self.model_config
         dev = self.device
         step = self.completed_steps + 1
+        self._check_kernels()
         self._enter_step(step)
         if self.cpu_slots is not None:
             self.cpu_slots.step = step
@@ -1032,6 +1056,7 @@ class SlideFSDP(nn.Module):
         self._offload_grads(emb, step)
         if self._exact_clip:
             self._apply_exact_clip()
+        self._read_kernel_errors(objective)
         self.acts.clear()
         self.completed_steps = step
         if self.tracer.enabled:
@@ -1063,6 +1088,7 @@ class SlideFSDP(nn.Module):
                    temperature: float = 1.0) -> torch.Tensor:
         """Forward only; returns logits [B, S, V], or with labels their
         log-probabilities [B, S]."""
+        self._check_kernels()
         ctx = self._make_context(input_ids, labels)
         S = self.layer_states
         L = self.num_decoder_layers
@@ -1083,18 +1109,21 @@ class SlideFSDP(nn.Module):
             else:
                 h = st.module.logprobs(h, ctx.targets, temperature)
             self._release(st, Event(self.device).record())
+        self._read_kernel_errors()
         B, T = input_ids.shape
         return h.view(B, T, -1) if labels is None else h.view(B, T)
 
     # ------------------------------------------------------------ control
     def wait_for_updates(self) -> None:
-        """Block until every scheduled optimizer update (all ranks) landed."""
+        """Block until every scheduled optimizer update (all ranks) landed.
+        Raises if a kernel gave up a wait meanwhile."""
         self.comm.check()
         if self._reducer is not None:
             self._reducer.drain()
         self.updates.drain()
         for st in self.layer_states:
             self.updates.wait_counter(st.idx, self._update_target(st))
+        self._check_kernels(wait=True)
 
     def update_learning_rate(self, new_lr: float) -> None:
         """Rate for the steps that start from now on.  Updates of earlier
