@@ -22,7 +22,7 @@ import torch
 from . import ops
 
 
-def _check_temperature(temperature: float) -> None:
+def check_temperature(temperature: float) -> None:
     if not 0 < temperature < float("inf"):
         raise ValueError(f"temperature must be positive, got {temperature}")
 
@@ -43,7 +43,7 @@ class PreferenceObjective:
 
     def __post_init__(self):
         ops.check_preference(self.beta, self.kind, self.label_smoothing)
-        _check_temperature(self.temperature)
+        check_temperature(self.temperature)
 
     def check(self, inputs, batch: int) -> None:
         if batch % 2:
@@ -71,7 +71,7 @@ class PolicyObjective:
 
     def __post_init__(self):
         ops.check_policy(self.clip_low, self.clip_high, self.kl_coef, self.reduction)
-        _check_temperature(self.temperature)
+        check_temperature(self.temperature)
 
     def check(self, inputs, batch: int) -> None:
         needed = ["old_logps", "advantages"] + (["ref_logps"] if self.kl_coef else [])

@@ -54,7 +54,7 @@ from .models import generic
 from .models.llama import LlamaConfig, LlamaDecoderLayer, LlamaForCausalLM, make_context
 from .optim.layer_adam import LayerAdam
 from .parallel.comm import CpuReduceSlots, make_comm
-from .objectives import ObjectiveStep
+from .objectives import ObjectiveStep, check_temperature
 from .runtime.activations import ActivationStore
 from .runtime.device import Event, Stream
 from .runtime import host_memory
@@ -849,6 +849,7 @@ class SlideFSDP(nn.Module):
             return CausalLMOutputWithPast(loss=None, logits=self._inference(input_ids))
         step = None
         if objective is not None:
+            self._check_label_shape(input_ids, labels)
             step = ObjectiveStep.build(objective, *input_ids.shape, self.device, ref_logps=ref_logps,
                                        old_logps=old_logps, advantages=advantages)
         loss = self._train_step(input_ids, labels, step)
@@ -862,7 +863,15 @@ class SlideFSDP(nn.Module):
         column.  With the weights of a run's start they are an objective's
         ``ref_logps``."""
         self._check_ids(input_ids, labels)
+        self._check_label_shape(input_ids, labels)
+        check_temperature(temperature)
         return self._inference(input_ids, labels, temperature)
+
+    @staticmethod
+    def _check_label_shape(input_ids: torch.Tensor, labels: torch.Tensor) -> None:
+        if input_ids.dim() != 2 or labels.shape != input_ids.shape:
+            raise ValueError(f"input_ids and labels must be [B, S], got {tuple(input_ids.shape)} and "
+                             f"{tuple(labels.shape)}")
 
     def _check_ids(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor]) -> None:
         """Token ids and labels that arrive in host memory are range-checked
