@@ -14,6 +14,7 @@ that sampled the answers.
 """
 from __future__ import annotations
 
+import warnings
 from dataclasses import dataclass, field
 from typing import Dict, Optional
 
@@ -43,11 +44,16 @@ class PreferenceObjective:
 
     def __post_init__(self):
         ops.check_preference(self.beta, self.kind, self.label_smoothing)
+        if self.label_smoothing and self.kind != "sigmoid":
+            warnings.warn(f"label_smoothing has no effect on the {self.kind} loss", stacklevel=3)
         check_temperature(self.temperature)
 
     def check(self, inputs, batch: int) -> None:
         if batch % 2:
             raise ValueError(f"a preference batch needs an even number of sequences, got {batch}")
+        unused = [n for n in ("old_logps", "advantages") if inputs.get(n) is not None]
+        if unused:
+            raise ValueError(f"a preference objective does not take {', '.join(unused)}")
 
     def loss_and_grad(self, logp, targets, seq_len, inputs):
         loss, dlogp, rewards = ops.preference_loss_fwd_bwd(

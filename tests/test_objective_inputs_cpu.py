@@ -34,3 +34,19 @@ def test_refused_labels_leave_the_engine_usable(labels, engine):
     with pytest.raises(ValueError):
         engine(input_ids=IDS, labels=labels, objective=PreferenceObjective())
     assert bool(torch.isfinite(engine(input_ids=IDS, labels=IDS, objective=PreferenceObjective()).loss))
+
+
+@pytest.mark.parametrize("extra", [dict(old_logps=torch.zeros(2, 16)), dict(advantages=torch.zeros(2))])
+def test_inputs_that_a_preference_objective_does_not_take(extra, engine):
+    with pytest.raises(ValueError, match="does not take"):
+        engine(input_ids=IDS, labels=IDS, objective=PreferenceObjective(), **extra)
+    assert engine.completed_steps == 0
+
+
+def test_label_smoothing_of_other_kinds_is_pointed_out(recwarn):
+    PreferenceObjective(kind="sigmoid", label_smoothing=0.1)
+    PreferenceObjective(kind="hinge")
+    assert not [w for w in recwarn if "label_smoothing" in str(w.message)]
+    for kind in ("hinge", "ipo"):
+        with pytest.warns(UserWarning, match="label_smoothing"):
+            PreferenceObjective(kind=kind, label_smoothing=0.1)
