@@ -353,7 +353,8 @@ def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, 
     are at ``ops.policy_loss_fwd_bwd``.  A token is clipped when its log ratio
     lies past log(1 +- clip) on the side its advantage pushes to."""
     valid = (targets != ignore_index).view(-1, seq_len)
-    a = advantages.float().view(valid.shape[0], -1)
+    a = advantages.float()
+    a = a.view(valid.shape) if a.shape[0] == valid.numel() else a[:, None]
     d = (logp.float() - old_logp.float()).view_as(valid)
     rho = torch.exp(d)
     over, under = d > math.log1p(clip_high), d < math.log1p(-clip_low)
