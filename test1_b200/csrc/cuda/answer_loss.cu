@@ -349,15 +349,20 @@ struct Clip {
         flat(-a * (a > 0.f ? p.edge_hi : p.edge_lo)) {}
 };
 
-// exp(e) - 1 - e: its series up to e^7 for small e, where the difference would
-// keep no digit (the first term left out is below 2^-25 of the sum).
-__device__ __forceinline__ float kl_term(float e) {
+// exp(e) - 1 and kl = exp(e) - 1 - e: kl's series up to e^7 for small e, where
+// the differences would keep no digit (the first term left out is below 2^-25
+// of the sum).  Elsewhere exp(e) - 1 comes first: it is at most 1 in size
+// where e is far below 0, and kl + e would not give it back.
+__device__ __forceinline__ float kl_term(float e, float& exp_m1) {
   float s = fmaf(e, 1.f / 5040, 1.f / 720);
   s = fmaf(e, s, 1.f / 120);
   s = fmaf(e, s, 1.f / 24);
   s = fmaf(e, s, 1.f / 6);
   s = fmaf(e, s, 0.5f);
-  return fabsf(e) < 0.25f ? s * e * e : (__expf(e) - 1.f) - e;
+  const bool near = fabsf(e) < 0.25f;
+  const float kl = s * e * e;
+  exp_m1 = near ? kl + e : __expf(e) - 1.f;
+  return near ? kl : exp_m1 - e;
 }
 
 __device__ __forceinline__ void policy_grad_phase(const LossParams& p, Sums* red) {
@@ -395,9 +400,10 @@ __device__ __forceinline__ void policy_grad_phase(const LossParams& p, Sums* red
         float l = clipped ? clip.flat : grad;
         g[k] = clipped ? 0.f : grad;
         if (p.ref != nullptr) {
-          const float e = rf[k] - lp[k], kl = kl_term(e);
+          float exp_m1;
+          const float e = rf[k] - lp[k], kl = kl_term(e, exp_m1);
           l = fmaf(p.kl_coef, kl, l);
-          g[k] = fmaf(-p.kl_coef, kl + e, g[k]);  // exp(e) - 1
+          g[k] = fmaf(-p.kl_coef, exp_m1, g[k]);
           if (ok[k]) kl_part += kl;
         }
         if (ok[k]) part += l;
