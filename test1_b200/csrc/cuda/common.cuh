@@ -48,6 +48,22 @@ inline int num_sms() {
   return n;
 }
 
+// A flag per device, for what is set up once on each (a kernel's shared memory
+// limit holds for one device).
+class DeviceFlags {
+ public:
+  bool& here() {
+    int dev = 0;
+    T1_CHECK_CUDA(cudaGetDevice(&dev));
+    TORCH_CHECK(dev < kMost, "device index out of range");
+    return flags_[dev];
+  }
+
+ private:
+  static constexpr int kMost = 64;
+  bool flags_[kMost] = {};
+};
+
 // 8 x bf16 = 16 bytes
 struct __align__(16) bf16x8 {
   __nv_bfloat162 h[4];

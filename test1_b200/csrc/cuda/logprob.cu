@@ -510,10 +510,10 @@ template <int JOB>
 static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta2, const CUtensorMap& tb2,
                          const CUtensorMap& tc, VocabParams& p, int64_t units) {
   auto kern = vocab::vocab_kernel<JOB>;
-  static bool configured = false;
-  if (!configured) {
+  static DeviceFlags configured;
+  if (bool& done = configured.here(); !done) {
     T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, vocab::V_SMEM_BYTES));
-    configured = true;
+    done = true;
   }
   p.err = gemm_error_word().data_ptr<int>();
   const int clusters = static_cast<int>(std::min<int64_t>(units, num_sms() / 2));
@@ -638,10 +638,10 @@ template <bool BWD>
 static void launch_few(const FewParams& p) {
   const int tokens8 = p.T <= 8 ? 8 : 16;
   auto kern = tokens8 == 8 ? logprob_few_kernel<1, BWD> : logprob_few_kernel<2, BWD>;
-  static bool configured[2] = {false, false};
-  if (!configured[tokens8 / 8 - 1]) {
+  static DeviceFlags configured[2];
+  if (bool& done = configured[tokens8 / 8 - 1].here(); !done) {
     T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
-    configured[tokens8 / 8 - 1] = true;
+    done = true;
   }
   launch_after("logprob_few", kern, dim3(few_grid(p.V, p.H)), kFewThreads, few_smem(tokens8, p.H), p);
 }
