@@ -53,6 +53,8 @@ struct LossParams {
   Arrivals arrivals;       // the grid barrier's counter; none: the blocks are one cluster
   int* err;
   uint8_t* answer;         // [T] phase A's finding, an eighth of the targets to read again
+  int64_t units_n;         // units and blocks that the workspace has room for
+  int blocks_n;
   double2* units;          // [B * chunks] (sum of log ratios, answer tokens)
   double2* totals;         // [block] preference: (loss, pairs); policy: (answer tokens, sequences that have one)
   float *loss, *dlogp;
@@ -110,6 +112,7 @@ __device__ __forceinline__ double group_sum(double v, int by) {
 __device__ __forceinline__ double2 join_units(const LossParams& p, int64_t b, int lane, int by) {
   double2 t = make_double2(0, 0);
   for (int c = lane; c < p.chunks; c += by) {
+    if (T1_OOB(b * p.chunks + c, p.units_n)) continue;
     const double2 v = __ldcg(&p.units[b * p.chunks + c]);
     t.x += v.x;
     t.y += v.y;
@@ -134,7 +137,7 @@ __device__ __forceinline__ double2 join_totals(const LossParams& p, Sums* red) {
 
 __device__ __forceinline__ void write_totals(const LossParams& p, double x, double y, Sums* red) {
   const Sums s = block_sums<2>(Sums{{x, y, 0}}, red);
-  if (threadIdx.x == 0) __stcg(&p.totals[blockIdx.x], make_double2(s.v[0], s.v[1]));
+  if (threadIdx.x == 0 && !T1_OOB(blockIdx.x, p.blocks_n)) __stcg(&p.totals[blockIdx.x], make_double2(s.v[0], s.v[1]));
 }
 
 // The warps' walk over units: body(unit, sequence, first token, tokens, lane
@@ -146,10 +149,10 @@ __device__ __forceinline__ void for_units(const LossParams& p, F body) {
   const int64_t count = p.B * p.chunks, step = static_cast<int64_t>(gridDim.x) * kLossWarps * per_warp;
   for (int64_t u0 = (static_cast<int64_t>(blockIdx.x) * kLossWarps + (threadIdx.x >> 5)) * per_warp; u0 < count; u0 += step) {
     const int64_t u = u0 + in_warp / p.lanes;
-    if (u < count) {
-      const int64_t b = u / p.chunks;
-      const int s0 = static_cast<int>(u - b * p.chunks) * p.unit;
-      body(u, b, b * p.S + s0, min(p.unit, p.S - s0), in_warp & (p.lanes - 1));
+    const int64_t b = u / p.chunks;
+    const int s0 = static_cast<int>(u - b * p.chunks) * p.unit, len = min(p.unit, p.S - s0);
+    if (u < count && !T1_OOB(u, p.units_n) && !T1_OOB(len - 1, p.S) && !T1_OOB(b * p.S + s0 + len - 1, p.B * p.S)) {
+      body(u, b, b * p.S + s0, len, in_warp & (p.lanes - 1));
     } else {
       body(-1, 0, 0, 0, in_warp & (p.lanes - 1));
     }
@@ -219,7 +222,8 @@ static_assert(kAhead == 4, "Four");
 template <class F>
 __device__ __forceinline__ void for_fours(const LossParams& p, int len, int lane, F body) {
   if (p.vectors) {
-    for (int s = 4 * lane; s < len; s += 4 * 32) body(Four<1>{s, 1, len, true});
+    for (int s = 4 * lane; s < len; s += 4 * 32)
+      if (!T1_OOB(s + 3, len)) body(Four<1>{s, 1, len, true});
   } else if (p.lanes == 32) {
     int s = lane;
     for (; s - lane + 32 * kAhead <= len; s += 32 * kAhead) body(Four<32>{s, 32, len, true});
@@ -274,6 +278,7 @@ __device__ __forceinline__ void pairs_phase(const LossParams& p, Sums* red) {
   const int64_t step = static_cast<int64_t>(gridDim.x) * kLossThreads / by;
   double loss = 0, live = 0;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kLossThreads + threadIdx.x) / by; i < P; i += step) {
+    if (T1_OOB(i + P, p.B)) continue;
     const double2 ch = join_units(p, i, lane, by), rj = join_units(p, i + P, lane, by);
     if (lane != 0) continue;
     const double pc = p.average ? 1 / fmax(1.0, ch.y) : 1, pr = p.average ? 1 / fmax(1.0, rj.y) : 1;
@@ -310,7 +315,7 @@ __device__ __forceinline__ void lengths_phase(const LossParams& p, Sums* red) {
   double tokens = 0, live = 0;
   for (int64_t b = static_cast<int64_t>(blockIdx.x) * kLossWarps + (threadIdx.x >> 5); b < p.B; b += static_cast<int64_t>(gridDim.x) * kLossWarps) {
     const double n = join_units(p, b, lane, 32).y;
-    if (lane != 0) continue;
+    if (lane != 0 || T1_OOB(b, p.B)) continue;
     __stcg(&p.lengths[b], static_cast<int>(n));
     tokens += n;
     live += n > 0 ? 1 : 0;
@@ -417,7 +422,7 @@ __device__ __forceinline__ void policy_grad_phase(const LossParams& p, Sums* red
     loss += unit_loss * w;
   });
   const Sums s = block_sums<3>(Sums{{loss, kls, static_cast<double>(cut)}}, red);
-  if (threadIdx.x == 0)
+  if (threadIdx.x == 0 && !T1_OOB(blockIdx.x, p.blocks_n))
     for (int k = 0; k < 3; ++k) __stcg(&p.sums[3 * blockIdx.x + k], s.v[k]);
 }
 
@@ -574,6 +579,8 @@ static void launch_loss(LossParams& p, const LossPlan& plan) {
   const torch::Tensor held =
       loss_workspace(pad(16 * units) + pad(16 * plan.blocks) + pad(24 * plan.blocks) + pad(4 * p.B) + p.B * p.S);
   uint8_t* ws = held.data_ptr<uint8_t>();
+  p.units_n = units;
+  p.blocks_n = plan.blocks;
   p.units = reinterpret_cast<double2*>(ws);
   p.totals = reinterpret_cast<double2*>(ws + pad(16 * units));
   p.sums = reinterpret_cast<double*>(ws + pad(16 * units) + pad(16 * plan.blocks));

@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const Voc
   s = 0.f;
   for (int w = 0; w < kJoinWarps; ++w) s += ss[w][lane] * ex2((sm[w][lane] - ref) * k2);
   const int t = p.index != nullptr ? p.index[row] : row;
+  if (T1_OOB(t, p.tokens)) return;
   const int64_t v = p.targets[row];
   vocab::write_logp(m, s, p.target_logit[row], v != p.ignore && v >= 0 && v < p.V, p.scale, p.logp + t, p.lse_out + t);
 }
@@ -233,7 +234,8 @@ __global__ void __launch_bounds__(kPlanesThreads) logprob_planes_kernel(const Vo
   const float4* plane = reinterpret_cast<const float4*>(p.planes + (static_cast<size_t>(tile) * e.splits * 8 + w8) * vocab::PLANE_BLOCK) +
                         (blockIdx.y * 16 + warp) * 32 + lane;
   float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (col0 + warp * 4 < p.H) {
+  const int64_t last_block = (static_cast<int64_t>(tile + 1) * e.splits - 1) * 8 + w8;
+  if (col0 + warp * 4 < p.H && !T1_OOB(last_block, p.plane_blocks)) {
     for (int s0 = 0; s0 < e.splits; s0 += 8) {
       float4 v[8];
 #pragma unroll
@@ -260,6 +262,7 @@ __global__ void __launch_bounds__(kPlanesThreads) logprob_planes_kernel(const Vo
   const int rr = threadIdx.x >> 3, j = threadIdx.x & 7, col = col0 + 8 * j;
   if (row0 + rr >= e.rows || col >= p.H) return;
   const int64_t t = p.index != nullptr ? p.index[row0 + rr] : row0 + rr;
+  if (T1_OOB(t, p.tokens)) return;
   *reinterpret_cast<uint4*>(p.dx + t * p.H + col) = *reinterpret_cast<const uint4*>(slab + rr * 128 + ((j ^ (rr & 7)) << 4));
 }
 
@@ -286,6 +289,7 @@ struct FewParams {
   float scale;
   // forward
   Arrivals ticket;       // of the blocks
+  int blocks;            // that part has room for
   float2* part;          // [block][16]
   float* target_logit;   // [16]
   float *logp, *lse_out;
@@ -385,12 +389,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
     lse = p.lse[token];
     gr = p.dlogp[token] * p.scale;
   }
-  if (BWD && blockIdx.x == 0 && cell && tid < TOK) p.g[token] = gr;
+  if (BWD && blockIdx.x == 0 && cell && tid < TOK && !T1_OOB(token, p.T)) p.g[token] = gr;
   __syncthreads();
   if (BWD) {  // a share of x per block
     const int nvec = p.H / 8;
     for (int i = blockIdx.x * kFewThreads + tid; i < p.T * nvec; i += gridDim.x * kFewThreads) {
       const int t = i / nvec, v = i % nvec;
+      if (T1_OOB(t, p.T)) continue;
       const int64_t tt = p.targets[t];
       const bool live = tt != p.ignore && tt >= 0 && tt < p.V && p.dlogp[t] != 0.f;
       *reinterpret_cast<uint4*>(p.xz + static_cast<size_t>(t) * p.H + 8 * v) =
@@ -435,10 +440,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
       for (int w = 0; w < p.share; ++w) l += red[(buf * kFewWarps + of * p.share + w) * CELLS + at];
       if (BWD) {
         const float uv = gr != 0.f ? gr * ((v == target ? 1.f : 0.f) - ex2(fmaf(l, p.scale, -lse) * kLog2e)) : 0.f;
-        p.u[token * p.ldu + v] = __float2bfloat16_rn(uv);
+        if (!T1_OOB(token, p.T) && !T1_OOB(v, p.ldu)) p.u[token * p.ldu + v] = __float2bfloat16_rn(uv);
       } else {
         vocab::lse_join(m, s, l, 1.f, k2);
-        if (v == target) __stcg(&p.target_logit[token], l);
+        if (v == target && !T1_OOB(token, 16)) __stcg(&p.target_logit[token], l);
       }
     }
     buf ^= 1;
@@ -453,7 +458,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   if (tid < TOK) {
     for (int r = 1; r < min(kFewThreads, CELLS * teams) / TOK; ++r)
       vocab::lse_join(m, s, cells[r * TOK + tid].x, cells[r * TOK + tid].y, k2);
-    __stcg(&p.part[blockIdx.x * 16 + tid], make_float2(m, s));
+    if (!T1_OOB(blockIdx.x, p.blocks) && !T1_OOB(tid, 16)) __stcg(&p.part[blockIdx.x * 16 + tid], make_float2(m, s));
   }
   __threadfence();
   __syncthreads();
@@ -671,6 +676,7 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
     FewParams p = few_params(x, w, tg, ignore_index, temperature);
     auto ws = torch::empty({32 * few_grid(V, H) + 16}, f32);
     p.part = reinterpret_cast<float2*>(ws.data_ptr<float>());
+    p.blocks = few_grid(V, H);
     p.target_logit = ws.data_ptr<float>() + 32 * few_grid(V, H);
     ArrivalCounters counters(1);
     p.ticket = counters.arrivals;
@@ -697,7 +703,7 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   p.targets = tg.data_ptr<int64_t>();
   p.ignore = ignore_index;
   p.V = V;
-  p.ld_part = static_cast<int>(T);
+  p.ld_part = p.tokens = static_cast<int>(T);
   p.part = reinterpret_cast<float2*>(base + o_part);
   p.target_logit = reinterpret_cast<float*>(base + o_logit);
   p.logp = logp.data_ptr<float>();
@@ -707,6 +713,7 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   if (p.join) {
     counters.emplace(tiles_t * 8);
     p.tickets = counters->arrivals;
+    p.tickets_n = static_cast<int>(tiles_t * 8);
   }
   if (pack) {
     PackParams k{};
@@ -797,6 +804,8 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   p.g = reinterpret_cast<float*>(base + o_g);
   p.dx = (bf16*)dx.data_ptr();
   p.planes = reinterpret_cast<float*>(base + o_planes);
+  p.plane_blocks = 8 * planes;
+  p.tokens = static_cast<int>(T);
   bf16 *u = reinterpret_cast<bf16*>(base + o_u), *xp = reinterpret_cast<bf16*>(base + o_x);
   const CUtensorMap txc = make_map_any(xp, H, u_rows, H, gemm::BK);
   if (few) {

@@ -69,8 +69,10 @@ struct VocabParams {
   float scale;             // 1 / temperature
   int col0;                // vocabulary index of column 0
   const int* index;        // [rows] token of a packed row; null: the row itself
+  int tokens;              // T
   const int64_t* targets;  // [rows] vocabulary index
   Arrivals tickets;        // kLse with join: arrivals per 32 rows
+  int tickets_n;
   // kLse
   int64_t ignore, V;
   int ld_part;
@@ -84,6 +86,7 @@ struct VocabParams {
   // kGrads
   bf16* dx;                // [T, H]
   float* planes;           // [tile][split][8] blocks of PLANE_BLOCK
+  int64_t plane_blocks;    // allocated
   int first, last;         // first / last piece of the vocabulary
   int* err;
 };
@@ -456,14 +459,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
           for (int j = 0; j < HALF; ++j) x = static_cast<int>(t) == j ? v[j] : x;
           if (mine) __stcg(&p.target_logit[row], x);
         }
-        if (row_ok && !T1_OOB(row, p.ld_part))
+        if (row_ok && !T1_OOB(row, p.ld_part) && !T1_OOB(2 * u.nb + half, 2 * e.tiles_n))
           __stcg(&p.part[static_cast<size_t>(2 * u.nb + half) * p.ld_part + row], make_float2(m, s));
         if (!p.join) continue;
         // the last of the row group's column blocks joins them all, in order
         __threadfence();
         __syncwarp();
         int last = 0;
-        if (lane == 0) last = atomicAdd(&p.tickets.use[u.mb * 8 + w8], 1) == 2 * e.tiles_n - 1;
+        if (lane == 0 && !T1_OOB(u.mb * 8 + w8, p.tickets_n)) last = atomicAdd(&p.tickets.use[u.mb * 8 + w8], 1) == 2 * e.tiles_n - 1;
         if (!__shfl_sync(0xffffffffu, last, 0)) continue;
         __threadfence();
         if (!row_ok) continue;
@@ -475,6 +478,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
           lse_join(m, s, w.x, w.y, k2);
         }
         const int at = p.index != nullptr ? p.index[row] : row;
+        if (T1_OOB(at, p.tokens)) continue;
         const int64_t target = p.targets[row];
         write_logp(m, s, __ldcg(&p.target_logit[row]), target != p.ignore && target >= 0 && target < p.V, p.scale,
                    p.logp + at, p.lse_out + at);
@@ -554,6 +558,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         const bool dead = row < e.rows && p.g[row] == 0.f;  // its dx is 0, whatever W holds
         const int at = row < e.rows && p.index != nullptr ? p.index[row] : row;
         const bool direct = e.splits == 1 && p.last;  // no other range, no later piece
+        // uniform over the warp
+        const bool plane_ok = !live || (direct && p.first) || !T1_OOB(block, p.plane_blocks);
         if (lane == 0) bulk_wait_group_read<0>();  // stores of an earlier dW tile have read the slab
         __syncwarp();
 #pragma unroll 1
@@ -562,7 +568,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
           tmem_ld_32x32b_x32(taddr + c, r);
           tmem_ld_wait();
           if (c + 32 == HALF) release(acc);
-          if (!live || col0 + c >= p.H) continue;
+          if (!live || !plane_ok || col0 + c >= p.H) continue;
           float f[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) f[j] = u.kb0 == u.kb1 ? 0.f : __uint_as_float(r[j]);
@@ -593,7 +599,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
             const int64_t t = __shfl_sync(0xffffffffu, at, rr);
             const uint4 v = *reinterpret_cast<const uint4*>(slab + rr * 128 + ((j ^ (rr & 7)) << 4));
             const int col = col0 + (c & ~63) + 8 * j;
-            if (row0 + rr < e.rows && col < p.H && (right || j < 4)) *reinterpret_cast<uint4*>(p.dx + t * p.H + col) = v;
+            if (row0 + rr < e.rows && col < p.H && (right || j < 4) && !T1_OOB(t, p.tokens)) *reinterpret_cast<uint4*>(p.dx + t * p.H + col) = v;
           }
           __syncwarp();
         }
