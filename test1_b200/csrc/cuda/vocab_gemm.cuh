@@ -107,8 +107,12 @@ __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.w
 // The tensor cores drop what falls below the accumulator's last bit at every
 // step, which adds up: over 4096 products the logits lose 2e-6 of their size.
 // The logits are therefore summed from accumulators of about 16 k blocks each
-// (equal parts of k, 1472 products at most), added up in registers, rounded:
-// 4e-7 at H = 4096, for 4 % more time.  kSoftmaxGrad sums them in the same
+// (equal parts of k, 1472 products at most), added up in registers, rounded.
+// Errors of logp (rms, of the row's largest logit; fp32 library arithmetic in
+// brackets): 3.6e-7 (4.2e-7) at H = 4096, for 4 % more time; 3.8e-7 (1.6e-7) at
+// 1024; 4.9e-7 (2.0e-7) at 1472, the longest accumulator.  At most 16 blocks
+// would give 2.5e-7 there for 1-4 % of the time of H between 1025 and 1472 (839
+// rows, H = 1032, V = 50021: 106 us against 102).  kSoftmaxGrad sums them in the same
 // order as kLse: where a target is nearly sure, u is what exp(logit - lse)
 // leaves of 1, and an error of the logit that lse does not share is all of u
 // (one accumulator there put dx rows of targets with p = 0.999 off by a half).

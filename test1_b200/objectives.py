@@ -3,10 +3,13 @@
 An objective is a function of the log-probabilities that the model gives to
 the labels.  ``SlideFSDP(..)(input_ids, labels, objective=..)`` runs the same
 step as cross-entropy training does; its output layer computes the
-log-probabilities without a [tokens, vocabulary] tensor of logits
-(``ops.linear_logprob_fwd``), the objective gives the loss and its gradient
-for them, and ``ops.linear_logprob_bwd`` carries that on to the hidden states
-and the output weights.  (The reference trains with cross-entropy only.)
+log-probabilities, the objective gives the loss and its gradient for them, and
+the output layer carries that on to the hidden states and the output weights.
+For Llama models it does so without a [tokens, vocabulary] tensor of logits
+(``ops.linear_logprob_fwd`` and ``ops.linear_logprob_bwd``); the generic path
+of other architectures runs their own head under autograd and holds the logits
+in fp32.  On several ranks every rank's loss is that of its own batch, and the
+gradients are their mean.  (The reference trains with cross-entropy only.)
 
 ``SlideFSDP.token_logprobs`` gives the log-probabilities that an objective
 compares with: those of a frozen reference model, and those of the policy
@@ -32,7 +35,7 @@ def check_temperature(temperature: float) -> None:
 class PreferenceObjective:
     """Paired answers: the first half of a batch are the chosen ones, the
     second half the rejected ones, in the same order (``labels`` -100 outside
-    the answers).  Takes ``ref_logps`` [B, S] (optional).  The loss, its kinds
+    the answers).  Takes ``ref_logps`` [B, S] (optional) and no other input.  The loss, its kinds
     and the padding rules are those of ``ops.preference_loss_fwd_bwd``.
     Results: ``rewards`` [B], the implicit rewards."""
 

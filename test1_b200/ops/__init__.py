@@ -113,8 +113,8 @@ def linear_logprob_fwd(x, w, targets, ignore_index=-100, temperature=1.0):
 
 def linear_logprob_bwd(dlogp, x, w, targets, lse, dx, dw, ignore_index=-100, temperature=1.0):
     """Gradients of ``linear_logprob_fwd``: from dlogp [T] (fp32) and the
-    forward's lse, writes dx [T, H] and dw [V, H].  Entries of dlogp at
-    ignored tokens are not used."""
+    forward's lse (of the same x and w: its logits' errors then cancel), writes
+    dx [T, H] and dw [V, H].  Entries of dlogp at ignored tokens are not used."""
     _impl(x).linear_logprob_bwd(dlogp, x, w, targets, lse, dx, dw, ignore_index, temperature)
 
 
@@ -133,8 +133,8 @@ def preference_loss_fwd_bwd(logp, ref_logp, targets, seq_len, beta=0.1, kind="si
       hinge    max(0, 1 - beta m)
       ipo      (m - 1 / (2 beta))^2
     averaged over the pairs that have an answer token (a pair of padding only
-    is left out); label_smoothing is the sigmoid loss's alone.  Returns (loss [] fp32, dloss/dlogp [T], rewards
-    [T / seq_len] = beta r)."""
+    is left out); label_smoothing is the sigmoid loss's alone.  Returns
+    (loss [] fp32, dloss/dlogp [T], rewards [T / seq_len] = beta r)."""
     _check_loss(logp, targets, seq_len)
     if (logp.shape[0] // seq_len) % 2:
         raise ValueError(f"a preference batch needs an even number of sequences, got {logp.shape[0] // seq_len}")
