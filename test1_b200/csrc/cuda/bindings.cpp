@@ -34,12 +34,21 @@ void fill_last_arrivals(int64_t value);
 void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, torch::Tensor targets,
                         torch::Tensor lse, torch::Tensor dx, torch::Tensor dw, int64_t ignore_index,
                         double temperature);
+torch::Tensor linear_logits(torch::Tensor x, torch::Tensor w);
+std::vector<torch::Tensor> linear_topk_logprob_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor ids, double temperature);
+void linear_topk_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, torch::Tensor ids, torch::Tensor lse,
+                             torch::Tensor dx, torch::Tensor dw, double temperature);
+std::vector<torch::Tensor> distillation_loss(torch::Tensor logp, torch::Tensor teacher, torch::Tensor ids, int64_t kind,
+                                             bool tail);
 std::vector<torch::Tensor> preference_loss(torch::Tensor logp, c10::optional<torch::Tensor> ref,
                                            torch::Tensor targets, int64_t S, double beta, int64_t kind,
                                            double smoothing, bool average, int64_t ignore_index);
 std::vector<torch::Tensor> policy_loss(torch::Tensor logp, torch::Tensor old, c10::optional<torch::Tensor> ref,
                                        torch::Tensor advantages, torch::Tensor targets, int64_t S, double clip_low,
                                        double clip_high, double kl_coef, bool per_sequence, int64_t ignore_index);
+std::vector<torch::Tensor> topk_logprobs(torch::Tensor logits, int64_t k, double temperature);
+std::vector<torch::Tensor> sample_tokens(torch::Tensor logits, torch::Tensor u, double temperature, int64_t top_k,
+                                         double top_p, double min_p);
 void gemm_bf16(torch::Tensor A, torch::Tensor B, torch::Tensor C, bool a_mn, bool b_mn,
                c10::optional<torch::Tensor> R);
 int64_t gemm_check_error(bool reset);
@@ -86,6 +95,7 @@ unsigned long long bounds_word_attention(bool);
 unsigned long long bounds_word_attention_tc(bool);
 unsigned long long bounds_word_attention_fwd2(bool);
 unsigned long long bounds_word_attention_bwd2(bool);
+unsigned long long bounds_word_distillation(bool);
 unsigned long long bounds_word_elementwise(bool);
 unsigned long long bounds_word_embed_ce(bool);
 unsigned long long bounds_word_fused_adam(bool);
@@ -94,6 +104,7 @@ unsigned long long bounds_word_fused_comm(bool);
 unsigned long long bounds_word_gemm(bool);
 unsigned long long bounds_word_logprob(bool);
 unsigned long long bounds_word_noalloc_rmsnorm(bool);
+unsigned long long bounds_word_row_select(bool);
 }  // namespace t1
 
 // [(source file, line, index)] of the first out-of-bounds access each
@@ -107,6 +118,7 @@ static std::vector<std::tuple<std::string, int64_t, int64_t>> bounds_errors(bool
       {"attention_tc.cu", &t1::bounds_word_attention_tc},
       {"attention_fwd2.cu", &t1::bounds_word_attention_fwd2},
       {"attention_bwd2.cu", &t1::bounds_word_attention_bwd2},
+      {"distillation.cu", &t1::bounds_word_distillation},
       {"elementwise.cu", &t1::bounds_word_elementwise},
       {"embed_ce.cu", &t1::bounds_word_embed_ce},
       {"fused_adam.cu", &t1::bounds_word_fused_adam},
@@ -115,6 +127,7 @@ static std::vector<std::tuple<std::string, int64_t, int64_t>> bounds_errors(bool
       {"gemm.cu", &t1::bounds_word_gemm},
       {"logprob.cu", &t1::bounds_word_logprob},
       {"noalloc_rmsnorm.cu", &t1::bounds_word_noalloc_rmsnorm},
+      {"row_select.cu", &t1::bounds_word_row_select},
   };
   std::vector<std::tuple<std::string, int64_t, int64_t>> out;
   for (const auto& r : readers) {
@@ -156,10 +169,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_logprob_fwd", &t1::linear_logprob_fwd,
         "log-probabilities of the targets under the output layer: (logp [T], lse [T])");
   m.def("linear_logprob_bwd", &t1::linear_logprob_bwd, "gradients of linear_logprob_fwd: writes dx and dW");
+  m.def("linear_logits", &t1::linear_logits, "logits of the output layer in fp32 [T, V]");
+  m.def("linear_topk_logprob_fwd", &t1::linear_topk_logprob_fwd,
+        "log-probabilities of a list of tokens per row under the output layer: (logp [T, K], lse [T])");
+  m.def("linear_topk_logprob_bwd", &t1::linear_topk_logprob_bwd, "gradients of linear_topk_logprob_fwd: writes dx and dW");
+  m.def("distillation_loss", &t1::distillation_loss,
+        "divergence from a teacher on its likeliest tokens: (loss, dlogp [T, K], divergence [T])");
   m.def("fill_last_arrivals", &t1::fill_last_arrivals,
         "leaves the arrival counters as an expired wait does (for tests of what follows one)");
   m.def("preference_loss", &t1::preference_loss, "paired log-ratio loss: (loss, dlogp [T], rewards [B])");
   m.def("policy_loss", &t1::policy_loss, "clipped policy loss with a KL term: (loss, dlogp [T], stats [2])");
+  m.def("topk_logprobs", &t1::topk_logprobs, "the likeliest tokens of every row of logits: (logp [T, k], ids [T, k])");
+  m.def("sample_tokens", &t1::sample_tokens,
+        "a token of every row, drawn with given random numbers: (token [B], logp [B])");
   m.def("gemm_bf16", &t1::gemm_bf16, pybind11::arg("A"), pybind11::arg("B"), pybind11::arg("C"),
         pybind11::arg("a_mn"), pybind11::arg("b_mn"), pybind11::arg("R") = pybind11::none());
   m.def("gemm_error_word", [] { return t1::gemm_error_word(); },

@@ -16,6 +16,12 @@
 //
 // A token whose target is ignored (ignore_index, or outside the vocabulary)
 // gives logp = lse = 0 and no gradient, whatever its hidden state holds.
+//
+// With a list of K tokens in place of the target (a teacher's likeliest):
+//   logp[t, k]  = logit[t, ids[t, k]] - lse[t]
+//   u[t, v]     = (sum_k dlogp[t, k] [ids[t, k] = v] - exp(logit[t, v] - lse[t]) sum_k dlogp[t, k]) / tau
+// and the same products; the listed tokens' part is added to u before it is
+// rounded, because where student and teacher agree the two nearly cancel.
 #include "vocab_gemm.cuh"
 
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
@@ -78,8 +84,9 @@ struct PackParams {
   int per_block;         // tokens of a block
   int per_slice;         // 8-column vectors of a block
   float scale;
-  const float* dlogp;    // null in the forward
+  const float* dlogp;    // null in the forward; of lists their sums over tau
   const float* lse;      // with dlogp
+  float* live;           // [T] 1, of lists with dlogp
   int k_blocks, tiles_n, tiles_h, clusters;  // of the products with u, with dlogp
   vocab::RowsMeta* meta;
   int* index;            // [T] the packed row's token
@@ -100,7 +107,8 @@ constexpr int kPackThreads = 256;
 // rows before its own tokens itself: T / 2 targets out of L2 on average
 // instead of a scan in a launch of its own.  Rows keep their order, so sums
 // over rows do not depend on timing.
-template <bool BWD>
+// Of lists (LISTS) the rows that take part are those that list_kernel marked.
+template <bool BWD, bool LISTS>
 __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackParams p) {
   __shared__ int counts[kPackThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -112,7 +120,7 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
   auto takes_part = [&](int t) {
     const int64_t v = p.targets[t];
     const bool valid = v != p.ignore && v >= 0 && v < p.V;
-    return BWD ? valid && p.dlogp[t] != 0.f : valid;
+    return BWD && !LISTS ? valid && p.dlogp[t] != 0.f : valid;
   };
   int n = 0;
 #pragma unroll 4
@@ -145,7 +153,8 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
         p.index[at] = t;
         p.target[at] = p.targets[t];
         if (BWD) {
-          p.g[at] = p.dlogp[t] * p.scale;
+          p.g[at] = LISTS ? p.dlogp[t] : p.dlogp[t] * p.scale;
+          if (LISTS) p.live[at] = 1.f;
           p.lse_packed[at] = p.lse[t];
         }
       }
@@ -181,8 +190,10 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
 // share the column blocks.  `meta` and `index` are null for rows that were
 // not packed.
 constexpr int kJoinWarps = 32;
+template <bool LISTS>
 __global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const VocabParams p, int blocks) {
   __shared__ float sm[kJoinWarps][32], ss[kJoinWarps][32];
+  __shared__ float top[32], log_s[32];
   vocab::launch_dependents();
   vocab::wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -202,6 +213,29 @@ __global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const Voc
   sm[warp][lane] = m;
   ss[warp][lane] = s;
   __syncthreads();
+  if (LISTS) {
+    if (warp == 0 && in) {
+      for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, sm[w][lane]);
+      top[lane] = m == -INFINITY ? 0.f : m;
+      s = 0.f;
+      for (int w = 0; w < kJoinWarps; ++w) s += ss[w][lane] * ex2((sm[w][lane] - top[lane]) * k2);
+      log_s[lane] = logf(s);
+    }
+    __syncthreads();
+    // a warp per row
+    const int at_row = blockIdx.x * 32 + warp;
+    if (at_row >= rows) return;
+    const int64_t t = p.index != nullptr ? p.index[at_row] : at_row;
+    if (T1_OOB(t, p.tokens)) return;
+    const int n = p.counts[t];
+    for (int i = lane; i < n; i += 32) {
+      const int64_t at = t * p.K + p.lists[t * p.K + i].y;
+      if (T1_OOB(at, static_cast<int64_t>(p.tokens) * p.K)) continue;
+      p.logp[at] = (__ldcg(p.picked + at) - top[warp]) * p.scale - log_s[warp];
+    }
+    if (lane == 0 && n > 0) p.lse_out[t] = top[warp] * p.scale + log_s[warp];
+    return;
+  }
   if (warp != 0 || !in) return;
   for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, sm[w][lane]);
   const float ref = m == -INFINITY ? 0.f : m;
@@ -298,9 +332,20 @@ struct FewParams {
   const float *dlogp, *lse;
   bf16* u;               // [T, ldu]
   long ldu;
-  float* g;              // [T] dlogp / tau
+  float* g;              // [T] dlogp / tau; of lists 1, 0 without a gradient
   bf16* xz;              // [T, H] x, zeros for tokens without a gradient
+  // lists, sorted by token (see list_kernel)
+  int K;
+  const int2* lists;     // [T, K]
+  const int* counts;     // [T]
+  float* picked;         // [T, K]
+  // logits
+  float* out;            // [T, ldo]
+  int64_t ldo;
 };
+
+// What the few-rows kernel makes of the logits.
+enum FewJob : int { kFewLse = 0, kFewGrad = 1, kFewLogits = 2 };
 
 constexpr int kFewThreads = 512;
 constexpr int kFewWarps = kFewThreads / 32;
@@ -332,8 +377,9 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NT, bool BWD>
+template <int NT, int JOB, bool LISTS>
 __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewParams p) {
+  constexpr bool BWD = JOB == kFewGrad;
   constexpr int TOK = 8 * NT;
   constexpr int CELLS = kFewRows * TOK;  // a group's logits
   extern __shared__ __align__(16) uint8_t few_raw[];
@@ -345,7 +391,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   const int g = lane >> 2, c = lane & 3;
   vocab::launch_dependents();
   vocab::wait_previous();
-  if (!BWD) clear_arrivals(p.ticket);
+  if (JOB == kFewLse) clear_arrivals(p.ticket);
 
   const int teams = kFewWarps / p.share, team = warp / p.share, part = warp % p.share;
   const int blocks32 = (p.H + 31) / 32;                       // of columns
@@ -382,23 +428,34 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   // what this thread's cells need to know: all are of one token
   const int token = tid % TOK;
   const bool cell = tid < CELLS * teams && token < p.T;
-  const int64_t target = cell ? p.targets[token] : -1;
-  const bool valid = cell && target != p.ignore && target >= 0 && target < p.V;
+  const int64_t target = !LISTS && JOB != kFewLogits && cell ? p.targets[token] : -1;
+  const int entries = LISTS && cell ? p.counts[token] : 0;
+  const bool valid = LISTS ? entries > 0 : cell && target != p.ignore && target >= 0 && target < p.V;
+  // of lists: the tokens' sorted entries, behind the warps' parts
+  int2* lists = reinterpret_cast<int2*>(red + 2 * kFewWarps * CELLS);
+  if (LISTS)
+    for (int i = tid; i < p.T * p.K; i += kFewThreads) lists[i] = p.lists[i];
+  const int2* list = lists + token * p.K;
   const float k2 = p.scale * kLog2e;
   float lse = 0.f, gr = 0.f;
   if (BWD && valid) {
     lse = p.lse[token];
-    gr = p.dlogp[token] * p.scale;
+    gr = LISTS ? p.dlogp[token] : p.dlogp[token] * p.scale;
   }
-  if (BWD && blockIdx.x == 0 && cell && tid < TOK && !T1_OOB(token, p.T)) p.g[token] = gr;
+  if (BWD && blockIdx.x == 0 && cell && tid < TOK && !T1_OOB(token, p.T)) p.g[token] = LISTS ? (valid ? 1.f : 0.f) : gr;
   __syncthreads();
   if (BWD) {  // a share of x per block
     const int nvec = p.H / 8;
     for (int i = blockIdx.x * kFewThreads + tid; i < p.T * nvec; i += gridDim.x * kFewThreads) {
       const int t = i / nvec, v = i % nvec;
       if (T1_OOB(t, p.T)) continue;
-      const int64_t tt = p.targets[t];
-      const bool live = tt != p.ignore && tt >= 0 && tt < p.V && p.dlogp[t] != 0.f;
+      bool live;
+      if (LISTS) {
+        live = p.counts[t] > 0;
+      } else {
+        const int64_t tt = p.targets[t];
+        live = tt != p.ignore && tt >= 0 && tt < p.V && p.dlogp[t] != 0.f;
+      }
       *reinterpret_cast<uint4*>(p.xz + static_cast<size_t>(t) * p.H + 8 * v) =
           live ? *reinterpret_cast<const uint4*>(xs + t * pitch + 16 * v) : make_uint4(0, 0, 0, 0);
     }
@@ -439,9 +496,32 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
       if (v >= p.V) continue;
       float l = 0.f;
       for (int w = 0; w < p.share; ++w) l += red[(buf * kFewWarps + of * p.share + w) * CELLS + at];
+      if (JOB == kFewLogits) {
+        if (!T1_OOB(token, p.T) && !T1_OOB(v, p.ldo)) p.out[token * p.ldo + v] = l;
+        continue;
+      }
+      int hit = entries;  // the first entry that is v
+      if (LISTS) {
+        int lo = 0;
+        while (lo < hit) {
+          const int mid = (lo + hit) >> 1;
+          if (list[mid].x < v) lo = mid + 1;
+          else hit = mid;
+        }
+      }
       if (BWD) {
-        const float uv = gr != 0.f ? gr * ((v == target ? 1.f : 0.f) - ex2(fmaf(l, p.scale, -lse) * kLog2e)) : 0.f;
+        float uv = 0.f;
+        if (LISTS) {
+          if (valid) uv = -gr * ex2(fmaf(l, p.scale, -lse) * kLog2e);
+          for (; hit < entries && list[hit].x == v; ++hit) uv += __int_as_float(list[hit].y);
+        } else if (gr != 0.f) {
+          uv = gr * ((v == target ? 1.f : 0.f) - ex2(fmaf(l, p.scale, -lse) * kLog2e));
+        }
         if (!T1_OOB(token, p.T) && !T1_OOB(v, p.ldu)) p.u[token * p.ldu + v] = __float2bfloat16_rn(uv);
+      } else if (LISTS) {
+        vocab::lse_join(m, s, l, 1.f, k2);
+        for (; hit < entries && list[hit].x == v; ++hit)
+          if (!T1_OOB(token, p.T) && !T1_OOB(list[hit].y, p.K)) __stcg(&p.picked[token * p.K + list[hit].y], l);
       } else {
         vocab::lse_join(m, s, l, 1.f, k2);
         if (v == target && !T1_OOB(token, 16)) __stcg(&p.target_logit[token], l);
@@ -449,7 +529,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
     }
     buf ^= 1;
   }
-  if (BWD) return;
+  if (JOB != kFewLse) return;
 
   // this block's (largest, sum) per token, then all blocks' by the last one
   float2* cells = reinterpret_cast<float2*>(red);
@@ -479,10 +559,123 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
     vocab::lse_join(m, s, m2, s2, k2);
   }
+  if (LISTS) {
+    const int n = p.counts[warp];
+    if (n == 0) return;
+    const float ref = m == -INFINITY ? 0.f : m, log_s = logf(s);
+    for (int i = lane; i < n; i += 32) {
+      const int at = warp * p.K + lists[warp * p.K + i].y;
+      if (!T1_OOB(at, p.T * p.K)) p.logp[at] = (__ldcg(&p.picked[at]) - ref) * p.scale - log_s;
+    }
+    if (lane == 0) p.lse_out[warp] = ref * p.scale + log_s;
+    return;
+  }
   if (lane == 0) {
     const int64_t t = p.targets[warp];
     vocab::write_logp(m, s, __ldcg(&p.target_logit[warp]), t != p.ignore && t >= 0 && t < p.V, p.scale, p.logp + warp,
                       p.lse_out + warp);
+  }
+}
+
+// ------------------------------------------------------------------ lists
+// Every row's list sorted by token, without the entries that name none (in the
+// gradient: nor those whose dlogp is 0), and where in it each 128-column block
+// of the vocabulary begins.  A warp per row sorts its list in shared memory (a
+// bitonic sort of token and place); then the block's 32 rows are the lanes and
+// its warps share the vocabulary's blocks, a binary search each, so that the
+// table is written 64 bytes at a time.  Latency: 10 us for 4096 rows of 64.
+struct ListParams {
+  const int64_t* ids;    // [T, K]
+  int T, K, V;
+  int slots;             // K rounded up to a power of two
+  float scale;
+  const float* dlogp;    // [T, K], in the gradient
+  int2* lists;           // [T, K]
+  int* counts;           // [T]
+  uint16_t* starts;      // [blocks + 1][T]; null: not needed
+  int blocks;
+  int64_t* flags;        // [T] 0, -1 for rows without an entry
+  float* sums;           // [T] sum of dlogp / tau, with dlogp
+  float *logp, *lse;     // forward: 0 where nothing else is written
+};
+
+constexpr int kListRows = 32;
+// An odd number of 8-byte words apart: the lanes' searches touch different banks.
+__host__ __device__ inline int list_pitch(int slots) { return slots + 1; }
+
+template <bool BWD>
+__global__ void __launch_bounds__(32 * kListRows) list_kernel(const ListParams p) {
+  extern __shared__ unsigned long long sorted[];
+  vocab::launch_dependents();
+  vocab::wait_previous();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t = blockIdx.x * kListRows + warp;
+  unsigned long long* mine = sorted + warp * list_pitch(p.slots);
+  constexpr unsigned long long kNone = ~0ull;
+  int n = 0;
+  for (int i = lane; i < p.slots; i += 32) {
+    unsigned long long e = kNone;
+    if (t < p.T && i < p.K) {
+      const int64_t at = static_cast<int64_t>(t) * p.K + i, id = p.ids[at];
+      const bool listed = id >= 0 && id < p.V;
+      if (listed && !(BWD && p.dlogp[at] == 0.f)) e = static_cast<unsigned long long>(id) << 32 | static_cast<unsigned>(i);
+      if (!BWD && !listed) p.logp[at] = 0.f;
+    }
+    n += e != kNone;
+    mine[i] = e;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  __syncwarp();
+  for (int size = 2; size <= p.slots; size *= 2) {
+    for (int step = size / 2; step > 0; step /= 2) {
+      for (int i = lane; i < p.slots; i += 32) {
+        const int j = i ^ step;
+        if (j > i) {
+          const unsigned long long a = mine[i], b = mine[j];
+          if ((a > b) == ((i & size) == 0)) {
+            mine[i] = b;
+            mine[j] = a;
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (t < p.T) {
+    float sum = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const int place = static_cast<int>(static_cast<unsigned>(mine[i]));
+      int second = place;
+      if (BWD) {
+        const float d = p.dlogp[static_cast<int64_t>(t) * p.K + place] * p.scale;
+        sum += d;
+        second = __float_as_int(d);
+      }
+      p.lists[static_cast<int64_t>(t) * p.K + i] = make_int2(static_cast<int>(mine[i] >> 32), second);
+    }
+    if (BWD) sum = warp_sum(sum);
+    if (lane == 0) {
+      p.counts[t] = n;
+      p.flags[t] = n > 0 ? 0 : -1;
+      if (BWD) p.sums[t] = sum;
+      else if (n == 0) p.lse[t] = 0.f;
+    }
+  }
+  if (p.starts == nullptr) return;
+  __syncthreads();
+  const int row = blockIdx.x * kListRows + lane;
+  const unsigned long long* of_row = sorted + lane * list_pitch(p.slots);
+  for (int b = warp; b <= p.blocks; b += kListRows) {
+    const unsigned long long first = static_cast<unsigned long long>(b) * vocab::HALF << 32;
+    int lo = 0, hi = p.slots;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (of_row[mid] < first) lo = mid + 1;
+      else hi = mid;
+    }
+    const int64_t at = static_cast<int64_t>(b) * p.T + row;
+    if (row < p.T && !T1_OOB(at, static_cast<int64_t>(p.blocks + 1) * p.T)) p.starts[at] = static_cast<uint16_t>(lo);
   }
 }
 
@@ -512,10 +705,10 @@ static void launch_after(const char* what, void (*kern)(P...), dim3 grid, int th
 }
 
 // `units`: the most units of work that the launch can have.
-template <int JOB>
+template <int JOB, bool LISTS = false>
 static void launch_vocab(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta2, const CUtensorMap& tb2,
                          const CUtensorMap& tc, VocabParams& p, int64_t units) {
-  auto kern = vocab::vocab_kernel<JOB>;
+  auto kern = vocab::vocab_kernel<JOB, LISTS>;
   static DeviceFlags configured;
   if (bool& done = configured.here(); !done) {
     T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, vocab::V_SMEM_BYTES));
@@ -580,24 +773,29 @@ static bool aligned_rows(const torch::Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_ld(t) % 8 == 0;
 }
 
-static void check_logprob(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets,
-                          double temperature) {
+static void check_layer(const torch::Tensor& x, const torch::Tensor& w) {
   T1_CHECK_INPUT(x, torch::kBFloat16);
   T1_CHECK_INPUT(w, torch::kBFloat16);
-  TORCH_CHECK(targets.is_cuda() && targets.scalar_type() == torch::kInt64, "targets must be int64 CUDA");
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "x must be [T, H] and w [V, H]");
   TORCH_CHECK(x.size(1) > 0 && x.size(1) % 8 == 0, "H must be a positive multiple of 8");
   TORCH_CHECK(w.size(0) > 0 && w.size(0) < (1ll << 30) && x.size(0) < (1ll << 30) && w.size(1) < (1ll << 30),
               "extents of x and w must lie below 2^30, and V above 0");
   TORCH_CHECK(x.stride(1) == 1 && w.stride(1) == 1 && (x.size(0) < 2 || x.stride(0) >= x.size(1)) &&
                   (w.size(0) < 2 || w.stride(0) >= w.size(1)), "x and w must be row-major");
-  TORCH_CHECK(targets.dim() == 1 && targets.size(0) == x.size(0), "targets must have T entries");
-  TORCH_CHECK(w.device() == x.device() && targets.device() == x.device(), "operands must be on one device");
+  TORCH_CHECK(w.device() == x.device(), "operands must be on one device");
   TORCH_CHECK(aligned_rows(x) && aligned_rows(w), "x and w must have 16-byte aligned rows");
+}
+
+static void check_logprob(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets,
+                          double temperature) {
+  TORCH_CHECK(targets.is_cuda() && targets.scalar_type() == torch::kInt64, "targets must be int64 CUDA");
+  check_layer(x, w);
+  TORCH_CHECK(targets.dim() == 1 && targets.size(0) == x.size(0), "targets must have T entries");
+  TORCH_CHECK(targets.device() == x.device(), "operands must be on one device");
   TORCH_CHECK(std::isfinite(temperature) && temperature > 0, "temperature must be positive");
 }
 
-static void launch_pack(PackParams& p) {
+static void launch_pack(PackParams& p, bool lists = false) {
   // about four blocks per SM: 8 to 32 tokens each and, when these are few,
   // slices of the columns (64 vectors at least, two per lane)
   p.per_block = static_cast<int>(std::min<int64_t>(32, std::max<int64_t>(8, ceil_div(p.T, 4 * num_sms()))));
@@ -605,13 +803,17 @@ static void launch_pack(PackParams& p) {
   const int64_t slices = std::max<int64_t>(1, std::min(ceil_div(p.H / 8, 64), 4 * num_sms() / groups));
   p.per_slice = static_cast<int>(ceil_div(p.H / 8, slices));
   const dim3 grid(groups, ceil_div(p.H / 8, p.per_slice));
-  if (p.dlogp != nullptr) launch_after("logprob_pack", logprob_pack_kernel<true>, grid, kPackThreads, 0, p);
-  else launch_after("logprob_pack", logprob_pack_kernel<false>, grid, kPackThreads, 0, p);
+  auto kern = p.dlogp == nullptr ? logprob_pack_kernel<false, false>
+              : lists            ? logprob_pack_kernel<true, true>
+                                 : logprob_pack_kernel<true, false>;
+  launch_after("logprob_pack", kern, grid, kPackThreads, 0, p);
 }
 
-// Whether a batch takes the few-rows kernel: x has to fit in shared memory.
+// Whether a batch takes the few-rows kernel: x, and lists of K tokens, have to
+// fit in shared memory.
 constexpr size_t kFewSmem = 200 * 1024;
-static bool few_rows(int64_t T, int64_t H) { return T <= 16 && few_smem(T <= 8 ? 8 : 16, H) <= kFewSmem; }
+static size_t few_bytes(int64_t T, int64_t H, int64_t K) { return few_smem(T <= 8 ? 8 : 16, H) + 8 * T * K; }
+static bool few_rows(int64_t T, int64_t H, int64_t K = 0) { return T <= 16 && few_bytes(T, H, K) <= kFewSmem; }
 
 static int few_share(int64_t H) {
   int share = 1;
@@ -623,14 +825,14 @@ static int few_grid(int64_t V, int64_t H) {
   return static_cast<int>(std::min<int64_t>(ceil_div(V, kFewRows * (kFewWarps / few_share(H))), num_sms()));
 }
 
-static FewParams few_params(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets, int64_t ignore,
+static FewParams few_params(const torch::Tensor& x, const torch::Tensor& w, const int64_t* targets, int64_t ignore,
                             double temperature) {
   FewParams p{};
   p.x = (const bf16*)x.data_ptr();
   p.ldx = row_ld(x);
   p.w = (const bf16*)w.data_ptr();
   p.ldw = row_ld(w);
-  p.targets = targets.data_ptr<int64_t>();
+  p.targets = targets;
   p.ignore = ignore;
   p.T = x.size(0);
   p.H = x.size(1);
@@ -640,16 +842,16 @@ static FewParams few_params(const torch::Tensor& x, const torch::Tensor& w, cons
   return p;
 }
 
-template <bool BWD>
+template <int JOB, bool LISTS = false>
 static void launch_few(const FewParams& p) {
   const int tokens8 = p.T <= 8 ? 8 : 16;
-  auto kern = tokens8 == 8 ? logprob_few_kernel<1, BWD> : logprob_few_kernel<2, BWD>;
+  auto kern = tokens8 == 8 ? logprob_few_kernel<1, JOB, LISTS> : logprob_few_kernel<2, JOB, LISTS>;
   static DeviceFlags configured[2];
   if (bool& done = configured[tokens8 / 8 - 1].here(); !done) {
     T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     done = true;
   }
-  launch_after("logprob_few", kern, dim3(few_grid(p.V, p.H)), kFewThreads, few_smem(tokens8, p.H), p);
+  launch_after("logprob_few", kern, dim3(few_grid(p.V, p.H)), kFewThreads, few_bytes(p.T, p.H, LISTS ? p.K : 0), p);
 }
 
 // Whether the forward packs its rows first.  Below 256 tokens there is one
@@ -663,18 +865,77 @@ static bool packs(int64_t T, int64_t H, int64_t V) {
 // launch of its own costs about as much as the 64 reads of 32 tiles.
 constexpr int kJoinBlocks = 32;
 
-// Returns (logp [T], lse [T]), fp32.
-std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets,
-                                              int64_t ignore_index, double temperature) {
-  check_logprob(x, w, targets, temperature);
-  const c10::cuda::CUDAGuard guard(x.device());
+// A batch's lists as list_kernel leaves them, in a workspace of their own.
+struct Lists {
+  torch::Tensor buf;
+  int K = 0;
+  int2* lists = nullptr;
+  int* counts = nullptr;
+  uint16_t* starts = nullptr;
+  int64_t* flags = nullptr;
+  float *sums = nullptr, *picked = nullptr;
+};
+
+static void check_lists(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& ids, double temperature) {
+  check_layer(x, w);
+  TORCH_CHECK(ids.is_cuda() && ids.scalar_type() == torch::kInt64, "ids must be int64 CUDA");
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == x.size(0), "ids must be [T, K]");
+  TORCH_CHECK(ids.size(1) >= 1 && ids.size(1) <= 512, "a list has 1 to 512 tokens");
+  TORCH_CHECK(ids.device() == x.device(), "operands must be on one device");
+  TORCH_CHECK(std::isfinite(temperature) && temperature > 0, "temperature must be positive");
+}
+
+// dlogp: null in the forward; logp and lse: null in the gradient.
+static Lists make_lists(const torch::Tensor& ids, int64_t V, double temperature, const float* dlogp, float* logp, float* lse,
+                        bool few) {
+  const int64_t T = ids.size(0), K = ids.size(1), blocks = ceil_div(V, vocab::HALF);
+  Lists l;
+  l.K = static_cast<int>(K);
+  Pieces ws;
+  const int64_t o_lists = ws.take(8 * T * K), o_counts = ws.take(4 * T), o_flags = ws.take(8 * T), o_sums = ws.take(4 * T),
+                o_picked = ws.take(dlogp == nullptr ? 4 * T * K : 0), o_starts = ws.take(few ? 0 : 2 * (blocks + 1) * T);
+  l.buf = torch::empty({ws.used}, ids.options().dtype(torch::kUInt8));
+  uint8_t* base = l.buf.data_ptr<uint8_t>();
+  l.lists = reinterpret_cast<int2*>(base + o_lists);
+  l.counts = reinterpret_cast<int*>(base + o_counts);
+  l.flags = reinterpret_cast<int64_t*>(base + o_flags);
+  l.sums = reinterpret_cast<float*>(base + o_sums);
+  l.picked = reinterpret_cast<float*>(base + o_picked);
+  l.starts = few ? nullptr : reinterpret_cast<uint16_t*>(base + o_starts);
+
+  ListParams p{};
+  p.ids = ids.data_ptr<int64_t>();
+  p.T = static_cast<int>(T);
+  p.K = l.K;
+  p.V = static_cast<int>(V);
+  p.slots = 1;
+  while (p.slots < p.K) p.slots *= 2;
+  p.scale = static_cast<float>(1.0 / temperature);
+  p.dlogp = dlogp;
+  p.lists = l.lists;
+  p.counts = l.counts;
+  p.starts = l.starts;
+  p.blocks = static_cast<int>(blocks);
+  p.flags = l.flags;
+  p.sums = l.sums;
+  p.logp = logp;
+  p.lse = lse;
+  auto kern = dlogp != nullptr ? list_kernel<true> : list_kernel<false>;
+  static DeviceFlags configured[2];
+  if (bool& done = configured[dlogp != nullptr].here(); !done) {
+    T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kListRows * list_pitch(512)));
+    done = true;
+  }
+  launch_after("logprob_lists", kern, dim3(ceil_div(T, kListRows)), 32 * kListRows, 8 * kListRows * list_pitch(p.slots), p);
+  return l;
+}
+
+static void logprob_forward(const torch::Tensor& x, const torch::Tensor& w, const int64_t* targets, const Lists* lists,
+                            const torch::Tensor& logp, const torch::Tensor& lse, int64_t ignore_index, double temperature) {
   const int64_t T = x.size(0), H = x.size(1), V = w.size(0);
   auto f32 = x.options().dtype(torch::kFloat32);
-  auto logp = torch::empty({T}, f32), lse = torch::empty({T}, f32);
-  if (T == 0) return {logp, lse};
-  auto tg = targets.contiguous();
-  if (few_rows(T, H)) {
-    FewParams p = few_params(x, w, tg, ignore_index, temperature);
+  if (few_rows(T, H, lists != nullptr ? lists->K : 0)) {
+    FewParams p = few_params(x, w, targets, ignore_index, temperature);
     auto ws = torch::empty({32 * few_grid(V, H) + 16}, f32);
     p.part = reinterpret_cast<float2*>(ws.data_ptr<float>());
     p.blocks = few_grid(V, H);
@@ -683,9 +944,17 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
     p.ticket = counters.arrivals;
     p.logp = logp.data_ptr<float>();
     p.lse_out = lse.data_ptr<float>();
-    launch_few<false>(p);
+    if (lists != nullptr) {
+      p.K = lists->K;
+      p.lists = lists->lists;
+      p.counts = lists->counts;
+      p.picked = lists->picked;
+      launch_few<kFewLse, true>(p);
+    } else {
+      launch_few<kFewLse>(p);
+    }
     counters.launched();
-    return {logp, lse};
+    return;
   }
   const int64_t blocks = ceil_div(V, vocab::TILE), tiles_t = ceil_div(T, vocab::TILE);
   const bool pack = packs(T, H, V);
@@ -701,7 +970,7 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   p.N = static_cast<int>(V);
   p.H = static_cast<int>(H);
   p.scale = static_cast<float>(1.0 / temperature);
-  p.targets = tg.data_ptr<int64_t>();
+  p.targets = targets;
   p.ignore = ignore_index;
   p.V = V;
   p.ld_part = p.tokens = static_cast<int>(T);
@@ -709,7 +978,8 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   p.target_logit = reinterpret_cast<float*>(base + o_logit);
   p.logp = logp.data_ptr<float>();
   p.lse_out = lse.data_ptr<float>();
-  p.join = blocks <= kJoinBlocks;
+  // a list's rows are joined in a launch of their own, a warp for each
+  p.join = lists == nullptr && blocks <= kJoinBlocks;
   std::optional<ArrivalCounters> counters;
   if (p.join) {
     counters.emplace(tiles_t * 8);
@@ -729,8 +999,9 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
     k.index = reinterpret_cast<int*>(base + o_index);
     k.target = reinterpret_cast<int64_t*>(base + o_target);
     k.xp = reinterpret_cast<bf16*>(base + o_x);
-    k.zero0 = p.logp;
-    k.zero1 = p.lse_out;
+    // what is zeroed for the rows left out; of lists it is done already, and part is spare until the product
+    k.zero0 = lists == nullptr ? p.logp : reinterpret_cast<float*>(p.part);
+    k.zero1 = lists == nullptr ? p.lse_out : reinterpret_cast<float*>(p.part);
     launch_pack(k);
     p.meta = k.meta;
     p.index = k.index;
@@ -738,10 +1009,73 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
   }
   CUtensorMap ta = make_map_any(pack ? base + o_x : x.data_ptr(), H, T, pack ? H : row_ld(x), vocab::HALF);
   CUtensorMap tb = make_map_any(w.data_ptr(), H, V, row_ld(w), vocab::HALF);
+  if (lists != nullptr) {
+    p.lists = lists->lists;
+    p.starts = lists->starts;
+    p.counts = lists->counts;
+    p.K = lists->K;
+    p.picked = lists->picked;
+    launch_vocab<vocab::kLse, true>(ta, tb, ta, tb, ta, p, tiles_t * blocks);
+    launch_after("logprob_join", logprob_join_kernel<true>, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, 2 * blocks);
+    return;
+  }
   launch_vocab<vocab::kLse>(ta, tb, ta, tb, ta, p, tiles_t * blocks);
   if (p.join) counters->launched();
-  else launch_after("logprob_join", logprob_join_kernel, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, 2 * blocks);
+  else launch_after("logprob_join", logprob_join_kernel<false>, dim3(ceil_div(T, 32)), 32 * kJoinWarps, 0, p, 2 * blocks);
+}
+
+// Returns (logp [T], lse [T]), fp32.
+std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets,
+                                              int64_t ignore_index, double temperature) {
+  check_logprob(x, w, targets, temperature);
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto f32 = x.options().dtype(torch::kFloat32);
+  auto logp = torch::empty({x.size(0)}, f32), lse = torch::empty({x.size(0)}, f32);
+  if (x.size(0) == 0) return {logp, lse};
+  auto tg = targets.contiguous();
+  logprob_forward(x, w, tg.data_ptr<int64_t>(), nullptr, logp, lse, ignore_index, temperature);
   return {logp, lse};
+}
+
+// Returns (logp [T, K], lse [T]), fp32.
+std::vector<torch::Tensor> linear_topk_logprob_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor ids, double temperature) {
+  check_lists(x, w, ids, temperature);
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto f32 = x.options().dtype(torch::kFloat32);
+  auto logp = torch::empty({ids.size(0), ids.size(1)}, f32), lse = torch::empty({x.size(0)}, f32);
+  if (x.size(0) == 0) return {logp, lse};
+  const Lists lists = make_lists(ids.contiguous(), w.size(0), temperature, nullptr, logp.data_ptr<float>(),
+                                 lse.data_ptr<float>(), few_rows(x.size(0), x.size(1), ids.size(1)));
+  logprob_forward(x, w, lists.flags, &lists, logp, lse, -1, temperature);
+  return {logp, lse};
+}
+
+// Logits x w^T [T, V] in fp32, the rows V rounded up to 4 apart so that every
+// one begins on 16 bytes.  Bound by writing them, by W's bytes or by the
+// product, in turn with T.
+torch::Tensor linear_logits(torch::Tensor x, torch::Tensor w) {
+  check_layer(x, w);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t T = x.size(0), H = x.size(1), V = w.size(0), ldo = round_up(V, 4);
+  auto out = torch::empty({T, ldo}, x.options().dtype(torch::kFloat32));
+  if (T == 0) return out.narrow(1, 0, V);
+  if (few_rows(T, H)) {
+    FewParams p = few_params(x, w, nullptr, 0, 1.0);
+    p.out = out.data_ptr<float>();
+    p.ldo = ldo;
+    launch_few<kFewLogits>(p);
+    return out.narrow(1, 0, V);
+  }
+  VocabParams p{};
+  p.rows = p.tokens = static_cast<int>(T);
+  p.N = static_cast<int>(V);
+  p.H = static_cast<int>(H);
+  p.out = out.data_ptr<float>();
+  p.ldo = ldo;
+  CUtensorMap ta = make_map_any(x.data_ptr(), H, T, row_ld(x), vocab::HALF);
+  CUtensorMap tb = make_map_any(w.data_ptr(), H, V, row_ld(w), vocab::HALF);
+  launch_vocab<vocab::kLogits>(ta, tb, ta, tb, ta, p, ceil_div(T, vocab::TILE) * ceil_div(V, vocab::TILE));
+  return out.narrow(1, 0, V);
 }
 
 // The softmax gradient u exists for as many vocabulary columns at a time as
@@ -749,36 +1083,32 @@ std::vector<torch::Tensor> linear_logprob_fwd(torch::Tensor x, torch::Tensor w, 
 // gathers the pieces' products in fp32.
 constexpr int64_t kGradBufferBytes = 1ll << 30;
 
-// Writes dx [T, H] and dw [V, H].
-void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, torch::Tensor targets,
-                        torch::Tensor lse, torch::Tensor dx, torch::Tensor dw, int64_t ignore_index,
-                        double temperature) {
-  check_logprob(x, w, targets, temperature);
+static void check_grads(const torch::Tensor& dlogp, const torch::Tensor& x, const torch::Tensor& w,
+                        const torch::Tensor& lse, const torch::Tensor& dx, const torch::Tensor& dw) {
   T1_CHECK_INPUT(dlogp, torch::kFloat32);
   T1_CHECK_INPUT(lse, torch::kFloat32);
   T1_CHECK_INPUT(dx, torch::kBFloat16);
   T1_CHECK_INPUT(dw, torch::kBFloat16);
-  const int64_t T = x.size(0), H = x.size(1), V = w.size(0);
-  TORCH_CHECK(dlogp.dim() == 1 && dlogp.size(0) == T && lse.dim() == 1 && lse.size(0) == T,
-              "dlogp and lse must have T entries");
+  TORCH_CHECK(lse.dim() == 1 && lse.size(0) == x.size(0), "lse must have T entries");
   TORCH_CHECK(dx.sizes() == x.sizes() && dx.is_contiguous(), "dx must be contiguous [T, H]");
   TORCH_CHECK(dw.sizes() == w.sizes() && dw.is_contiguous(), "dw must be contiguous [V, H]");
   TORCH_CHECK(dlogp.device() == x.device() && lse.device() == x.device() && dx.device() == x.device() &&
                   dw.device() == x.device(), "operands must be on one device");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(dx.data_ptr()) % 16 == 0, "dx must be 16-byte aligned");
-  const c10::cuda::CUDAGuard guard(x.device());
-  if (T == 0) {
-    dw.zero_();
-    return;
-  }
-  auto tg = targets.contiguous(), up = dlogp.contiguous(), ls = lse.contiguous();
+}
+
+// dlogp: [T], of lists their sums over tau.
+static void logprob_grads(const float* dlogp, const torch::Tensor& x, const torch::Tensor& w, const int64_t* targets,
+                          const float* lse, const Lists* lists, const torch::Tensor& dx, const torch::Tensor& dw,
+                          int64_t ignore_index, double temperature) {
+  const int64_t T = x.size(0), H = x.size(1), V = w.size(0);
   const int clusters = num_sms() / 2;
   const int64_t tiles_t = ceil_div(T, vocab::TILE), tiles_h = ceil_div(H, vocab::TILE);
 
   const int64_t most = std::max<int64_t>(vocab::TILE, kGradBufferBytes / (2 * T) / vocab::TILE * vocab::TILE);
   const int64_t pieces = ceil_div(V, most);
   const int64_t width = std::min(V, round_up(ceil_div(V, pieces), vocab::TILE));
-  const bool few = few_rows(T, H) && pieces == 1;
+  const bool few = few_rows(T, H, lists != nullptr ? lists->K : 0) && pieces == 1;
   // with few rows nothing is packed: u and x have T rows, and TMA reads zeros
   // past them
   const int64_t ldu = round_up(width, 8), u_rows = few ? T : round_up(T, gemm::BK), k_v = ceil_div(width, gemm::BK);
@@ -795,7 +1125,7 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   const bool may_split = split_tiles > 0;
   Pieces ws;
   const int64_t o_meta = ws.take(sizeof(vocab::RowsMeta)), o_index = ws.take(4 * T), o_target = ws.take(8 * T),
-                o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_x = ws.take(2 * u_rows * H),
+                o_g = ws.take(4 * T), o_lse = ws.take(4 * T), o_live = ws.take(4 * T), o_x = ws.take(2 * u_rows * H),
                 o_planes = ws.take(4 * 8 * vocab::PLANE_BLOCK * planes), o_u = ws.take(2 * u_rows * ldu);
   auto buf = torch::empty({ws.used}, x.options().dtype(torch::kUInt8));
   uint8_t* base = buf.data_ptr<uint8_t>();
@@ -810,14 +1140,21 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   bf16 *u = reinterpret_cast<bf16*>(base + o_u), *xp = reinterpret_cast<bf16*>(base + o_x);
   const CUtensorMap txc = make_map_any(xp, H, u_rows, H, gemm::BK);
   if (few) {
-    FewParams f = few_params(x, w, tg, ignore_index, temperature);
-    f.dlogp = up.data_ptr<float>();
-    f.lse = ls.data_ptr<float>();
+    FewParams f = few_params(x, w, targets, ignore_index, temperature);
+    f.dlogp = dlogp;
+    f.lse = lse;
     f.u = u;
     f.ldu = ldu;
     f.g = reinterpret_cast<float*>(base + o_g);
     f.xz = xp;
-    launch_few<true>(f);
+    if (lists != nullptr) {
+      f.K = lists->K;
+      f.lists = lists->lists;
+      f.counts = lists->counts;
+      launch_few<kFewGrad, true>(f);
+    } else {
+      launch_few<kFewGrad>(f);
+    }
     p.rows = static_cast<int>(T);
     p.splits = pick_splits(tiles_h, k_v, tiles_v * tiles_h, 1, clusters);
     p.N = static_cast<int>(V);
@@ -833,14 +1170,15 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   PackParams k{};
   k.x = (const bf16*)x.data_ptr();
   k.ldx = row_ld(x);
-  k.targets = tg.data_ptr<int64_t>();
+  k.targets = targets;
   k.ignore = ignore_index;
   k.V = V;
   k.T = T;
   k.H = H;
   k.scale = static_cast<float>(1.0 / temperature);
-  k.dlogp = up.data_ptr<float>();
-  k.lse = ls.data_ptr<float>();
+  k.dlogp = dlogp;
+  k.lse = lse;
+  k.live = reinterpret_cast<float*>(base + o_live);
   k.k_blocks = k_v;
   k.tiles_n = tiles_v;
   k.tiles_h = tiles_h;
@@ -852,13 +1190,19 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
   k.lse_packed = reinterpret_cast<float*>(base + o_lse);
   k.xp = xp;
   k.dx = p.dx;
-  launch_pack(k);
+  launch_pack(k, lists != nullptr);
 
   p.meta = k.meta;
   p.scale = k.scale;
   p.index = k.index;
   p.targets = k.target;
   p.lse = k.lse_packed;
+  if (lists != nullptr) {
+    p.lists = lists->lists;
+    p.starts = lists->starts;
+    p.counts = lists->counts;
+    p.K = lists->K;
+  }
   const CUtensorMap tx = make_map_any(xp, H, u_rows, H, vocab::HALF);
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int64_t n = std::min(width, V - v0);
@@ -873,10 +1217,48 @@ void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, t
     const CUtensorMap tuc = make_map_any(u, n, u_rows, ldu, gemm::BK);
     const CUtensorMap tus = make_map_any(u, n, u_rows, ldu, 32);
     const CUtensorMap tdw = make_map_any((bf16*)dw.data_ptr() + v0 * H, H, n, H, 32);
-    launch_vocab<vocab::kSoftmaxGrad>(tx, tw, tx, tw, tus, p, tiles_t * ceil_div(n, vocab::TILE));
+    const int64_t tiles = tiles_t * ceil_div(n, vocab::TILE);
+    p.g = k.g;
+    if (lists != nullptr) launch_vocab<vocab::kSoftmaxGrad, true>(tx, tw, tx, tw, tus, p, tiles);
+    else launch_vocab<vocab::kSoftmaxGrad>(tx, tw, tx, tw, tus, p, tiles);
+    // a list's gradients may add up to 0: every packed row counts
+    if (lists != nullptr) p.g = k.live;
     launch_vocab<vocab::kGrads>(tu, twc, tuc, txc, tdw, p, most_units + ceil_div(n, vocab::TILE) * tiles_h);
   }
   if (may_split) launch_after("logprob_planes", logprob_planes_kernel, dim3(split_tiles * 8, 4), kPlanesThreads, 0, p);
+}
+
+// Writes dx [T, H] and dw [V, H].
+void linear_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, torch::Tensor targets,
+                        torch::Tensor lse, torch::Tensor dx, torch::Tensor dw, int64_t ignore_index,
+                        double temperature) {
+  check_logprob(x, w, targets, temperature);
+  check_grads(dlogp, x, w, lse, dx, dw);
+  TORCH_CHECK(dlogp.dim() == 1 && dlogp.size(0) == x.size(0), "dlogp must have T entries");
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (x.size(0) == 0) {
+    dw.zero_();
+    return;
+  }
+  auto tg = targets.contiguous(), up = dlogp.contiguous(), ls = lse.contiguous();
+  logprob_grads(up.data_ptr<float>(), x, w, tg.data_ptr<int64_t>(), ls.data_ptr<float>(), nullptr, dx, dw, ignore_index,
+                temperature);
+}
+
+// Writes dx [T, H] and dw [V, H].
+void linear_topk_logprob_bwd(torch::Tensor dlogp, torch::Tensor x, torch::Tensor w, torch::Tensor ids, torch::Tensor lse,
+                             torch::Tensor dx, torch::Tensor dw, double temperature) {
+  check_lists(x, w, ids, temperature);
+  check_grads(dlogp, x, w, lse, dx, dw);
+  TORCH_CHECK(dlogp.sizes() == ids.sizes(), "dlogp must be [T, K]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (x.size(0) == 0) {
+    dw.zero_();
+    return;
+  }
+  auto up = dlogp.contiguous(), ls = lse.contiguous();
+  const Lists lists = make_lists(ids.contiguous(), w.size(0), temperature, up.data_ptr<float>(), nullptr, nullptr, false);
+  logprob_grads(lists.sums, x, w, lists.flags, ls.data_ptr<float>(), &lists, dx, dw, -1, temperature);
 }
 
 }  // namespace t1

@@ -1,10 +1,16 @@
 // tcgen05 products of the output layer whose [T, V] result is consumed on
-// the spot.  One kernel, three jobs:
+// the spot.  One kernel, four jobs:
 //   kLse          logits x W^T, reduced to (largest, sum of exponentials) per
 //                 row and 128-column block, and the target's logit;
 //   kSoftmaxGrad  the same logits turned into u = g (onehot - softmax), bf16;
 //   kGrads        both products with u in one launch: the rows of dx = u W, and
-//                 dW = u^T x.
+//                 dW = u^T x;
+//   kLogits       the logits themselves, in fp32.
+// kLse and kSoftmaxGrad also take a list of tokens per row instead of one
+// target (LISTS).  A list is sorted by token, and a table says where in it the
+// tokens of each 128-column block begin, so a warp knows at once whether its
+// block holds any of a row's; where it does, 32 columns at a time go through
+// shared memory, the lane's own 32 words, because registers have no index.
 //
 // The main loop is that of gemm_pair.cuh: CTA pairs (cta_group::2), 256 x 256
 // tiles, 128B-swizzled TMA loads into a 6-stage ring, one elected thread
@@ -31,6 +37,8 @@
 #include "arrivals.cuh"
 #include "gemm_core.cuh"
 
+#include <climits>
+
 namespace t1 {
 namespace vocab {
 
@@ -48,7 +56,7 @@ constexpr int V_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int V_SMEM_BYTES = VSTAGES * V_STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 static_assert(V_SMEM_BYTES <= 232448, "exceeds 227 KB of shared memory");
 
-enum Job : int { kLse = 0, kSoftmaxGrad = 1, kGrads = 2 };
+enum Job : int { kLse = 0, kSoftmaxGrad = 1, kGrads = 2, kLogits = 3 };
 
 // What the packing of the batch's rows found out on the GPU.
 struct RowsMeta {
@@ -88,6 +96,15 @@ struct VocabParams {
   float* planes;           // [tile][split][8] blocks of PLANE_BLOCK
   int64_t plane_blocks;    // allocated
   int first, last;         // first / last piece of the vocabulary
+  // kLogits
+  float* out;              // [rows, ldo]
+  int64_t ldo;             // a multiple of 4
+  // LISTS
+  const int2* lists;       // [T, K] by token: (vocabulary index, kLse: place in the list, kSoftmaxGrad: dlogp / tau)
+  const uint16_t* starts;  // [128-column blocks of the vocabulary + 1][T]
+  const int* counts;       // [T] entries
+  int K;
+  float* picked;           // [T, K] unscaled logits
   int* err;
 };
 
@@ -214,7 +231,7 @@ __device__ __forceinline__ bool get_unit(const Shape& e, int i, int c, int C, Un
 // Operands: kLse, kSoftmaxGrad: A = rows of x, B = W.  kGrads, dx: A = u, B =
 // W by columns; dW: A2 = u by columns, B2 = x by columns.  tma_c: u
 // (kSoftmaxGrad) or dW (kGrads).
-template <int JOB>
+template <int JOB, bool LISTS = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
     vocab_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_a2, const __grid_constant__ CUtensorMap tma_b2,
@@ -255,7 +272,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&tma_a);
     prefetch_tensormap(&tma_b);
-    if (JOB != kLse) prefetch_tensormap(&tma_c);
+    if (JOB != kLse && JOB != kLogits) prefetch_tensormap(&tma_c);
     if (JOB == kGrads) {
       prefetch_tensormap(&tma_a2);
       prefetch_tensormap(&tma_b2);
@@ -435,6 +452,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         return true;
       };
 
+      // the row's list entries in this warp's columns: a cursor on the next one
+      int entry = 0, entry_end = 0, next_col = INT_MAX;
+      const int2* list = nullptr;
+      int2 next = make_int2(0, 0);
+      auto next_entry = [&] {
+        next_col = INT_MAX;
+        if (entry < entry_end) {
+          next = __ldg(list + entry++);
+          next_col = next.x - (p.col0 + tcol0 + half * HALF);
+        }
+      };
+      int64_t token_at = 0;
+      if (LISTS && row < e.rows) {
+        token_at = p.index != nullptr ? p.index[row] : row;
+        if (!T1_OOB(token_at, p.tokens)) {
+          const uint16_t* s = p.starts + (static_cast<int64_t>((p.col0 + tcol0) / HALF) + half) * p.tokens + token_at;
+          entry = __ldg(s);
+          // the last tile's second half may lie past the vocabulary
+          entry_end = tcol0 + half * HALF < p.N ? __ldg(s + p.tokens) : entry;
+          list = p.lists + token_at * p.K;
+          next_entry();
+        }
+      }
+      // the lane's 32 words of the slab: no two lanes share one, nor a bank
+      float* words = reinterpret_cast<float*>(slab) + lane;
+
+      if (JOB == kLogits) {
+        float v[HALF];
+        if (!take_logits(v)) break;
+        const int col0 = tcol0 + half * HALF;
+#pragma unroll
+        for (int c = 0; c < HALF; c += 32) {
+          if (col0 + c >= p.N || row0 >= e.rows) break;  // uniform over the warp
+          // 32 rows x 32 columns, turned so that 8 lanes write 128 bytes of a row
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(slab + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_float4(v[c + 4 * j], v[c + 4 * j + 1], v[c + 4 * j + 2], v[c + 4 * j + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int rr = it * 4 + (lane >> 3), j = lane & 7, col = col0 + c + 4 * j;
+            const float4 f = *reinterpret_cast<const float4*>(slab + rr * 128 + ((j ^ (rr & 7)) << 4));
+            const int64_t at = static_cast<int64_t>(row0 + rr) * p.ldo + col;
+            if (row0 + rr < e.rows && col < p.N && !T1_OOB(at + 3, e.rows * p.ldo)) __stcs(reinterpret_cast<float4*>(p.out + at), f);
+          }
+        }
+        continue;
+      }
+
       if (JOB == kLse) {
         float v[HALF];
         if (!take_logits(v)) break;
@@ -455,13 +523,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < HALF; ++j) a[j & 3] += ex2((v[j] - ref) * k2);
         float s = (a[0] + a[1]) + (a[2] + a[3]);
-        const int64_t t = row_ok ? p.targets[row] - col0 : -1;
-        const bool mine = t >= 0 && t < min(cols, HALF) && !T1_OOB(row, p.ld_part);
-        if (__any_sync(0xffffffffu, mine)) {
-          float x = 0.f;
+        if (LISTS) {
 #pragma unroll
-          for (int j = 0; j < HALF; ++j) x = static_cast<int>(t) == j ? v[j] : x;
-          if (mine) __stcg(&p.target_logit[row], x);
+          for (int c = 0; c < HALF; c += 32) {
+            if (!__any_sync(0xffffffffu, next_col < c + 32)) continue;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) words[32 * j] = v[c + j];
+            while (next_col < c + 32) {
+              if (!T1_OOB(next_col - c, 32) && !T1_OOB(next.y, p.K)) __stcg(&p.picked[token_at * p.K + next.y], words[32 * (next_col - c)]);
+              next_entry();
+            }
+            __syncwarp();
+          }
+        } else {
+          const int64_t t = row_ok ? p.targets[row] - col0 : -1;
+          const bool mine = t >= 0 && t < min(cols, HALF) && !T1_OOB(row, p.ld_part);
+          if (__any_sync(0xffffffffu, mine)) {
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) x = static_cast<int>(t) == j ? v[j] : x;
+            if (mine) __stcg(&p.target_logit[row], x);
+          }
         }
         if (row_ok && !T1_OOB(row, p.ld_part) && !T1_OOB(2 * u.nb + half, 2 * e.tiles_n))
           __stcg(&p.part[static_cast<size_t>(2 * u.nb + half) * p.ld_part + row], make_float2(m, s));
@@ -526,8 +608,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
         if (row_ok) {
           gr = p.g[row];
           lse = p.lse[row];
-          const int64_t t = p.targets[row] - p.col0 - col0;
-          tcol = t >= 0 && t < HALF ? static_cast<int>(t) : -1;
+          if (!LISTS) {
+            const int64_t t = p.targets[row] - p.col0 - col0;
+            tcol = t >= 0 && t < HALF ? static_cast<int>(t) : -1;
+          }
         }
 #pragma unroll
         for (int c = 0; c < HALF; c += 64) {
@@ -535,6 +619,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
           // the store issued from the slab before has read it
           if (lane == 0) bulk_wait_group_read<0>();
           __syncwarp();
+          if (LISTS) {
+#pragma unroll
+            for (int right = 0; right < 2; ++right) {
+              const int cc = c + 32 * right;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[cc + j] = -gr * ex2(fmaf(v[cc + j], p.scale, -lse) * kLog2e);
+              if (!__any_sync(0xffffffffu, next_col < cc + 32)) continue;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) words[32 * j] = v[cc + j];
+              while (next_col < cc + 32) {
+                if (!T1_OOB(next_col - cc, 32)) words[32 * (next_col - cc)] += __int_as_float(next.y);
+                next_entry();
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[cc + j] = words[32 * j];
+              __syncwarp();
+            }
+#pragma unroll
+            for (int right = 0; right < 2; ++right) {
+              float f[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] = v[c + 32 * right + j];
+              to_slab(f, right, !row_ok);
+            }
+            store_slab(c);
+            continue;
+          }
 #pragma unroll
           for (int right = 0; right < 2; ++right) {
             float f[32];

@@ -14,6 +14,8 @@ from __future__ import annotations
 
 import os
 
+import torch
+
 from . import reference
 
 _FORCE_TORCH = os.environ.get("T1_OPS", "native").lower() == "torch"
@@ -161,6 +163,135 @@ def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, 
         raise ValueError(f"advantages must be [T] or [T / seq_len], got {tuple(advantages.shape)}")
     return _impl(logp).policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, clip_low,
                                            clip_high, kl_coef, reduction, ignore_index)
+
+
+MAX_LIST = 512  # tokens of a row's list
+
+
+def linear_logits(x, w):
+    """Logits x @ w^T in fp32: x [T, H], w [V, H] -> [T, V].  The rows of the
+    result may lie further apart than V."""
+    return _impl(x).linear_logits(x, w)
+
+
+def topk_logprobs(logits, k, temperature=1.0):
+    """The k likeliest tokens of every row of ``logits`` [T, V] (fp32 or bf16)
+    and their log-probabilities under softmax(logits / temperature):
+    (logp [T, k] fp32, ids [T, k] int64), likeliest first, of equals the lowest
+    index first.  Logits of -inf and NaN are no tokens; a row that has fewer
+    than k ends with ids of -1 and log-probabilities of 0.  k is at most
+    MAX_LIST."""
+    _check_logits(logits, temperature)
+    if not 1 <= k <= min(MAX_LIST, logits.shape[1]):
+        raise ValueError(f"k must lie in [1, {min(MAX_LIST, logits.shape[1])}], got {k}")
+    return _impl(logits).topk_logprobs(logits, int(k), float(temperature))
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token of every row of ``logits`` [B, V] (fp32 or bf16), drawn with
+    the random numbers u [B] (fp32, in [0, 1)) from softmax(logits /
+    temperature) after three cuts, all on the tokens' order by logit (of equals
+    the lowest index first): ``top_k`` keeps the first top_k (0: all); ``top_p``
+    keeps, of these, the ones before which less than top_p of their probability
+    has come (1: all); ``min_p`` keeps those at least min_p times as likely as
+    the likeliest.  The draw takes the lowest index whose running sum over the
+    kept tokens, in index order, exceeds u times their sum, and is the same for
+    the same inputs.  Returns (token [B] int64, logp [B] fp32), logp under the
+    tempered distribution before the cuts, as ``linear_logprob_fwd`` gives it.
+    Logits of -inf and NaN are no tokens; a row without any gives -1 and 0."""
+    _check_logits(logits, temperature)
+    check_sampling(temperature, top_k, top_p, min_p)
+    if u.dim() != 1 or u.shape[0] != logits.shape[0]:
+        raise ValueError(f"u must be [{logits.shape[0]}], got {tuple(u.shape)}")
+    if u.dtype != torch.float32:
+        raise ValueError(f"u must be float32, got {u.dtype}")
+    return _impl(logits).sample_tokens(logits, u, float(temperature), int(top_k), float(top_p), float(min_p))
+
+
+def linear_topk_logprob_fwd(x, w, ids, temperature=1.0):
+    """Log-probabilities of a list of tokens of every row under the output
+    layer: logits = x @ w^T / temperature, of which no [T, V] tensor is kept.
+    x [T, H], w [V, H], ids [T, K] int64 (a teacher's likeliest tokens; K at
+    most MAX_LIST) -> (logp [T, K], lse [T]) in fp32.  Entries outside the
+    vocabulary give 0, and rows without any other give 0 in lse too: they take
+    no part."""
+    _check_lists(x, w, ids, temperature)
+    return _impl(x).linear_topk_logprob_fwd(x, w, ids, float(temperature))
+
+
+def linear_topk_logprob_bwd(dlogp, x, w, ids, lse, dx, dw, temperature=1.0):
+    """Gradients of ``linear_topk_logprob_fwd``: from dlogp [T, K] (fp32) and
+    the forward's lse, writes dx [T, H] and dw [V, H].  A token that a list
+    names twice gets both gradients.  Entries of dlogp whose token is outside
+    the vocabulary are not used."""
+    _check_lists(x, w, ids, temperature)
+    if dlogp.shape != ids.shape:
+        raise ValueError(f"dlogp must be {tuple(ids.shape)}, got {tuple(dlogp.shape)}")
+    _impl(x).linear_topk_logprob_bwd(dlogp, x, w, ids, lse, dx, dw, float(temperature))
+
+
+DISTILLATION_KINDS = reference.DISTILLATION_KINDS
+
+
+def distillation_loss_fwd_bwd(logp, teacher_logp, ids, kind="forward", tail=True):
+    """Divergence of a student from its teacher on the teacher's likeliest
+    tokens.
+
+    logp and teacher_logp [T, K] (fp32; the teacher's also bf16) are both
+    models' log-probabilities of the tokens ids [T, K] (int64).  Entries of a
+    negative id, or of a teacher's log-probability of -inf, are left out, and
+    rows without any entry take no part; a row's ids must differ.  With p the
+    student's and q the teacher's probabilities of the listed tokens and, with
+    ``tail``, of the rest of the vocabulary as one more outcome (at least
+    2^-20: less is the rounding of what is listed), without it scaled to sum to
+    1 over the list:
+      forward  sum q log(q / p)
+      reverse  sum p log(p / q)
+      jensen   half of sum p log(p / m) + q log(q / m), m = (p + q) / 2
+    Returns (loss [] fp32, the mean over the rows that take part; dloss/dlogp
+    [T, K]; the divergence of every row [T])."""
+    if logp.dim() != 2 or teacher_logp.shape != logp.shape or ids.shape != logp.shape:
+        raise ValueError(f"logp, teacher_logp and ids must be [T, K], got {tuple(logp.shape)}, "
+                         f"{tuple(teacher_logp.shape)} and {tuple(ids.shape)}")
+    if not 1 <= logp.shape[1] <= MAX_LIST:
+        raise ValueError(f"a list has 1 to {MAX_LIST} tokens, got {logp.shape[1]}")
+    check_distillation(kind)
+    return _impl(logp).distillation_loss_fwd_bwd(logp, teacher_logp, ids, kind, bool(tail))
+
+
+def check_distillation(kind):
+    if kind not in DISTILLATION_KINDS:
+        raise ValueError(f"kind must be one of {DISTILLATION_KINDS}, got {kind!r}")
+
+
+def check_sampling(temperature, top_k, top_p, min_p):
+    if not 0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    if top_k < 0 or top_k != int(top_k):
+        raise ValueError(f"top_k must be a whole number, 0 for all tokens, got {top_k}")
+    if not 0 < top_p <= 1:
+        raise ValueError(f"top_p must lie in (0, 1], got {top_p}")
+    if not 0 <= min_p <= 1:
+        raise ValueError(f"min_p must lie in [0, 1], got {min_p}")
+
+
+def _check_logits(logits, temperature):
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be [T, V], got {tuple(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    if not 0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive, got {temperature}")
+
+
+def _check_lists(x, w, ids, temperature):
+    if x.dim() != 2 or w.dim() != 2 or ids.dim() != 2 or ids.shape[0] != x.shape[0]:
+        raise ValueError(f"x must be [T, H], w [V, H] and ids [T, K], got {tuple(x.shape)}, {tuple(w.shape)} and "
+                         f"{tuple(ids.shape)}")
+    if not 1 <= ids.shape[1] <= MAX_LIST:
+        raise ValueError(f"a list has 1 to {MAX_LIST} tokens, got {ids.shape[1]}")
+    if not 0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive, got {temperature}")
 
 
 def check_preference(beta, kind, label_smoothing):

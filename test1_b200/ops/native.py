@@ -211,3 +211,33 @@ def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, 
                                           float(clip_low), float(clip_high), float(kl_coef),
                                           reduction == "sequence", int(ignore_index))
     return loss, dlogp, stats
+
+
+# --------------------------------------------- logits, their likeliest tokens, a draw
+def linear_logits(x, w):
+    return _c().linear_logits(x, w)
+
+
+def topk_logprobs(logits, k, temperature=1.0):
+    logp, ids = _c().topk_logprobs(logits, k, temperature)
+    return logp, ids
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    token, logp = _c().sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+    return token, logp
+
+
+# --------------------------- log-probabilities at lists of tokens, distillation
+def linear_topk_logprob_fwd(x, w, ids, temperature=1.0):
+    logp, lse = _c().linear_topk_logprob_fwd(x, w, ids, temperature)
+    return logp, lse
+
+
+def linear_topk_logprob_bwd(dlogp, x, w, ids, lse, dx, dw, temperature=1.0):
+    _c().linear_topk_logprob_bwd(dlogp, x, w, ids, lse, dx, dw, temperature)
+
+
+def distillation_loss_fwd_bwd(logp, teacher_logp, ids, kind="forward", tail=True):
+    loss, dlogp, each = _c().distillation_loss(logp, teacher_logp, ids, _ref.DISTILLATION_KINDS.index(kind), tail)
+    return loss, dlogp, each

@@ -378,6 +378,140 @@ def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, 
     return loss, torch.where(valid, grad * weight[:, None], 0.0).reshape(-1), stats
 
 
+# --------------------------------------------- logits, their likeliest tokens, a draw
+
+
+def linear_logits(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    return x.float() @ w.float().t()
+
+
+def _tokens_of(logits: torch.Tensor, temperature: float, dtype):
+    """Logits in ``dtype`` with NaN as -inf, and log of the tempered
+    distribution: an infinite logit outweighs all finite ones."""
+    z = logits.to(dtype)
+    z = torch.where(torch.isnan(z), -math.inf, z)
+    top = z.max(dim=-1, keepdim=True).values
+    t = torch.where(z == top, 0.0, (z - top) / temperature)
+    t = torch.where(z == -math.inf, -math.inf, t)
+    total = torch.exp(t).sum(dim=-1, keepdim=True)
+    return z, t, torch.where(total > 0, t - torch.log(total), t)
+
+
+def topk_logprobs(logits: torch.Tensor, k: int, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The formulas are at ``ops.topk_logprobs``."""
+    z, _, logp = _tokens_of(logits, temperature, torch.float32)
+    z, ids = torch.sort(z, dim=-1, descending=True, stable=True)
+    none = z[:, :k] == -math.inf
+    ids = ids[:, :k]
+    return torch.where(none, 0.0, logp.gather(1, ids)), torch.where(none, -1, ids)
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                  min_p: float = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The formulas are at ``ops.sample_tokens``.  Weights in 64 bits: in 32 a
+    draw near a border takes a neighbour."""
+    z, t, logp = _tokens_of(logits, temperature, torch.float64)
+    order = torch.sort(z, dim=-1, descending=True, stable=True).indices
+    w = torch.exp(t).gather(1, order)
+    if top_k:
+        w[:, top_k:] = 0
+    if top_p < 1:
+        before = w.cumsum(dim=1) - w
+        w = torch.where(before < top_p * w.sum(dim=1, keepdim=True), w, 0.0)
+    w = torch.where(w >= min_p, w, 0.0)
+    cdf = torch.zeros_like(w).scatter_(1, order, w).cumsum(dim=1)
+    u = u.double().nan_to_num(0.0).clamp(0.0, 1.0 - 2.0 ** -53)
+    token = (cdf <= u[:, None] * cdf[:, -1:]).sum(dim=1).clamp_max(z.shape[1] - 1)
+    none = (z == -math.inf).all(dim=1)
+    logp = logp.gather(1, token[:, None])[:, 0]
+    return torch.where(none, -1, token), torch.where(none, 0.0, logp).float()
+
+
+# --------------------------- log-probabilities at lists of tokens, distillation
+
+
+def _listed(ids: torch.Tensor, vocab: int) -> torch.Tensor:
+    return (ids >= 0) & (ids < vocab)
+
+
+def linear_topk_logprob_fwd(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor,
+                            temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """log softmax(x w^T / temperature)[t, ids[t, k]] and the row's log-sum-exp
+    (fp32); entries that name no token, and rows without any that does, give 0."""
+    keep = _listed(ids, w.shape[0])
+    logits = (x.float() @ w.float().t()) / temperature
+    top = logits.max(dim=-1).values
+    log_sum = torch.logsumexp(logits - top[:, None], dim=-1)
+    picked = logits.gather(1, torch.where(keep, ids, 0))
+    return (torch.where(keep, (picked - top[:, None]) - log_sum[:, None], 0.0),
+            torch.where(keep.any(dim=1), top + log_sum, 0.0))
+
+
+def linear_topk_logprob_bwd(dlogp: torch.Tensor, x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor,
+                            dx: torch.Tensor, dw: torch.Tensor, temperature: float = 1.0) -> None:
+    """Writes dx and dw from dlogp and the forward's lse (fp32 arithmetic,
+    rounded once)."""
+    keep = _listed(ids, w.shape[0])
+    up = torch.where(keep, dlogp.float() / temperature, 0.0)
+    rows = (up != 0).any(dim=1).nonzero()[:, 0]
+    xf, wf, up = x[rows].float(), w.float(), up[rows]
+    u = torch.exp(xf @ wf.t() / temperature - lse[rows, None]) * -up.sum(dim=1, keepdim=True)
+    u.scatter_add_(1, torch.where(keep, ids, 0)[rows], up)
+    dx.zero_()
+    dx[rows] = (u @ wf).to(dx.dtype)
+    dw.copy_(u.t() @ xf)
+
+
+DISTILLATION_KINDS = ("forward", "reverse", "jensen")
+REST_FLOOR = 2.0 ** -20
+
+
+def distillation_loss_fwd_bwd(logp: torch.Tensor, teacher_logp: torch.Tensor, ids: torch.Tensor, kind: str = "forward",
+                              tail: bool = True):
+    """Returns (loss, dloss/dlogp [T, K], divergence [T]); the formulas are at
+    ``ops.distillation_loss_fwd_bwd``."""
+    b = teacher_logp.float()
+    keep = (ids >= 0) & (b > -math.inf)
+    live = keep.any(dim=1)
+    a, b = torch.where(keep, logp.float(), 0.0), torch.where(keep, b, 0.0)
+    if not tail:
+        def log_sum(v):
+            s = torch.logsumexp(torch.where(keep, v, -math.inf), dim=1, keepdim=True)
+            return torch.where(live[:, None], s, 0.0)
+        a, b = a - log_sum(a), b - log_sum(b)
+    p, q = (torch.where(keep, torch.exp(v), 0.0) for v in (a, b))
+
+    def divergence(p, q, a, b):
+        """f(p, q) and p df/dp, with a = log p and b = log q; 0 log 0 is 0."""
+        def times(weight, log):
+            return torch.where(weight > 0, weight * log, 0.0)
+        if kind == "forward":
+            return times(q, b - a), -q
+        if kind == "reverse":
+            f = times(p, a - b)
+            return f, f + p
+        log_m = torch.log((p + q) / 2)
+        f = times(p / 2, a - log_m)
+        return f + times(q / 2, b - log_m), f
+
+    f, g = divergence(p, q, a, b)
+    f, g = torch.where(keep, f, 0.0), torch.where(keep, g, 0.0)
+    each = f.sum(dim=1)
+    if tail:
+        def rest(v):  # what is left of 1, whose last bits count
+            return 1 - torch.where(keep, torch.exp(v.double()), 0.0).sum(dim=1, keepdim=True)
+        rp, rq = rest(a), rest(b)
+        pr, qr = rp.clamp_min(REST_FLOOR).float(), rq.clamp_min(REST_FLOOR).float()
+        fr, gr = divergence(pr, qr, torch.log(pr), torch.log(qr))
+        each = each + fr[:, 0]
+        d = g - p * torch.where(rp > REST_FLOOR, gr / pr, 0.0)
+    else:
+        d = g - p * g.sum(dim=1, keepdim=True)
+    n = live.sum().clamp_min(1).float()
+    each = torch.where(live, each, 0.0)
+    return each.sum() / n, torch.where(keep, d / n, 0.0), each
+
+
 # ------------------------------------------------ fused-layout entry points
 # The model keeps q/k/v as column blocks of one [T, (Hq + 2 Hkv) * D] buffer
 # and gate/up as the two halves of one [T, 2 I] buffer; these wrappers state
