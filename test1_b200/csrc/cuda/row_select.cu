@@ -11,9 +11,18 @@
 // -inf and NaN are no tokens; a logit of +inf outweighs all finite ones.
 //
 // A cluster of CTAs holds one row in shared memory: one read of the logits, and
-// every thread keeps to the same few of them in every pass.  Thresholds are found digit by
-// digit of the order-preserving integer of a logit (8 bits at a time), with the
-// CTAs' histograms added up over distributed shared memory.
+// every thread keeps to the same few of them in every pass.  Three ways to the
+// cut, of which the first two touch few logits more than once:
+//   list   the first n <= 1024: no n tokens can all lie below the n-th largest
+//          of the threads' own largest ones, which a histogram of their
+//          distances from m finds.  What lies above (little more than n) goes to
+//          the first CTA, which sorts it and does all the rest.
+//   bins   top_p alone: weights added up by distance from m, 16 bins per unit of
+//          the exponent; the tokens of the bin where top_p is reached are sorted
+//          by the first CTA.
+//   digits where neither applies (more tokens are asked for, or too many are
+//          equal): the threshold is found digit by digit, 8 bits at a time, of
+//          the order-preserving integer of a logit.
 //
 // Weights are 64-bit whole numbers, round(w 2^s) with V 2^s <= 2^62, from
 // exponentials in 64 bits: their sums do not depend on the order of the
@@ -34,14 +43,19 @@ namespace cg = cooperative_groups;
 using bf16_t = __nv_bfloat16;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMostCtas = 16;   // of a cluster
-constexpr int kMostList = 512;  // tokens of `top`
+constexpr int kMostCtas = 8;      // of a cluster
+constexpr int kMostList = 512;    // tokens of `top`
+constexpr int kListSlots = 1024;  // tokens that the first CTA sorts
 constexpr int kDigits = 256;
+constexpr int kBins = 256;
+constexpr int kExps = 128;        // steps of an octave in the table of exponentials
 
 struct Params {
   const void* logits;
   int64_t ld;
   int rows, V;
+  int per_thread;  // columns
+  bool aligned;    // rows begin on 16 bytes
   float scale;     // 1 / tau
   double scale64;
   // top
@@ -50,20 +64,44 @@ struct Params {
   int64_t* ids;    // [rows, k]; sample: [rows]
   // sample
   const float* u;
-  int top_k;                  // 0: all
-  double top_p;               // 1: all
-  double log_min_p;           // -inf: all
-  double one;                 // the weight of the largest logit, 2^s
-  int per_thread;             // columns
+  int top_k;         // 0: all
+  double top_p;      // 1: all
+  double log_min_p;  // -inf: all
+  int one;           // s: the largest logit's weight is 2^s
 };
 
-// A logit to shared memory: 32-bit ones without a stop in a register.
-__device__ __forceinline__ void fetch(float* to, const float* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from)
-               : "memory");
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// Logits from..from + n to shared memory as fp32, by one warp.
+__device__ __forceinline__ void fetch(float* to, const float* from, int n, bool aligned, int lane) {
+  if (aligned) {
+    const int vecs = n / 4;
+    for (int i = lane; i < vecs; i += 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(to + 4 * i)), "l"(from + 4 * i) : "memory");
+    to += 4 * vecs;
+    from += 4 * vecs;
+    n -= 4 * vecs;
+  }
+  for (int i = lane; i < n; i += 32)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(to + i)), "l"(from + i) : "memory");
 }
-__device__ __forceinline__ void fetch(float* to, const bf16_t* from) {
-  *to = __bfloat162float(__ushort_as_bfloat16(__ldcs(reinterpret_cast<const unsigned short*>(from))));
+__device__ __forceinline__ void fetch(float* to, const bf16_t* from, int n, bool aligned, int lane) {
+  if (aligned) {
+    const int vecs = n / 8;
+#pragma unroll 4
+    for (int i = lane; i < vecs; i += 32) {
+      float f[8];
+      load8(from + 8 * i, f);
+      reinterpret_cast<float4*>(to)[2 * i] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(to)[2 * i + 1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    to += 8 * vecs;
+    from += 8 * vecs;
+    n -= 8 * vecs;
+  }
+#pragma unroll 8
+  for (int i = lane; i < n; i += 32)
+    to[i] = __bfloat162float(__ushort_as_bfloat16(__ldcs(reinterpret_cast<const unsigned short*>(from + i))));
 }
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -75,6 +113,14 @@ __device__ __forceinline__ unsigned key_of(float z) {
 __device__ __forceinline__ float logit_of(unsigned key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+// The order of tokens as one number: larger ones come first.
+__device__ __forceinline__ unsigned long long place_of(float z, int column) {
+  return static_cast<unsigned long long>(key_of(z)) << 32 | ~static_cast<unsigned>(column);
+}
+__device__ __forceinline__ float logit_at(unsigned long long place) { return logit_of(static_cast<unsigned>(place >> 32)); }
+__device__ __forceinline__ int column_at(unsigned long long place) { return static_cast<int>(~static_cast<unsigned>(place)); }
+
+__device__ __forceinline__ bool is_token(float z) { return z > -INFINITY; }
 
 __device__ __forceinline__ unsigned long long warp_sum64(unsigned long long v) {
 #pragma unroll
@@ -91,28 +137,77 @@ __device__ __forceinline__ unsigned long long warp_scan64(unsigned long long v, 
 }
 
 struct Shared {
-  unsigned hist[2][kDigits];
-  unsigned long long weights[2][kDigits];
+  double exps[kExps];              // 2^(j / 128)
   unsigned long long red[kWarps];
+  unsigned bins[3][kBins];         // counts; of weights 16 bits each
+  union {
+    struct {
+      unsigned hist[2][kDigits];
+      unsigned long long weights[2][kDigits];
+    };
+    unsigned long long list[kListSlots];  // of the first CTA
+    unsigned long long cells[32][33];     // weights of the warp that holds the drawn token
+  };
   // what every CTA of the cluster tells all others, once each
   float max_of[kMostCtas];
   float sum_of[kMostCtas];
   unsigned count_of[kMostCtas], ties_of[kMostCtas];
-  unsigned long long total_of[kMostCtas], kept_of[kMostCtas];
-  // the digit that a threshold falls into
-  unsigned digit, before32, in32;
+  unsigned long long total_of[kMostCtas], kept_of[kMostCtas], cut_of[kMostCtas];
+  // where a threshold falls
+  unsigned digit, before32;
+  int bin;
   unsigned long long before64;
   unsigned listed;
-  unsigned long long list[kMostList];   // of the first CTA
-  unsigned long long cells[32][33];     // weights of the warp that holds the drawn token
 };
+
+__device__ __forceinline__ void sync_all(cg::cluster_group& cluster) {
+  if (cluster.num_blocks() == 1) __syncthreads();
+  else cluster.sync();
+}
 
 // Every CTA's value to all of the cluster, in slots[rank]; one barrier.
 template <typename V>
 __device__ __forceinline__ void tell_all(cg::cluster_group& cluster, V* slots, V value) {
   const unsigned n = cluster.num_blocks();
   if (threadIdx.x < n) cluster.map_shared_rank(slots, threadIdx.x)[cluster.block_rank()] = value;
-  cluster.sync();
+  sync_all(cluster);
+}
+
+// Sum of the threads' values; every thread gets it, and the sum of the threads
+// before it.
+__device__ __forceinline__ unsigned long long block_scan64(unsigned long long v, unsigned long long& before,
+                                                           unsigned long long* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned long long upto = warp_scan64(v, lane);
+  __syncthreads();
+  if (lane == 31) red[warp] = upto;
+  __syncthreads();
+  unsigned long long sum = 0, of_warps = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) of_warps = sum;
+    sum += red[w];
+  }
+  before = of_warps + upto - v;
+  return sum;
+}
+
+// Descending, slots a power of two.
+__device__ __forceinline__ void sort_list(unsigned long long* list, unsigned slots) {
+  for (unsigned size = 2; size <= slots; size *= 2) {
+    for (unsigned step = size / 2; step > 0; step /= 2) {
+      __syncthreads();
+      for (unsigned q = threadIdx.x; q < slots / 2; q += kThreads) {
+        const unsigned i = 2 * q - (q & (step - 1)), j = i + step;
+        const unsigned long long a = list[i], b = list[j];
+        if ((a < b) == ((i & size) == 0)) {
+          list[i] = b;
+          list[j] = a;
+        }
+      }
+    }
+  }
+  __syncthreads();
 }
 
 // A prefix of the order: all tokens of a larger key, and the first `ties` of
@@ -125,80 +220,271 @@ struct Cut {
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
   __shared__ Shared sh;
-  extern __shared__ float held[];
+  __shared__ float red[32];
+  extern __shared__ __align__(16) float held[];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / ctas;
   // a warp has 32 n columns in a row, a thread every 32nd of them
   const int n = p.per_thread;
-  const int col0 = (rank * kWarps + warp) * 32 * n + lane;
+  const int warp_col0 = (rank * kWarps + warp) * 32 * n, col0 = warp_col0 + lane;
   float* v = held + warp * 32 * n + lane;  // v[32 i]: the thread's i-th
   constexpr int kLowest = sizeof(T) == 2 ? 16 : 0;  // key bits below are the same in all of a type's values
+  if (T1_OOB(row, p.rows)) return;
 
-  const T* src = static_cast<const T*>(p.logits) + row * p.ld;
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) {
-    const int c = col0 + 32 * i;
-    if (c < p.V) fetch(&v[32 * i], src + c);
-    else v[32 * i] = -INFINITY;
+  {
+    const int cols = max(0, min(32 * n, p.V - warp_col0));
+    fetch(held + warp * 32 * n, static_cast<const T*>(p.logits) + row * p.ld + warp_col0, cols, p.aligned, lane);
+    for (int c = cols + lane; c < 32 * n; c += 32) held[warp * 32 * n + c] = -INFINITY;
   }
+  for (int i = tid; i < 3 * kBins; i += kThreads) sh.bins[0][i] = 0;
+  if (tid == 0) sh.listed = 0;
+  if (!TOP && tid < kExps) sh.exps[tid] = exp2(tid / static_cast<double>(kExps));
   fetched();
-  float m = -INFINITY;
+  __syncwarp();
+  float own_max = -INFINITY;
   unsigned count = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = 0; i < n; ++i) {
     float z = v[32 * i];
     z = z == z ? z + 0.f : -INFINITY;  // -0 is 0
     v[32 * i] = z;
-    m = fmaxf(m, z);
-    count += z > -INFINITY;
+    own_max = fmaxf(own_max, z);
+    count += is_token(z);
   }
 
   // ---- largest logit, number of tokens
-  __shared__ float red[32];
-  m = block_max(m, red);
+  float m = block_max(own_max, red);
   {
-    unsigned long long c = warp_sum64(count);
+    unsigned c = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) sh.red[warp] = c;
     __syncthreads();
-    c = 0;
-    for (int w = 0; w < kWarps; ++w) c += sh.red[w];
-    count = static_cast<unsigned>(c);
+    count = 0;
+    for (int w = 0; w < kWarps; ++w) count += static_cast<unsigned>(sh.red[w]);
   }
-  if (tid < static_cast<unsigned>(ctas)) cluster.map_shared_rank(sh.max_of, tid)[rank] = m;
+  if (tid < ctas) cluster.map_shared_rank(sh.max_of, tid)[rank] = m;
   tell_all(cluster, sh.count_of, count);
   count = 0;
   for (int r = 0; r < ctas; ++r) {
     m = fmaxf(m, sh.max_of[r]);
     count += sh.count_of[r];
   }
+  if (count == 0) {
+    if (rank != 0) return;
+    for (int i = tid; i < (TOP ? p.k : 1); i += kThreads) {
+      p.ids[static_cast<int64_t>(row) * (TOP ? p.k : 1) + i] = -1;
+      p.logp[static_cast<int64_t>(row) * (TOP ? p.k : 1) + i] = 0.f;
+    }
+    return;
+  }
 
-  // ---- log of the sum of all weights
-  float sum = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) sum += v[32 * i] == m ? 1.f : __expf((v[32 * i] - m) * p.scale);
-  if (m == -INFINITY) sum = 0.f;
-  sum = block_sum(sum, red);
-  tell_all(cluster, sh.sum_of, sum);
-  sum = 0.f;
-  for (int r = 0; r < ctas; ++r) sum += sh.sum_of[r];
-  const float log_sum = logf(sum);
-
-  auto log_weight = [&](float z) {
-    return z == m ? 0.0 : (static_cast<double>(z) - static_cast<double>(m)) * p.scale64;
+  const double m64 = m;
+  auto log_weight = [&](float z) { return z == m ? 0.0 : (static_cast<double>(z) - m64) * p.scale64; };
+  // exp(t) 2^s for t <= 0: 2^(j / 128) from the table, the rest of the exponent (|r| < 0.0028) by its series, whose
+  // first term left out is below 1.4e-15
+  auto weight_at = [&](double t) -> unsigned long long {
+    if (t < -64.0) return 0ull;
+    constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: adding it leaves a whole number in the low bits
+    const double y = fma(t, 1.4426950408889634 * kExps, kRound);
+    const int j = __double2loint(y);
+    const double r = fma(y - kRound, -0.6931471805599453 / kExps, t);
+    double e = fma(r, 1.0 / 24, 1.0 / 6);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    const double base = sh.exps[j & (kExps - 1)];
+    const double scaled = __hiloint2double(__double2hiint(base) + (((j >> 7) + p.one) << 20), __double2loint(base));
+    constexpr double kWhole = 4503599627370496.0;  // 2^52
+    return __double_as_longlong(fma(e, scaled, kWhole)) - __double_as_longlong(kWhole);
   };
-  auto weight = [&](float z) -> unsigned long long { return __double2ull_rn(exp(log_weight(z)) * p.one); };
-  // a key from its digits: the bits below are 0, of a negative logit 1
-  auto with_low_bits = [](unsigned prefix) { return kLowest == 0 || prefix & 0x80000000u ? prefix : prefix | ((1u << kLowest) - 1); };
-  auto is_token = [](float z) { return z > -INFINITY; };
+  static_assert(kExps == 128, "j >> 7");
+  auto weight = [&](float z) { return weight_at(log_weight(z)); };
+  // Distance from m in steps of a sixteenth of its octave, 2^-8 to 2^8.
+  auto step_of = [&](float z) {
+    const int s = static_cast<int>(__float_as_uint(z == m ? 0.f : m - z) >> 19) - (119 << 4);
+    return min(max(s, 0), kBins - 1);
+  };
+  // Distance from m in sixteenths of the exponent's unit.
+  auto bin_of = [&](float z) { return z == m ? 0 : static_cast<int>(fminf((m - z) * p.scale * 16.f, kBins - 1.f)); };
 
+  const unsigned first = TOP ? p.k : p.top_k;
+  const bool cut_first = first != 0 && first < count;
+  const bool by_list = cut_first && first <= kListSlots / 2 && first <= static_cast<unsigned>(ctas * kThreads);
+  const bool by_bins = !TOP && !cut_first && p.top_p < 1.0;
+
+  // ---- log of the sum of all weights, and the sum by bins
+  float log_sum;
+  unsigned long long total = 0, own = 0;  // own: the thread's kept weight
+  if (TOP || cut_first) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) sum += v[32 * i] == m ? 1.f : __expf((v[32 * i] - m) * p.scale);
+    if (by_list && is_token(own_max)) atomicAdd(&sh.bins[0][step_of(own_max)], 1u);
+    sum = block_sum(sum, red);
+    tell_all(cluster, sh.sum_of, sum);
+    sum = 0.f;
+    for (int r = 0; r < ctas; ++r) sum += sh.sum_of[r];
+    log_sum = logf(sum);
+  } else {
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
+      const float z = v[32 * i];
+      if (!is_token(z)) continue;
+      const unsigned long long w = weight(z);
+      own += w;
+      if (by_bins) {
+        const int b = bin_of(z);
+        if (b < kBins - 1) {
+          const unsigned lo = static_cast<unsigned>(w) & 0xffffu, mid = static_cast<unsigned>(w >> 16) & 0xffffu,
+                         hi = static_cast<unsigned>(w >> 32);
+          atomicAdd(&sh.bins[0][b], lo);
+          if (mid != 0) atomicAdd(&sh.bins[1][b], mid);
+          if (hi != 0) atomicAdd(&sh.bins[2][b], hi);
+        }
+      }
+    }
+    unsigned long long before;
+    tell_all(cluster, sh.total_of, block_scan64(own, before, sh.red));
+    for (int r = 0; r < ctas; ++r) total += sh.total_of[r];
+    log_sum = static_cast<float>(log(ldexp(static_cast<double>(total), -p.one)));
+  }
+
+  // ---- list and bins: the step or bin that the cut falls into, and its tokens to the first CTA
+  bool done = false;           // by the list or bins
+  unsigned listed = 0;
+  int cut_bin = 0;
+  unsigned long long cut_place = 0;
+  if (by_list || by_bins) {
+    const unsigned long long need =
+        by_list ? first : max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(total)));
+    unsigned long long here = 0, before;
+    if (tid < kBins) {
+      for (int r = 0; r < ctas; ++r) {
+        const unsigned* b = cluster.map_shared_rank(&sh.bins[0][0], r);
+        here += b[tid];
+        if (!by_list) here += (static_cast<unsigned long long>(b[kBins + tid]) << 16) + (static_cast<unsigned long long>(b[2 * kBins + tid]) << 32);
+      }
+    }
+    if (tid == 0) sh.bin = kBins;
+    block_scan64(here, before, sh.red);
+    if (before < need && before + here >= need) {
+      sh.bin = tid;
+      sh.before64 = before;
+    }
+    __syncthreads();
+    cut_bin = sh.bin;
+    if (cut_bin < kBins - 1) {
+      unsigned* to = cluster.map_shared_rank(&sh.listed, 0);
+      unsigned long long* list = cluster.map_shared_rank(sh.list, 0);
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float z = v[32 * i];
+        if (is_token(z) && (by_list ? step_of(z) <= cut_bin : bin_of(z) == cut_bin)) {
+          const unsigned at = atomicAdd(to, 1u);
+          if (at < kListSlots) list[at] = place_of(z, col0 + 32 * i);
+        }
+      }
+      sync_all(cluster);
+      listed = *to;
+      done = listed <= kListSlots;
+    }
+  }
+
+  if (by_list && done) {
+    if (rank != 0) return;  // the first CTA waits for that before it leaves
+    unsigned slots = 1;
+    while (slots < listed) slots *= 2;
+    for (unsigned i = listed + tid; i < slots; i += kThreads) sh.list[i] = 0;
+    sort_list(sh.list, slots);
+    if (TOP) {
+      for (int i = tid; i < p.k; i += kThreads) {
+        const float z = logit_at(sh.list[i]);
+        const int64_t at = static_cast<int64_t>(row) * p.k + i;
+        p.logp[at] = (z == m ? 0.f : (z - m) * p.scale) - log_sum;
+        p.ids[at] = column_at(sh.list[i]);
+      }
+    } else {
+      // two neighbours of the order a thread: kept by top_p and min_p?
+      unsigned long long w[2], e[2], before;
+      bool in[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned i = 2 * tid + j;
+        in[j] = i < first;
+        e[j] = in[j] ? sh.list[i] : 0ull;
+        w[j] = in[j] ? weight(logit_at(e[j])) : 0ull;
+      }
+      const unsigned long long sum = block_scan64(w[0] + w[1], before, sh.red);
+      const unsigned long long need =
+          p.top_p < 1.0 ? max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(sum))) : sum;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        in[j] = in[j] && (p.top_p == 1.0 || before < need) && log_weight(logit_at(e[j])) >= p.log_min_p;
+        before += w[j];
+      }
+      // by index, the lowest first: the complement of the column, then the logit's key
+      unsigned kept_slots = 1;
+      while (kept_slots < first) kept_slots *= 2;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (2 * tid + j < static_cast<int>(kept_slots)) sh.list[2 * tid + j] = in[j] ? e[j] << 32 | e[j] >> 32 : 0ull;
+      sort_list(sh.list, kept_slots);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        e[j] = 2 * tid + j < static_cast<int>(kept_slots) ? sh.list[2 * tid + j] : 0ull;
+        w[j] = e[j] != 0 ? weight(logit_of(static_cast<unsigned>(e[j]))) : 0ull;
+      }
+      const unsigned long long kept = block_scan64(w[0] + w[1], before, sh.red);
+      const double ud = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0 - 0x1p-53);  // NaN: 0
+      const unsigned long long target = __umul64hi(kept, static_cast<unsigned long long>(ud * 0x1p64));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (before <= target && target < before + w[j]) {
+          const float z = logit_of(static_cast<unsigned>(e[j]));
+          p.ids[row] = static_cast<int>(~static_cast<unsigned>(e[j] >> 32));
+          p.logp[row] = (z == m ? 0.f : (z - m) * p.scale) - log_sum;
+        }
+        before += w[j];
+      }
+    }
+    sync_all(cluster);
+    return;
+  }
+  if (by_bins && done) {
+    if (rank == 0) {
+      // the last token before which less than top_p has come
+      unsigned slots = 1;
+      while (slots < listed) slots *= 2;
+      for (unsigned i = listed + tid; i < slots; i += kThreads) sh.list[i] = 0;
+      sort_list(sh.list, slots);
+      const unsigned long long need = max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(total)));
+      unsigned long long e[2], w[2], before;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        e[j] = 2 * tid + j < static_cast<int>(listed) ? sh.list[2 * tid + j] : 0ull;
+        w[j] = e[j] != 0 ? weight(logit_at(e[j])) : 0ull;
+      }
+      block_scan64(w[0] + w[1], before, sh.red);
+      before += sh.before64;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (e[j] != 0 && before < need && before + w[j] >= need)
+          for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(sh.cut_of, r)[0] = e[j];
+        before += w[j];
+      }
+    }
+    sync_all(cluster);
+    cut_place = sh.cut_of[0];
+  }
+
+  // ---- digits
   Cut cut{0u, 0u};  // all tokens
   int pass = 0;     // of both kinds of histogram
-
-  // ---- the n-th token's key
-  const unsigned first = TOP ? p.k : p.top_k;
-  if (first != 0 && first < count) {
+  // a key from its digits: the bits below are 0, of a negative logit 1
+  auto with_low_bits = [](unsigned prefix) { return kLowest == 0 || prefix & 0x80000000u ? prefix : prefix | ((1u << kLowest) - 1); };
+  if (cut_first) {
+    sync_all(cluster);  // the list lies where the histograms are
     unsigned need = first, prefix = 0, mask = 0;
     for (int shift = 24; shift >= kLowest; shift -= 8, ++pass) {
       unsigned* hist = sh.hist[pass & 1];
@@ -210,17 +496,17 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         const unsigned key = key_of(z);
         if (is_token(z) && (key & mask) == prefix) atomicAdd(&hist[key >> shift & 255], 1u);
       }
-      cluster.sync();
+      sync_all(cluster);
       if (warp == 0) {
         // a lane has 8 digits, lane 0 the largest
-        unsigned h[8], own = 0;
+        unsigned h[8], sum = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           h[j] = 0;
           for (int r = 0; r < ctas; ++r) h[j] += cluster.map_shared_rank(hist, r)[255 - (8 * lane + j)];
-          own += h[j];
+          sum += h[j];
         }
-        unsigned before = static_cast<unsigned>(warp_scan64(own, lane)) - own;
+        unsigned before = static_cast<unsigned>(warp_scan64(sum, lane)) - sum;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (before < need && before + h[j] >= need) {
@@ -238,26 +524,19 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     }
     cut = {with_low_bits(prefix), need};
   }
-
-  if (!TOP && p.top_p < 1.0 && count > 0) {
-    // ---- the key where top_p of the sum is reached
-    unsigned long long total = 0;
+  if (!TOP && p.top_p < 1.0 && !done) {
+    // the key where top_p of the sum is reached
+    unsigned long long sum = 0, before;
 #pragma unroll 2
     for (int i = 0; i < n; ++i) {
       const float z = v[32 * i];
-      if (is_token(z) && key_of(z) > cut.key) total += weight(z);
+      if (is_token(z) && key_of(z) > cut.key) sum += weight(z);
     }
-    total = warp_sum64(total);
-    __syncthreads();
-    if (lane == 0) sh.red[warp] = total;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < kWarps; ++w) total += sh.red[w];
-    tell_all(cluster, sh.total_of, total);
-    total = cut.ties != 0 ? cut.ties * weight(logit_of(cut.key)) : 0ull;
-    for (int r = 0; r < ctas; ++r) total += sh.total_of[r];
+    tell_all(cluster, sh.cut_of, block_scan64(sum, before, sh.red));
+    sum = cut.ties != 0 ? cut.ties * weight(logit_of(cut.key)) : 0ull;
+    for (int r = 0; r < ctas; ++r) sum += sh.cut_of[r];
     // in 64-bit floating point, which gives what was meant where 0.9 of equal weights is a whole number of them
-    unsigned long long need = max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(total)));
+    unsigned long long need = max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(sum)));
     unsigned prefix = 0, mask = 0;
     for (int shift = 24; shift >= kLowest; shift -= 8, ++pass) {
       unsigned long long* hist = sh.weights[pass & 1];
@@ -268,23 +547,23 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         const unsigned key = key_of(z);
         if (is_token(z) && key >= cut.key && (key & mask) == prefix) atomicAdd(&hist[key >> shift & 255], weight(z));
       }
-      cluster.sync();
+      sync_all(cluster);
       if (warp == 0) {
-        unsigned long long h[8], own = 0;
+        unsigned long long h[8], all = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           h[j] = 0;
           for (int r = 0; r < ctas; ++r) h[j] += cluster.map_shared_rank(hist, r)[255 - (8 * lane + j)];
-          own += h[j];
+          all += h[j];
         }
-        unsigned long long before = warp_scan64(own, lane) - own;
+        unsigned long long upto = warp_scan64(all, lane) - all;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (before < need && before + h[j] >= need) {
+          if (upto < need && upto + h[j] >= need) {
             sh.digit = 255 - (8 * lane + j);
-            sh.before64 = before;
+            sh.before64 = upto;
           }
-          before += h[j];
+          upto += h[j];
         }
       }
       __syncthreads();
@@ -300,39 +579,43 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
   }
 
   // ---- which of the tokens with the threshold's key are kept: the first ones
-  unsigned tie = 0, ties_here = 0;  // rank of the warp's first
+  unsigned tie = 0;  // rank of the warp's first
   if (cut.ties != 0) {
+    unsigned here = 0;
 #pragma unroll 4
     for (int i = 0; i < n; ++i)
-      ties_here += __popc(__ballot_sync(0xffffffffu, is_token(v[32 * i]) && key_of(v[32 * i]) == cut.key));
-    __syncthreads();
-    if (lane == 0) sh.red[warp] = ties_here;
-    __syncthreads();
-    unsigned of_cta = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) tie = of_cta;
-      of_cta += static_cast<unsigned>(sh.red[w]);
-    }
+      here += __popc(__ballot_sync(0xffffffffu, is_token(v[32 * i]) && key_of(v[32 * i]) == cut.key));
+    unsigned long long before;
+    const unsigned of_cta = static_cast<unsigned>(block_scan64(lane == 0 ? here : 0u, before, sh.red));
+    tie = __shfl_sync(0xffffffffu, static_cast<unsigned>(before), 0);
     tell_all(cluster, sh.ties_of, of_cta);
     for (int r = 0; r < rank; ++r) tie += sh.ties_of[r];
   }
-  unsigned long long own = 0;  // weight of the thread's kept tokens
+  const bool cuts = cut_first || by_bins || (!TOP && p.log_min_p > -INFINITY);
+  if (cuts) {
+    own = 0;
 #pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const float z = v[32 * i];
-    const unsigned key = key_of(z);
-    bool in = is_token(z) && key > cut.key;
-    if (cut.ties != 0) {
-      const bool equal = is_token(z) && key == cut.key;
-      const unsigned all = __ballot_sync(0xffffffffu, equal);
-      in = in || (equal && tie + __popc(all & ((1u << lane) - 1)) < cut.ties);
-      tie += __popc(all);
+    for (int i = 0; i < n; ++i) {
+      const float z = v[32 * i];
+      const unsigned key = key_of(z);
+      bool in = is_token(z) && key > cut.key;
+      if (cut.ties != 0) {
+        const bool equal = is_token(z) && key == cut.key;
+        const unsigned all = __ballot_sync(0xffffffffu, equal);
+        in = in || (equal && tie + __popc(all & ((1u << lane) - 1)) < cut.ties);
+        tie += __popc(all);
+      }
+      if (!TOP && in && done) {
+        const int b = bin_of(z);
+        in = b < cut_bin || (b == cut_bin && place_of(z, col0 + 32 * i) >= cut_place);
+      }
+      if (!TOP && in) {
+        const double t = log_weight(z);
+        in = t >= p.log_min_p;
+        if (in) own += weight_at(t);
+      }
+      if (!in) v[32 * i] = -INFINITY;  // from here on no token
     }
-    if (!TOP && in) {
-      in = log_weight(z) >= p.log_min_p;
-      if (in) own += weight(z);
-    }
-    if (!in) v[32 * i] = -INFINITY;  // from here on no token
   }
 
   if (TOP) {
@@ -340,72 +623,43 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     const unsigned have = min(static_cast<unsigned>(p.k), count);
     unsigned slots = 1;
     while (slots < static_cast<unsigned>(p.k)) slots *= 2;
+    sync_all(cluster);  // the list lies where the histograms are
     if (rank == 0) {
       if (tid == 0) sh.listed = 0;
       for (unsigned i = tid; i < slots; i += kThreads) sh.list[i] = 0;
     }
-    cluster.sync();
-    unsigned* listed = cluster.map_shared_rank(&sh.listed, 0);
+    sync_all(cluster);
+    unsigned* to = cluster.map_shared_rank(&sh.listed, 0);
     unsigned long long* list = cluster.map_shared_rank(sh.list, 0);
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
       if (is_token(v[32 * i])) {
-        const unsigned at = atomicAdd(listed, 1u);
-        if (at < kMostList)
-          list[at] = static_cast<unsigned long long>(key_of(v[32 * i])) << 32 | ~static_cast<unsigned>(col0 + 32 * i);
+        const unsigned at = atomicAdd(to, 1u);
+        if (at < slots) list[at] = place_of(v[32 * i], col0 + 32 * i);
       }
     }
-    cluster.sync();
+    sync_all(cluster);
     if (rank != 0) return;
-    for (unsigned size = 2; size <= slots; size *= 2) {
-      for (unsigned step = size / 2; step > 0; step /= 2) {
-        const unsigned i = tid, j = i ^ step;
-        if (i < slots && j > i) {
-          const unsigned long long a = sh.list[i], b = sh.list[j];
-          if ((a < b) == ((i & size) == 0)) {
-            sh.list[i] = b;
-            sh.list[j] = a;
-          }
-        }
-        __syncthreads();
-      }
-    }
-    if (tid < p.k) {
-      const unsigned long long e = sh.list[tid];
-      const float z = logit_of(static_cast<unsigned>(e >> 32));
-      const bool in = tid < static_cast<int>(have);
-      const int64_t at = static_cast<int64_t>(row) * p.k + tid;
-      if (!T1_OOB(at, static_cast<int64_t>(p.rows) * p.k)) {
-        p.logp[at] = in ? (z == m ? 0.f : (z - m) * p.scale) - log_sum : 0.f;
-        p.ids[at] = in ? static_cast<int64_t>(~static_cast<unsigned>(e)) : -1;
-      }
+    sort_list(sh.list, slots);
+    for (int i = tid; i < p.k; i += kThreads) {
+      const float z = logit_at(sh.list[i]);
+      const bool in = i < static_cast<int>(have);
+      const int64_t at = static_cast<int64_t>(row) * p.k + i;
+      p.logp[at] = in ? (z == m ? 0.f : (z - m) * p.scale) - log_sum : 0.f;
+      p.ids[at] = in ? column_at(sh.list[i]) : -1;
     }
     return;
   }
 
   // ---- the draw
-  unsigned long long of_warp = warp_sum64(own);
-  __syncthreads();
-  if (lane == 0) sh.red[warp] = of_warp;
-  __syncthreads();
-  unsigned long long before = 0, of_cta = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) before = of_cta;
-    of_cta += sh.red[w];
-  }
-  tell_all(cluster, sh.kept_of, of_cta);
-  unsigned long long total = 0;
+  unsigned long long before;
+  const unsigned long long of_warp = warp_sum64(own);
+  tell_all(cluster, sh.kept_of, block_scan64(own, before, sh.red));
+  total = 0;
+  before = __shfl_sync(0xffffffffu, before, 0);  // the warp's
   for (int r = 0; r < ctas; ++r) {
     if (r == rank) before += total;
     total += sh.kept_of[r];
-  }
-  if (T1_OOB(row, p.rows)) return;
-  if (total == 0) {
-    if (rank == 0 && tid == 0) {
-      p.ids[row] = -1;
-      p.logp[row] = 0.f;
-    }
-    return;
   }
   const double ud = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0 - 0x1p-53);  // NaN: 0
   const unsigned long long target = __umul64hi(total, static_cast<unsigned long long>(ud * 0x1p64));
@@ -495,6 +749,7 @@ static void run_rows(rows::Params& p, const torch::Tensor& logits, double temper
   p.ld = logits.size(0) > 1 ? logits.stride(0) : 0;
   p.rows = static_cast<int>(logits.size(0));
   p.V = static_cast<int>(logits.size(1));
+  p.aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * logits.element_size() % 16 == 0;
   p.scale64 = 1.0 / temperature;
   p.scale = static_cast<float>(p.scale64);
   if (p.rows == 0) return;
@@ -541,7 +796,7 @@ std::vector<torch::Tensor> sample_tokens(torch::Tensor logits, torch::Tensor u, 
   p.log_min_p = std::log(min_p);
   int bits = 0;
   while ((1ll << bits) < logits.size(1)) ++bits;
-  p.one = std::ldexp(1.0, 62 - bits);
+  p.one = std::min(51, 62 - bits);  // a weight fits the 52 bits of a double
   run_rows<false>(p, logits, temperature);
   return {token, logp};
 }
