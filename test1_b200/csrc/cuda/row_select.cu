@@ -11,15 +11,15 @@
 // -inf and NaN are no tokens; a logit of +inf outweighs all finite ones.
 //
 // A cluster of CTAs holds one row in shared memory: one read of the logits, and
-// every thread keeps to the same few of them in every pass.  Three ways to the
-// cut, of which the first two touch few logits more than once:
-//   list   the first n <= 1024: no n tokens can all lie below the n-th largest
+// every warp keeps to the same stretch of them in every pass.  Three ways to the
+// cut, of which the first two look at most logits twice or three times:
+//   list   the first n <= 512: no n tokens can all lie below the n-th largest
 //          of the threads' own largest ones, which a histogram of their
 //          distances from m finds.  What lies above (little more than n) goes to
 //          the first CTA, which sorts it and does all the rest.
-//   bins   top_p alone: weights added up by distance from m, 16 bins per unit of
-//          the exponent; the tokens of the bin where top_p is reached are sorted
-//          by the first CTA.
+//   bins   top_p alone: weights added up by distance from m, 8 bins per factor
+//          of two, the bin where top_p is reached once more in 256 parts, and
+//          the tokens of that part sorted by the first CTA.
 //   digits where neither applies (more tokens are asked for, or too many are
 //          equal): the threshold is found digit by digit, 8 bits at a time, of
 //          the order-preserving integer of a logit.
@@ -46,6 +46,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMostCtas = 8;      // of a cluster
 constexpr int kMostList = 512;    // tokens of `top`
 constexpr int kListSlots = 1024;  // tokens that the first CTA sorts
+constexpr int kRankSlots = 128;   // up to so many by counting
 constexpr int kDigits = 256;
 constexpr int kBins = 256;
 constexpr int kExps = 128;        // steps of an octave in the table of exponentials
@@ -56,8 +57,10 @@ struct Params {
   int rows, V;
   int per_thread;  // columns
   bool aligned;    // rows begin on 16 bytes
+  float tau;
   float scale;     // 1 / tau
-  double scale64;
+  float scale2;    // log2(e) / tau
+  double steps;    // kExps log2(e) / tau
   // top
   int k;
   float* logp;     // [rows, k]; sample: [rows]
@@ -66,7 +69,7 @@ struct Params {
   const float* u;
   int top_k;         // 0: all
   double top_p;      // 1: all
-  double log_min_p;  // -inf: all
+  double log_min_p;  // in units of 1 / kExps of a factor of two; -inf: all
   int one;           // s: the largest logit's weight is 2^s
 };
 
@@ -139,7 +142,7 @@ __device__ __forceinline__ unsigned long long warp_scan64(unsigned long long v, 
 struct Shared {
   double exps[kExps];              // 2^(j / 128)
   unsigned long long red[kWarps];
-  unsigned bins[3][kBins];         // counts; of weights 16 bits each
+  unsigned bins[2][3][kBins];      // counts; of weights 16 bits each
   union {
     struct {
       unsigned hist[2][kDigits];
@@ -156,9 +159,21 @@ struct Shared {
   // where a threshold falls
   unsigned digit, before32;
   int bin;
-  unsigned long long before64;
+  unsigned long long before64, here64;
   unsigned listed;
 };
+
+__device__ __forceinline__ float exp2f_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// u times the sum, rounded down; u of NaN is 0.
+__device__ __forceinline__ unsigned long long target_of(float u, unsigned long long sum) {
+  const double d = fmin(fmax(static_cast<double>(u), 0.0), 1.0 - 0x1p-53);
+  return __umul64hi(sum, static_cast<unsigned long long>(d * 0x1p64));
+}
 
 __device__ __forceinline__ void sync_all(cg::cluster_group& cluster) {
   if (cluster.num_blocks() == 1) __syncthreads();
@@ -210,6 +225,31 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, unsigned slo
   __syncthreads();
 }
 
+// The same; kRankSlots or fewer by counting for each how many are larger, four
+// threads to one.  Places differ, except for the zeros that fill the list up.
+__device__ __forceinline__ void order_list(unsigned long long* list, unsigned listed) {
+  if (listed <= kRankSlots) {
+    __syncthreads();
+    const unsigned i = threadIdx.x >> 2, part = threadIdx.x & 3;
+    const unsigned long long mine = i < listed ? list[i] : 0ull;
+    unsigned larger = 0;
+    if ((threadIdx.x & ~31u) < 4 * listed) {  // whole warps
+#pragma unroll 4
+      for (unsigned j = part; j < listed; j += 4) larger += list[j] > mine;
+      larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+      larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+    }
+    __syncthreads();
+    if (i < listed && part == 0) list[larger] = mine;
+    __syncthreads();
+    return;
+  }
+  unsigned slots = 1;
+  while (slots < listed) slots *= 2;
+  for (unsigned i = listed + threadIdx.x; i < slots; i += kThreads) list[i] = 0;
+  sort_list(list, slots);
+}
+
 // A prefix of the order: all tokens of a larger key, and the first `ties` of
 // those that have it.
 struct Cut {
@@ -218,7 +258,7 @@ struct Cut {
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
   __shared__ Shared sh;
   __shared__ float red[32];
   extern __shared__ __align__(16) float held[];
@@ -226,10 +266,12 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / ctas;
-  // a warp has 32 n columns in a row, a thread every 32nd of them
+  // a warp has 32 n columns in a row, n a multiple of 4.  A thread has every 32nd of them, v[32 i], or, where only
+  // sums count, four at a time, quads[32 i]
   const int n = p.per_thread;
   const int warp_col0 = (rank * kWarps + warp) * 32 * n, col0 = warp_col0 + lane;
-  float* v = held + warp * 32 * n + lane;  // v[32 i]: the thread's i-th
+  float* v = held + warp * 32 * n + lane;
+  const float4* quads = reinterpret_cast<const float4*>(held + warp * 32 * n) + lane;
   constexpr int kLowest = sizeof(T) == 2 ? 16 : 0;  // key bits below are the same in all of a type's values
   if (T1_OOB(row, p.rows)) return;
 
@@ -238,39 +280,22 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     fetch(held + warp * 32 * n, static_cast<const T*>(p.logits) + row * p.ld + warp_col0, cols, p.aligned, lane);
     for (int c = cols + lane; c < 32 * n; c += 32) held[warp * 32 * n + c] = -INFINITY;
   }
-  for (int i = tid; i < 3 * kBins; i += kThreads) sh.bins[0][i] = 0;
+  for (int i = tid; i < 6 * kBins; i += kThreads) sh.bins[0][0][i] = 0;
   if (tid == 0) sh.listed = 0;
   if (!TOP && tid < kExps) sh.exps[tid] = exp2(tid / static_cast<double>(kExps));
   fetched();
   __syncwarp();
+  // ---- largest logit (a NaN is never the larger of two)
   float own_max = -INFINITY;
-  unsigned count = 0;
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) {
-    float z = v[32 * i];
-    z = z == z ? z + 0.f : -INFINITY;  // -0 is 0
-    v[32 * i] = z;
-    own_max = fmaxf(own_max, z);
-    count += is_token(z);
+#pragma unroll 4
+  for (int i = 0; i < n / 4; ++i) {
+    const float4 q = quads[32 * i];
+    own_max = fmaxf(fmaxf(own_max, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
   }
-
-  // ---- largest logit, number of tokens
   float m = block_max(own_max, red);
-  {
-    unsigned c = __reduce_add_sync(0xffffffffu, count);
-    if (lane == 0) sh.red[warp] = c;
-    __syncthreads();
-    count = 0;
-    for (int w = 0; w < kWarps; ++w) count += static_cast<unsigned>(sh.red[w]);
-  }
-  if (tid < ctas) cluster.map_shared_rank(sh.max_of, tid)[rank] = m;
-  tell_all(cluster, sh.count_of, count);
-  count = 0;
-  for (int r = 0; r < ctas; ++r) {
-    m = fmaxf(m, sh.max_of[r]);
-    count += sh.count_of[r];
-  }
-  if (count == 0) {
+  tell_all(cluster, sh.max_of, m);
+  for (int r = 0; r < ctas; ++r) m = fmaxf(m, sh.max_of[r]);
+  if (m == -INFINITY) {
     if (rank != 0) return;
     for (int i = tid; i < (TOP ? p.k : 1); i += kThreads) {
       p.ids[static_cast<int64_t>(row) * (TOP ? p.k : 1) + i] = -1;
@@ -278,69 +303,179 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     }
     return;
   }
+  // Where m is infinite, or its neighbours lie far below it, the largest logits have all the weight.
+  const bool sharp = !(fabsf(m) * 0x1p-23f <= 100.f * p.tau);
+  const float top = m;
+  if (!TOP && sharp) {
+    for (int i = 0; i < n; ++i) v[32 * i] = v[32 * i] == m ? 0.f : -INFINITY;
+    own_max = own_max == m ? 0.f : -INFINITY;
+    m = 0.f;
+    __syncwarp();
+  }
+  // exp(-350) is no weight in any precision here: below, and NaN, counts as that
+  const float low = m - 400.f * p.tau;
+  auto log_p = [&](float z, float log_sum) {
+    return (z == m ? 0.f : TOP && top == INFINITY ? -INFINITY : (z - m) * p.scale) - log_sum;
+  };
 
   const double m64 = m;
-  auto log_weight = [&](float z) { return z == m ? 0.0 : (static_cast<double>(z) - m64) * p.scale64; };
-  // exp(t) 2^s for t <= 0: 2^(j / 128) from the table, the rest of the exponent (|r| < 0.0028) by its series, whose
-  // first term left out is below 1.4e-15
-  auto weight_at = [&](double t) -> unsigned long long {
-    if (t < -64.0) return 0ull;
-    constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: adding it leaves a whole number in the low bits
-    const double y = fma(t, 1.4426950408889634 * kExps, kRound);
+  // log2 of the weight, of 1 for m, in steps of 1 / kExps
+  auto steps_of = [&](float z) { return (static_cast<double>(fmaxf(z, low)) - m64) * p.steps; };
+  // 2^(x / kExps + s): a power from the table, the rest of it (|f| <= 1/2) by the series of the exponential function,
+  // whose first term left out is below 5e-15; rounded to a whole number by the last addition
+  constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: adding it leaves a whole number in the low bits
+  auto weight_at = [&](double x) -> unsigned long long {
+    constexpr double L = 0.6931471805599453 / kExps;
+    const double y = x + kRound;
     const int j = __double2loint(y);
-    const double r = fma(y - kRound, -0.6931471805599453 / kExps, t);
-    double e = fma(r, 1.0 / 24, 1.0 / 6);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
+    const double f = x - (y - kRound);
+    double e = fma(f, L * L * L * L / 24, L * L * L / 6);
+    e = fma(e, f, L * L / 2);
+    e = fma(e, f, L);
+    e = fma(e, f, 1.0);
     const double base = sh.exps[j & (kExps - 1)];
     const double scaled = __hiloint2double(__double2hiint(base) + (((j >> 7) + p.one) << 20), __double2loint(base));
     constexpr double kWhole = 4503599627370496.0;  // 2^52
     return __double_as_longlong(fma(e, scaled, kWhole)) - __double_as_longlong(kWhole);
   };
   static_assert(kExps == 128, "j >> 7");
-  auto weight = [&](float z) { return weight_at(log_weight(z)); };
+  auto weight = [&](float z) { return weight_at(steps_of(z)); };
   // Distance from m in steps of a sixteenth of its octave, 2^-8 to 2^8.
   auto step_of = [&](float z) {
-    const int s = static_cast<int>(__float_as_uint(z == m ? 0.f : m - z) >> 19) - (119 << 4);
+    const int s = static_cast<int>(__float_as_uint(m - z) >> 19) - (119 << 4);
     return min(max(s, 0), kBins - 1);
   };
-  // Distance from m in sixteenths of the exponent's unit.
-  auto bin_of = [&](float z) { return z == m ? 0 : static_cast<int>(fminf((m - z) * p.scale * 16.f, kBins - 1.f)); };
+  // Bins of 16 steps of a weight's logarithm, and 256 parts of one.
+  auto bin_at = [&](double x) { return -__double2loint(x + kRound) >> 4; };
+  auto part_at = [&](double x, int bin) { return min(max(static_cast<int>((0.5 - x - 16 * bin) * 16.0), 0), kBins - 1); };
+  auto add_to = [](unsigned (*bins)[kBins], int b, unsigned long long w) {
+    const unsigned lo = static_cast<unsigned>(w) & 0xffffu, mid = static_cast<unsigned>(w >> 16) & 0xffffu,
+                   hi = static_cast<unsigned>(w >> 32);
+    atomicAdd(&bins[0][b], lo);
+    if (mid != 0) atomicAdd(&bins[1][b], mid);
+    if (hi != 0) atomicAdd(&bins[2][b], hi);
+  };
+  // The bin in which `need` is reached (-1: in none), and in sh.before64 what comes before it; all CTAs' bins.
+  auto reach = [&](unsigned (*bins)[kBins], bool weights, unsigned long long need) {
+    unsigned long long here = 0, before;
+    if (tid < kBins) {
+      for (int r = 0; r < ctas; ++r) {
+        const unsigned* b = cluster.map_shared_rank(&bins[0][0], r);
+        here += b[tid];
+        if (weights)
+          here += (static_cast<unsigned long long>(b[kBins + tid]) << 16) + (static_cast<unsigned long long>(b[2 * kBins + tid]) << 32);
+      }
+    }
+    if (tid == 0) sh.bin = -1;
+    block_scan64(here, before, sh.red);
+    if (before < need && before + here >= need) {
+      sh.bin = tid;
+      sh.before64 = before;
+      sh.here64 = here;
+    }
+    __syncthreads();
+    return sh.bin;
+  };
+  // A token to the first CTA's list.
+  unsigned* const list_length = cluster.map_shared_rank(&sh.listed, 0);
+  unsigned long long* const first_list = cluster.map_shared_rank(sh.list, 0);
+  auto push = [&](float z, int column) {
+    const unsigned at = atomicAdd(list_length, 1u);
+    if (at < kListSlots) first_list[at] = place_of(z + 0.f, column);  // -0 is 0
+  };
 
   const unsigned first = TOP ? p.k : p.top_k;
-  const bool cut_first = first != 0 && first < count;
-  const bool by_list = cut_first && first <= kListSlots / 2 && first <= static_cast<unsigned>(ctas * kThreads);
-  const bool by_bins = !TOP && !cut_first && p.top_p < 1.0;
-
-  // ---- log of the sum of all weights, and the sum by bins
   float log_sum;
   unsigned long long total = 0, own = 0;  // own: the thread's kept weight
-  if (TOP || cut_first) {
+  bool done = false;                      // the cut is found
+  unsigned long long cut_place = 0;       // with done: the last token kept
+
+  if (TOP || first != 0) {
+    // ---- list
+    const bool by_list = !sharp && first <= kListSlots / 2 && first <= static_cast<unsigned>(ctas * kThreads);
+    float bound = INFINITY;
+    if (by_list) {
+      if (is_token(own_max)) atomicAdd(&sh.bins[0][0][step_of(own_max)], 1u);
+      sync_all(cluster);
+      const int bin = reach(sh.bins[0], false, first);
+      // the far edge of that step, and a little more for the rounding of m - z
+      if (bin >= 0 && bin < kBins - 1) bound = m - __uint_as_float(static_cast<unsigned>(bin + 1 + (119 << 4)) << 19) * 1.000001f;
+    }
     float sum = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) sum += v[32 * i] == m ? 1.f : __expf((v[32 * i] - m) * p.scale);
-    if (by_list && is_token(own_max)) atomicAdd(&sh.bins[0][step_of(own_max)], 1u);
+    if (TOP && sharp) {
+      for (int i = 0; i < n; ++i) sum += v[32 * i] == m;
+    } else {
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int i = 0; i < n / 4; ++i) {
+        const float4 q = quads[32 * i];
+        const float z[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast((fmaxf(z[j], low) - m) * p.scale2);
+        if (fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= bound) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (z[j] >= bound) push(z[j], warp_col0 + 4 * (32 * i + lane) + j);
+        }
+      }
+      sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    }
     sum = block_sum(sum, red);
     tell_all(cluster, sh.sum_of, sum);
     sum = 0.f;
     for (int r = 0; r < ctas; ++r) sum += sh.sum_of[r];
     log_sum = logf(sum);
+    const unsigned listed = *list_length;
+    if (bound < INFINITY && listed <= kListSlots) {
+      if (rank != 0) return;  // the first CTA waits for that before it leaves
+      order_list(sh.list, listed);
+      if (TOP) {
+        for (int i = tid; i < p.k; i += kThreads) {
+          const int64_t at = static_cast<int64_t>(row) * p.k + i;
+          p.logp[at] = log_p(logit_at(sh.list[i]), log_sum);
+          p.ids[at] = column_at(sh.list[i]);
+        }
+      } else {
+        // kept by top_p and min_p?
+        unsigned long long before, e = tid < static_cast<int>(first) ? sh.list[tid] : 0ull;
+        const double x = e != 0 ? steps_of(logit_at(e)) : 0.0;
+        const unsigned long long w = e != 0 ? weight_at(x) : 0ull;
+        const unsigned long long sum64 = block_scan64(w, before, sh.red);
+        const unsigned long long need = max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(sum64)));
+        const bool in = e != 0 && (p.top_p == 1.0 || before < need) && x >= p.log_min_p;
+        // by index, the lowest first: the complement of the column, then the logit's key
+        if (tid < static_cast<int>(first)) sh.list[tid] = in ? e << 32 | e >> 32 : 0ull;
+        const unsigned kept = __syncthreads_count(in);
+        // the tokens kept are a prefix of the list
+        order_list(sh.list, kept);
+        e = tid < static_cast<int>(kept) ? sh.list[tid] : 0ull;
+        const float z = logit_of(static_cast<unsigned>(e));
+        const unsigned long long w2 = e != 0 ? weight(z) : 0ull;
+        const unsigned long long all = block_scan64(w2, before, sh.red);
+        const unsigned long long target = target_of(p.u[row], all);
+        if (before <= target && target < before + w2) {
+          p.ids[row] = static_cast<int>(~static_cast<unsigned>(e >> 32));
+          p.logp[row] = log_p(z, log_sum);
+        }
+      }
+      sync_all(cluster);
+      return;
+    }
   } else {
+    // ---- bins
+    const bool by_bins = p.top_p < 1.0;
 #pragma unroll 2
-    for (int i = 0; i < n; ++i) {
-      const float z = v[32 * i];
-      if (!is_token(z)) continue;
-      const unsigned long long w = weight(z);
-      own += w;
-      if (by_bins) {
-        const int b = bin_of(z);
-        if (b < kBins - 1) {
-          const unsigned lo = static_cast<unsigned>(w) & 0xffffu, mid = static_cast<unsigned>(w >> 16) & 0xffffu,
-                         hi = static_cast<unsigned>(w >> 32);
-          atomicAdd(&sh.bins[0][b], lo);
-          if (mid != 0) atomicAdd(&sh.bins[1][b], mid);
-          if (hi != 0) atomicAdd(&sh.bins[2][b], hi);
+    for (int i = 0; i < n / 4; ++i) {
+      const float4 q = quads[32 * i];
+      const float z[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double x = steps_of(z[j]);
+        const unsigned long long w = weight_at(x);
+        own += w;
+        if (by_bins) {
+          const int b = bin_at(x);
+          if (b < kBins && w != 0) add_to(sh.bins[0], b, w);
         }
       }
     }
@@ -348,143 +483,76 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     tell_all(cluster, sh.total_of, block_scan64(own, before, sh.red));
     for (int r = 0; r < ctas; ++r) total += sh.total_of[r];
     log_sum = static_cast<float>(log(ldexp(static_cast<double>(total), -p.one)));
-  }
-
-  // ---- list and bins: the step or bin that the cut falls into, and its tokens to the first CTA
-  bool done = false;           // by the list or bins
-  unsigned listed = 0;
-  int cut_bin = 0;
-  unsigned long long cut_place = 0;
-  if (by_list || by_bins) {
-    const unsigned long long need =
-        by_list ? first : max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(total)));
-    unsigned long long here = 0, before;
-    if (tid < kBins) {
-      for (int r = 0; r < ctas; ++r) {
-        const unsigned* b = cluster.map_shared_rank(&sh.bins[0][0], r);
-        here += b[tid];
-        if (!by_list) here += (static_cast<unsigned long long>(b[kBins + tid]) << 16) + (static_cast<unsigned long long>(b[2 * kBins + tid]) << 32);
-      }
-    }
-    if (tid == 0) sh.bin = kBins;
-    block_scan64(here, before, sh.red);
-    if (before < need && before + here >= need) {
-      sh.bin = tid;
-      sh.before64 = before;
-    }
-    __syncthreads();
-    cut_bin = sh.bin;
-    if (cut_bin < kBins - 1) {
-      unsigned* to = cluster.map_shared_rank(&sh.listed, 0);
-      unsigned long long* list = cluster.map_shared_rank(sh.list, 0);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float z = v[32 * i];
-        if (is_token(z) && (by_list ? step_of(z) <= cut_bin : bin_of(z) == cut_bin)) {
-          const unsigned at = atomicAdd(to, 1u);
-          if (at < kListSlots) list[at] = place_of(z, col0 + 32 * i);
+    if (by_bins) {
+      unsigned long long need = max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(total)));
+      const int bin = reach(sh.bins[0], true, need);
+      if (bin >= 0) {
+        need -= sh.before64;
+        // no more tokens than this have the bin's weight
+        const bool few = sh.here64 / max(1ull, weight_at(-16.0 * (bin + 1))) < kListSlots;
+        int part = 0;
+        if (!few) {
+#pragma unroll 4
+          for (int i = 0; i < n; ++i) {
+            const double x = steps_of(v[32 * i]);
+            if (bin_at(x) == bin) add_to(sh.bins[1], part_at(x, bin), weight_at(x));
+          }
+          sync_all(cluster);
+          part = reach(sh.bins[1], true, need);
+          need -= sh.before64;
+        }
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+          const float z = v[32 * i];
+          const double x = steps_of(z);
+          if (bin_at(x) == bin && is_token(z) && (few || part_at(x, bin) == part)) push(z, col0 + 32 * i);
+        }
+        sync_all(cluster);
+        const unsigned listed = *list_length;
+        done = listed <= kListSlots;
+        if (done) {
+          if (rank == 0) {
+            // the last token before which less than top_p has come
+            order_list(sh.list, listed);
+            unsigned long long e[2], w[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              e[j] = 2 * tid + j < static_cast<int>(listed) ? sh.list[2 * tid + j] : 0ull;
+              w[j] = e[j] != 0 ? weight(logit_at(e[j])) : 0ull;
+            }
+            block_scan64(w[0] + w[1], before, sh.red);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (e[j] != 0 && before < need && before + w[j] >= need)
+                for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(sh.cut_of, r)[0] = e[j];
+              before += w[j];
+            }
+          }
+          sync_all(cluster);
+          cut_place = sh.cut_of[0];
         }
       }
-      sync_all(cluster);
-      listed = *to;
-      done = listed <= kListSlots;
     }
-  }
-
-  if (by_list && done) {
-    if (rank != 0) return;  // the first CTA waits for that before it leaves
-    unsigned slots = 1;
-    while (slots < listed) slots *= 2;
-    for (unsigned i = listed + tid; i < slots; i += kThreads) sh.list[i] = 0;
-    sort_list(sh.list, slots);
-    if (TOP) {
-      for (int i = tid; i < p.k; i += kThreads) {
-        const float z = logit_at(sh.list[i]);
-        const int64_t at = static_cast<int64_t>(row) * p.k + i;
-        p.logp[at] = (z == m ? 0.f : (z - m) * p.scale) - log_sum;
-        p.ids[at] = column_at(sh.list[i]);
-      }
-    } else {
-      // two neighbours of the order a thread: kept by top_p and min_p?
-      unsigned long long w[2], e[2], before;
-      bool in[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const unsigned i = 2 * tid + j;
-        in[j] = i < first;
-        e[j] = in[j] ? sh.list[i] : 0ull;
-        w[j] = in[j] ? weight(logit_at(e[j])) : 0ull;
-      }
-      const unsigned long long sum = block_scan64(w[0] + w[1], before, sh.red);
-      const unsigned long long need =
-          p.top_p < 1.0 ? max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(sum))) : sum;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        in[j] = in[j] && (p.top_p == 1.0 || before < need) && log_weight(logit_at(e[j])) >= p.log_min_p;
-        before += w[j];
-      }
-      // by index, the lowest first: the complement of the column, then the logit's key
-      unsigned kept_slots = 1;
-      while (kept_slots < first) kept_slots *= 2;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (2 * tid + j < static_cast<int>(kept_slots)) sh.list[2 * tid + j] = in[j] ? e[j] << 32 | e[j] >> 32 : 0ull;
-      sort_list(sh.list, kept_slots);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        e[j] = 2 * tid + j < static_cast<int>(kept_slots) ? sh.list[2 * tid + j] : 0ull;
-        w[j] = e[j] != 0 ? weight(logit_of(static_cast<unsigned>(e[j]))) : 0ull;
-      }
-      const unsigned long long kept = block_scan64(w[0] + w[1], before, sh.red);
-      const double ud = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0 - 0x1p-53);  // NaN: 0
-      const unsigned long long target = __umul64hi(kept, static_cast<unsigned long long>(ud * 0x1p64));
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (before <= target && target < before + w[j]) {
-          const float z = logit_of(static_cast<unsigned>(e[j]));
-          p.ids[row] = static_cast<int>(~static_cast<unsigned>(e[j] >> 32));
-          p.logp[row] = (z == m ? 0.f : (z - m) * p.scale) - log_sum;
-        }
-        before += w[j];
-      }
-    }
-    sync_all(cluster);
-    return;
-  }
-  if (by_bins && done) {
-    if (rank == 0) {
-      // the last token before which less than top_p has come
-      unsigned slots = 1;
-      while (slots < listed) slots *= 2;
-      for (unsigned i = listed + tid; i < slots; i += kThreads) sh.list[i] = 0;
-      sort_list(sh.list, slots);
-      const unsigned long long need = max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(total)));
-      unsigned long long e[2], w[2], before;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        e[j] = 2 * tid + j < static_cast<int>(listed) ? sh.list[2 * tid + j] : 0ull;
-        w[j] = e[j] != 0 ? weight(logit_at(e[j])) : 0ull;
-      }
-      block_scan64(w[0] + w[1], before, sh.red);
-      before += sh.before64;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (e[j] != 0 && before < need && before + w[j] >= need)
-          for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(sh.cut_of, r)[0] = e[j];
-        before += w[j];
-      }
-    }
-    sync_all(cluster);
-    cut_place = sh.cut_of[0];
   }
 
   // ---- digits
   Cut cut{0u, 0u};  // all tokens
   int pass = 0;     // of both kinds of histogram
+  unsigned count = 0;
   // a key from its digits: the bits below are 0, of a negative logit 1
   auto with_low_bits = [](unsigned prefix) { return kLowest == 0 || prefix & 0x80000000u ? prefix : prefix | ((1u << kLowest) - 1); };
-  if (cut_first) {
-    sync_all(cluster);  // the list lies where the histograms are
+  if (first != 0) {
+    for (int i = 0; i < n; ++i) {
+      const float z = v[32 * i];
+      v[32 * i] = z == z ? z + 0.f : -INFINITY;  // -0 is 0
+      count += is_token(z);
+    }
+    unsigned long long before;
+    tell_all(cluster, sh.count_of, static_cast<unsigned>(block_scan64(count, before, sh.red)));
+    count = 0;
+    for (int r = 0; r < ctas; ++r) count += sh.count_of[r];
+  }
+  if (first != 0 && first < count) {
     unsigned need = first, prefix = 0, mask = 0;
     for (int shift = 24; shift >= kLowest; shift -= 8, ++pass) {
       unsigned* hist = sh.hist[pass & 1];
@@ -543,7 +611,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
       if (tid < kDigits) hist[tid] = 0;
       __syncthreads();
       for (int i = 0; i < n; ++i) {
-        const float z = v[32 * i];
+        const float z = v[32 * i] + 0.f;
         const unsigned key = key_of(z);
         if (is_token(z) && key >= cut.key && (key & mask) == prefix) atomicAdd(&hist[key >> shift & 255], weight(z));
       }
@@ -584,35 +652,37 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     unsigned here = 0;
 #pragma unroll 4
     for (int i = 0; i < n; ++i)
-      here += __popc(__ballot_sync(0xffffffffu, is_token(v[32 * i]) && key_of(v[32 * i]) == cut.key));
+      here += __popc(__ballot_sync(0xffffffffu, is_token(v[32 * i]) && key_of(v[32 * i] + 0.f) == cut.key));
     unsigned long long before;
     const unsigned of_cta = static_cast<unsigned>(block_scan64(lane == 0 ? here : 0u, before, sh.red));
     tie = __shfl_sync(0xffffffffu, static_cast<unsigned>(before), 0);
     tell_all(cluster, sh.ties_of, of_cta);
     for (int r = 0; r < rank; ++r) tie += sh.ties_of[r];
   }
-  const bool cuts = cut_first || by_bins || (!TOP && p.log_min_p > -INFINITY);
-  if (cuts) {
+  if (first != 0 || (!TOP && (p.top_p < 1.0 || p.log_min_p > -INFINITY))) {
     own = 0;
+    const float cut_logit = done ? logit_at(cut_place) : -INFINITY;
+    const int cut_column = done ? column_at(cut_place) : 0;
 #pragma unroll 2
     for (int i = 0; i < n; ++i) {
       const float z = v[32 * i];
-      const unsigned key = key_of(z);
-      bool in = is_token(z) && key > cut.key;
-      if (cut.ties != 0) {
-        const bool equal = is_token(z) && key == cut.key;
-        const unsigned all = __ballot_sync(0xffffffffu, equal);
-        in = in || (equal && tie + __popc(all & ((1u << lane) - 1)) < cut.ties);
-        tie += __popc(all);
-      }
-      if (!TOP && in && done) {
-        const int b = bin_of(z);
-        in = b < cut_bin || (b == cut_bin && place_of(z, col0 + 32 * i) >= cut_place);
+      bool in;
+      if (done) {
+        in = z > cut_logit || (z == cut_logit && col0 + 32 * i <= cut_column);
+      } else {
+        const unsigned key = key_of(z + 0.f);
+        in = is_token(z) && key > cut.key;
+        if (cut.ties != 0) {
+          const bool equal = is_token(z) && key == cut.key;
+          const unsigned all = __ballot_sync(0xffffffffu, equal);
+          in = in || (equal && tie + __popc(all & ((1u << lane) - 1)) < cut.ties);
+          tie += __popc(all);
+        }
       }
       if (!TOP && in) {
-        const double t = log_weight(z);
-        in = t >= p.log_min_p;
-        if (in) own += weight_at(t);
+        const double x = steps_of(z);
+        in = x >= p.log_min_p;
+        if (in) own += weight_at(x);
       }
       if (!in) v[32 * i] = -INFINITY;  // from here on no token
     }
@@ -621,31 +691,19 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
   if (TOP) {
     // ---- the kept tokens to the first CTA, which sorts them
     const unsigned have = min(static_cast<unsigned>(p.k), count);
-    unsigned slots = 1;
-    while (slots < static_cast<unsigned>(p.k)) slots *= 2;
     sync_all(cluster);  // the list lies where the histograms are
-    if (rank == 0) {
-      if (tid == 0) sh.listed = 0;
-      for (unsigned i = tid; i < slots; i += kThreads) sh.list[i] = 0;
-    }
+    if (rank == 0 && tid == 0) sh.listed = 0;
     sync_all(cluster);
-    unsigned* to = cluster.map_shared_rank(&sh.listed, 0);
-    unsigned long long* list = cluster.map_shared_rank(sh.list, 0);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      if (is_token(v[32 * i])) {
-        const unsigned at = atomicAdd(to, 1u);
-        if (at < slots) list[at] = place_of(v[32 * i], col0 + 32 * i);
-      }
-    }
+    for (int i = 0; i < n; ++i)
+      if (is_token(v[32 * i])) push(v[32 * i], col0 + 32 * i);
     sync_all(cluster);
     if (rank != 0) return;
-    sort_list(sh.list, slots);
+    order_list(sh.list, have);
     for (int i = tid; i < p.k; i += kThreads) {
-      const float z = logit_at(sh.list[i]);
       const bool in = i < static_cast<int>(have);
       const int64_t at = static_cast<int64_t>(row) * p.k + i;
-      p.logp[at] = in ? (z == m ? 0.f : (z - m) * p.scale) - log_sum : 0.f;
+      p.logp[at] = in ? log_p(logit_at(sh.list[i]), log_sum) : 0.f;
       p.ids[at] = in ? column_at(sh.list[i]) : -1;
     }
     return;
@@ -661,17 +719,13 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     if (r == rank) before += total;
     total += sh.kept_of[r];
   }
-  const double ud = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0 - 0x1p-53);  // NaN: 0
-  const unsigned long long target = __umul64hi(total, static_cast<unsigned long long>(ud * 0x1p64));
+  const unsigned long long target = target_of(p.u[row], total);
   if (target < before || target >= before + of_warp) return;
   // this warp has it: the sums of 32 times 32 columns i, then the lanes of one i
   unsigned long long at = before;
   for (int i0 = 0; i0 < n; i0 += 32) {
     __syncwarp();
-    for (int i = 0; i < min(32, n - i0); ++i) {
-      const float z = v[32 * (i0 + i)];
-      sh.cells[i][lane] = is_token(z) ? weight(z) : 0ull;
-    }
+    for (int i = 0; i < min(32, n - i0); ++i) sh.cells[i][lane] = weight(v[32 * (i0 + i)]);
     __syncwarp();
     unsigned long long s = 0;
     if (i0 + lane < n)
@@ -686,9 +740,8 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     at = __shfl_sync(0xffffffffu, upto - s, l);
     const unsigned long long mine = at + warp_scan64(sh.cells[l][lane], lane);
     if (lane == __ffs(__ballot_sync(0xffffffffu, target < mine)) - 1) {
-      const float z = v[32 * (i0 + l)];
       p.ids[row] = col0 + 32 * (i0 + l);
-      p.logp[row] = (z == m ? 0.f : (z - m) * p.scale) - log_sum;
+      p.logp[row] = log_p(v[32 * (i0 + l)], log_sum);
     }
     return;
   }
@@ -718,7 +771,7 @@ static void launch_rows(rows::Params& p) {
   // 32 columns a thread (64 KB a CTA, so that several rows share an SM) as long as 8 CTAs are enough
   int ctas = 1;
   while (ctas < 8 && ctas * 32 * rows::kThreads < p.V) ctas *= 2;
-  p.per_thread = (p.V + ctas * rows::kThreads - 1) / (ctas * rows::kThreads);
+  p.per_thread = (p.V + 4 * ctas * rows::kThreads - 1) / (4 * ctas * rows::kThreads) * 4;
   auto kern = rows::rows_kernel<T, TOP>;
   static DeviceFlags configured;
   if (bool& done = configured.here(); !done) {
@@ -750,8 +803,10 @@ static void run_rows(rows::Params& p, const torch::Tensor& logits, double temper
   p.rows = static_cast<int>(logits.size(0));
   p.V = static_cast<int>(logits.size(1));
   p.aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * logits.element_size() % 16 == 0;
-  p.scale64 = 1.0 / temperature;
-  p.scale = static_cast<float>(p.scale64);
+  p.tau = static_cast<float>(temperature);
+  p.scale = static_cast<float>(1.0 / temperature);
+  p.scale2 = static_cast<float>(1.4426950408889634 / temperature);
+  p.steps = rows::kExps * 1.4426950408889634 / temperature;
   if (p.rows == 0) return;
   if (logits.scalar_type() == torch::kFloat32) launch_rows<float, TOP>(p);
   else launch_rows<rows::bf16_t, TOP>(p);
@@ -793,7 +848,7 @@ std::vector<torch::Tensor> sample_tokens(torch::Tensor logits, torch::Tensor u, 
   p.u = uc.data_ptr<float>();
   p.top_k = static_cast<int>(top_k >= logits.size(1) ? 0 : top_k);
   p.top_p = top_p;
-  p.log_min_p = std::log(min_p);
+  p.log_min_p = rows::kExps * std::log2(min_p);
   int bits = 0;
   while ((1ll << bits) < logits.size(1)) ++bits;
   p.one = std::min(51, 62 - bits);  // a weight fits the 52 bits of a double
