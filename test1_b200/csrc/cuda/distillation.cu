@@ -1,30 +1,45 @@
 // Divergence of a student from its teacher on the teacher's likeliest tokens,
 // and its gradient for the student's log-probabilities.
 //
-// Per row, with a_k = log p_k and b_k = log q_k of the listed tokens k and, with
-// a tail, p_r = 1 - sum p_k and q_r = 1 - sum q_k of the rest (at least 2^-20):
-//   forward  f(p, q) = q log(q / p)                     p f' = -q
-//   reverse  f(p, q) = p log(p / q)                     p f' = p (a - b + 1)
-//   jensen   f(p, q) = (p log(p/m) + q log(q/m)) / 2    p f' = p (a - log m) / 2,  m = (p + q) / 2
+// Per row, with a_k = log p_k and b_k = log q_k of the listed tokens k, d = b - a
+// and, with a tail, p_r = 1 - sum p_k and q_r = 1 - sum q_k of the rest (at least
+// 2^-20):
+//   forward  f(p, q) = q d                                     p f' = -q
+//   reverse  f(p, q) = -p d                                    p f' = f + p
+//   jensen   f(p, q) = (p log(p/m) + q log(q/m)) / 2           p f' = p log(p/m) / 2
+//            with m = (p + q) / 2, log(p/m) = -log((1 + e^d) / 2)
 //   L = sum f,  dL/da_k = p_k f'(p_k) - p_k f'(p_r), the second term only above the floor
 // Without a tail both are scaled to sum to 1 over the list first:
 //   dL/da_k = p_k f'(p_k) - p_k sum_j p_j f'(p_j)
+// Everything goes by d, the difference of two inputs, and not by logarithms of
+// rounded probabilities: where student and teacher are near each other the
+// terms cancel, and 2^-24 of a logarithm of 10 is more than is left of them.
 //
 // What is left of 1 is the difference of two numbers that nearly agree where
-// the list holds nearly all, so p and q are summed in 64 bits there (their
-// exponentials too: 2^-24 of a p near 1 would be all of a rest of 1e-7).
+// the list holds nearly all, so p and q are summed in 64 bits there, from
+// exponentials that are good to 2^-31 (2^-24 of a p near 1 would be all of a rest
+// of 1e-7): a power from a table in 64 bits, times a short series of what is left
+// of the exponent, below 0.003, for which 32 bits are enough.  The library's
+// 64-bit exponential takes twice the instructions, and instructions bound this.
 //
-// A warp per row, one read of the inputs.  The rows that take part are counted
-// first, in a launch of its own, because every gradient is divided by their
-// number.
+// G lanes have a row, PER entries each; the inputs are read once, a round ahead.
+// Every gradient is divided by the number of rows that take part.  A batch that
+// one cluster of 8 CTAs has in one round waits for the others' counts and then
+// writes; a larger one is scaled by a second launch, out of L2.
+#include "arrivals.cuh"
 #include "common.cuh"
+
+#include <cooperative_groups.h>
 
 namespace t1 {
 namespace distil {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr float kFloor = 0x1p-20f;
+constexpr int kExps = 128;  // steps of an octave in the table of exponentials
 
 enum Kind : int { kForward = 0, kReverse = 1, kJensen = 2 };
 
@@ -34,171 +49,280 @@ struct Params {
   const int64_t* ids;      // [T, K]
   int64_t T;
   int K, kind;
-  int* count;              // rows that take part
-  int* ticket;             // blocks that are done
+  Arrivals ticket;         // blocks that are done
   double* sums;            // [blocks]
+  int* counts;             // [blocks]
+  float* scale;            // 1 / rows that take part, for the second launch
   float* loss;
   float* dlogp;            // [T, K]
   float* each;             // [T]
 };
 
-template <typename V>
-__device__ __forceinline__ float as_float(const V* p);
-template <>
-__device__ __forceinline__ float as_float<float>(const float* p) {
-  return __ldg(p);
-}
-template <>
-__device__ __forceinline__ float as_float<__nv_bfloat16>(const __nv_bfloat16* p) {
-  return __bfloat162float(*p);
-}
+__device__ __forceinline__ float as_float(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float as_float(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-__device__ __forceinline__ double warp_sum(double v) {
+// Sums over G neighbouring lanes.
+template <int G, typename V>
+__device__ __forceinline__ V lanes_sum(V v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
-template <typename V>
-__global__ void __launch_bounds__(kThreads) count_kernel(const Params p) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int n = 0;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp; t < p.T; t += static_cast<int64_t>(gridDim.x) * kWarps) {
-    bool any = false;
-    for (int k = lane; k < p.K; k += 32)
-      any = any || (p.ids[t * p.K + k] >= 0 && as_float(static_cast<const V*>(p.teacher) + t * p.K + k) > -INFINITY);
-    n += __any_sync(0xffffffffu, any);
-  }
-  if (lane == 0 && n > 0) atomicAdd(p.count, n);
+// log((1 + e^-x) / 2) for x >= 0, to a few 2^-24 of itself however small x is:
+// with y = e^-x - 1 it is log(1 + y / 2) = 2 artanh(y / (4 + y)), |y / (4 + y)| < 1/3.
+__device__ __forceinline__ float log_half_sum(float x) {
+  // e^-x - 1: the exponential's series where the difference would cancel (its first term left out is 0.5^8 / 9!)
+  float s = fmaf(x, 1.f / 40320, -1.f / 5040);
+  s = fmaf(x, s, 1.f / 720);
+  s = fmaf(x, s, -1.f / 120);
+  s = fmaf(x, s, 1.f / 24);
+  s = fmaf(x, s, -1.f / 6);
+  s = fmaf(x, s, 0.5f);
+  s = fmaf(x, s, -1.f);
+  const float y = x < 0.5f ? x * s : __expf(-x) - 1.f;
+  const float z = __fdividef(y, 4.f + y), z2 = z * z;
+  float a = fmaf(z2, 2.f / 15, 2.f / 13);
+  a = fmaf(z2, a, 2.f / 11);
+  a = fmaf(z2, a, 2.f / 9);
+  a = fmaf(z2, a, 2.f / 7);
+  a = fmaf(z2, a, 2.f / 5);
+  a = fmaf(z2, a, 2.f / 3);
+  a = fmaf(z2, a, 2.f);
+  return z * a;
 }
 
-// f(p, q) and p f'(p) of an outcome, a = log p and b = log q.
-__device__ __forceinline__ void divergence(int kind, float p, float q, float a, float b, float& f, float& g) {
+// f(p, q) and p f'(p) of an outcome, d = log(q / p).
+__device__ __forceinline__ void divergence(int kind, float p, float q, float d, float& f, float& g) {
   if (kind == kForward) {
-    f = q > 0.f ? q * (b - a) : 0.f;
+    f = q > 0.f ? q * d : 0.f;
     g = -q;
   } else if (kind == kReverse) {
-    f = p > 0.f ? p * (a - b) : 0.f;
+    f = p > 0.f ? -p * d : 0.f;
     g = f + p;
   } else {
-    const float log_m = logf(0.5f * (p + q));
-    const float fp = p > 0.f ? 0.5f * p * (a - log_m) : 0.f;
-    f = fp + (q > 0.f ? 0.5f * q * (b - log_m) : 0.f);
-    g = fp;
+    const float l = log_half_sum(fabsf(d));
+    g = p > 0.f ? -0.5f * p * (fmaxf(d, 0.f) + l) : 0.f;
+    f = g + (q > 0.f ? -0.5f * q * (fmaxf(-d, 0.f) + l) : 0.f);
   }
 }
 
-// PER entries a lane.
-template <typename V, int PER, bool TAIL>
+// ONE: one cluster has the batch in one round.
+template <typename V, int G, int PER, bool TAIL, bool ONE>
 __global__ void __launch_bounds__(kThreads) loss_kernel(const Params p) {
+  __shared__ double exps[kExps];  // 2^(j / 128)
   __shared__ double of_warp[kWarps];
+  __shared__ int live_of_warp[kWarps];
+  __shared__ double of_cta[8];    // of the cluster
+  __shared__ int live_of_cta[8];
   __shared__ int last;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float scale = 1.f / static_cast<float>(max(1, *p.count));
-  double sum = 0.0;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp; t < p.T; t += static_cast<int64_t>(gridDim.x) * kWarps) {
-    float a[PER], b[PER];
-    bool keep[PER];
-    bool any = false;
+  constexpr int kRows = 32 / G;   // of a warp
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, of_row = lane % G;
+  // a row's entries, asked for one round ahead
+  const int64_t t_step = static_cast<int64_t>(gridDim.x) * kWarps * kRows;
+  const int64_t t_first = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * kRows;
+  int64_t t0 = t_first;
+  float next_a[PER], next_b[PER];
+  int64_t next_id[PER];
+  auto load = [&] {
+    const int64_t at = (t0 + lane / G) * p.K + of_row;
+    const int left = t0 + lane / G < p.T ? p.K - of_row : 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int k = lane + 32 * j;
-      const int64_t at = t * p.K + k;
-      keep[j] = false;
-      a[j] = b[j] = 0.f;
-      if (k < p.K) {
-        keep[j] = p.ids[at] >= 0;
-        b[j] = as_float(static_cast<const V*>(p.teacher) + at);
-        a[j] = __ldg(p.logp + at);
-      }
-      keep[j] = keep[j] && b[j] > -INFINITY;
-      any = any || keep[j];
+      const bool in = G * j < left;
+      next_id[j] = in ? __ldcs(p.ids + at + G * j) : -1;
+      next_b[j] = in ? as_float(static_cast<const V*>(p.teacher) + at + G * j) : 0.f;
+      next_a[j] = in ? __ldcs(p.logp + at + G * j) : 0.f;
     }
-    any = __any_sync(0xffffffffu, any);
-    float pk[PER], qk[PER], g[PER];
+  };
+  load();
+  if (TAIL) {
+    if (threadIdx.x < kExps) exps[threadIdx.x] = exp2(threadIdx.x / static_cast<double>(kExps));
+    __syncthreads();
+  }
+  if (!ONE) clear_arrivals(p.ticket);
+
+  // exp(v) for v <= about 1
+  auto exp64 = [&](float at) {
+    constexpr float kRound = 12582912.f;  // 1.5 2^23: adding it leaves a whole number in the low bits
+    const float v = fmaxf(at, -600.f);
+    const float y = fmaf(v, 1.4426950408889634f * kExps, kRound);
+    const int j = __float_as_int(y) - 0x4b400000;
+    const float n = y - kRound;
+    // v - n ln 2 / 128, the constant in two parts
+    const float r = fmaf(n, 1.4880111e-11f, fmaf(n, -0.00541521236f, v));
+    const float e = fmaf(fmaf(r, 1.f / 6, 0.5f) * r, r, r);
+    const double base = exps[j & (kExps - 1)];
+    const double power = __hiloint2double(__double2hiint(base) + ((j >> 7) << 20), __double2loint(base));
+    return fma(power, static_cast<double>(e), power);
+  };
+  static_assert(kExps == 128, "j >> 7");
+
+  double sum = 0.0;
+  int rows = 0;
+  float g[PER];
+  unsigned keep = 0;
+  auto store = [&](int64_t t, float scale) {
+    const int64_t at = t * p.K + of_row;
+    const int left = t < p.T ? p.K - of_row : 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (G * j < left && !T1_OOB(at + G * j, p.T * p.K)) p.dlogp[at + G * j] = keep >> j & 1 ? g[j] * scale : 0.f;
+  };
+  while (t0 < p.T) {
+    const int64_t t = t0 + lane / G;
+    float a[PER], b[PER];
+    keep = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      a[j] = next_a[j];
+      b[j] = next_b[j];
+      if (next_id[j] >= 0 && b[j] > -INFINITY) keep |= 1u << j;
+    }
+    t0 += t_step;
+    if (!ONE && t0 < p.T) load();
+    const unsigned lanes = __ballot_sync(0xffffffffu, keep != 0);
+    const bool live = (G == 32 ? lanes : (lanes >> (lane & ~(G - 1))) & ((1u << (G & 31)) - 1)) != 0;
+    float pk[PER], qk[PER];
     float loss = 0.f, rest = 0.f;  // rest: f'(p_r), without a tail sum p f'
+    float shift = 0.f;             // of d
     if (TAIL) {
       double ps = 0.0, qs = 0.0;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const double pd = keep[j] ? exp(static_cast<double>(a[j])) : 0.0, qd = keep[j] ? exp(static_cast<double>(b[j])) : 0.0;
-        ps += pd;
-        qs += qd;
-        pk[j] = static_cast<float>(pd);
-        qk[j] = static_cast<float>(qd);
+        const bool in = keep >> j & 1;
+        const double pd = exp64(a[j]), qd = exp64(b[j]);
+        ps += in ? pd : 0.0;
+        qs += in ? qd : 0.0;
+        pk[j] = in ? static_cast<float>(pd) : 0.f;
+        qk[j] = in ? static_cast<float>(qd) : 0.f;
       }
-      ps = 1.0 - warp_sum(ps);
-      qs = 1.0 - warp_sum(qs);
+      ps = 1.0 - lanes_sum<G>(ps);
+      qs = 1.0 - lanes_sum<G>(qs);
       const float pr = fmaxf(static_cast<float>(ps), kFloor), qr = fmaxf(static_cast<float>(qs), kFloor);
       float fr, gr;
-      divergence(p.kind, pr, qr, logf(pr), logf(qr), fr, gr);
+      divergence(p.kind, pr, qr, logf(qr / pr), fr, gr);
       rest = ps > kFloor ? gr / pr : 0.f;
-      if (lane == 0) loss = fr;
+      if (of_row == 0) loss = fr;
     } else {
       // scaled to sum to 1
-      float am = -INFINITY, bm = -INFINITY;
+      float am = -INFINITY, bm = -INFINITY, as = 0.f, bs = 0.f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        if (!keep[j]) continue;
-        am = fmaxf(am, a[j]);
-        bm = fmaxf(bm, b[j]);
+        if (keep >> j & 1) am = fmaxf(am, a[j]);
+        if (keep >> j & 1) bm = fmaxf(bm, b[j]);
       }
-      am = warp_max(am);
-      bm = warp_max(bm);
-      float as = 0.f, bs = 0.f;
+      am = lanes_max<G>(am);
+      bm = lanes_max<G>(bm);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        if (!keep[j]) continue;
-        as += expf(a[j] - am);
-        bs += expf(b[j] - bm);
+        pk[j] = keep >> j & 1 ? expf(a[j] - am) : 0.f;
+        qk[j] = keep >> j & 1 ? expf(b[j] - bm) : 0.f;
+        as += pk[j];
+        bs += qk[j];
       }
-      am += logf(t1::warp_sum(as));
-      bm += logf(t1::warp_sum(bs));
+      as = lanes_sum<G>(as);
+      bs = lanes_sum<G>(bs);
+      shift = (bm - am) + logf(bs / as);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        a[j] -= am;
-        b[j] -= bm;
-        pk[j] = keep[j] ? expf(a[j]) : 0.f;
-        qk[j] = keep[j] ? expf(b[j]) : 0.f;
+        pk[j] = keep >> j & 1 ? pk[j] / as : 0.f;
+        qk[j] = keep >> j & 1 ? qk[j] / bs : 0.f;
       }
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      float f = 0.f;
-      g[j] = 0.f;
-      if (keep[j]) divergence(p.kind, pk[j], qk[j], a[j], b[j], f, g[j]);
-      loss += f;
-      if (!TAIL) rest += g[j];
+      float f;
+      divergence(p.kind, pk[j], qk[j], (b[j] - a[j]) - shift, f, g[j]);
+      loss += keep >> j & 1 ? f : 0.f;
+      if (!TAIL) rest += keep >> j & 1 ? g[j] : 0.f;
     }
-    loss = t1::warp_sum(loss);
-    if (!TAIL) rest = t1::warp_sum(rest);
+    loss = lanes_sum<G>(loss);
+    if (!TAIL) rest = lanes_sum<G>(rest);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int k = lane + 32 * j;
-      const int64_t at = t * p.K + k;
-      if (k < p.K && !T1_OOB(at, p.T * p.K)) p.dlogp[at] = keep[j] ? (g[j] - pk[j] * rest) * scale : 0.f;
+    for (int j = 0; j < PER; ++j) g[j] -= pk[j] * rest;
+    if (!live) loss = 0.f;
+    if (of_row == 0) {
+      if (t < p.T && !T1_OOB(t, p.T)) p.each[t] = loss;
+      sum += loss;
+      rows += live;
     }
-    if (!any) loss = 0.f;
-    if (lane == 0 && !T1_OOB(t, p.T)) p.each[t] = loss;
-    sum += loss;
+    if (!ONE) store(t, 1.f);
+  }
+  sum = lanes_sum<32>(sum);
+  rows = __reduce_add_sync(0xffffffffu, rows);
+  if (lane == 0) {
+    of_warp[warp] = sum;
+    live_of_warp[warp] = rows;
+  }
+  __syncthreads();
+  sum = 0.0;
+  rows = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    sum += of_warp[w];
+    rows += live_of_warp[w];
+  }
+  if (ONE) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const unsigned ctas = cluster.num_blocks();
+    if (threadIdx.x < ctas) {
+      cluster.map_shared_rank(of_cta, threadIdx.x)[cluster.block_rank()] = sum;
+      cluster.map_shared_rank(live_of_cta, threadIdx.x)[cluster.block_rank()] = rows;
+    }
+    cluster.sync();
+    sum = 0.0;
+    rows = 0;
+    for (unsigned r = 0; r < ctas; ++r) {
+      sum += of_cta[r];
+      rows += live_of_cta[r];
+    }
+    const float scale = 1.f / static_cast<float>(max(1, rows));
+    store(t_first + lane / G, scale);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.loss = static_cast<float>(sum * scale);
+    return;
   }
   // the blocks' sums in their order, by the last one
-  if (lane == 0) of_warp[warp] = sum;
-  __syncthreads();
   if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int w = 0; w < kWarps; ++w) sum += of_warp[w];
     __stcg(p.sums + blockIdx.x, sum);
+    __stcg(p.counts + blockIdx.x, rows);
     __threadfence();
-    last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+    last = atomicAdd(p.ticket.use, 1) == static_cast<int>(gridDim.x) - 1;
   }
   __syncthreads();
   if (!last || warp != 0) return;
   __threadfence();
   sum = 0.0;
-  for (int i = lane; i < static_cast<int>(gridDim.x); i += 32) sum += __ldcg(p.sums + i);
-  sum = warp_sum(sum);
-  if (lane == 0) *p.loss = static_cast<float>(sum * scale);
+  rows = 0;
+  for (int i = lane; i < static_cast<int>(gridDim.x); i += 32) {
+    sum += __ldcg(p.sums + i);
+    rows += __ldcg(p.counts + i);
+  }
+  sum = lanes_sum<32>(sum);
+  rows = __reduce_add_sync(0xffffffffu, rows);
+  const float scale = 1.f / static_cast<float>(max(1, rows));
+  if (lane == 0) {
+    *p.loss = static_cast<float>(sum * scale);
+    *p.scale = scale;
+  }
+}
+
+// dlogp times the scale; dlogp is freshly allocated and so begins on 16 bytes.
+__global__ void __launch_bounds__(kThreads) scale_kernel(float* dlogp, int64_t n, const float* scale) {
+  const float s = *scale;
+  const int64_t vecs = n / 4, step = static_cast<int64_t>(gridDim.x) * kThreads;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  for (int64_t i = i0; i < vecs; i += step) {
+    float4 v = reinterpret_cast<float4*>(dlogp)[i];
+    v = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
+    reinterpret_cast<float4*>(dlogp)[i] = v;
+  }
+  if (i0 < n - 4 * vecs) dlogp[4 * vecs + i0] *= s;
 }
 
 }  // namespace distil
@@ -206,23 +330,52 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Params p) {
 // ================================================================ host side
 T1_BOUNDS_READER(distillation)
 
-template <typename V, int PER>
-static void launch_loss(const distil::Params& p, int blocks, bool tail) {
-  if (tail) distil::loss_kernel<V, PER, true><<<blocks, distil::kThreads, 0, stream()>>>(p);
-  else distil::loss_kernel<V, PER, false><<<blocks, distil::kThreads, 0, stream()>>>(p);
+template <typename V, int G, int PER>
+static void launch_loss(distil::Params& p, bool tail) {
+  const int64_t per_block = distil::kWarps * (32 / G), blocks_one = (p.T + per_block - 1) / per_block;
+  if (blocks_one <= 8) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks_one);
+    cfg.blockDim = dim3(distil::kThreads);
+    cfg.stream = stream();
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = blocks_one;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    auto kern = tail ? distil::loss_kernel<V, G, PER, true, true> : distil::loss_kernel<V, G, PER, false, true>;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<const distil::Params>(p));
+    TORCH_CHECK(e == cudaSuccess, "distillation_loss launch failed: ", cudaGetErrorString(e));
+    count_launch();
+    return;
+  }
+  const int blocks = static_cast<int>(std::min<int64_t>(blocks_one, 8 * num_sms()));
+  auto ws = torch::empty({2 * blocks + 1}, torch::TensorOptions().dtype(torch::kFloat64).device(torch::kCUDA, at::cuda::current_device()));
+  p.sums = ws.data_ptr<double>();
+  p.counts = reinterpret_cast<int*>(p.sums + blocks);
+  p.scale = reinterpret_cast<float*>(p.sums + 2 * blocks);
+  ArrivalCounters counters(1);
+  p.ticket = counters.arrivals;
+  auto kern = tail ? distil::loss_kernel<V, G, PER, true, false> : distil::loss_kernel<V, G, PER, false, false>;
+  kern<<<blocks, distil::kThreads, 0, stream()>>>(p);
   check_launch("distillation_loss");
-  count_launch();
+  counters.launched();
+  const int64_t n = p.T * p.K;
+  distil::scale_kernel<<<static_cast<int>(std::min<int64_t>((n / 4 + distil::kThreads) / distil::kThreads, 8 * num_sms())),
+                         distil::kThreads, 0, stream()>>>(p.dlogp, n, p.scale);
+  check_launch("distillation_loss");
+  count_launch(2);
 }
 
 template <typename V>
-static void run_loss(const distil::Params& p, int blocks, bool tail) {
-  distil::count_kernel<V><<<blocks, distil::kThreads, 0, stream()>>>(p);
-  check_launch("distillation_loss");
-  count_launch();
-  if (p.K <= 32) launch_loss<V, 1>(p, blocks, tail);
-  else if (p.K <= 64) launch_loss<V, 2>(p, blocks, tail);
-  else if (p.K <= 128) launch_loss<V, 4>(p, blocks, tail);
-  else launch_loss<V, 16>(p, blocks, tail);
+static void run_loss(distil::Params& p, bool tail) {
+  if (p.K <= 8) launch_loss<V, 8, 1>(p, tail);
+  else if (p.K <= 16) launch_loss<V, 8, 2>(p, tail);
+  else if (p.K <= 32) launch_loss<V, 8, 4>(p, tail);
+  else if (p.K <= 64) launch_loss<V, 16, 4>(p, tail);
+  else if (p.K <= 128) launch_loss<V, 32, 4>(p, tail);
+  else launch_loss<V, 32, 16>(p, tail);
 }
 
 // Returns (loss [], dlogp [T, K], divergence of every row [T]), fp32.
@@ -241,12 +394,10 @@ std::vector<torch::Tensor> distillation_loss(torch::Tensor logp, torch::Tensor t
   const c10::cuda::CUDAGuard guard(logp.device());
   const int64_t T = logp.size(0), K = logp.size(1);
   auto f32 = logp.options();
-  auto dlogp = torch::empty({T, K}, f32), each = torch::empty({T}, f32), loss = torch::zeros({}, f32);
-  if (T == 0) return {loss, dlogp, each};
+  auto dlogp = torch::empty({T, K}, f32), each = torch::empty({T}, f32);
+  if (T == 0) return {torch::zeros({}, f32), dlogp, each};
+  auto loss = torch::empty({}, f32);
   auto lp = logp.contiguous(), te = teacher.contiguous(), id = ids.contiguous();
-  const int blocks = static_cast<int>(std::min<int64_t>((T + distil::kWarps - 1) / distil::kWarps, 8 * num_sms()));
-  auto counters = torch::zeros({2}, f32.dtype(torch::kInt32));
-  auto sums = torch::empty({blocks}, f32.dtype(torch::kFloat64));
   distil::Params p{};
   p.logp = lp.data_ptr<float>();
   p.teacher = te.data_ptr();
@@ -254,14 +405,11 @@ std::vector<torch::Tensor> distillation_loss(torch::Tensor logp, torch::Tensor t
   p.T = T;
   p.K = static_cast<int>(K);
   p.kind = static_cast<int>(kind);
-  p.count = counters.data_ptr<int>();
-  p.ticket = p.count + 1;
-  p.sums = sums.data_ptr<double>();
   p.loss = loss.data_ptr<float>();
   p.dlogp = dlogp.data_ptr<float>();
   p.each = each.data_ptr<float>();
-  if (te.scalar_type() == torch::kFloat32) run_loss<float>(p, blocks, tail);
-  else run_loss<__nv_bfloat16>(p, blocks, tail);
+  if (te.scalar_type() == torch::kFloat32) run_loss<float>(p, tail);
+  else run_loss<__nv_bfloat16>(p, tail);
   return {loss, dlogp, each};
 }
 

@@ -293,8 +293,77 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     own_max = fmaxf(fmaxf(own_max, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
   }
   float m = block_max(own_max, red);
+  // A token to the first CTA's list.
+  unsigned* const list_length = cluster.map_shared_rank(&sh.listed, 0);
+  unsigned long long* const first_list = cluster.map_shared_rank(sh.list, 0);
+  auto push = [&](float z, int column) {
+    const unsigned at = atomicAdd(list_length, 1u);
+    if (at < kListSlots) first_list[at] = place_of(z + 0.f, column);  // -0 is 0
+  };
+  // Distance from a largest logit in steps of a sixteenth of its octave, 2^-8 to 2^8, and the least logit of a step (a
+  // little lower, for the rounding of the distance).
+  auto step_of = [](float from, float z) {
+    const int s = static_cast<int>(__float_as_uint(from - z) >> 19) - (119 << 4);
+    return min(max(s, 0), kBins - 1);
+  };
+  auto least_of = [](float from, int step) {
+    return from - __uint_as_float(static_cast<unsigned>(step + 1 + (119 << 4)) << 19) * 1.000001f;
+  };
+  // Sum of exp((z - from) / tau) over this CTA's logits, and the tokens from `bound` on to the list.  Where `from` is
+  // infinite, or its neighbours lie far below it, it has all the weight.
+  auto is_sharp = [&](float from) { return !(fabsf(from) * 0x1p-23f <= 100.f * p.tau); };
+  auto sum_and_push = [&](float from, float bound) {
+    if (is_sharp(from)) {
+      float sum = 0.f;
+      for (int i = 0; i < n; ++i) sum += v[32 * i] == from;
+      if (bound < INFINITY)
+        for (int i = 0; i < n; ++i)
+          if (is_token(v[32 * i]) && v[32 * i] >= bound) push(v[32 * i], col0 + 32 * i);
+      return block_sum(sum, red);
+    }
+    const float low = from - 400.f * p.tau;  // exp(-350) is no weight here: below, and NaN, counts as that
+    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < n / 4; ++i) {
+      const float4 q = quads[32 * i];
+      const float z[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast((fmaxf(z[j], low) - from) * p.scale2);
+      if (fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= bound) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (is_token(z[j]) && z[j] >= bound) push(z[j], warp_col0 + 4 * (32 * i + lane) + j);
+      }
+    }
+    return block_sum((s4[0] + s4[1]) + (s4[2] + s4[3]), red);
+  };
+  // The bin in which `need` is reached (-1: in none) of all CTAs' bins, and in sh.before64 what comes before.
+  auto reach = [&](unsigned (*bins)[kBins], bool weights, unsigned long long need) {
+    unsigned long long here = 0, before;
+    if (tid < kBins) {
+      for (int r = 0; r < ctas; ++r) {
+        const unsigned* b = cluster.map_shared_rank(&bins[0][0], r);
+        here += b[tid];
+        if (weights)
+          here += (static_cast<unsigned long long>(b[kBins + tid]) << 16) + (static_cast<unsigned long long>(b[2 * kBins + tid]) << 32);
+      }
+    }
+    if (tid == 0) sh.bin = -1;
+    block_scan64(here, before, sh.red);
+    if (before < need && before + here >= need) {
+      sh.bin = tid;
+      sh.before64 = before;
+      sh.here64 = here;
+    }
+    __syncthreads();
+    return sh.bin;
+  };
+
+  const unsigned first = TOP ? p.k : p.top_k;
+  float log_sum = 0.f;  // log of the sum of all weights
   tell_all(cluster, sh.max_of, m);
   for (int r = 0; r < ctas; ++r) m = fmaxf(m, sh.max_of[r]);
+  // m is the row's largest from here on
   if (m == -INFINITY) {
     if (rank != 0) return;
     for (int i = tid; i < (TOP ? p.k : 1); i += kThreads) {
@@ -303,19 +372,16 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     }
     return;
   }
-  // Where m is infinite, or its neighbours lie far below it, the largest logits have all the weight.
-  const bool sharp = !(fabsf(m) * 0x1p-23f <= 100.f * p.tau);
-  const float top = m;
+  const bool sharp = is_sharp(m);
   if (!TOP && sharp) {
     for (int i = 0; i < n; ++i) v[32 * i] = v[32 * i] == m ? 0.f : -INFINITY;
     own_max = own_max == m ? 0.f : -INFINITY;
     m = 0.f;
     __syncwarp();
   }
-  // exp(-350) is no weight in any precision here: below, and NaN, counts as that
   const float low = m - 400.f * p.tau;
-  auto log_p = [&](float z, float log_sum) {
-    return (z == m ? 0.f : TOP && top == INFINITY ? -INFINITY : (z - m) * p.scale) - log_sum;
+  auto log_p = [&](float z) {
+    return (z == m ? 0.f : m == INFINITY ? -INFINITY : (z - m) * p.scale) - log_sum;
   };
 
   const double m64 = m;
@@ -340,11 +406,6 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
   };
   static_assert(kExps == 128, "j >> 7");
   auto weight = [&](float z) { return weight_at(steps_of(z)); };
-  // Distance from m in steps of a sixteenth of its octave, 2^-8 to 2^8.
-  auto step_of = [&](float z) {
-    const int s = static_cast<int>(__float_as_uint(m - z) >> 19) - (119 << 4);
-    return min(max(s, 0), kBins - 1);
-  };
   // Bins of 16 steps of a weight's logarithm, and 256 parts of one.
   auto bin_at = [&](double x) { return -__double2loint(x + kRound) >> 4; };
   auto part_at = [&](double x, int bin) { return min(max(static_cast<int>((0.5 - x - 16 * bin) * 16.0), 0), kBins - 1); };
@@ -352,77 +413,29 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     const unsigned lo = static_cast<unsigned>(w) & 0xffffu, mid = static_cast<unsigned>(w >> 16) & 0xffffu,
                    hi = static_cast<unsigned>(w >> 32);
     atomicAdd(&bins[0][b], lo);
-    if (mid != 0) atomicAdd(&bins[1][b], mid);
+    atomicAdd(&bins[1][b], mid);
     if (hi != 0) atomicAdd(&bins[2][b], hi);
   };
-  // The bin in which `need` is reached (-1: in none), and in sh.before64 what comes before it; all CTAs' bins.
-  auto reach = [&](unsigned (*bins)[kBins], bool weights, unsigned long long need) {
-    unsigned long long here = 0, before;
-    if (tid < kBins) {
-      for (int r = 0; r < ctas; ++r) {
-        const unsigned* b = cluster.map_shared_rank(&bins[0][0], r);
-        here += b[tid];
-        if (weights)
-          here += (static_cast<unsigned long long>(b[kBins + tid]) << 16) + (static_cast<unsigned long long>(b[2 * kBins + tid]) << 32);
-      }
-    }
-    if (tid == 0) sh.bin = -1;
-    block_scan64(here, before, sh.red);
-    if (before < need && before + here >= need) {
-      sh.bin = tid;
-      sh.before64 = before;
-      sh.here64 = here;
-    }
-    __syncthreads();
-    return sh.bin;
-  };
-  // A token to the first CTA's list.
-  unsigned* const list_length = cluster.map_shared_rank(&sh.listed, 0);
-  unsigned long long* const first_list = cluster.map_shared_rank(sh.list, 0);
-  auto push = [&](float z, int column) {
-    const unsigned at = atomicAdd(list_length, 1u);
-    if (at < kListSlots) first_list[at] = place_of(z + 0.f, column);  // -0 is 0
-  };
-
-  const unsigned first = TOP ? p.k : p.top_k;
-  float log_sum;
   unsigned long long total = 0, own = 0;  // own: the thread's kept weight
+  unsigned long long before_cta = 0;
+  bool alone = false;                     // the other CTAs have left
   bool done = false;                      // the cut is found
   unsigned long long cut_place = 0;       // with done: the last token kept
+  float cut_logit = -INFINITY;
+  int cut_column = 0;
 
   if (TOP || first != 0) {
     // ---- list
-    const bool by_list = !sharp && first <= kListSlots / 2 && first <= static_cast<unsigned>(ctas * kThreads);
+    const bool by_list = !sharp && first <= kThreads;
     float bound = INFINITY;
     if (by_list) {
-      if (is_token(own_max)) atomicAdd(&sh.bins[0][0][step_of(own_max)], 1u);
+      if (is_token(own_max)) atomicAdd(&sh.bins[0][0][step_of(m, own_max)], 1u);
       sync_all(cluster);
       const int bin = reach(sh.bins[0], false, first);
-      // the far edge of that step, and a little more for the rounding of m - z
-      if (bin >= 0 && bin < kBins - 1) bound = m - __uint_as_float(static_cast<unsigned>(bin + 1 + (119 << 4)) << 19) * 1.000001f;
+      if (bin >= 0 && bin < kBins - 1) bound = least_of(m, bin);
     }
+    tell_all(cluster, sh.sum_of, sum_and_push(m, bound));
     float sum = 0.f;
-    if (TOP && sharp) {
-      for (int i = 0; i < n; ++i) sum += v[32 * i] == m;
-    } else {
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int i = 0; i < n / 4; ++i) {
-        const float4 q = quads[32 * i];
-        const float z[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast((fmaxf(z[j], low) - m) * p.scale2);
-        if (fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= bound) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (z[j] >= bound) push(z[j], warp_col0 + 4 * (32 * i + lane) + j);
-        }
-      }
-      sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-    }
-    sum = block_sum(sum, red);
-    tell_all(cluster, sh.sum_of, sum);
-    sum = 0.f;
     for (int r = 0; r < ctas; ++r) sum += sh.sum_of[r];
     log_sum = logf(sum);
     const unsigned listed = *list_length;
@@ -431,13 +444,14 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
       order_list(sh.list, listed);
       if (TOP) {
         for (int i = tid; i < p.k; i += kThreads) {
+          const bool in = i < static_cast<int>(listed);  // of fewer tokens than k all are listed
           const int64_t at = static_cast<int64_t>(row) * p.k + i;
-          p.logp[at] = log_p(logit_at(sh.list[i]), log_sum);
-          p.ids[at] = column_at(sh.list[i]);
+          p.logp[at] = in ? log_p(logit_at(sh.list[i])) : 0.f;
+          p.ids[at] = in ? column_at(sh.list[i]) : -1;
         }
       } else {
         // kept by top_p and min_p?
-        unsigned long long before, e = tid < static_cast<int>(first) ? sh.list[tid] : 0ull;
+        unsigned long long before, e = tid < static_cast<int>(min(first, listed)) ? sh.list[tid] : 0ull;
         const double x = e != 0 ? steps_of(logit_at(e)) : 0.0;
         const unsigned long long w = e != 0 ? weight_at(x) : 0ull;
         const unsigned long long sum64 = block_scan64(w, before, sh.red);
@@ -450,12 +464,12 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
         order_list(sh.list, kept);
         e = tid < static_cast<int>(kept) ? sh.list[tid] : 0ull;
         const float z = logit_of(static_cast<unsigned>(e));
-        const unsigned long long w2 = e != 0 ? weight(z) : 0ull;
+        const unsigned long long w2 = e != 0 ? weight_at(steps_of(z)) : 0ull;
         const unsigned long long all = block_scan64(w2, before, sh.red);
         const unsigned long long target = target_of(p.u[row], all);
         if (before <= target && target < before + w2) {
           p.ids[row] = static_cast<int>(~static_cast<unsigned>(e >> 32));
-          p.logp[row] = log_p(z, log_sum);
+          p.logp[row] = log_p(z);
         }
       }
       sync_all(cluster);
@@ -475,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
         own += w;
         if (by_bins) {
           const int b = bin_at(x);
-          if (b < kBins && w != 0) add_to(sh.bins[0], b, w);
+          if (b < kBins) add_to(sh.bins[0], b, w);
         }
       }
     }
@@ -490,22 +504,30 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
         need -= sh.before64;
         // no more tokens than this have the bin's weight
         const bool few = sh.here64 / max(1ull, weight_at(-16.0 * (bin + 1))) < kListSlots;
+        // the bin's logits lie between these
+        const float least = __double2float_rd(m64 - 16.0 * (bin + 1) / p.steps), most = __double2float_ru(m64 - (16.0 * bin - 1) / p.steps);
         int part = 0;
         if (!few) {
-#pragma unroll 4
+#pragma unroll 8
           for (int i = 0; i < n; ++i) {
-            const double x = steps_of(v[32 * i]);
+            const float z = v[32 * i];
+            if (!(z >= least && z <= most)) continue;
+            const double x = steps_of(z);
             if (bin_at(x) == bin) add_to(sh.bins[1], part_at(x, bin), weight_at(x));
           }
           sync_all(cluster);
           part = reach(sh.bins[1], true, need);
           need -= sh.before64;
         }
-#pragma unroll 4
+        auto at_border = [&](float z) {
+          if (!(z >= least && z <= most)) return false;
+          const double x = steps_of(z);
+          return bin_at(x) == bin && (few || part_at(x, bin) == part);
+        };
+#pragma unroll 8
         for (int i = 0; i < n; ++i) {
           const float z = v[32 * i];
-          const double x = steps_of(z);
-          if (bin_at(x) == bin && is_token(z) && (few || part_at(x, bin) == part)) push(z, col0 + 32 * i);
+          if (is_token(z) && at_border(z)) push(z, col0 + 32 * i);
         }
         sync_all(cluster);
         const unsigned listed = *list_length;
@@ -530,6 +552,35 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
           }
           sync_all(cluster);
           cut_place = sh.cut_of[0];
+          cut_logit = logit_at(cut_place);
+          cut_column = column_at(cut_place);
+          if (steps_of(cut_logit) >= p.log_min_p) {
+            // min_p takes no more away: the CTA's kept weight from its bins and the border's tokens
+            own = 0;
+            if (tid < kBins) {
+              auto of = [&](unsigned (*bins)[kBins]) {
+                return bins[0][tid] + (static_cast<unsigned long long>(bins[1][tid]) << 16) + (static_cast<unsigned long long>(bins[2][tid]) << 32);
+              };
+              if (tid < bin) own = of(sh.bins[0]);
+              if (!few && tid < part) own += of(sh.bins[1]);
+            }
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) {
+              const float z = v[32 * i];
+              if ((z > cut_logit || (z == cut_logit && col0 + 32 * i <= cut_column)) && at_border(z)) own += weight(z);
+            }
+            tell_all(cluster, sh.kept_of, block_scan64(own, before, sh.red));
+            unsigned long long kept = 0, mine = 0;
+            for (int r = 0; r < ctas; ++r) {
+              if (r == rank) mine = kept;
+              kept += sh.kept_of[r];
+            }
+            const unsigned long long target = target_of(p.u[row], kept);
+            if (target < mine || target >= mine + sh.kept_of[rank]) return;
+            alone = true;  // the token drawn is this CTA's
+            before_cta = mine;
+            total = kept;
+          }
         }
       }
     }
@@ -659,30 +710,17 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     tell_all(cluster, sh.ties_of, of_cta);
     for (int r = 0; r < rank; ++r) tie += sh.ties_of[r];
   }
-  if (first != 0 || (!TOP && (p.top_p < 1.0 || p.log_min_p > -INFINITY))) {
-    own = 0;
-    const float cut_logit = done ? logit_at(cut_place) : -INFINITY;
-    const int cut_column = done ? column_at(cut_place) : 0;
+  if (cut.key != 0) {
 #pragma unroll 2
     for (int i = 0; i < n; ++i) {
       const float z = v[32 * i];
-      bool in;
-      if (done) {
-        in = z > cut_logit || (z == cut_logit && col0 + 32 * i <= cut_column);
-      } else {
-        const unsigned key = key_of(z + 0.f);
-        in = is_token(z) && key > cut.key;
-        if (cut.ties != 0) {
-          const bool equal = is_token(z) && key == cut.key;
-          const unsigned all = __ballot_sync(0xffffffffu, equal);
-          in = in || (equal && tie + __popc(all & ((1u << lane) - 1)) < cut.ties);
-          tie += __popc(all);
-        }
-      }
-      if (!TOP && in) {
-        const double x = steps_of(z);
-        in = x >= p.log_min_p;
-        if (in) own += weight_at(x);
+      const unsigned key = key_of(z + 0.f);
+      bool in = is_token(z) && key > cut.key;
+      if (cut.ties != 0) {
+        const bool equal = is_token(z) && key == cut.key;
+        const unsigned all = __ballot_sync(0xffffffffu, equal);
+        in = in || (equal && tie + __popc(all & ((1u << lane) - 1)) < cut.ties);
+        tie += __popc(all);
       }
       if (!in) v[32 * i] = -INFINITY;  // from here on no token
     }
@@ -703,21 +741,41 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     for (int i = tid; i < p.k; i += kThreads) {
       const bool in = i < static_cast<int>(have);
       const int64_t at = static_cast<int64_t>(row) * p.k + i;
-      p.logp[at] = in ? log_p(logit_at(sh.list[i]), log_sum) : 0.f;
+      p.logp[at] = in ? log_p(logit_at(sh.list[i])) : 0.f;
       p.ids[at] = in ? column_at(sh.list[i]) : -1;
     }
     return;
   }
 
   // ---- the draw
+  const float min_logit = p.log_min_p > -INFINITY ? __double2float_rd(m64 + (p.log_min_p - 1.0) / p.steps) : -INFINITY;
+  auto kept_at = [&](float z, int column) {
+    if (!is_token(z) || z < min_logit) return false;
+    if (done && !(z > cut_logit || (z == cut_logit && column <= cut_column))) return false;
+    return p.log_min_p == -INFINITY || steps_of(z) >= p.log_min_p;
+  };
+  if (first != 0 || done || p.top_p < 1.0 || p.log_min_p > -INFINITY) {
+    own = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      // which of 32 are kept, then those alone: a thread's few rather than a warp's many
+      unsigned kept = 0;
+#pragma unroll 8
+      for (int i = 0; i < min(32, n - i0); ++i) kept |= kept_at(v[32 * (i0 + i)], col0 + 32 * (i0 + i)) ? 1u << i : 0u;
+      for (; kept != 0; kept &= kept - 1) own += weight(v[32 * (i0 + __ffs(kept) - 1)]);
+    }
+  }
   unsigned long long before;
-  const unsigned long long of_warp = warp_sum64(own);
-  tell_all(cluster, sh.kept_of, block_scan64(own, before, sh.red));
-  total = 0;
+  const unsigned long long of_warp = warp_sum64(own), of_cta = block_scan64(own, before, sh.red);
   before = __shfl_sync(0xffffffffu, before, 0);  // the warp's
-  for (int r = 0; r < ctas; ++r) {
-    if (r == rank) before += total;
-    total += sh.kept_of[r];
+  if (alone) {
+    before += before_cta;
+  } else {
+    tell_all(cluster, sh.kept_of, of_cta);
+    total = 0;
+    for (int r = 0; r < ctas; ++r) {
+      if (r == rank) before += total;
+      total += sh.kept_of[r];
+    }
   }
   const unsigned long long target = target_of(p.u[row], total);
   if (target < before || target >= before + of_warp) return;
@@ -725,7 +783,10 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
   unsigned long long at = before;
   for (int i0 = 0; i0 < n; i0 += 32) {
     __syncwarp();
-    for (int i = 0; i < min(32, n - i0); ++i) sh.cells[i][lane] = weight(v[32 * (i0 + i)]);
+    for (int i = 0; i < min(32, n - i0); ++i) {
+      const float z = v[32 * (i0 + i)];
+      sh.cells[i][lane] = kept_at(z, col0 + 32 * (i0 + i)) ? weight(z) : 0ull;
+    }
     __syncwarp();
     unsigned long long s = 0;
     if (i0 + lane < n)
@@ -741,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     const unsigned long long mine = at + warp_scan64(sh.cells[l][lane], lane);
     if (lane == __ffs(__ballot_sync(0xffffffffu, target < mine)) - 1) {
       p.ids[row] = col0 + 32 * (i0 + l);
-      p.logp[row] = log_p(v[32 * (i0 + l)], log_sum);
+      p.logp[row] = log_p(v[32 * (i0 + l)]);
     }
     return;
   }
