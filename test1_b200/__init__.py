@@ -4,12 +4,14 @@ Public API (same names as the SlideFSDP reference):
     SlideFSDPConfig, SlideFSDP, LayerAdam, SlidingCheckpoint
 and for training on preferences or sampled answers:
     PreferenceObjective, PolicyObjective
+or on a teacher's likeliest tokens:
+    DistillationObjective
 """
 from .config import SlideFSDPConfig
 from .optim.layer_adam import LayerAdam
 
 __all__ = ["SlideFSDPConfig", "SlideFSDP", "LayerAdam", "SlidingCheckpoint", "LlamaConfig",
-           "LlamaForCausalLM", "PreferenceObjective", "PolicyObjective"]
+           "LlamaForCausalLM", "PreferenceObjective", "PolicyObjective", "DistillationObjective"]
 __version__ = "0.1.0"
 
 
@@ -22,7 +24,7 @@ def __getattr__(name):
         from .sliding_checkpoint import SlidingCheckpoint
 
         return SlidingCheckpoint
-    if name in ("PreferenceObjective", "PolicyObjective"):
+    if name in ("PreferenceObjective", "PolicyObjective", "DistillationObjective"):
         from . import objectives
 
         return getattr(objectives, name)

@@ -22,7 +22,9 @@
 // of the exponent, below 0.003, for which 32 bits are enough.  The library's
 // 64-bit exponential takes twice the instructions, and instructions bound this.
 //
-// G lanes have a row, PER entries each; the inputs are read once, a round ahead.
+// G lanes have a row, PER entries each; the inputs are read once.  (Asking for
+// them a round ahead takes the registers of half of the warps: 46 us for 64 x
+// 1025 x 64 against 40.)
 // Every gradient is divided by the number of rows that take part.  A batch that
 // one cluster of 8 CTAs has in one round waits for the others' counts and then
 // writes; a larger one is scaled by a second launch, out of L2.
@@ -46,6 +48,7 @@ enum Kind : int { kForward = 0, kReverse = 1, kJensen = 2 };
 struct Params {
   const float* logp;       // [T, K]
   const void* teacher;     // [T, K]
+  bool teacher_bf16;
   const int64_t* ids;      // [T, K]
   int64_t T;
   int K, kind;
@@ -57,9 +60,6 @@ struct Params {
   float* dlogp;            // [T, K]
   float* each;             // [T]
 };
-
-__device__ __forceinline__ float as_float(const float* p) { return __ldg(p); }
-__device__ __forceinline__ float as_float(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
 // Sums over G neighbouring lanes.
 template <int G, typename V>
@@ -98,24 +98,25 @@ __device__ __forceinline__ float log_half_sum(float x) {
   return z * a;
 }
 
-// f(p, q) and p f'(p) of an outcome, d = log(q / p).
+// f(p, q) and p f'(p) of an outcome, d = log(q / p), finite: 0 times it is 0.
 __device__ __forceinline__ void divergence(int kind, float p, float q, float d, float& f, float& g) {
   if (kind == kForward) {
-    f = q > 0.f ? q * d : 0.f;
+    f = q * d;
     g = -q;
   } else if (kind == kReverse) {
-    f = p > 0.f ? -p * d : 0.f;
+    f = -p * d;
     g = f + p;
   } else {
     const float l = log_half_sum(fabsf(d));
-    g = p > 0.f ? -0.5f * p * (fmaxf(d, 0.f) + l) : 0.f;
-    f = g + (q > 0.f ? -0.5f * q * (fmaxf(-d, 0.f) + l) : 0.f);
+    g = -0.5f * p * (fmaxf(d, 0.f) + l);
+    f = fmaf(-0.5f * q, fmaxf(-d, 0.f) + l, g);
   }
 }
 
-// ONE: one cluster has the batch in one round.
-template <typename V, int G, int PER, bool TAIL, bool ONE>
-__global__ void __launch_bounds__(kThreads) loss_kernel(const Params p) {
+// ONE: one cluster has the batch in one round.  VEC: four neighbouring entries
+// a load (K a multiple of 4, tensors on 16 bytes).
+template <int G, int PER, bool VEC, bool TAIL, bool ONE>
+__global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const Params p) {
   __shared__ double exps[kExps];  // 2^(j / 128)
   __shared__ double of_warp[kWarps];
   __shared__ int live_of_warp[kWarps];
@@ -123,25 +124,50 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Params p) {
   __shared__ int live_of_cta[8];
   __shared__ int last;
   constexpr int kRows = 32 / G;   // of a warp
+  constexpr int kStep = VEC ? 4 : 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, of_row = lane % G;
-  // a row's entries, asked for one round ahead
+  // entry j of the lane
+  auto entry = [&](int j) { return VEC ? 4 * of_row + 4 * G * (j / 4) + j % 4 : of_row + G * j; };
   const int64_t t_step = static_cast<int64_t>(gridDim.x) * kWarps * kRows;
   const int64_t t_first = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * kRows;
   int64_t t0 = t_first;
-  float next_a[PER], next_b[PER];
-  int64_t next_id[PER];
+  float in_a[PER], in_b[PER];
+  int64_t in_id[PER];
   auto load = [&] {
-    const int64_t at = (t0 + lane / G) * p.K + of_row;
-    const int left = t0 + lane / G < p.T ? p.K - of_row : 0;
+    const int64_t row = (t0 + lane / G) * p.K;
+    const int cols = t0 + lane / G < p.T ? p.K : 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const bool in = G * j < left;
-      next_id[j] = in ? __ldcs(p.ids + at + G * j) : -1;
-      next_b[j] = in ? as_float(static_cast<const V*>(p.teacher) + at + G * j) : 0.f;
-      next_a[j] = in ? __ldcs(p.logp + at + G * j) : 0.f;
+    for (int j = 0; j < PER; j += kStep) {
+      const int k = entry(j);
+      if (VEC) {
+        longlong2 i0 = make_longlong2(-1, -1), i1 = i0;
+        float4 a4 = make_float4(0.f, 0.f, 0.f, 0.f), b4 = a4;
+        if (k < cols) {
+          i0 = __ldcs(reinterpret_cast<const longlong2*>(p.ids + row + k));
+          i1 = __ldcs(reinterpret_cast<const longlong2*>(p.ids + row + k) + 1);
+          a4 = __ldcs(reinterpret_cast<const float4*>(p.logp + row + k));
+          if (p.teacher_bf16) {
+            const uint2 u = __ldcs(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.teacher) + row + k));
+            b4 = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                             __uint_as_float(u.y & 0xffff0000u));
+          } else {
+            b4 = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(p.teacher) + row + k));
+          }
+        }
+        in_id[j] = i0.x, in_id[j + 1] = i0.y, in_id[j + 2] = i1.x, in_id[j + 3] = i1.y;
+        in_a[j] = a4.x, in_a[j + 1] = a4.y, in_a[j + 2] = a4.z, in_a[j + 3] = a4.w;
+        in_b[j] = b4.x, in_b[j + 1] = b4.y, in_b[j + 2] = b4.z, in_b[j + 3] = b4.w;
+      } else {
+        const bool in = k < cols;
+        in_id[j] = in ? __ldcs(p.ids + row + k) : -1;
+        in_a[j] = in ? __ldcs(p.logp + row + k) : 0.f;
+        in_b[j] = !in              ? 0.f
+                    : p.teacher_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.teacher)[row + k])
+                                     : __ldcs(static_cast<const float*>(p.teacher) + row + k);
+      }
     }
   };
-  load();
+  if (ONE) load();
   if (TAIL) {
     if (threadIdx.x < kExps) exps[threadIdx.x] = exp2(threadIdx.x / static_cast<double>(kExps));
     __syncthreads();
@@ -167,27 +193,35 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Params p) {
   double sum = 0.0;
   int rows = 0;
   float g[PER];
-  unsigned keep = 0;
-  auto store = [&](int64_t t, float scale) {
-    const int64_t at = t * p.K + of_row;
-    const int left = t < p.T ? p.K - of_row : 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (G * j < left && !T1_OOB(at + G * j, p.T * p.K)) p.dlogp[at + G * j] = keep >> j & 1 ? g[j] * scale : 0.f;
+  for (int j = 0; j < PER; ++j) g[j] = 0.f;
+  auto store = [&](int64_t t, float scale) {
+    const int64_t row = t * p.K;
+    const int cols = t < p.T ? p.K : 0;
+#pragma unroll
+    for (int j = 0; j < PER; j += kStep) {
+      const int k = entry(j);
+      if (k >= cols || T1_OOB(row + k + kStep - 1, p.T * p.K)) continue;
+      if (VEC) *reinterpret_cast<float4*>(p.dlogp + row + k) = make_float4(g[j] * scale, g[j + 1] * scale, g[j + 2] * scale, g[j + 3] * scale);
+      else p.dlogp[row + k] = g[j] * scale;
+    }
   };
+  // An entry left out has the logarithm of no probability at all, in both, and so no part in anything below.
+  constexpr float kNothing = -1e4f;
   while (t0 < p.T) {
+    if (!ONE) load();
     const int64_t t = t0 + lane / G;
     float a[PER], b[PER];
-    keep = 0;
+    bool any = false;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      a[j] = next_a[j];
-      b[j] = next_b[j];
-      if (next_id[j] >= 0 && b[j] > -INFINITY) keep |= 1u << j;
+      const bool keep = in_id[j] >= 0 && in_b[j] > -INFINITY;
+      a[j] = keep ? in_a[j] : kNothing;
+      b[j] = keep ? in_b[j] : kNothing;
+      any = any || keep;
     }
     t0 += t_step;
-    if (!ONE && t0 < p.T) load();
-    const unsigned lanes = __ballot_sync(0xffffffffu, keep != 0);
+    const unsigned lanes = __ballot_sync(0xffffffffu, any);
     const bool live = (G == 32 ? lanes : (lanes >> (lane & ~(G - 1))) & ((1u << (G & 31)) - 1)) != 0;
     float pk[PER], qk[PER];
     float loss = 0.f, rest = 0.f;  // rest: f'(p_r), without a tail sum p f'
@@ -196,58 +230,59 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Params p) {
       double ps = 0.0, qs = 0.0;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const bool in = keep >> j & 1;
         const double pd = exp64(a[j]), qd = exp64(b[j]);
-        ps += in ? pd : 0.0;
-        qs += in ? qd : 0.0;
-        pk[j] = in ? static_cast<float>(pd) : 0.f;
-        qk[j] = in ? static_cast<float>(qd) : 0.f;
+        ps += pd;
+        qs += qd;
+        pk[j] = static_cast<float>(pd);
+        qk[j] = static_cast<float>(qd);
       }
       ps = 1.0 - lanes_sum<G>(ps);
       qs = 1.0 - lanes_sum<G>(qs);
       const float pr = fmaxf(static_cast<float>(ps), kFloor), qr = fmaxf(static_cast<float>(qs), kFloor);
       float fr, gr;
-      divergence(p.kind, pr, qr, logf(qr / pr), fr, gr);
-      rest = ps > kFloor ? gr / pr : 0.f;
+      divergence(p.kind, pr, qr, logf(__fdividef(qr, pr)), fr, gr);
+      rest = ps > kFloor ? __fdividef(gr, pr) : 0.f;
       if (of_row == 0) loss = fr;
     } else {
       // scaled to sum to 1
-      float am = -INFINITY, bm = -INFINITY, as = 0.f, bs = 0.f;
+      float am = a[0], bm = b[0], as = 0.f, bs = 0.f;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        if (keep >> j & 1) am = fmaxf(am, a[j]);
-        if (keep >> j & 1) bm = fmaxf(bm, b[j]);
+      for (int j = 1; j < PER; ++j) {
+        am = fmaxf(am, a[j]);
+        bm = fmaxf(bm, b[j]);
       }
       am = lanes_max<G>(am);
       bm = lanes_max<G>(bm);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        pk[j] = keep >> j & 1 ? expf(a[j] - am) : 0.f;
-        qk[j] = keep >> j & 1 ? expf(b[j] - bm) : 0.f;
+        pk[j] = expf(a[j] - am);
+        qk[j] = expf(b[j] - bm);
         as += pk[j];
         bs += qk[j];
       }
       as = lanes_sum<G>(as);
       bs = lanes_sum<G>(bs);
       shift = (bm - am) + logf(bs / as);
+      as = live ? 1.f / as : 0.f;
+      bs = live ? 1.f / bs : 0.f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        pk[j] = keep >> j & 1 ? pk[j] / as : 0.f;
-        qk[j] = keep >> j & 1 ? qk[j] / bs : 0.f;
+        pk[j] *= as;
+        qk[j] *= bs;
       }
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       float f;
-      divergence(p.kind, pk[j], qk[j], (b[j] - a[j]) - shift, f, g[j]);
-      loss += keep >> j & 1 ? f : 0.f;
-      if (!TAIL) rest += keep >> j & 1 ? g[j] : 0.f;
+      // of a student's -inf as much as there is
+      divergence(p.kind, pk[j], qk[j], fminf((b[j] - a[j]) - shift, 3e38f), f, g[j]);
+      loss += f;
+      if (!TAIL) rest += g[j];
     }
     loss = lanes_sum<G>(loss);
     if (!TAIL) rest = lanes_sum<G>(rest);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) g[j] -= pk[j] * rest;
-    if (!live) loss = 0.f;
+    for (int j = 0; j < PER; ++j) g[j] = fmaf(-pk[j], rest, g[j]);
     if (of_row == 0) {
       if (t < p.T && !T1_OOB(t, p.T)) p.each[t] = loss;
       sum += loss;
@@ -330,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(float* dlogp, int64_t n
 // ================================================================ host side
 T1_BOUNDS_READER(distillation)
 
-template <typename V, int G, int PER>
+template <int G, int PER, bool VEC>
 static void launch_loss(distil::Params& p, bool tail) {
   const int64_t per_block = distil::kWarps * (32 / G), blocks_one = (p.T + per_block - 1) / per_block;
   if (blocks_one <= 8) {
@@ -344,7 +379,7 @@ static void launch_loss(distil::Params& p, bool tail) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    auto kern = tail ? distil::loss_kernel<V, G, PER, true, true> : distil::loss_kernel<V, G, PER, false, true>;
+    auto kern = tail ? distil::loss_kernel<G, PER, VEC, true, true> : distil::loss_kernel<G, PER, VEC, false, true>;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<const distil::Params>(p));
     TORCH_CHECK(e == cudaSuccess, "distillation_loss launch failed: ", cudaGetErrorString(e));
     count_launch();
@@ -357,7 +392,7 @@ static void launch_loss(distil::Params& p, bool tail) {
   p.scale = reinterpret_cast<float*>(p.sums + 2 * blocks);
   ArrivalCounters counters(1);
   p.ticket = counters.arrivals;
-  auto kern = tail ? distil::loss_kernel<V, G, PER, true, false> : distil::loss_kernel<V, G, PER, false, false>;
+  auto kern = tail ? distil::loss_kernel<G, PER, VEC, true, false> : distil::loss_kernel<G, PER, VEC, false, false>;
   kern<<<blocks, distil::kThreads, 0, stream()>>>(p);
   check_launch("distillation_loss");
   counters.launched();
@@ -368,14 +403,22 @@ static void launch_loss(distil::Params& p, bool tail) {
   count_launch(2);
 }
 
-template <typename V>
+template <int G, int PER>
+static void launch_loss(distil::Params& p, bool tail, bool vec) {
+  if (vec) launch_loss<G, PER, true>(p, tail);
+  else launch_loss<G, PER, false>(p, tail);
+}
+
+// Few lanes and many entries each, as far as registers go: what a row costs
+// besides its entries is shared by more of them.
 static void run_loss(distil::Params& p, bool tail) {
-  if (p.K <= 8) launch_loss<V, 8, 1>(p, tail);
-  else if (p.K <= 16) launch_loss<V, 8, 2>(p, tail);
-  else if (p.K <= 32) launch_loss<V, 8, 4>(p, tail);
-  else if (p.K <= 64) launch_loss<V, 16, 4>(p, tail);
-  else if (p.K <= 128) launch_loss<V, 32, 4>(p, tail);
-  else launch_loss<V, 32, 16>(p, tail);
+  const auto at = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+  const bool vec = p.K % 4 == 0 && (at(p.logp) | at(p.teacher) | at(p.ids) | at(p.dlogp)) % 16 == 0;
+  if (p.K <= 8) launch_loss<8, 1, false>(p, tail);
+  else if (p.K <= 32) launch_loss<8, 4>(p, tail, vec);
+  else if (p.K <= 64) launch_loss<8, 8>(p, tail, vec);
+  else if (p.K <= 128) launch_loss<16, 8>(p, tail, vec);
+  else launch_loss<32, 16>(p, tail, vec);
 }
 
 // Returns (loss [], dlogp [T, K], divergence of every row [T]), fp32.
@@ -408,8 +451,8 @@ std::vector<torch::Tensor> distillation_loss(torch::Tensor logp, torch::Tensor t
   p.loss = loss.data_ptr<float>();
   p.dlogp = dlogp.data_ptr<float>();
   p.each = each.data_ptr<float>();
-  if (te.scalar_type() == torch::kFloat32) run_loss<float>(p, tail);
-  else run_loss<__nv_bfloat16>(p, tail);
+  p.teacher_bf16 = te.scalar_type() == torch::kBFloat16;
+  run_loss(p, tail);
   return {loss, dlogp, each};
 }
 

@@ -18,6 +18,8 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from .. import ops
+
 
 def _zero_grads(module: nn.Module) -> None:
     for p in module.parameters():
@@ -109,6 +111,14 @@ def _label_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: fl
     return -nll
 
 
+def _list_logprobs(logits: torch.Tensor, ids: torch.Tensor, temperature: float) -> torch.Tensor:
+    """Log-probabilities of every row's listed tokens [T, K], 0 where an id is
+    outside the vocabulary."""
+    keep = (ids >= 0) & (ids < logits.shape[-1])
+    logp = torch.log_softmax(logits.view(ids.shape[0], -1) / temperature, dim=-1)
+    return torch.where(keep, logp.gather(1, torch.where(keep, ids, 0)), 0.0)
+
+
 class GenericOutputLayer(nn.Module):
     """Final norm + lm_head of any architecture; loss = mean token
     cross-entropy on shifted labels (ignore_index -100)."""
@@ -124,7 +134,11 @@ class GenericOutputLayer(nn.Module):
         with torch.enable_grad():
             logits = self.lm_head(self.norm(x)).float()
             if getattr(ctx, "objective", None) is not None:
-                logp = _label_logprobs(logits, ctx.targets, ctx.objective.temperature)
+                ids = ctx.objective.token_lists(ctx.targets)
+                if ids is None:
+                    logp = _label_logprobs(logits, ctx.targets, ctx.objective.temperature)
+                else:
+                    logp = _list_logprobs(logits, ids, ctx.objective.temperature)
                 loss, dlogp = ctx.objective.loss_and_grad(logp.detach(), ctx.targets, ctx.seq_len)
                 logp.backward(dlogp)
                 return loss, x.grad
@@ -139,6 +153,13 @@ class GenericOutputLayer(nn.Module):
     def logprobs(self, h: torch.Tensor, targets: torch.Tensor, temperature: float) -> torch.Tensor:
         with torch.no_grad():
             return _label_logprobs(self.logits(h).float(), targets, temperature)
+
+    def logits_fp32(self, h: torch.Tensor) -> torch.Tensor:
+        return self.logits(h).float()
+
+    def top_logprobs(self, h: torch.Tensor, k: int, temperature: float):
+        parts = [ops.topk_logprobs(self.logits_fp32(c), k, temperature) for c in h.split(2048)]
+        return tuple(torch.cat(p) for p in zip(*parts))
 
 
 def causal_masks(config, batch: int, seq_len: int, hidden: int, position_ids, device, dtype) -> dict:

@@ -13,7 +13,9 @@ gradients are their mean.  (The reference trains with cross-entropy only.)
 
 ``SlideFSDP.token_logprobs`` gives the log-probabilities that an objective
 compares with: those of a frozen reference model, and those of the policy
-that sampled the answers.
+that sampled the answers.  ``SlideFSDP.generate`` samples answers and gives the
+latter with them; ``SlideFSDP.top_logprobs`` gives a teacher's likeliest tokens
+at every position, from which ``DistillationObjective`` trains.
 """
 from __future__ import annotations
 
@@ -54,7 +56,7 @@ class PreferenceObjective:
     def check(self, inputs, batch: int) -> None:
         if batch % 2:
             raise ValueError(f"a preference batch needs an even number of sequences, got {batch}")
-        unused = [n for n in ("old_logps", "advantages") if inputs.get(n) is not None]
+        unused = [n for n in ("old_logps", "advantages", "teacher_logps", "teacher_ids") if inputs.get(n) is not None]
         if unused:
             raise ValueError(f"a preference objective does not take {', '.join(unused)}")
 
@@ -87,12 +89,51 @@ class PolicyObjective:
         missing = [n for n in needed if inputs.get(n) is None]
         if missing:
             raise ValueError(f"this policy objective needs {', '.join(missing)}")
+        unused = [n for n in ("teacher_logps", "teacher_ids") if inputs.get(n) is not None]
+        if unused:
+            raise ValueError(f"a policy objective does not take {', '.join(unused)}")
 
     def loss_and_grad(self, logp, targets, seq_len, inputs):
         loss, dlogp, stats = ops.policy_loss_fwd_bwd(
             logp, inputs["old_logps"], inputs.get("ref_logps"), inputs["advantages"], targets, seq_len,
             self.clip_low, self.clip_high, self.kl_coef, self.reduction)
         return loss, dlogp, {"stats": stats}
+
+
+@dataclass
+class DistillationObjective:
+    """Learning from a teacher's likeliest tokens.  Takes ``teacher_logps`` and
+    ``teacher_ids`` [B, S, K] as ``SlideFSDP.top_logprobs`` of the teacher gives
+    them (at this ``temperature``, of the same vocabulary); positions whose label
+    is -100 take no part, nor do entries of id -1.  The divergences and ``tail``
+    are those of ``ops.distillation_loss_fwd_bwd``.  Results: ``divergence``
+    [B, S], of every position; ``logps`` [B, S, K], of the teacher's tokens."""
+
+    kind: str = "forward"
+    tail: bool = True
+    temperature: float = 1.0
+
+    def __post_init__(self):
+        ops.check_distillation(self.kind)
+        check_temperature(self.temperature)
+
+    def check(self, inputs, batch: int) -> None:
+        missing = [n for n in ("teacher_logps", "teacher_ids") if inputs.get(n) is None]
+        if missing:
+            raise ValueError(f"a distillation objective needs {', '.join(missing)}")
+        unused = [n for n in ("ref_logps", "old_logps", "advantages") if inputs.get(n) is not None]
+        if unused:
+            raise ValueError(f"a distillation objective does not take {', '.join(unused)}")
+
+    def token_lists(self, targets, inputs):
+        """[T, K] tokens whose log-probabilities the loss is a function of."""
+        ids = inputs["teacher_ids"]
+        return torch.where((targets != -100)[:, None], ids, -1)
+
+    def loss_and_grad(self, logp, targets, seq_len, inputs):
+        loss, dlogp, each = ops.distillation_loss_fwd_bwd(logp, inputs["teacher_logps"], self.token_lists(targets, inputs),
+                                                          self.kind, self.tail)
+        return loss, dlogp, {"divergence": each.view(-1, seq_len)}
 
 
 @dataclass
@@ -109,9 +150,20 @@ class ObjectiveStep:
         tensors.  Per-token inputs are [batch, seq_len] as ``token_logprobs``
         returns them: entry [b, s] belongs to labels[b, s + 1]."""
         flat = {}
+        lists = [t.shape for n, t in inputs.items() if n.startswith("teacher_") and t is not None]
         for name, t in inputs.items():
             if t is None:
                 flat[name] = None
+                continue
+            if name.startswith("teacher_"):
+                if t.dim() != 3 or t.shape != lists[0] or t.shape[:2] != (batch, seq_len):
+                    raise ValueError(f"{name} must be [{batch}, {seq_len}, K], got {tuple(t.shape)}")
+                if not 1 <= t.shape[2] <= ops.MAX_LIST:
+                    raise ValueError(f"{name} must have 1 to {ops.MAX_LIST} entries a position, got {t.shape[2]}")
+                if name == "teacher_ids" and t.is_floating_point():
+                    raise ValueError(f"teacher_ids must be whole numbers, got {t.dtype}")
+                kept = torch.int64 if name == "teacher_ids" else t.dtype if t.dtype == torch.bfloat16 else torch.float32
+                flat[name] = t.to(device=device, dtype=kept, non_blocking=True).reshape(-1, t.shape[2])
                 continue
             if tuple(t.shape) != (batch, seq_len) and not (name == "advantages" and tuple(t.shape) == (batch,)):
                 raise ValueError(f"{name} must be [{batch}, {seq_len}], got {tuple(t.shape)}")
@@ -119,9 +171,15 @@ class ObjectiveStep:
         objective.check(flat, batch)  # before anything of the step has started
         return cls(objective, flat)
 
+    def token_lists(self, targets: torch.Tensor) -> Optional[torch.Tensor]:
+        """[T, K] tokens whose log-probabilities the objective takes; None: the
+        targets alone."""
+        lists = getattr(self.objective, "token_lists", None)
+        return None if lists is None else lists(targets, self.inputs)
+
     def loss_and_grad(self, logp: torch.Tensor, targets: torch.Tensor, seq_len: int):
         loss, dlogp, results = self.objective.loss_and_grad(logp, targets, seq_len, self.inputs)
-        self.results = dict(results, logps=logp.view(-1, seq_len))
+        self.results = dict(results, logps=logp.view(-1, seq_len, *logp.shape[1:]))
         return loss, dlogp
 
     @property

@@ -74,6 +74,18 @@ except Exception:  # pragma: no cover
         logits: Optional[torch.Tensor] = None
 
 
+@dataclass
+class GeneratedAnswers:
+    """What ``SlideFSDP.generate`` gives, all on the engine's device.  With
+    ``labels`` as a policy step's labels, ``logps`` are its ``old_logps`` (if its
+    temperature is the one that was sampled with)."""
+
+    input_ids: torch.Tensor  # [B, S + max_new_tokens]: prompts, answers, 0 behind them
+    labels: torch.Tensor     # the answers' tokens, -100 elsewhere
+    logps: torch.Tensor      # fp32, entry [b, s] is that of labels[b, s + 1]
+    lengths: torch.Tensor    # [B] tokens of prompt and answer
+
+
 class OutputLayer(nn.Module):
     """Final norm + lm_head moved as one unit (reference slide_fsdp.py:45-113).
     ``named_parameters``: norm.weight, lm_head.weight.
@@ -107,10 +119,16 @@ class OutputLayer(nn.Module):
         g_n, g_lm = self._grads()
         if getattr(ctx, "objective", None) is not None:
             tau = ctx.objective.temperature
-            logp, lse = ops.linear_logprob_fwd(x, w_lm, ctx.targets, temperature=tau)
-            loss, dlogp = ctx.objective.loss_and_grad(logp, ctx.targets, ctx.seq_len)
+            ids = ctx.objective.token_lists(ctx.targets)
             dx = torch.empty_like(x)
-            ops.linear_logprob_bwd(dlogp, x, w_lm, ctx.targets, lse, dx, g_lm, temperature=tau)
+            if ids is None:
+                logp, lse = ops.linear_logprob_fwd(x, w_lm, ctx.targets, temperature=tau)
+                loss, dlogp = ctx.objective.loss_and_grad(logp, ctx.targets, ctx.seq_len)
+                ops.linear_logprob_bwd(dlogp, x, w_lm, ctx.targets, lse, dx, g_lm, temperature=tau)
+            else:
+                logp, lse = ops.linear_topk_logprob_fwd(x, w_lm, ids, temperature=tau)
+                loss, dlogp = ctx.objective.loss_and_grad(logp, ctx.targets, ctx.seq_len)
+                ops.linear_topk_logprob_bwd(dlogp, x, w_lm, ids, lse, dx, g_lm, temperature=tau)
         elif self.chunk_tokens > 0:
             dx = torch.empty_like(x)
             loss, _ = ops.linear_cross_entropy(x, w_lm, ctx.targets, dx, g_lm, self.chunk_tokens)
@@ -132,6 +150,16 @@ class OutputLayer(nn.Module):
     def logprobs(self, h: torch.Tensor, targets: torch.Tensor, temperature: float) -> torch.Tensor:
         x, _ = ops.rmsnorm_fwd(h, self.norm.weight.data, self.eps)
         return ops.linear_logprob_fwd(x, self.lm_head.weight.data, targets, temperature=temperature)[0]
+
+    def logits_fp32(self, h: torch.Tensor) -> torch.Tensor:
+        x, _ = ops.rmsnorm_fwd(h, self.norm.weight.data, self.eps)
+        return ops.linear_logits(x, self.lm_head.weight.data)
+
+    def top_logprobs(self, h: torch.Tensor, k: int, temperature: float):
+        """Log-probabilities and ids [T, k] of every row's likeliest tokens;
+        logits of ``chunk_tokens`` rows at a time."""
+        parts = [ops.topk_logprobs(self.logits_fp32(c), k, temperature) for c in h.split(self.chunk_tokens or 2048)]
+        return tuple(torch.cat(p) for p in zip(*parts))
 
 
 def _convert_hf_llama(model: nn.Module) -> LlamaForCausalLM:
@@ -833,16 +861,20 @@ class SlideFSDP(nn.Module):
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 labels: Optional[torch.Tensor] = None, *, objective=None,
                 ref_logps: Optional[torch.Tensor] = None, old_logps: Optional[torch.Tensor] = None,
-                advantages: Optional[torch.Tensor] = None, **kwargs) -> CausalLMOutputWithPast:
+                advantages: Optional[torch.Tensor] = None, teacher_logps: Optional[torch.Tensor] = None,
+                teacher_ids: Optional[torch.Tensor] = None, **kwargs) -> CausalLMOutputWithPast:
         """One training step with labels, logits without.  ``objective``
-        (``objectives.PreferenceObjective``, ``objectives.PolicyObjective``)
-        replaces the cross-entropy loss; the tensors after it are what it
-        takes, and ``last_objective`` holds its results."""
+        (``objectives.PreferenceObjective``, ``objectives.PolicyObjective``,
+        ``objectives.DistillationObjective``) replaces the cross-entropy loss;
+        the tensors after it are what it takes, and ``last_objective`` holds its
+        results."""
         if attention_mask is not None:
             self._check_mask(attention_mask)
         self._check_ids(input_ids, labels)
-        if objective is None and any(t is not None for t in (ref_logps, old_logps, advantages)):
-            raise ValueError("ref_logps, old_logps and advantages go with an objective")
+        inputs = dict(ref_logps=ref_logps, old_logps=old_logps, advantages=advantages, teacher_logps=teacher_logps,
+                      teacher_ids=teacher_ids)
+        if objective is None and any(t is not None for t in inputs.values()):
+            raise ValueError("ref_logps, old_logps, advantages, teacher_logps and teacher_ids go with an objective")
         if labels is None:
             if objective is not None:
                 raise ValueError("an objective needs labels")
@@ -850,8 +882,9 @@ class SlideFSDP(nn.Module):
         step = None
         if objective is not None:
             self._check_label_shape(input_ids, labels)
-            step = ObjectiveStep.build(objective, *input_ids.shape, self.device, ref_logps=ref_logps,
-                                       old_logps=old_logps, advantages=advantages)
+            if teacher_ids is not None:
+                self._check_teacher_ids(teacher_ids)
+            step = ObjectiveStep.build(objective, *input_ids.shape, self.device, **inputs)
         loss = self._train_step(input_ids, labels, step)
         return CausalLMOutputWithPast(loss=loss, logits=None)
 
@@ -866,6 +899,86 @@ class SlideFSDP(nn.Module):
         self._check_label_shape(input_ids, labels)
         check_temperature(temperature)
         return self._inference(input_ids, labels, temperature)
+
+    @torch.no_grad()
+    def top_logprobs(self, input_ids: torch.Tensor, k: int, temperature: float = 1.0):
+        """The k likeliest next tokens at every position under the present
+        weights, forward only: (log-probabilities [B, S, k] fp32, ids [B, S, k]
+        int64), likeliest first (``ops.topk_logprobs``).  Those of a teacher are
+        a ``DistillationObjective``'s ``teacher_logps`` and ``teacher_ids``."""
+        self._check_ids(input_ids, None)
+        check_temperature(temperature)
+        most = min(ops.MAX_LIST, self.model_config.vocab_size)
+        if input_ids.dim() != 2 or not input_ids.numel():
+            raise ValueError(f"input_ids must be [B, S], got {tuple(input_ids.shape)}")
+        if not 1 <= k <= most:
+            raise ValueError(f"k must lie in [1, {most}], got {k}")
+        logp, ids = self._forward_only(input_ids, None, lambda layer, h, ctx: layer.top_logprobs(h, k, temperature))
+        return logp.view(*input_ids.shape, k), ids.view(*input_ids.shape, k)
+
+    @torch.no_grad()
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, lengths: Optional[torch.Tensor] = None, *,
+                 temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 eos_token_id: Optional[int] = None, generator: Optional[torch.Generator] = None) -> GeneratedAnswers:
+        """Samples an answer to every prompt: ``input_ids`` [B, S], right-padded,
+        with ``lengths`` [B] tokens each (default: all of them).  Every token is
+        drawn by ``ops.sample_tokens`` with numbers of ``generator``; an answer
+        ends with ``eos_token_id`` or after ``max_new_tokens``.
+
+        A token is one forward pass over prompts and answers so far, without a
+        cache of keys and values: the pass streams every layer's weights from
+        host memory, which for the Llama-3.1-8B architecture takes as long as
+        the arithmetic of about 25 thousand tokens.  On several ranks every rank
+        generates its own batch, in as many passes as the longest."""
+        self._check_ids(input_ids, None)
+        ops.check_sampling(temperature, top_k, top_p, min_p)
+        if input_ids.dim() != 2 or not input_ids.numel():
+            raise ValueError(f"input_ids must be [B, S], got {tuple(input_ids.shape)}")
+        if max_new_tokens < 1:
+            raise ValueError(f"max_new_tokens must be positive, got {max_new_tokens}")
+        B, S = input_ids.shape
+        dev = self.device
+        lengths = torch.full((B,), S) if lengths is None else lengths.to("cpu", torch.int64)
+        if lengths.shape != (B,) or int(lengths.min()) < 1 or int(lengths.max()) > S:
+            raise ValueError(f"lengths must be [{B}] of 1 to {S} tokens")
+        longest, length = int(lengths.max()), lengths.to(dev)
+        # the attention kernels take whole tiles; what lies behind a sequence's last token does not reach it
+        tile = 256 if self.is_cuda else 1
+        total = S + max_new_tokens
+        width = -(-total // tile) * tile
+        ids = torch.zeros(B, width, dtype=torch.int64, device=dev)
+        ids[:, :S] = torch.where(torch.arange(S, device=dev) < length[:, None], input_ids.to(dev), 0)
+        labels = torch.full_like(ids, -100)
+        logps = torch.zeros(B, width, dtype=torch.float32, device=dev)
+        done = torch.zeros(B, dtype=torch.bool, device=dev)
+        for step in range(max_new_tokens):
+            run = min(width, -(-(longest + step) // tile) * tile)
+            last = torch.arange(B, device=dev) * run + length - 1
+            logits = self._forward_only(ids[:, :run].contiguous(), None,
+                                        lambda layer, h, ctx: layer.logits_fp32(h.index_select(0, last)))
+            source = dev if generator is None else generator.device
+            u = torch.rand(B, generator=generator, device=source, dtype=torch.float32).to(dev, non_blocking=True)
+            token, logp = ops.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+            done = done | (token < 0)  # no finite logit
+            at, new = length[:, None], ~done[:, None]
+            ids.scatter_(1, at, torch.where(new, token[:, None], ids.gather(1, at)))
+            labels.scatter_(1, at, torch.where(new, token[:, None], labels.gather(1, at)))
+            logps.scatter_(1, at - 1, torch.where(new, logp[:, None], logps.gather(1, at - 1)))
+            length = length + (~done)
+            if eos_token_id is not None:
+                done = done | (token == eos_token_id)
+                ended = done.all().to(torch.int32)
+                if self.world_size > 1:
+                    dist.all_reduce(ended, op=dist.ReduceOp.MIN)
+                if bool(ended):
+                    break
+        return GeneratedAnswers(ids[:, :total], labels[:, :total], logps[:, :total], length)
+
+    def _check_teacher_ids(self, ids: torch.Tensor) -> None:
+        """As ``_check_ids``, for those in host memory."""
+        V = self.model_config.vocab_size
+        if ids.device.type == "cpu" and ids.numel() and int(ids.max()) >= V:
+            raise ValueError(f"teacher_ids must lie below the vocabulary's {V}, got {int(ids.max())}")
 
     @staticmethod
     def _check_label_shape(input_ids: torch.Tensor, labels: torch.Tensor) -> None:
@@ -1097,6 +1210,15 @@ class SlideFSDP(nn.Module):
                    temperature: float = 1.0) -> torch.Tensor:
         """Forward only; returns logits [B, S, V], or with labels their
         log-probabilities [B, S]."""
+        B, T = input_ids.shape
+        if labels is None:
+            return self._forward_only(input_ids, None, lambda layer, h, ctx: layer.logits(h)).view(B, T, -1)
+        return self._forward_only(input_ids, labels,
+                                  lambda layer, h, ctx: layer.logprobs(h, ctx.targets, temperature)).view(B, T)
+
+    def _forward_only(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor], head):
+        """All layers' forward pass; ``head(output_layer, h, ctx)`` makes the
+        result of the last decoder layer's h [B S, H]."""
         self._check_kernels()
         ctx = self._make_context(input_ids, labels)
         S = self.layer_states
@@ -1111,16 +1233,10 @@ class SlideFSDP(nn.Module):
             if i + 1 < L + 2 and S[i + 1].pool.num_free:
                 self._fetch(S[i + 1], with_grad=False)
             self._wait_loaded(st)
-            if i <= L:
-                h = st.module(h, ctx)
-            elif labels is None:
-                h = st.module.logits(h)
-            else:
-                h = st.module.logprobs(h, ctx.targets, temperature)
+            h = st.module(h, ctx) if i <= L else head(st.module, h, ctx)
             self._release(st, Event(self.device).record())
         self._read_kernel_errors()
-        B, T = input_ids.shape
-        return h.view(B, T, -1) if labels is None else h.view(B, T)
+        return h
 
     # ------------------------------------------------------------ control
     def wait_for_updates(self) -> None:
