@@ -18,8 +18,10 @@
 //          distances from m finds.  What lies above (little more than n) goes to
 //          the first CTA, which sorts it and does all the rest.
 //   bins   top_p alone: weights added up by distance from m, 8 bins per factor
-//          of two, the bin where top_p is reached once more in 256 parts, and
-//          the tokens of that part sorted by the first CTA.
+//          of two.  The tokens of the bin where top_p is reached go to the first
+//          CTA, which finds the last one kept (by 256 parts of the bin, then by
+//          order) and, since it has every CTA's weight above the bin too, the
+//          CTA that the draw falls into.  The others are done.
 //   digits where neither applies (more tokens are asked for, or too many are
 //          equal): the threshold is found digit by digit, 8 bits at a time, of
 //          the order-preserving integer of a logit.
@@ -45,8 +47,10 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostCtas = 8;      // of a cluster
 constexpr int kMostList = 512;    // tokens of `top`
-constexpr int kListSlots = 1024;  // tokens that the first CTA sorts
+constexpr int kListSlots = 2048;  // tokens that the first CTA takes from all
+constexpr int kSortSlots = 1024;  // of bins: tokens of the last part
 constexpr int kRankSlots = 128;   // up to so many by counting
+constexpr int kMostColumns = 96;  // of a thread: what fits in shared memory next to the rest
 constexpr int kDigits = 256;
 constexpr int kBins = 256;
 constexpr int kExps = 128;        // steps of an octave in the table of exponentials
@@ -142,7 +146,8 @@ __device__ __forceinline__ unsigned long long warp_scan64(unsigned long long v, 
 struct Shared {
   double exps[kExps];              // 2^(j / 128)
   unsigned long long red[kWarps];
-  unsigned bins[2][3][kBins];      // counts; of weights 16 bits each
+  unsigned bins[2][3][kBins];      // counts; of weights 16 bits each; the second of a bin's parts
+  unsigned long long border[kWarps][kMostCtas];
   union {
     struct {
       unsigned hist[2][kDigits];
@@ -155,11 +160,14 @@ struct Shared {
   float max_of[kMostCtas];
   float sum_of[kMostCtas];
   unsigned count_of[kMostCtas], ties_of[kMostCtas];
-  unsigned long long total_of[kMostCtas], kept_of[kMostCtas], cut_of[kMostCtas];
+  unsigned long long total_of[kMostCtas], kept_of[kMostCtas], cut_of[kMostCtas], above_of[kMostCtas];
+  // what the first CTA finds
+  unsigned long long found_cut, found_before, found_total;
+  int found_cta;
   // where a threshold falls
   unsigned digit, before32;
   int bin;
-  unsigned long long before64, here64;
+  unsigned long long before64;
   unsigned listed;
 };
 
@@ -337,15 +345,17 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     }
     return block_sum((s4[0] + s4[1]) + (s4[2] + s4[3]), red);
   };
-  // The bin in which `need` is reached (-1: in none) of all CTAs' bins, and in sh.before64 what comes before.
-  auto reach = [&](unsigned (*bins)[kBins], bool weights, unsigned long long need) {
+  // A bin of weights.
+  auto bin_sum = [](const unsigned* bins, int b) {
+    return bins[b] + (static_cast<unsigned long long>(bins[kBins + b]) << 16) + (static_cast<unsigned long long>(bins[2 * kBins + b]) << 32);
+  };
+  // The bin in which `need` is reached (-1: in none) of the first `of` CTAs' bins, and in sh.before64 what comes before.
+  auto reach = [&](unsigned (*bins)[kBins], bool weights, unsigned long long need, int of) {
     unsigned long long here = 0, before;
     if (tid < kBins) {
-      for (int r = 0; r < ctas; ++r) {
+      for (int r = 0; r < of; ++r) {
         const unsigned* b = cluster.map_shared_rank(&bins[0][0], r);
-        here += b[tid];
-        if (weights)
-          here += (static_cast<unsigned long long>(b[kBins + tid]) << 16) + (static_cast<unsigned long long>(b[2 * kBins + tid]) << 32);
+        here += weights ? bin_sum(b, tid) : b[tid];
       }
     }
     if (tid == 0) sh.bin = -1;
@@ -353,7 +363,6 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     if (before < need && before + here >= need) {
       sh.bin = tid;
       sh.before64 = before;
-      sh.here64 = here;
     }
     __syncthreads();
     return sh.bin;
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
   unsigned long long before_cta = 0;
   bool alone = false;                     // the other CTAs have left
   bool done = false;                      // the cut is found
-  unsigned long long cut_place = 0;       // with done: the last token kept
+  // with done: the last token kept
   float cut_logit = -INFINITY;
   int cut_column = 0;
 
@@ -431,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     if (by_list) {
       if (is_token(own_max)) atomicAdd(&sh.bins[0][0][step_of(m, own_max)], 1u);
       sync_all(cluster);
-      const int bin = reach(sh.bins[0], false, first);
+      const int bin = reach(sh.bins[0], false, first, ctas);
       if (bin >= 0 && bin < kBins - 1) bound = least_of(m, bin);
     }
     tell_all(cluster, sh.sum_of, sum_and_push(m, bound));
@@ -499,88 +508,122 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Params p) {
     log_sum = static_cast<float>(log(ldexp(static_cast<double>(total), -p.one)));
     if (by_bins) {
       unsigned long long need = max(1ull, static_cast<unsigned long long>(p.top_p * static_cast<double>(total)));
-      const int bin = reach(sh.bins[0], true, need);
+      const int bin = reach(sh.bins[0], true, need, ctas);
       if (bin >= 0) {
         need -= sh.before64;
-        // no more tokens than this have the bin's weight
-        const bool few = sh.here64 / max(1ull, weight_at(-16.0 * (bin + 1))) < kListSlots;
         // the bin's logits lie between these
         const float least = __double2float_rd(m64 - 16.0 * (bin + 1) / p.steps), most = __double2float_ru(m64 - (16.0 * bin - 1) / p.steps);
-        int part = 0;
-        if (!few) {
+        // the CTA's weight above the bin, and its tokens in the bin
+        const unsigned long long above = block_scan64(tid < bin ? bin_sum(sh.bins[0][0], tid) : 0ull, before, sh.red);
+        if (tid == 0) cluster.map_shared_rank(sh.above_of, 0)[rank] = above;
+        unsigned in_bin[kMostColumns / 32], mine = 0;
+#pragma unroll
+        for (int b = 0; b < kMostColumns / 32; ++b) {
+          in_bin[b] = 0;
 #pragma unroll 8
-          for (int i = 0; i < n; ++i) {
+          for (int i = 32 * b; i < min(n, 32 * b + 32); ++i) {
             const float z = v[32 * i];
-            if (!(z >= least && z <= most)) continue;
-            const double x = steps_of(z);
-            if (bin_at(x) == bin) add_to(sh.bins[1], part_at(x, bin), weight_at(x));
+            if (z >= least && z <= most && bin_at(steps_of(z)) == bin) in_bin[b] |= 1u << (i - 32 * b);
           }
-          sync_all(cluster);
-          part = reach(sh.bins[1], true, need);
-          need -= sh.before64;
+          mine += __popc(in_bin[b]);
         }
-        auto at_border = [&](float z) {
-          if (!(z >= least && z <= most)) return false;
-          const double x = steps_of(z);
-          return bin_at(x) == bin && (few || part_at(x, bin) == part);
-        };
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-          const float z = v[32 * i];
-          if (is_token(z) && at_border(z)) push(z, col0 + 32 * i);
+        const unsigned of_cta = static_cast<unsigned>(block_scan64(mine, before, sh.red));
+        if (tid == 0) sh.digit = of_cta == 0 ? 0 : atomicAdd(list_length, of_cta);
+        __syncthreads();
+        unsigned at = sh.digit + static_cast<unsigned>(before);
+#pragma unroll
+        for (int b = 0; b < kMostColumns / 32; ++b) {
+          for (; in_bin[b] != 0; in_bin[b] &= in_bin[b] - 1, ++at) {
+            const int i = 32 * b + __ffs(in_bin[b]) - 1;
+            if (at < kListSlots) first_list[at] = place_of(v[32 * i] + 0.f, col0 + 32 * i);  // -0 is 0
+          }
         }
         sync_all(cluster);
-        const unsigned listed = *list_length;
-        done = listed <= kListSlots;
+        if (rank == 0) {
+          // -2: not found here, -1: the CTAs go on together
+          int found = -2;
+          const unsigned listed = sh.listed;
+          constexpr int kPer = kListSlots / kThreads;
+          unsigned long long e[kPer], w[kPer];
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            const unsigned i = j * kThreads + tid;
+            e[j] = listed <= kListSlots && i < listed ? sh.list[i] : 0ull;
+            w[j] = e[j] != 0 ? weight(logit_at(e[j])) : 0ull;
+            if (e[j] != 0) add_to(sh.bins[1], part_at(steps_of(logit_at(e[j])), bin), w[j]);
+          }
+          __syncthreads();
+          const int part = listed <= kListSlots ? reach(sh.bins[1], true, need, 1) : -1;
+          if (part >= 0) {
+            // the last token before which less than top_p has come is one of this part
+            need -= sh.before64;
+            if (tid == 0) sh.listed = 0;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              if (e[j] != 0 && part_at(steps_of(logit_at(e[j])), bin) == part) push(logit_at(e[j]), column_at(e[j]));
+            __syncthreads();
+            const unsigned few = sh.listed;
+            if (few <= kSortSlots) {
+              order_list(sh.list, few);
+              unsigned long long f[2], wf[2];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                f[j] = 2 * tid + j < static_cast<int>(few) ? sh.list[2 * tid + j] : 0ull;
+                wf[j] = f[j] != 0 ? weight(logit_at(f[j])) : 0ull;
+              }
+              block_scan64(wf[0] + wf[1], before, sh.red);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                if (f[j] != 0 && before < need && before + wf[j] >= need) sh.found_cut = f[j];
+                before += wf[j];
+              }
+              __syncthreads();
+              const unsigned long long cut = sh.found_cut;
+              found = -1;
+              if (steps_of(logit_at(cut)) >= p.log_min_p) {
+                // min_p takes no more away: the CTAs' kept weights, and whose the draw is
+                for (int r = 0; r < ctas; ++r) {
+                  unsigned long long kept = 0;
+#pragma unroll
+                  for (int j = 0; j < kPer; ++j)
+                    if (e[j] >= cut && column_at(e[j]) / (kThreads * n) == r) kept += w[j];
+                  kept = warp_sum64(kept);
+                  if (lane == 0) sh.border[warp][r] = kept;
+                }
+                __syncthreads();
+                if (tid < ctas) {
+                  unsigned long long kept = sh.above_of[tid];
+                  for (int w = 0; w < kWarps; ++w) kept += sh.border[w][tid];
+                  sh.kept_of[tid] = kept;
+                }
+                __syncthreads();
+                unsigned long long all = 0, upto = 0;
+                for (int r = 0; r < ctas; ++r) all += sh.kept_of[r];
+                const unsigned long long target = target_of(p.u[row], all);
+                for (found = 0; target >= upto + sh.kept_of[found]; ++found) upto += sh.kept_of[found];
+                if (tid < ctas) {
+                  Shared* to = cluster.map_shared_rank(&sh, tid);
+                  to->found_before = upto;
+                  to->found_total = all;
+                }
+              }
+              if (tid < ctas) cluster.map_shared_rank(&sh, tid)->found_cut = cut;
+            }
+          }
+          if (tid < ctas) cluster.map_shared_rank(&sh, tid)->found_cta = found;
+        }
+        sync_all(cluster);
+        if (sh.found_cta >= 0 && sh.found_cta != rank) return;
+        alone = sh.found_cta >= 0;
+        done = sh.found_cta >= -1;
         if (done) {
-          if (rank == 0) {
-            // the last token before which less than top_p has come
-            order_list(sh.list, listed);
-            unsigned long long e[2], w[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              e[j] = 2 * tid + j < static_cast<int>(listed) ? sh.list[2 * tid + j] : 0ull;
-              w[j] = e[j] != 0 ? weight(logit_at(e[j])) : 0ull;
-            }
-            block_scan64(w[0] + w[1], before, sh.red);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if (e[j] != 0 && before < need && before + w[j] >= need)
-                for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(sh.cut_of, r)[0] = e[j];
-              before += w[j];
-            }
-          }
-          sync_all(cluster);
-          cut_place = sh.cut_of[0];
-          cut_logit = logit_at(cut_place);
-          cut_column = column_at(cut_place);
-          if (steps_of(cut_logit) >= p.log_min_p) {
-            // min_p takes no more away: the CTA's kept weight from its bins and the border's tokens
-            own = 0;
-            if (tid < kBins) {
-              auto of = [&](unsigned (*bins)[kBins]) {
-                return bins[0][tid] + (static_cast<unsigned long long>(bins[1][tid]) << 16) + (static_cast<unsigned long long>(bins[2][tid]) << 32);
-              };
-              if (tid < bin) own = of(sh.bins[0]);
-              if (!few && tid < part) own += of(sh.bins[1]);
-            }
-#pragma unroll 8
-            for (int i = 0; i < n; ++i) {
-              const float z = v[32 * i];
-              if ((z > cut_logit || (z == cut_logit && col0 + 32 * i <= cut_column)) && at_border(z)) own += weight(z);
-            }
-            tell_all(cluster, sh.kept_of, block_scan64(own, before, sh.red));
-            unsigned long long kept = 0, mine = 0;
-            for (int r = 0; r < ctas; ++r) {
-              if (r == rank) mine = kept;
-              kept += sh.kept_of[r];
-            }
-            const unsigned long long target = target_of(p.u[row], kept);
-            if (target < mine || target >= mine + sh.kept_of[rank]) return;
-            alone = true;  // the token drawn is this CTA's
-            before_cta = mine;
-            total = kept;
-          }
+          cut_logit = logit_at(sh.found_cut);
+          cut_column = column_at(sh.found_cut);
+        }
+        if (alone) {
+          before_cta = sh.found_before;
+          total = sh.found_total;
         }
       }
     }
@@ -823,9 +866,7 @@ static void check_rows(const torch::Tensor& logits, double temperature) {
   TORCH_CHECK(std::isfinite(temperature) && temperature > 0, "temperature must be positive");
 }
 
-// Columns of a thread that fit in shared memory next to the rest.
-constexpr int kMostColumns = 96;
-constexpr int64_t kMostVocab = 8ll * kMostColumns * rows::kThreads;
+constexpr int64_t kMostVocab = static_cast<int64_t>(rows::kMostCtas) * rows::kMostColumns * rows::kThreads;
 
 template <typename T, bool TOP>
 static void launch_rows(rows::Params& p) {
@@ -836,7 +877,7 @@ static void launch_rows(rows::Params& p) {
   auto kern = rows::rows_kernel<T, TOP>;
   static DeviceFlags configured;
   if (bool& done = configured.here(); !done) {
-    T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostColumns * rows::kThreads));
+    T1_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * rows::kMostColumns * rows::kThreads));
     done = true;
   }
   cudaLaunchConfig_t cfg{};
