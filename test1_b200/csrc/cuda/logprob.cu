@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(kPackThreads) logprob_pack_kernel(const PackPa
   __shared__ int counts[kPackThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kWarps = kPackThreads / 32;
-  vocab::launch_dependents();
-  vocab::wait_previous();
+  launch_dependents();
+  wait_previous();
   const int t0 = blockIdx.x * p.per_block, t1 = min(p.T, t0 + p.per_block);
   const bool first_slice = blockIdx.y == 0;
   auto takes_part = [&](int t) {
@@ -194,8 +194,8 @@ template <bool LISTS>
 __global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const VocabParams p, int blocks) {
   __shared__ float sm[kJoinWarps][32], ss[kJoinWarps][32];
   __shared__ float top[32], log_s[32];
-  vocab::launch_dependents();
-  vocab::wait_previous();
+  launch_dependents();
+  wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
   const int rows = p.meta != nullptr ? p.meta->rows : p.rows;
@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) logprob_join_kernel(const Voc
 constexpr int kPlanesThreads = 512;
 __global__ void __launch_bounds__(kPlanesThreads) logprob_planes_kernel(const VocabParams p) {
   __shared__ __align__(16) uint8_t slab[32 * 128];
-  vocab::launch_dependents();
-  vocab::wait_previous();
+  launch_dependents();
+  wait_previous();
   const vocab::Shape e = vocab::shape_of(p, true);
   if (e.splits == 1) return;  // written by the product
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -389,8 +389,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
-  vocab::launch_dependents();
-  vocab::wait_previous();
+  launch_dependents();
+  wait_previous();
   if (JOB == kFewLse) clear_arrivals(p.ticket);
 
   const int teams = kFewWarps / p.share, team = warp / p.share, part = warp % p.share;
@@ -606,8 +606,8 @@ __host__ __device__ inline int list_pitch(int slots) { return slots + 1; }
 template <bool BWD>
 __global__ void __launch_bounds__(32 * kListRows) list_kernel(const ListParams p) {
   extern __shared__ unsigned long long sorted[];
-  vocab::launch_dependents();
-  vocab::wait_previous();
+  launch_dependents();
+  wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = blockIdx.x * kListRows + warp;
   unsigned long long* mine = sorted + warp * list_pitch(p.slots);
@@ -684,25 +684,6 @@ T1_BOUNDS_READER(logprob)
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
-
-// A launch whose prologue may overlap the end of the stream's previous
-// kernel (every kernel here waits for it before it touches memory).
-template <class... P, class... A>
-static void launch_after(const char* what, void (*kern)(P...), dim3 grid, int threads, size_t smem, const A&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream();
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
-  TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e));
-  count_launch();
-}
 
 // `units`: the most units of work that the launch can have.
 template <int JOB, bool LISTS = false>

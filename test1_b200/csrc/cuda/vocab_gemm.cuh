@@ -36,6 +36,7 @@
 
 #include "arrivals.cuh"
 #include "gemm_core.cuh"
+#include "programmatic.cuh"
 
 #include <climits>
 
@@ -115,11 +116,6 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-
-// Programmatic launch: the next kernel of the stream may start its prologue,
-// and this one touches nothing of the previous kernel's before it has ended.
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // The tensor cores drop what falls below the accumulator's last bit at every
 // step, which adds up: over 4096 products the logits lose 2e-6 of their size.
