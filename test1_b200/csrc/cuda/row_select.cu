@@ -13,12 +13,16 @@
 // A scan of the whole row by many CTAs, then what is left of it by one (finish),
 // which starts in the scan's tail.  Two kinds of scan:
 //   scan_list  top, and top_k of at most 1024.  No r tokens of a stretch can all
-//              lie below the r-th largest of the 1024 largest logits of its parts,
-//              which a histogram of their distances from the stretch's own
-//              largest finds: what lies above, little more than r, is listed.
-//              The stretches know nothing of each other: as one cluster per
-//              row that agreed on m and on the bound, the same work waited in
-//              barriers most of the time (1024 rows of 128256, k = 64: 264 us).
+//              lie below the r-th largest of the largest logits of its 256 or
+//              1024 parts, which a histogram of their distances from the
+//              stretch's own largest finds: what lies above, little more than r,
+//              is listed.  r is a stretch's share of what is asked for and some
+//              more; finish looks once more at those that have held back a
+//              token that matters.  The stretches know nothing of each other: as
+//              one cluster per row that agreed on m and on the bound, the same
+//              work waited in barriers most of the time (1024 rows of 128256,
+//              k = 64: 264 us), and with r = k its CTAs spent theirs on listing
+//              (172 us).
 //   scan_bins  all other draws.  A cluster of CTAs holds the row in shared
 //              memory and agrees on m; weights are added up, with top_p by
 //              distance from m as well, 8 bins per factor of two, and the tokens
@@ -282,7 +286,6 @@ static_assert(kBinThreads * kMostColumns <= 65536 && kListSlots <= 65536, "add_t
 // the tokens that may be among the row's first ones.
 struct ListShared {
   unsigned bins[kBins];
-  u64 red[kWarps];
   float fred[32];
   int bin;
   unsigned listed;
@@ -322,15 +325,35 @@ __device__ __forceinline__ void scan_stretch(const Params& p, int row, int segme
     }
     return;
   }
+  // few tokens need few parts
+  if (p.rank <= kThreads / 4) {
+    const float own = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    if (is_token(own)) atomicAdd(&sh.bins[step_of(m, own)], 1u);
+  } else {
 #pragma unroll
-  for (int j = 0; j < kParts; ++j)
-    if (is_token(part[j])) atomicAdd(&sh.bins[step_of(m, part[j])], 1u);
-  if (tid == 0) sh.bin = -1;
-  u64 before;
+    for (int j = 0; j < kParts; ++j)
+      if (is_token(part[j])) atomicAdd(&sh.bins[step_of(m, part[j])], 1u);
+  }
   __syncthreads();
-  const unsigned here = sh.bins[tid];
-  block_scan64<kWarps>(here, before, sh.red);
-  if (before < p.rank && before + here >= p.rank) sh.bin = tid;
+  if (warp == 0) {
+    int h[kBins / 32], own = 0, upto = 0, bin = -1;
+#pragma unroll
+    for (int j = 0; j < kBins / 32; ++j) own += h[j] = sh.bins[kBins / 32 * lane + j];
+    upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    upto -= own;
+#pragma unroll
+    for (int j = 0; j < kBins / 32; ++j) {
+      if (upto < p.rank && upto + h[j] >= p.rank) bin = kBins / 32 * lane + j;
+      upto += h[j];
+    }
+    bin = __reduce_max_sync(0xffffffffu, bin);
+    if (lane == 0) sh.bin = bin;
+  }
   __syncthreads();
   // where too few parts have a token, all tokens; where they lie too far from the largest, none: the list is given up
   const float bound = sh.bin < 0 ? -INFINITY : sh.bin < kBins - 1 ? least_of(m, sh.bin) : INFINITY;
@@ -346,14 +369,13 @@ __device__ __forceinline__ void scan_stretch(const Params& p, int row, int segme
       if (is_token(mine[c]) && mine[c] >= bound) push(mine[c], col0 + c);
     }
   } else {
-    const float low = m - 400.f * p.tau;  // as a Weigher's
     float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < n / 4; ++i) {
       const float4 q = quads[32 * i];
       const float z[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast((fmaxf(z[j], low) - m) * p.scale2);
+      for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast((z[j] - m) * p.scale2);
       if (fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= bound) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -361,6 +383,15 @@ __device__ __forceinline__ void scan_stretch(const Params& p, int row, int segme
       }
     }
     sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    if (!(sum == sum)) {  // NaN among them, which is no token
+      sum = 0.f;
+      for (int i = 0; i < n / 4; ++i) {
+        const float4 q = quads[32 * i];
+        const float z[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += z[j] == z[j] ? exp2f_fast((z[j] - m) * p.scale2) : 0.f;
+      }
+    }
   }
   sum = block_sum(sum, sh.fred);
   if (tid == 0) {
@@ -652,6 +683,18 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     }
   };
 
+  // columns of the row, 16 at a time; a warp's in a row
+  auto each_column = [&](int lo, int hi, auto&& of) {
+    const int per = ((hi - lo + kThreads - 1) / kThreads) * 32;
+    const int c0 = lo + warp * per, c1 = min(hi, c0 + per);
+    for (int c = c0 + lane; c - lane < c1; c += 16 * 32) {
+      float z[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) z[j] = c + 32 * j < c1 ? logit(src + c + 32 * j) : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) of(z[j] == z[j] ? z[j] + 0.f : -INFINITY, c + 32 * j);
+    }
+  };
   // ---- by list: the row's first tokens in order
   if (p.by_list && complete && !w.sharp) {
     each_listed([&](u64 e) { atomicAdd(&sh.bins[0][step_of(m, logit_at(e))], 1u); });
@@ -661,11 +704,26 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
       if (bin < 0 || step_of(m, logit_at(e)) <= bin) push(e);
     });
     __syncthreads();
-    const unsigned listed = sh.listed;
-    if (listed <= kListSlots) {
+    unsigned listed = sh.listed;
+    if (listed <= kListSlots && (bin >= 0 || bound == -INFINITY)) {
       order_list(sh.list, listed);
-      // no stretch has kept back one that comes before the last of these
-      if (bin < 0 ? bound == -INFINITY : listed >= first && logit_at(sh.list[first - 1]) >= bound) {
+      if (bin >= 0) {
+        // stretches that may have held back a token that comes before the last of these
+        const float last = logit_at(sh.list[first - 1]);
+        if (bound > last) {
+          for (int s = 0; s < p.segments; ++s) {
+            const float of = p.part[seg0 + s].z;
+            if (of <= last) continue;
+            each_column(s * p.per_segment, min(p.V, (s + 1) * p.per_segment), [&](float z, int c) {
+              if (z >= last && z < of) push(place_of(z, c));
+            });
+          }
+          __syncthreads();
+          listed = sh.listed;
+          if (listed <= kListSlots) order_list(sh.list, listed);
+        }
+      }
+      if (listed <= kListSlots) {
         if (TOP) return write_top(listed);
         // kept by top_p and min_p?  Four neighbours of the order a thread.
         constexpr int kPer = kMostFirst / kThreads;
@@ -726,18 +784,6 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     cut_column = column;
   };
   auto in_cut = [&](float z, int column) { return is_token(z) && (z > cut_logit || (z == cut_logit && column <= cut_column)); };
-  // columns of the row, 16 at a time; a warp's in a row
-  auto each_column = [&](int lo, int hi, auto&& of) {
-    const int per = ((hi - lo + kThreads - 1) / kThreads) * 32;
-    const int c0 = lo + warp * per, c1 = min(hi, c0 + per);
-    for (int c = c0 + lane; c - lane < c1; c += 16 * 32) {
-      float z[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) z[j] = c + 32 * j < c1 ? logit(src + c + 32 * j) : -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) of(z[j] == z[j] ? z[j] + 0.f : -INFINITY, c + 32 * j);
-    }
-  };
   // the token drawn of those kept in columns lo to hi: of weight `target`, from the first of them on
   const float min_logit = p.log_min_p > -INFINITY && !w.sharp ? __double2float_rd(w.m64 + (p.log_min_p - 1.0) / p.steps) : -INFINITY;
   auto kept_weight = [&](float z, int column) -> u64 {
@@ -1033,9 +1079,9 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
   if (p.by_list) {
     p.segments = static_cast<int>(up(p.V, rows::kStretch));
     p.per_segment = static_cast<int>(up(up(p.V, p.segments), 4 * rows::kThreads) * 4 * rows::kThreads);
-    // With several stretches and many tokens asked for, not each could hold them all: twice its share and 64, which
-    // finish checks.
-    p.rank = p.segments == 1 ? p.first : std::min<int>(p.first, std::max<int>(256, 2 * up(p.first, p.segments) + 64));
+    // a stretch's share and four standard deviations more, where the first tokens lie anywhere
+    const double share = static_cast<double>(p.first) / p.segments;
+    p.rank = p.segments == 1 ? p.first : std::min(p.first, static_cast<int>(share + 4 * std::sqrt(share)) + 8);
     p.cap = std::min(p.per_segment, p.rank + p.rank / 2 + 64);
     auto space = scan_space(p, logits);
     const size_t held = sizeof(float) * p.per_segment;
