@@ -50,9 +50,9 @@ namespace cg = cooperative_groups;
 using bf16_t = __nv_bfloat16;
 using u64 = unsigned long long;
 
-constexpr int kThreads = 256;     // of scan_list and finish
-constexpr int kWarps = kThreads / 32;
-constexpr int kBinThreads = 512;  // of scan_bins
+constexpr int kThreads = 256;     // of scan_list, and of finish behind it
+constexpr int kBinThreads = 512;  // of scan_bins, and of finish behind it
+constexpr int kBatch = 256;       // columns that a warp of finish looks at at a time
 constexpr int kMostCtas = 8;      // of a cluster
 constexpr int kMostColumns = 96;  // of a thread of scan_bins: what fits in shared memory next to the rest
 constexpr int kStretch = 8192;    // columns of a CTA of scan_list
@@ -545,14 +545,14 @@ __global__ void __launch_bounds__(kBinThreads, 2) scan_bins_kernel(const Params 
 // ==================================================================== finish
 struct FinishShared {
   double exps[kExps];
-  u64 red[kWarps];
+  u64 red[kBinThreads / 32];
   float fred[32];
   unsigned bins[3][kBins];
-  u64 border[kWarps][kMostCtas];
+  u64 border[kBinThreads / 32][kMostCtas];
   u64 kept_of[kMostCtas];
   union {
     u64 list[kListSlots];
-    u64 cells[32][33];  // weights of the warp that holds the drawn token
+    float kept[kBinThreads / 32][kBatch];  // of a warp's batch, in order
     unsigned hist[kDigits];
     u64 weights[kDigits];
   };
@@ -562,11 +562,12 @@ struct FinishShared {
 };
 
 // Descending, slots a power of two.
+template <int THREADS>
 __device__ __forceinline__ void sort_list(u64* list, unsigned slots) {
   for (unsigned size = 2; size <= slots; size *= 2) {
     for (unsigned step = size / 2; step > 0; step /= 2) {
       __syncthreads();
-      for (unsigned q = threadIdx.x; q < slots / 2; q += kThreads) {
+      for (unsigned q = threadIdx.x; q < slots / 2; q += THREADS) {
         const unsigned i = 2 * q - (q & (step - 1)), j = i + step;
         const u64 a = list[i], b = list[j];
         if ((a < b) == ((i & size) == 0)) {
@@ -581,6 +582,7 @@ __device__ __forceinline__ void sort_list(u64* list, unsigned slots) {
 
 // The same of `listed` tokens; kRankSlots or fewer by counting for each how many
 // are larger, two threads to one.
+template <int THREADS>
 __device__ __forceinline__ void order_list(u64* list, unsigned listed) {
   if (listed <= kRankSlots) {
     __syncthreads();
@@ -599,20 +601,21 @@ __device__ __forceinline__ void order_list(u64* list, unsigned listed) {
   }
   unsigned slots = 1;
   while (slots < listed) slots *= 2;
-  for (unsigned i = listed + threadIdx.x; i < slots; i += kThreads) list[i] = 0;
-  sort_list(list, slots);
+  for (unsigned i = listed + threadIdx.x; i < slots; i += THREADS) list[i] = 0;
+  sort_list<THREADS>(list, slots);
 }
-static_assert(2 * kRankSlots <= kThreads && kBins == kThreads && kDigits == kThreads, "a thread each");
+static_assert(2 * kRankSlots <= kThreads && kBins <= kThreads && kDigits <= kThreads, "a thread each");
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, int THREADS>
 __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShared& sh) {
+  constexpr int kWarps = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* src = static_cast<const T*>(p.logits) + row * p.ld;
   const int64_t seg0 = static_cast<int64_t>(row) * p.segments;
   constexpr int kLowest = sizeof(T) == 2 ? 16 : 0;  // key bits below are the same in all of a type's values
   const unsigned first = p.first;
   if (!TOP) fill_exps(sh.exps);
-  for (int i = tid; i < 3 * kBins; i += kThreads) sh.bins[0][i] = 0;
+  for (int i = tid; i < 3 * kBins; i += THREADS) sh.bins[0][i] = 0;
   if (tid == 0) sh.listed = 0;
 
   // ---- the row's largest logit; by list also the sum of its weights
@@ -620,7 +623,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   bool complete = true;  // the lists are
   float bound = -INFINITY;
   if (p.by_list) {
-    for (int s = tid; s < p.segments; s += kThreads) {
+    for (int s = tid; s < p.segments; s += THREADS) {
       const float4 of = p.part[seg0 + s];
       m = fmaxf(m, of.x);
       bound = fmaxf(bound, of.z);
@@ -628,18 +631,18 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     }
     m = block_max(m, sh.fred);
     bound = block_max(bound, sh.fred);
-    for (int s = tid; s < p.segments; s += kThreads) {
+    for (int s = tid; s < p.segments; s += THREADS) {
       const float4 of = p.part[seg0 + s];
       sum += of.x == m ? of.y : of.y * exp2f_fast((of.x - m) * p.scale2);
     }
     sum = block_sum(sum, sh.fred);
   } else {
     m = p.states[row].m;
-    for (int s = tid; s < p.segments; s += kThreads) complete = complete && p.counts[seg0 + s] <= p.cap;
+    for (int s = tid; s < p.segments; s += THREADS) complete = complete && p.counts[seg0 + s] <= p.cap;
   }
   complete = __syncthreads_and(complete);
   if (m == -INFINITY) {
-    for (int i = tid; i < (TOP ? p.first : 1); i += kThreads) {
+    for (int i = tid; i < (TOP ? p.first : 1); i += THREADS) {
       p.ids[static_cast<int64_t>(row) * (TOP ? p.first : 1) + i] = -1;
       p.logp[static_cast<int64_t>(row) * (TOP ? p.first : 1) + i] = 0.f;
     }
@@ -674,7 +677,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   };
   // the first `n` of the ordered list
   auto write_top = [&](unsigned n) {
-    for (int i = tid; i < p.first; i += kThreads) {
+    for (int i = tid; i < p.first; i += THREADS) {
       const bool in = i < static_cast<int>(n);
       const int64_t at = static_cast<int64_t>(row) * p.first + i;
       if (T1_OOB(at, static_cast<int64_t>(p.rows) * p.first)) continue;
@@ -685,7 +688,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
 
   // columns of the row, 16 at a time; a warp's in a row
   auto each_column = [&](int lo, int hi, auto&& of) {
-    const int per = ((hi - lo + kThreads - 1) / kThreads) * 32;
+    const int per = ((hi - lo + THREADS - 1) / THREADS) * 32;
     const int c0 = lo + warp * per, c1 = min(hi, c0 + per);
     for (int c = c0 + lane; c - lane < c1; c += 16 * 32) {
       float z[16];
@@ -699,14 +702,14 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   if (p.by_list && complete && !w.sharp) {
     each_listed([&](u64 e) { atomicAdd(&sh.bins[0][step_of(m, logit_at(e))], 1u); });
     __syncthreads();
-    const int bin = reach(sh.bins[0][tid], first);  // none: they are fewer
+    const int bin = reach(tid < kBins ? sh.bins[0][tid] : 0ull, first);  // none: they are fewer
     each_listed([&](u64 e) {
       if (bin < 0 || step_of(m, logit_at(e)) <= bin) push(e);
     });
     __syncthreads();
     unsigned listed = sh.listed;
     if (listed <= kListSlots && (bin >= 0 || bound == -INFINITY)) {
-      order_list(sh.list, listed);
+      order_list<THREADS>(sh.list, listed);
       if (bin >= 0) {
         // stretches that may have held back a token that comes before the last of these
         const float last = logit_at(sh.list[first - 1]);
@@ -720,13 +723,13 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
           }
           __syncthreads();
           listed = sh.listed;
-          if (listed <= kListSlots) order_list(sh.list, listed);
+          if (listed <= kListSlots) order_list<THREADS>(sh.list, listed);
         }
       }
       if (listed <= kListSlots) {
         if (TOP) return write_top(listed);
         // kept by top_p and min_p?  Four neighbours of the order a thread.
-        constexpr int kPer = kMostFirst / kThreads;
+        constexpr int kPer = kMostFirst / THREADS;
         const unsigned have = min(first, listed);
         u64 e[kPer], of[kPer], own = 0, before;
         double x[kPer];
@@ -750,7 +753,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
           if (i < have) sh.list[i] = in ? e[j] << 32 | e[j] >> 32 : 0ull;
         }
         kept = static_cast<unsigned>(block_scan64<kWarps>(kept, before, sh.red));
-        order_list(sh.list, kept);  // the tokens kept are a prefix of the list
+        order_list<THREADS>(sh.list, kept);  // the tokens kept are a prefix of the list
         own = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
@@ -784,53 +787,59 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     cut_column = column;
   };
   auto in_cut = [&](float z, int column) { return is_token(z) && (z > cut_logit || (z == cut_logit && column <= cut_column)); };
-  // the token drawn of those kept in columns lo to hi: of weight `target`, from the first of them on
+  // A token of weight `target`, from the first of them on, of those kept in columns lo to hi.  A batch's kept tokens
+  // are put together first: where one in ten is kept, weights are not worked out ten lanes in vain.
   const float min_logit = p.log_min_p > -INFINITY && !w.sharp ? __double2float_rd(w.m64 + (p.log_min_p - 1.0) / p.steps) : -INFINITY;
-  auto kept_weight = [&](float z, int column) -> u64 {
-    if (!in_cut(z, column) || z < min_logit) return 0;
-    const double x = w.steps_of(z);
-    return x >= p.log_min_p ? w.weight_at(x) : 0ull;
+  auto is_kept = [&](float z, int column) {
+    return in_cut(z, column) && z >= min_logit && (p.log_min_p == -INFINITY || w.steps_of(z) >= p.log_min_p);
   };
-  // Weight of the tokens kept in lo to hi before the warp's columns, in `before`; and of the warp's and all of them.
-  auto weigh = [&](int lo, int hi, u64& before, u64& of_warp) {
-    u64 own = 0;
-    each_column(lo, hi, [&](float z, int c) { own += kept_weight(z, c); });
-    of_warp = warp_sum64(own);
+  // a batch from column c on, to c1: `put` gets its kept tokens' places in order; their number
+  auto batch = [&](int c, int c1, auto&& put) {
+    float z[kBatch / 32];
+#pragma unroll
+    for (int j = 0; j < kBatch / 32; ++j) z[j] = c + 32 * j + lane < c1 ? logit(src + c + 32 * j + lane) : -INFINITY;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kBatch / 32; ++j) {
+      const bool in = is_kept(z[j], c + 32 * j + lane);
+      const unsigned all = __ballot_sync(0xffffffffu, in);
+      if (in) put(n + __popc(all & ((1u << lane) - 1)), z[j], c + 32 * j + lane);
+      n += __popc(all);
+    }
+    __syncwarp();
+    return n;
+  };
+  auto draw = [&](int lo, int hi, bool have_target, u64 target) {
+    const int per = ((hi - lo + THREADS - 1) / THREADS) * 32;
+    const int c0 = lo + warp * per, c1 = min(hi, c0 + per);
+    u64 own = 0, before;
+    for (int c = c0; c < c1; c += kBatch) {
+      const int n = batch(c, c1, [&](int i, float z, int) { sh.kept[warp][i] = z; });
+      for (int i = lane; i < n; i += 32) own += w.weight(sh.kept[warp][i]);
+      __syncwarp();
+    }
+    const u64 of_warp = warp_sum64(own);
     const u64 all = block_scan64<kWarps>(own, before, sh.red);
     before = __shfl_sync(0xffffffffu, before, 0);
-    return all;
-  };
-  auto draw = [&](int lo, int hi, u64 target, u64 before, u64 of_warp) {
+    if (!have_target) target = target_of(p.u[row], all);
     if (target < before || target >= before + of_warp) return;
-    // this warp has it: the sums of 32 times 32 columns, then the lanes of one
-    const int per = ((hi - lo + kThreads - 1) / kThreads) * 32;
-    const int c0 = lo + warp * per, c1 = min(hi, c0 + per);
-    for (int c = c0; c < c1; c += 32 * 32) {
-      __syncwarp();
-#pragma unroll 8
-      for (int i = 0; i < 32; ++i) {
-        const int column = c + 32 * i + lane;
-        const float z = column < c1 ? logit(src + column) : -INFINITY;
-        sh.cells[i][lane] = kept_weight(z + 0.f, column);
-      }
-      __syncwarp();
-      u64 s = 0;
-      for (int l = 0; l < 32; ++l) s += sh.cells[lane][l];
-      const u64 upto = before + warp_scan64(s, lane);
-      const unsigned past = __ballot_sync(0xffffffffu, target < upto);
-      if (past == 0) {
+    // this warp has it, and the list's place to itself
+    for (int c = c0; c < c1; c += kBatch) {
+      const int n = batch(c, c1, [&](int i, float z, int column) { sh.list[i] = place_of(z, column); });
+      for (int i = lane; i - lane < n; i += 32) {
+        const u64 e = i < n ? sh.list[i] : 0ull;
+        const u64 upto = before + warp_scan64(i < n ? w.weight(logit_at(e)) : 0ull, lane);
+        const unsigned past = __ballot_sync(0xffffffffu, target < upto);
+        if (past != 0) {
+          if (lane == __ffs(past) - 1) {
+            p.ids[row] = column_at(e);
+            p.logp[row] = log_p(logit_at(e));
+          }
+          return;
+        }
         before = __shfl_sync(0xffffffffu, upto, 31);
-        continue;
       }
-      const int i = __ffs(past) - 1;
-      before = __shfl_sync(0xffffffffu, upto - s, i);
-      const u64 mine = before + warp_scan64(sh.cells[i][lane], lane);
-      if (lane == __ffs(__ballot_sync(0xffffffffu, target < mine)) - 1) {
-        const int column = c + 32 * i + lane;
-        p.ids[row] = column;
-        p.logp[row] = log_p(logit(src + column));
-      }
-      return;
+      __syncwarp();
     }
   };
 
@@ -851,11 +860,11 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
       __syncthreads();
       const unsigned listed = sh.listed;
       if (listed <= kListSlots) {
-        constexpr int kPer = kListSlots / kThreads;
+        constexpr int kPer = kListSlots / THREADS;
         u64 e[kPer], of[kPer], before;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-          const unsigned i = j * kThreads + tid;
+          const unsigned i = j * THREADS + tid;
           e[j] = i < listed ? sh.list[i] : 0ull;
           of[j] = 0;
           if (e[j] != 0) {
@@ -866,7 +875,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
         }
         __syncthreads();
         if (tid == 0) sh.listed = 0;
-        const int part = reach(bin_sum(sh.bins[0], tid), st.need);
+        const int part = reach(tid < kBins ? bin_sum(sh.bins[0], tid) : 0ull, st.need);
         // the last token before which less than top_p has come is one of this part
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
@@ -874,7 +883,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
         __syncthreads();
         const unsigned few = sh.listed;
         const u64 need = st.need - sh.before64;
-        order_list(sh.list, few);
+        order_list<THREADS>(sh.list, few);
         u64 own = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
@@ -918,9 +927,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
       const u64 target = target_of(p.u[row], of_segments);
       while (target >= before_segment + sh.kept_of[segment]) before_segment += sh.kept_of[segment++];
       const int lo = segment * p.per_segment, hi = min(p.V, lo + p.per_segment);
-      u64 before, of_warp;
-      weigh(lo, hi, before, of_warp);
-      draw(lo, hi, target - before_segment, before, of_warp);
+      draw(lo, hi, true, target - before_segment);
       return;
     }
   }
@@ -959,14 +966,14 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     if (first < tokens) {
       unsigned need = first, prefix = 0, mask = 0;
       for (int shift = 24; shift >= kLowest; shift -= 8) {
-        sh.hist[tid] = 0;
+        if (tid < kDigits) sh.hist[tid] = 0;
         __syncthreads();
         each_column(0, p.V, [&](float z, int) {
           const unsigned key = key_of(z);
           if (is_token(z) && (key & mask) == prefix) atomicAdd(&sh.hist[key >> shift & 255], 1u);
         });
         __syncthreads();
-        const int digit = 255 - reach(sh.hist[255 - tid], need);
+        const int digit = 255 - reach(tid < kDigits ? sh.hist[kDigits - 1 - tid] : 0ull, need);
         need -= static_cast<unsigned>(sh.before64);
         prefix |= static_cast<unsigned>(digit) << shift;
         mask |= 255u << shift;
@@ -982,7 +989,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
       if (in_cut(z, c)) push(place_of(z, c));
     });
     __syncthreads();
-    order_list(sh.list, have);
+    order_list<THREADS>(sh.list, have);
     return write_top(have);
   }
   if (p.top_p < 1.0 && !found) {
@@ -993,14 +1000,14 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     u64 need = share_of(p.top_p, block_scan64<kWarps>(own, before, sh.red));
     unsigned prefix = 0, mask = 0;
     for (int shift = 24; shift >= kLowest; shift -= 8) {
-      sh.weights[tid] = 0;
+      if (tid < kDigits) sh.weights[tid] = 0;
       __syncthreads();
       each_column(0, p.V, [&](float z, int c) {
         const unsigned key = key_of(z);
         if (in_cut(z, c) && (key & mask) == prefix) atomicAdd(&sh.weights[key >> shift & 255], w.weight(z));
       });
       __syncthreads();
-      const int digit = 255 - reach(sh.weights[255 - tid], need);
+      const int digit = 255 - reach(tid < kDigits ? sh.weights[kDigits - 1 - tid] : 0ull, need);
       need -= sh.before64;
       prefix |= static_cast<unsigned>(digit) << shift;
       mask |= 255u << shift;
@@ -1010,17 +1017,15 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     const u64 one = w.weight(logit_of(key));
     cut_at_tie(key, static_cast<unsigned>((need + one - 1) / one));  // of these it takes so many to reach `need`
   }
-  u64 before, of_warp;
-  const u64 all = weigh(0, p.V, before, of_warp);
-  draw(0, p.V, target_of(p.u[row], all), before, of_warp);
+  draw(0, p.V, false, 0);
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) finish_kernel(const Params p) {
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS) finish_kernel(const Params p) {
   __shared__ FinishShared sh;
   launch_dependents();
   wait_previous();
-  finish_row<T, TOP>(p, blockIdx.x, sh);
+  finish_row<T, TOP, THREADS>(p, blockIdx.x, sh);
 }
 
 // `ALONE`: a row is one stretch, and the CTA that scans it finishes it too.
@@ -1035,7 +1040,7 @@ __global__ void __launch_bounds__(kThreads) scan_list_kernel(const Params p) {
   if constexpr (ALONE) {
     __shared__ FinishShared rest;
     __syncthreads();
-    finish_row<T, TOP>(p, row, rest);
+    finish_row<T, TOP, kThreads>(p, row, rest);
   }
 }
 
@@ -1092,39 +1097,41 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
       done = true;
     }
     launch_after(what, scan, dim3(static_cast<unsigned>(p.rows) * p.segments), rows::kThreads, held, p);
-    if (p.segments > 1) launch_after(what, rows::finish_kernel<T, TOP>, dim3(p.rows), rows::kThreads, 0, p);
+    if (p.segments > 1) launch_after(what, rows::finish_kernel<T, TOP, rows::kThreads>, dim3(p.rows), rows::kThreads, 0, p);
     return;
   }
-  // 32 columns a thread (64 KB a CTA, so that several rows share an SM) as long as 8 CTAs are enough
-  p.segments = 1;
-  while (p.segments < rows::kMostCtas && p.segments * 32 * rows::kBinThreads < p.V) p.segments *= 2;
-  p.per_segment = static_cast<int>(up(up(p.V, p.segments), 4 * rows::kBinThreads) * 4 * rows::kBinThreads);
-  p.cap = rows::kBinCap;
-  auto space = scan_space(p, logits);
-  auto scan = rows::scan_bins_kernel<T>;
-  static DeviceFlags configured;
-  if (bool& done = configured.here(); !done) {
-    T1_CHECK_CUDA(cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       sizeof(float) * rows::kMostColumns * rows::kBinThreads));
-    done = true;
+  if constexpr (!TOP) {
+    // 32 columns a thread (64 KB a CTA, so that several rows share an SM) as long as 8 CTAs are enough
+    p.segments = 1;
+    while (p.segments < rows::kMostCtas && p.segments * 32 * rows::kBinThreads < p.V) p.segments *= 2;
+    p.per_segment = static_cast<int>(up(up(p.V, p.segments), 4 * rows::kBinThreads) * 4 * rows::kBinThreads);
+    p.cap = rows::kBinCap;
+    auto space = scan_space(p, logits);
+    auto scan = rows::scan_bins_kernel<T>;
+    static DeviceFlags configured;
+    if (bool& done = configured.here(); !done) {
+      T1_CHECK_CUDA(cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         sizeof(float) * rows::kMostColumns * rows::kBinThreads));
+      done = true;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * p.segments);
+    cfg.blockDim = dim3(rows::kBinThreads);
+    cfg.dynamicSmemBytes = sizeof(float) * p.per_segment;
+    cfg.stream = stream();
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.segments;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, scan, static_cast<const rows::Params>(p));
+    TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e));
+    count_launch();
+    launch_after(what, rows::finish_kernel<T, TOP, rows::kBinThreads>, dim3(p.rows), rows::kBinThreads, 0, p);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * p.segments);
-  cfg.blockDim = dim3(rows::kBinThreads);
-  cfg.dynamicSmemBytes = sizeof(float) * p.per_segment;
-  cfg.stream = stream();
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.segments;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, scan, static_cast<const rows::Params>(p));
-  TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e));
-  count_launch();
-  launch_after(what, rows::finish_kernel<T, TOP>, dim3(p.rows), rows::kThreads, 0, p);
 }
 
 template <bool TOP>
