@@ -427,7 +427,7 @@ __device__ __forceinline__ void tell_all(cg::cluster_group& cluster, V* slots, V
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kBinThreads, 2) scan_bins_kernel(const Params p) {
+__global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params p) {
   __shared__ BinShared sh;
   extern __shared__ __align__(16) float held[];
   cg::cluster_group cluster = cg::this_cluster();
