@@ -25,8 +25,9 @@
 //              (172 us).
 //   scan_bins  all other draws.  A cluster of CTAs holds the row in shared
 //              memory and agrees on m; weights are added up, with top_p by
-//              distance from m as well, 8 bins per factor of two, and the tokens
-//              of the bin where top_p is reached are listed.
+//              distance from m as well, 16 bins per factor of two, and the tokens
+//              of the bin where top_p is reached are listed (a tenth of the
+//              vocabulary may fall into one).
 // Where a list is too long (many equal logits) or does not hold what is asked
 // for, finish finds the cut digit by digit, 8 bits at a time, of the
 // order-preserving integer of a logit, reading the row anew each time.
@@ -61,9 +62,11 @@ constexpr int kMostList = 512;    // tokens of `top`
 constexpr int kMostFirst = kParts * kThreads;  // tokens that a list can be asked for
 constexpr int kListSlots = 2048;  // tokens that finish orders
 constexpr int kRankSlots = 128;   // up to so many by counting
-constexpr int kBinCap = 1024;     // tokens that a CTA of scan_bins lists
+constexpr int kBinCap = 2048;     // tokens that a CTA of scan_bins lists
 constexpr int kDigits = 256;
-constexpr int kBins = 256;
+constexpr int kBins = 256;        // of distances, and parts of a bin of weights
+constexpr int kWeightBins = 512;  // of scan_bins
+constexpr int kBinSteps = 8;
 constexpr int kExps = 128;        // steps of an octave in the table of exponentials
 
 // What scan_bins has found out about a row.
@@ -260,26 +263,29 @@ struct Weigher {
     return __double_as_longlong(fma(e, scaled, kWhole)) - __double_as_longlong(kWhole);
   }
   __device__ __forceinline__ u64 weight(float z) const { return weight_at(steps_of(z)); }
-  // Bins of 16 steps, and 256 parts of one.
-  __device__ __forceinline__ static int bin_at(double x) { return -__double2loint(x + kRound) >> 4; }
+  // Bins of 8 steps, and 256 parts of one.
+  __device__ __forceinline__ static int bin_at(double x) { return -__double2loint(x + kRound) >> 3; }
   __device__ __forceinline__ static int part_at(double x, int bin) {
-    return min(max(static_cast<int>((0.5 - x - 16 * bin) * 16.0), 0), kBins - 1);
+    return min(max(static_cast<int>((0.5 - x - kBinSteps * bin) * (kBins / kBinSteps)), 0), kBins - 1);
   }
 };
+static_assert(kBinSteps == 8, "bin_at: >> 3");
 static_assert(kExps == 128, "weight_at: j >> 7");
 
 // Bins of weights, 16 bits each: a bin of 2^16 tokens stays below 2^32.
-__device__ __forceinline__ void add_to(unsigned (*bins)[kBins], int b, u64 w) {
+template <int N>
+__device__ __forceinline__ void add_to(unsigned (&bins)[3][N], int b, u64 w) {
   const unsigned lo = static_cast<unsigned>(w) & 0xffffu, mid = static_cast<unsigned>(w >> 16) & 0xffffu,
                  hi = static_cast<unsigned>(w >> 32);
   atomicAdd(&bins[0][b], lo);
   atomicAdd(&bins[1][b], mid);
   if (hi != 0) atomicAdd(&bins[2][b], hi);
 }
-__device__ __forceinline__ u64 bin_sum(const unsigned* bins, int b) {
-  return bins[b] + (static_cast<u64>(bins[kBins + b]) << 16) + (static_cast<u64>(bins[2 * kBins + b]) << 32);
+template <int N>
+__device__ __forceinline__ u64 bin_sum(const unsigned (&bins)[3][N], int b) {
+  return bins[0][b] + (static_cast<u64>(bins[1][b]) << 16) + (static_cast<u64>(bins[2][b]) << 32);
 }
-static_assert(kBinThreads * kMostColumns <= 65536 && kListSlots <= 65536, "add_to");
+static_assert(kBinThreads * kMostColumns <= 65536 && kMostCtas * kBinCap <= 65536, "add_to");
 
 // =============================================================== scan by list
 // A CTA takes a stretch of a row: its largest logit, the sum of its weights and
@@ -403,7 +409,7 @@ __device__ __forceinline__ void scan_stretch(const Params& p, int row, int segme
 // =============================================================== scan by bins
 struct BinShared {
   double exps[kExps];
-  unsigned bins[3][kBins];
+  unsigned bins[3][kWeightBins];
   u64 red[kBinThreads / 32];
   float fred[32];
   // what every CTA of the cluster tells all others, once each
@@ -447,7 +453,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
     fetch(held + warp * 32 * n, static_cast<const T*>(p.logits) + row * p.ld + warp_col0, cols, p.aligned, lane);
     for (int c = cols + lane; c < 32 * n; c += 32) held[warp * 32 * n + c] = -INFINITY;
   }
-  for (int i = tid; i < 3 * kBins; i += kBinThreads) sh.bins[0][i] = 0;
+  for (int i = tid; i < 3 * kWeightBins; i += kBinThreads) sh.bins[0][i] = 0;
   fill_exps(sh.exps);
   fetched();
   __syncwarp();
@@ -481,7 +487,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
       own += of;
       if (by_bins) {
         const int b = Weigher::bin_at(x);
-        if (b < kBins) add_to(sh.bins, b, of);
+        if (b < kWeightBins) add_to(sh.bins, b, of);
       } else if (by_min && x >= p.log_min_p) {
         kept += of;
       }
@@ -501,8 +507,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   // the bin in which top_p is reached, of all CTAs' weights
   const u64 need = share_of(p.top_p, total);
   u64 here = 0;
-  if (tid < kBins)
-    for (int r = 0; r < ctas; ++r) here += bin_sum(cluster.map_shared_rank(&sh.bins[0][0], r), tid);
+  for (int r = 0; r < ctas; ++r) here += bin_sum(cluster.map_shared_rank(&sh, r)->bins, tid);
   if (tid == 0) sh.bin = -1;
   block_scan64<kBinThreads / 32>(here, before, sh.red);
   if (before < need && before + here >= need) {
@@ -514,10 +519,10 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   if (rank == 0 && tid == 0) p.states[row] = {m, bin, total, need - (bin < 0 ? 0 : sh.before64)};
   if (bin < 0) return;
   // the CTA's weight above that bin, and its tokens in it
-  const u64 above = block_scan64<kBinThreads / 32>(tid < bin ? bin_sum(sh.bins[0], tid) : 0ull, before, sh.red);
+  const u64 above = block_scan64<kBinThreads / 32>(tid < bin ? bin_sum(sh.bins, tid) : 0ull, before, sh.red);
   if (tid == 0) p.weights[at] = above;
   // between which the bin's logits lie
-  const float least = __double2float_rd(w.m64 - 16.0 * (bin + 1) / p.steps), most = __double2float_ru(w.m64 - (16.0 * bin - 1) / p.steps);
+  const float least = __double2float_rd(w.m64 - kBinSteps * (bin + 1.0) / p.steps), most = __double2float_ru(w.m64 - (kBinSteps * bin - 1.0) / p.steps);
   unsigned in_bin[kMostColumns / 32], mine = 0;
 #pragma unroll
   for (int b = 0; b < kMostColumns / 32; ++b) {
@@ -548,7 +553,7 @@ struct FinishShared {
   u64 red[kBinThreads / 32];
   float fred[32];
   unsigned bins[3][kBins];
-  u64 border[kBinThreads / 32][kMostCtas];
+  u64 border[kBinThreads / 32];
   u64 kept_of[kMostCtas];
   union {
     u64 list[kListSlots];
@@ -604,6 +609,7 @@ __device__ __forceinline__ void order_list(u64* list, unsigned listed) {
   for (unsigned i = listed + threadIdx.x; i < slots; i += THREADS) list[i] = 0;
   sort_list<THREADS>(list, slots);
 }
+static_assert(kMostCtas <= kBinThreads / 32, "each_listed: a warp or more to a segment of scan_bins");
 static_assert(2 * kRankSlots <= kThreads && kBins <= kThreads && kDigits <= kThreads, "a thread each");
 
 template <typename T, bool TOP, int THREADS>
@@ -656,11 +662,12 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     if (to < kListSlots) sh.list[to] = place;
   };
   // every token that the scan has listed
+  const int warps_each = max(1, kWarps / p.segments);  // of a segment
   auto each_listed = [&](auto&& of) {
-    for (int s = warp; s < p.segments; s += kWarps) {
+    for (int s = warp / warps_each; s < p.segments; s += kWarps / warps_each) {
       const int n = p.counts[seg0 + s];
       const u64* list = p.lists + (seg0 + s) * p.cap;
-      for (int i = lane; i < n; i += 32) of(list[i]);
+      for (int i = warp % warps_each * 32 + lane; i < n; i += 32 * warps_each) of(list[i]);
     }
   };
   // the thread's bin in which `need` is reached (-1: in none), and in sh.before64 what comes before
@@ -856,35 +863,23 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
       __syncthreads();
       segment = 0;
     } else if (st.bin >= 0 && complete) {
-      each_listed(push);
+      each_listed([&](u64 e) {
+        const double x = w.blunt_steps(logit_at(e));
+        add_to(sh.bins, Weigher::part_at(x, st.bin), w.weight_at(x));
+      });
       __syncthreads();
-      const unsigned listed = sh.listed;
-      if (listed <= kListSlots) {
-        constexpr int kPer = kListSlots / THREADS;
-        u64 e[kPer], of[kPer], before;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const unsigned i = j * THREADS + tid;
-          e[j] = i < listed ? sh.list[i] : 0ull;
-          of[j] = 0;
-          if (e[j] != 0) {
-            const double x = w.blunt_steps(logit_at(e[j]));
-            of[j] = w.weight_at(x);
-            add_to(sh.bins, Weigher::part_at(x, st.bin), of[j]);
-          }
-        }
-        __syncthreads();
-        if (tid == 0) sh.listed = 0;
-        const int part = reach(tid < kBins ? bin_sum(sh.bins[0], tid) : 0ull, st.need);
-        // the last token before which less than top_p has come is one of this part
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (e[j] != 0 && Weigher::part_at(w.blunt_steps(logit_at(e[j])), st.bin) == part) push(e[j]);
-        __syncthreads();
-        const unsigned few = sh.listed;
-        const u64 need = st.need - sh.before64;
+      // the last token before which less than top_p has come is one of this part
+      const int part = reach(tid < kBins ? bin_sum(sh.bins, tid) : 0ull, st.need);
+      const u64 need = st.need - sh.before64;
+      each_listed([&](u64 e) {
+        if (Weigher::part_at(w.blunt_steps(logit_at(e)), st.bin) == part) push(e);
+      });
+      __syncthreads();
+      const unsigned few = sh.listed;
+      if (few <= kListSlots) {
         order_list<THREADS>(sh.list, few);
-        u64 own = 0;
+        constexpr int kPer = kListSlots / THREADS;
+        u64 own = 0, before;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
           const unsigned i = kPer * tid + j;
@@ -903,18 +898,16 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
         found = true;
         if (w.blunt_steps(cut_logit) >= p.log_min_p) {
           // min_p takes no more away: the segments' kept weights
-          for (int s = 0; s < p.segments; ++s) {
-            u64 kept = 0;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-              if (e[j] >= cut && column_at(e[j]) / p.per_segment == s) kept += of[j];
-            kept = warp_sum64(kept);
-            if (lane == 0) sh.border[warp][s] = kept;
-          }
+          u64 kept = 0;
+          each_listed([&](u64 e) {
+            if (e >= cut) kept += w.weight(logit_at(e));
+          });
+          kept = warp_sum64(kept);
+          if (lane == 0) sh.border[warp] = kept;
           __syncthreads();
           if (tid < p.segments) {
-            u64 kept = p.weights[seg0 + tid];
-            for (int v = 0; v < kWarps; ++v) kept += sh.border[v][tid];
+            kept = p.weights[seg0 + tid];
+            for (int v = 0; v < warps_each; ++v) kept += sh.border[tid * warps_each + v];
             sh.kept_of[tid] = kept;
           }
           __syncthreads();
@@ -1087,7 +1080,7 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
     // a stretch's share and four standard deviations more, where the first tokens lie anywhere
     const double share = static_cast<double>(p.first) / p.segments;
     p.rank = p.segments == 1 ? p.first : std::min(p.first, static_cast<int>(share + 4 * std::sqrt(share)) + 8);
-    p.cap = std::min(p.per_segment, p.rank + p.rank / 2 + 64);
+    p.cap = std::min(p.per_segment, 2 * p.rank + 64);
     auto space = scan_space(p, logits);
     const size_t held = sizeof(float) * p.per_segment;
     auto scan = p.segments == 1 ? rows::scan_list_kernel<T, TOP, true> : rows::scan_list_kernel<T, TOP, false>;
