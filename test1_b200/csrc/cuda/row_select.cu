@@ -53,7 +53,7 @@ using u64 = unsigned long long;
 
 constexpr int kThreads = 256;     // of scan_list, and of finish behind it
 constexpr int kBinThreads = 512;  // of scan_bins, and of finish behind it
-constexpr int kBatch = 256;       // columns that a warp of finish looks at at a time
+constexpr int kBatch = 512;       // columns that a warp of finish looks at at a time
 constexpr int kMostCtas = 8;      // of a cluster
 constexpr int kMostColumns = 96;  // of a thread of scan_bins: what fits in shared memory next to the rest
 constexpr int kStretch = 8192;    // columns of a CTA of scan_list
@@ -297,8 +297,14 @@ struct ListShared {
   unsigned listed;
 };
 
+// What a scan by list has found out about a stretch.
+struct Scan {
+  float m, sum, bound;  // largest logit, sum of weights; no token from `bound` on is missing in the list
+  unsigned listed;      // above the list's length: not all
+};
+
 template <typename T>
-__device__ __forceinline__ void scan_stretch(const Params& p, int row, int segment, ListShared& sh, float* held) {
+__device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segment, u64* list, unsigned cap, ListShared& sh, float* held) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // a warp has 32 n columns in a row, a thread four of every 128, quads[32 i]
   const int n = p.per_segment / kThreads;
@@ -323,14 +329,7 @@ __device__ __forceinline__ void scan_stretch(const Params& p, int row, int segme
     part[3] = fmaxf(part[3], q.w);
   }
   const float m = block_max(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), sh.fred);
-  const int64_t at = static_cast<int64_t>(row) * p.segments + segment;
-  if (m == -INFINITY) {
-    if (tid == 0) {
-      p.part[at] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-      p.counts[at] = 0;
-    }
-    return;
-  }
+  if (m == -INFINITY) return {m, 0.f, m, 0};
   // few tokens need few parts
   if (p.rank <= kThreads / 4) {
     const float own = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
@@ -363,10 +362,9 @@ __device__ __forceinline__ void scan_stretch(const Params& p, int row, int segme
   __syncthreads();
   // where too few parts have a token, all tokens; where they lie too far from the largest, none: the list is given up
   const float bound = sh.bin < 0 ? -INFINITY : sh.bin < kBins - 1 ? least_of(m, sh.bin) : INFINITY;
-  u64* list = p.lists + at * p.cap;
   auto push = [&](float z, int column) {
     const unsigned to = atomicAdd(&sh.listed, 1u);
-    if (to < p.cap) list[to] = place_of(z, column);
+    if (to < cap) list[to] = place_of(z, column);
   };
   float sum = 0.f;
   if (is_sharp(m, p.tau)) {
@@ -400,10 +398,7 @@ __device__ __forceinline__ void scan_stretch(const Params& p, int row, int segme
     }
   }
   sum = block_sum(sum, sh.fred);
-  if (tid == 0) {
-    p.part[at] = make_float4(m, sum, bound, 0.f);
-    p.counts[at] = bound == INFINITY ? p.cap + 1 : static_cast<int>(min(sh.listed, p.cap + 1u));
-  }
+  return {m, sum, bound, bound == INFINITY ? cap + 1 : min(sh.listed, cap + 1)};
 }
 
 // =============================================================== scan by bins
@@ -612,8 +607,10 @@ __device__ __forceinline__ void order_list(u64* list, unsigned listed) {
 static_assert(kMostCtas <= kBinThreads / 32, "each_listed: a warp or more to a segment of scan_bins");
 static_assert(2 * kRankSlots <= kThreads && kBins <= kThreads && kDigits <= kThreads, "a thread each");
 
-template <typename T, bool TOP, int THREADS>
-__device__ __forceinline__ void finish_row(const Params& p, int row, FinishShared& sh) {
+// ALONE: the row is one stretch, which this CTA has scanned itself and whose
+// list is in place.
+template <typename T, bool TOP, int THREADS, bool ALONE>
+__device__ __forceinline__ void finish_row(const Params& p, int row, FinishShared& sh, const Scan& scan) {
   constexpr int kWarps = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* src = static_cast<const T*>(p.logits) + row * p.ld;
@@ -621,14 +618,19 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   constexpr int kLowest = sizeof(T) == 2 ? 16 : 0;  // key bits below are the same in all of a type's values
   const unsigned first = p.first;
   if (!TOP) fill_exps(sh.exps);
-  for (int i = tid; i < 3 * kBins; i += THREADS) sh.bins[0][i] = 0;
-  if (tid == 0) sh.listed = 0;
+  for (int i = tid; !ALONE && i < 3 * kBins; i += THREADS) sh.bins[0][i] = 0;
+  if (tid == 0) sh.listed = ALONE ? scan.listed : 0;
 
   // ---- the row's largest logit; by list also the sum of its weights
   float m = -INFINITY, sum = 0.f;
   bool complete = true;  // the lists are
   float bound = -INFINITY;
-  if (p.by_list) {
+  if (ALONE) {
+    m = scan.m;
+    sum = scan.sum;
+    bound = scan.bound;
+    complete = scan.listed <= kListSlots;
+  } else if (p.by_list) {
     for (int s = tid; s < p.segments; s += THREADS) {
       const float4 of = p.part[seg0 + s];
       m = fmaxf(m, of.x);
@@ -707,17 +709,21 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   };
   // ---- by list: the row's first tokens in order
   if (p.by_list && complete && !w.sharp) {
-    each_listed([&](u64 e) { atomicAdd(&sh.bins[0][step_of(m, logit_at(e))], 1u); });
-    __syncthreads();
-    const int bin = reach(tid < kBins ? sh.bins[0][tid] : 0ull, first);  // none: they are fewer
-    each_listed([&](u64 e) {
-      if (bin < 0 || step_of(m, logit_at(e)) <= bin) push(e);
-    });
-    __syncthreads();
+    bool enough = ALONE && bound > -INFINITY;  // not only all that there are
+    if (!ALONE) {
+      each_listed([&](u64 e) { atomicAdd(&sh.bins[0][step_of(m, logit_at(e))], 1u); });
+      __syncthreads();
+      const int bin = reach(tid < kBins ? sh.bins[0][tid] : 0ull, first);
+      enough = bin >= 0;
+      each_listed([&](u64 e) {
+        if (!enough || step_of(m, logit_at(e)) <= bin) push(e);
+      });
+      __syncthreads();
+    }
     unsigned listed = sh.listed;
-    if (listed <= kListSlots && (bin >= 0 || bound == -INFINITY)) {
+    if (listed <= kListSlots && (enough || bound == -INFINITY)) {
       order_list<THREADS>(sh.list, listed);
-      if (bin >= 0) {
+      if (!ALONE && enough) {
         // stretches that may have held back a token that comes before the last of these
         const float last = logit_at(sh.list[first - 1]);
         if (bound > last) {
@@ -1018,7 +1024,7 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(const Params p) {
   __shared__ FinishShared sh;
   launch_dependents();
   wait_previous();
-  finish_row<T, TOP, THREADS>(p, blockIdx.x, sh);
+  finish_row<T, TOP, THREADS, false>(p, blockIdx.x, sh, Scan{});
 }
 
 // `ALONE`: a row is one stretch, and the CTA that scans it finishes it too.
@@ -1028,12 +1034,19 @@ __global__ void __launch_bounds__(kThreads) scan_list_kernel(const Params p) {
   extern __shared__ __align__(16) float held[];
   launch_dependents();
   wait_previous();
-  const int row = blockIdx.x / p.segments;
-  scan_stretch<T>(p, row, blockIdx.x % p.segments, sh, held);
   if constexpr (ALONE) {
     __shared__ FinishShared rest;
+    const Scan scan = scan_stretch<T>(p, blockIdx.x, 0, rest.list, kListSlots, sh, held);
     __syncthreads();
-    finish_row<T, TOP, kThreads>(p, row, rest);
+    finish_row<T, TOP, kThreads, true>(p, blockIdx.x, rest, scan);
+  } else {
+    const int segment = blockIdx.x % p.segments;
+    const Scan scan = scan_stretch<T>(p, blockIdx.x / p.segments, segment, p.lists + static_cast<int64_t>(blockIdx.x) * p.cap,
+                                      p.cap, sh, held);
+    if (threadIdx.x == 0) {
+      p.part[blockIdx.x] = make_float4(scan.m, scan.sum, scan.bound, 0.f);
+      p.counts[blockIdx.x] = static_cast<int>(scan.listed);
+    }
   }
 }
 
@@ -1081,7 +1094,8 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
     const double share = static_cast<double>(p.first) / p.segments;
     p.rank = p.segments == 1 ? p.first : std::min(p.first, static_cast<int>(share + 4 * std::sqrt(share)) + 8);
     p.cap = std::min(p.per_segment, 2 * p.rank + 64);
-    auto space = scan_space(p, logits);
+    torch::Tensor space;
+    if (p.segments > 1) space = scan_space(p, logits);
     const size_t held = sizeof(float) * p.per_segment;
     auto scan = p.segments == 1 ? rows::scan_list_kernel<T, TOP, true> : rows::scan_list_kernel<T, TOP, false>;
     static DeviceFlags configured[2];
