@@ -22,7 +22,9 @@
 //              one cluster per row that agreed on m and on the bound, the same
 //              work waited in barriers most of the time (1024 rows of 128256,
 //              k = 64: 264 us), and with r = k its CTAs spent theirs on listing
-//              (172 us).
+//              (172 us).  A warp's stretches of 1024 in registers, without any
+//              barrier, are scanned in 106 us where these take 118, and cost
+//              finish more than that: it has eight times as many lists.
 //   scan_bins  all other draws.  A cluster of CTAs holds the row in shared
 //              memory and agrees on m; weights are added up, with top_p by
 //              distance from m as well, 16 bins per factor of two, and the tokens
@@ -373,20 +375,22 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
       if (is_token(mine[c]) && mine[c] >= bound) push(mine[c], col0 + c);
     }
   } else {
+    // (z - m) / tau as one operation; what rounds off m / tau is the same for all, and made good in the end
+    const float shift = -m * p.scale2, off = fmaf(m, p.scale2, shift);
     float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < n / 4; ++i) {
       const float4 q = quads[32 * i];
       const float z[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast((z[j] - m) * p.scale2);
+      for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast(fmaf(z[j], p.scale2, shift));
       if (fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= bound) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (is_token(z[j]) && z[j] >= bound) push(z[j], col0 + 4 * (32 * i + lane) + j);
       }
     }
-    sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    sum = ((s4[0] + s4[1]) + (s4[2] + s4[3])) * exp2f_fast(-off);
     if (!(sum == sum)) {  // NaN among them, which is no token
       sum = 0.f;
       for (int i = 0; i < n / 4; ++i) {
@@ -1090,9 +1094,10 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
   if (p.by_list) {
     p.segments = static_cast<int>(up(p.V, rows::kStretch));
     p.per_segment = static_cast<int>(up(up(p.V, p.segments), 4 * rows::kThreads) * 4 * rows::kThreads);
-    // a stretch's share and four standard deviations more, where the first tokens lie anywhere
+    // A stretch's share and three standard deviations and four more: where the first tokens lie anywhere, one row in
+    // two thousand has a stretch that is looked at again (k = 64).  Each token more costs every stretch a store.
     const double share = static_cast<double>(p.first) / p.segments;
-    p.rank = p.segments == 1 ? p.first : std::min(p.first, static_cast<int>(share + 4 * std::sqrt(share)) + 8);
+    p.rank = p.segments == 1 ? p.first : std::min(p.first, static_cast<int>(share + 3 * std::sqrt(share)) + 4);
     p.cap = std::min(p.per_segment, 2 * p.rank + 64);
     torch::Tensor space;
     if (p.segments > 1) space = scan_space(p, logits);
