@@ -431,7 +431,10 @@ __device__ __forceinline__ void tell_all(cg::cluster_group& cluster, V* slots, V
   sync_all(cluster);
 }
 
-template <typename T>
+// What a draw without top_k needs besides the sum of all weights.
+enum BinMode : int { kAll = 0, kMinP = 1, kTopP = 2 };
+
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params p) {
   __shared__ BinShared sh;
   extern __shared__ __align__(16) float held[];
@@ -439,11 +442,9 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / ctas;
-  // a warp has 32 n columns in a row: a thread every 32nd of them, v[32 i], or, where only sums count, four of every
-  // 128, quads[32 i]
+  // a warp has 32 n columns in a row, a thread four of every 128, quads[32 i]
   const int n = p.per_segment / kBinThreads;
-  const int warp_col0 = rank * p.per_segment + warp * 32 * n, col0 = warp_col0 + lane;
-  float* v = held + warp * 32 * n + lane;
+  const int warp_col0 = rank * p.per_segment + warp * 32 * n;
   const float4* quads = reinterpret_cast<const float4*>(held + warp * 32 * n) + lane;
   launch_dependents();
   wait_previous();
@@ -473,8 +474,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
     return;
   }
 
-  const bool by_bins = p.top_p < 1.0, by_min = !by_bins && p.log_min_p > -INFINITY;
-  u64 own = 0, kept = 0, before;
+  u64 own = 0, kept = 0, before;  // with top_p: what lies below all bins
 #pragma unroll 2
   for (int i = 0; i < n / 4; ++i) {
     const float4 q = quads[32 * i];
@@ -483,22 +483,27 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
     for (int j = 0; j < 4; ++j) {
       const double x = w.blunt_steps(z[j]);
       const u64 of = w.weight_at(x);
-      own += of;
-      if (by_bins) {
+      if (MODE == kTopP) {
         const int b = Weigher::bin_at(x);
         if (b < kWeightBins) add_to(sh.bins, b, of);
-      } else if (by_min && x >= p.log_min_p) {
-        kept += of;
+        else own += of;
+      } else {
+        own += of;
+        if (MODE == kMinP && x >= p.log_min_p) kept += of;
       }
     }
+  }
+  if (MODE == kTopP) {
+    __syncthreads();
+    own += bin_sum(sh.bins, tid);
   }
   const u64 of_cta = block_scan64<kBinThreads / 32>(own, before, sh.red);
   tell_all(cluster, sh.total_of, of_cta);
   u64 total = 0;
   for (int r = 0; r < ctas; ++r) total += sh.total_of[r];
-  if (!by_bins) {
-    kept = by_min ? block_scan64<kBinThreads / 32>(kept, before, sh.red) : of_cta;
-    if (tid == 0) p.weights[at] = kept;
+  if (MODE != kTopP) {
+    if (MODE == kMinP) kept = block_scan64<kBinThreads / 32>(kept, before, sh.red);
+    if (tid == 0) p.weights[at] = MODE == kMinP ? kept : of_cta;
     if (rank == 0 && tid == 0) p.states[row] = {m, -1, total, 0};
     return;
   }
@@ -520,16 +525,26 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   // the CTA's weight above that bin, and its tokens in it
   const u64 above = block_scan64<kBinThreads / 32>(tid < bin ? bin_sum(sh.bins, tid) : 0ull, before, sh.red);
   if (tid == 0) p.weights[at] = above;
+  auto column_of = [&](int k) { return 128 * (k / 4) + 4 * lane + k % 4; };  // of the warp's, the thread's k-th
+  auto mine_at = [&](int k) { return held[warp * 32 * n + column_of(k)]; };
   // between which the bin's logits lie
   const float least = __double2float_rd(w.m64 - kBinSteps * (bin + 1.0) / p.steps), most = __double2float_ru(w.m64 - (kBinSteps * bin - 1.0) / p.steps);
-  unsigned in_bin[kMostColumns / 32], mine = 0;
+  unsigned in_bin[kMostColumns / 32], mine = 0;  // bit 4 i + j: of the thread's i-th four the j-th
 #pragma unroll
   for (int b = 0; b < kMostColumns / 32; ++b) {
     in_bin[b] = 0;
-#pragma unroll 8
-    for (int i = 32 * b; i < min(n, 32 * b + 32); ++i) {
-      const float z = v[32 * i];
-      if (z >= least && z <= most && Weigher::bin_at(w.blunt_steps(z)) == bin) in_bin[b] |= 1u << (i - 32 * b);
+#pragma unroll 4
+    for (int i = 8 * b; i < min(n / 4, 8 * b + 8); ++i) {
+      const float4 q = quads[32 * i];
+      const float z[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (z[j] >= least && z[j] <= most) in_bin[b] |= 1u << (4 * (i - 8 * b) + j);
+    }
+    // few of these lie beyond the bin after all
+    for (unsigned left = in_bin[b]; left != 0; left &= left - 1) {
+      const int k = __ffs(left) - 1;
+      if (Weigher::bin_at(w.blunt_steps(mine_at(32 * b + k))) != bin) in_bin[b] &= ~(1u << k);
     }
     mine += __popc(in_bin[b]);
   }
@@ -540,8 +555,8 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
 #pragma unroll
   for (int b = 0; b < kMostColumns / 32; ++b) {
     for (; in_bin[b] != 0; in_bin[b] &= in_bin[b] - 1, ++to) {
-      const int i = 32 * b + __ffs(in_bin[b]) - 1;
-      if (to < p.cap) list[to] = place_of(v[32 * i], col0 + 32 * i);
+      const int k = 32 * b + __ffs(in_bin[b]) - 1;
+      if (to < p.cap) list[to] = place_of(mine_at(k), warp_col0 + column_of(k));
     }
   }
 }
@@ -1119,9 +1134,12 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
     p.per_segment = static_cast<int>(up(up(p.V, p.segments), 4 * rows::kBinThreads) * 4 * rows::kBinThreads);
     p.cap = rows::kBinCap;
     auto space = scan_space(p, logits);
-    auto scan = rows::scan_bins_kernel<T>;
-    static DeviceFlags configured;
-    if (bool& done = configured.here(); !done) {
+    const int mode = p.top_p < 1.0 ? rows::kTopP : std::isfinite(p.log_min_p) ? rows::kMinP : rows::kAll;
+    auto scan = mode == rows::kTopP  ? rows::scan_bins_kernel<T, rows::kTopP>
+                : mode == rows::kMinP ? rows::scan_bins_kernel<T, rows::kMinP>
+                                      : rows::scan_bins_kernel<T, rows::kAll>;
+    static DeviceFlags configured[3];
+    if (bool& done = configured[mode].here(); !done) {
       T1_CHECK_CUDA(cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          sizeof(float) * rows::kMostColumns * rows::kBinThreads));
       done = true;
