@@ -169,31 +169,27 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ u64 warp_scan64(u64 v, int lane) {
+template <int LANES = 32, typename V>
+__device__ __forceinline__ V warp_scan(V v, int lane) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+  for (int o = 1; o < LANES; o <<= 1) {
+    const V up = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += up;
   }
   return v;
 }
 // Sum of the threads' values; every thread gets it, and the sum of the threads
 // before it.
-template <int WARPS>
-__device__ __forceinline__ u64 block_scan64(u64 v, u64& before, u64* red) {
+template <int WARPS, typename V>
+__device__ __forceinline__ V block_scan(V v, V& before, V* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const u64 upto = warp_scan64(v, lane);
+  const V upto = warp_scan(v, lane);
   __syncthreads();
   if (lane == 31) red[warp] = upto;
   __syncthreads();
-  u64 sum = 0, of_warps = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w == warp) of_warps = sum;
-    sum += red[w];
-  }
-  before = of_warps + upto - v;
-  return sum;
+  const V of_warp = lane < WARPS ? red[lane] : V(0), of_warps = warp_scan<WARPS>(of_warp, lane);
+  before = __shfl_sync(0xffffffffu, of_warps - of_warp, warp) + upto - v;
+  return __shfl_sync(0xffffffffu, of_warps, WARPS - 1);
 }
 
 __device__ __forceinline__ float exp2f_fast(float x) {
@@ -408,8 +404,12 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
 // =============================================================== scan by bins
 struct BinShared {
   double exps[kExps];
-  unsigned bins[3][kWeightBins];
+  union {
+    unsigned bins[3][kWeightBins];
+    u64 sums[kWeightBins];  // then
+  };
   u64 red[kBinThreads / 32];
+  unsigned red32[kBinThreads / 32];
   float fred[32];
   // what every CTA of the cluster tells all others, once each
   float max_of[kMostCtas];
@@ -493,16 +493,20 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
       }
     }
   }
+  u64 my_bin = 0;
   if (MODE == kTopP) {
     __syncthreads();
-    own += bin_sum(sh.bins, tid);
+    my_bin = bin_sum(sh.bins, tid);
+    own += my_bin;
+    __syncthreads();
+    sh.sums[tid] = my_bin;
   }
-  const u64 of_cta = block_scan64<kBinThreads / 32>(own, before, sh.red);
+  const u64 of_cta = block_scan<kBinThreads / 32>(own, before, sh.red);
   tell_all(cluster, sh.total_of, of_cta);
   u64 total = 0;
   for (int r = 0; r < ctas; ++r) total += sh.total_of[r];
   if (MODE != kTopP) {
-    if (MODE == kMinP) kept = block_scan64<kBinThreads / 32>(kept, before, sh.red);
+    if (MODE == kMinP) kept = block_scan<kBinThreads / 32>(kept, before, sh.red);
     if (tid == 0) p.weights[at] = MODE == kMinP ? kept : of_cta;
     if (rank == 0 && tid == 0) p.states[row] = {m, -1, total, 0};
     return;
@@ -511,9 +515,9 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   // the bin in which top_p is reached, of all CTAs' weights
   const u64 need = share_of(p.top_p, total);
   u64 here = 0;
-  for (int r = 0; r < ctas; ++r) here += bin_sum(cluster.map_shared_rank(&sh, r)->bins, tid);
+  for (int r = 0; r < ctas; ++r) here += cluster.map_shared_rank(sh.sums, r)[tid];
   if (tid == 0) sh.bin = -1;
-  block_scan64<kBinThreads / 32>(here, before, sh.red);
+  block_scan<kBinThreads / 32>(here, before, sh.red);
   if (before < need && before + here >= need) {
     sh.bin = tid;
     sh.before64 = before;
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   if (rank == 0 && tid == 0) p.states[row] = {m, bin, total, need - (bin < 0 ? 0 : sh.before64)};
   if (bin < 0) return;
   // the CTA's weight above that bin, and its tokens in it
-  const u64 above = block_scan64<kBinThreads / 32>(tid < bin ? bin_sum(sh.bins, tid) : 0ull, before, sh.red);
+  const u64 above = block_scan<kBinThreads / 32>(tid < bin ? my_bin : 0ull, before, sh.red);
   if (tid == 0) p.weights[at] = above;
   auto column_of = [&](int k) { return 128 * (k / 4) + 4 * lane + k % 4; };  // of the warp's, the thread's k-th
   auto mine_at = [&](int k) { return held[warp * 32 * n + column_of(k)]; };
@@ -548,9 +552,9 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
     }
     mine += __popc(in_bin[b]);
   }
-  const unsigned listed = static_cast<unsigned>(block_scan64<kBinThreads / 32>(mine, before, sh.red));
+  unsigned to;
+  const unsigned listed = block_scan<kBinThreads / 32>(mine, to, sh.red32);
   if (tid == 0) p.counts[at] = static_cast<int>(min(listed, p.cap + 1u));
-  unsigned to = static_cast<unsigned>(before);
   u64* list = p.lists + at * p.cap;
 #pragma unroll
   for (int b = 0; b < kMostColumns / 32; ++b) {
@@ -695,7 +699,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   auto reach = [&](u64 here, u64 need) {
     u64 before;
     if (tid == 0) sh.bin = -1;
-    block_scan64<kWarps>(here, before, sh.red);
+    block_scan<kWarps>(here, before, sh.red);
     if (before < need && before + here >= need) {
       sh.bin = tid;
       sh.before64 = before;
@@ -773,7 +777,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
           of[j] = e[j] != 0 ? w.weight_at(x[j]) : 0ull;
           own += of[j];
         }
-        const u64 need = share_of(p.top_p, block_scan64<kWarps>(own, before, sh.red));
+        const u64 need = share_of(p.top_p, block_scan<kWarps>(own, before, sh.red));
         unsigned kept = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
@@ -784,7 +788,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
           // by index, the lowest first: the complement of the column, then the logit's key
           if (i < have) sh.list[i] = in ? e[j] << 32 | e[j] >> 32 : 0ull;
         }
-        kept = static_cast<unsigned>(block_scan64<kWarps>(kept, before, sh.red));
+        kept = static_cast<unsigned>(block_scan<kWarps>(static_cast<u64>(kept), before, sh.red));
         order_list<THREADS>(sh.list, kept);  // the tokens kept are a prefix of the list
         own = 0;
 #pragma unroll
@@ -794,7 +798,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
           of[j] = e[j] != 0 ? w.weight(logit_of(static_cast<unsigned>(e[j]))) : 0ull;
           own += of[j];
         }
-        const u64 target = target_of(p.u[row], block_scan64<kWarps>(own, before, sh.red));
+        const u64 target = target_of(p.u[row], block_scan<kWarps>(own, before, sh.red));
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
           if (before <= target && target < before + of[j]) {
@@ -851,7 +855,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
       __syncwarp();
     }
     const u64 of_warp = warp_sum64(own);
-    const u64 all = block_scan64<kWarps>(own, before, sh.red);
+    const u64 all = block_scan<kWarps>(own, before, sh.red);
     before = __shfl_sync(0xffffffffu, before, 0);
     if (!have_target) target = target_of(p.u[row], all);
     if (target < before || target >= before + of_warp) return;
@@ -860,7 +864,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
       const int n = batch(c, c1, [&](int i, float z, int column) { sh.list[i] = place_of(z, column); });
       for (int i = lane; i - lane < n; i += 32) {
         const u64 e = i < n ? sh.list[i] : 0ull;
-        const u64 upto = before + warp_scan64(i < n ? w.weight(logit_at(e)) : 0ull, lane);
+        const u64 upto = before + warp_scan(i < n ? w.weight(logit_at(e)) : 0ull, lane);
         const unsigned past = __ballot_sync(0xffffffffu, target < upto);
         if (past != 0) {
           if (lane == __ffs(past) - 1) {
@@ -910,7 +914,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
           const unsigned i = kPer * tid + j;
           own += i < few ? w.weight(logit_at(sh.list[i])) : 0ull;
         }
-        block_scan64<kWarps>(own, before, sh.red);
+        block_scan<kWarps>(own, before, sh.red);
         if (before < need && before + own >= need) {
           for (unsigned i = kPer * tid; before < need; ++i) {
             before += w.weight(logit_at(sh.list[i]));
@@ -959,7 +963,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     unsigned here = 0;
     each_column(0, p.V, [&](float q, int) { here += __popc(__ballot_sync(0xffffffffu, q == z)); });
     u64 before;
-    block_scan64<kWarps>(lane == 0 ? here : 0u, before, sh.red);
+    block_scan<kWarps>(static_cast<u64>(lane == 0 ? here : 0u), before, sh.red);
     unsigned tie = __shfl_sync(0xffffffffu, static_cast<unsigned>(before), 0);
     each_column(0, p.V, [&](float q, int c) {
       const unsigned all = __ballot_sync(0xffffffffu, q == z);
@@ -973,13 +977,13 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   if (!TOP && !p.by_list && w.sharp) {
     u64 before, own = 0;
     each_column(0, p.V, [&](float z, int) { own += z == m; });
-    log_sum = logf(static_cast<float>(block_scan64<kWarps>(own, before, sh.red)));
+    log_sum = logf(static_cast<float>(block_scan<kWarps>(own, before, sh.red)));
   }
   unsigned have = 0;
   if (first != 0) {
     u64 before, count = 0;
     each_column(0, p.V, [&](float z, int) { count += is_token(z); });
-    const unsigned tokens = static_cast<unsigned>(block_scan64<kWarps>(count, before, sh.red));
+    const unsigned tokens = static_cast<unsigned>(block_scan<kWarps>(count, before, sh.red));
     have = min(first, tokens);
     if (first < tokens) {
       unsigned need = first, prefix = 0, mask = 0;
@@ -1015,7 +1019,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     each_column(0, p.V, [&](float z, int c) {
       if (in_cut(z, c)) own += w.weight(z);
     });
-    u64 need = share_of(p.top_p, block_scan64<kWarps>(own, before, sh.red));
+    u64 need = share_of(p.top_p, block_scan<kWarps>(own, before, sh.red));
     unsigned prefix = 0, mask = 0;
     for (int shift = 24; shift >= kLowest; shift -= 8) {
       if (tid < kDigits) sh.weights[tid] = 0;
