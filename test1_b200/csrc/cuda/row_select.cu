@@ -116,39 +116,35 @@ struct Params {
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-// Logits from..from + n to shared memory as fp32, by one warp.
-__device__ __forceinline__ void fetch(float* to, const float* from, int n, bool aligned, int lane) {
-  if (aligned) {
-    const int vecs = n / 4;
-    for (int i = lane; i < vecs; i += 32)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(to + 4 * i)), "l"(from + 4 * i) : "memory");
-    to += 4 * vecs;
-    from += 4 * vecs;
-    n -= 4 * vecs;
-  }
-  for (int i = lane; i < n; i += 32)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(to + i)), "l"(from + i) : "memory");
-}
 __device__ __forceinline__ float logit(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float logit(const bf16_t* p) {
   return __bfloat162float(__ushort_as_bfloat16(__ldg(reinterpret_cast<const unsigned short*>(p))));
 }
-__device__ __forceinline__ void fetch(float* to, const bf16_t* from, int n, bool aligned, int lane) {
-  if (aligned) {
-    const int vecs = n / 8;
-#pragma unroll 4
-    for (int i = lane; i < vecs; i += 32) {
-      float f[8];
-      load8(from + 8 * i, f);
-      reinterpret_cast<float4*>(to)[2 * i] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(to)[2 * i + 1] = make_float4(f[4], f[5], f[6], f[7]);
-    }
-    to += 8 * vecs;
-    from += 8 * vecs;
-    n -= 8 * vecs;
-  }
+__device__ __forceinline__ float held_logit(const float* p) { return *p; }
+__device__ __forceinline__ float held_logit(const bf16_t* p) { return __bfloat162float(*p); }
+// Four neighbours in shared memory.
+__device__ __forceinline__ float4 held_quad(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 held_quad(const bf16_t* p) {
+  const uint2 q = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16),
+                     __uint_as_float(q.y & 0xffff0000u));
+}
+
+// A warp's `cols` logits from `from` on to shared memory, and -inf up to `all`.
+template <typename T>
+__device__ __forceinline__ void fetch(T* to, const T* from, int cols, int all, bool aligned, int lane) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int vecs = aligned ? cols / kVec : 0;
+  for (int i = lane; i < vecs; i += 32)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(to + kVec * i)), "l"(from + kVec * i) : "memory");
 #pragma unroll 8
-  for (int i = lane; i < n; i += 32) to[i] = logit(from + i);
+  for (int c = vecs * kVec + lane; c < cols; c += 32) {
+    if (sizeof(T) == 4)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(to + c)), "l"(from + c) : "memory");
+    else
+      to[c] = from[c];
+  }
+  for (int c = cols + lane; c < all; c += 32) to[c] = static_cast<T>(-INFINITY);
 }
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -307,16 +303,14 @@ struct Scan {
 };
 
 template <typename T>
-__device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segment, u64* list, unsigned cap, ListShared& sh, float* held) {
+__device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segment, u64* list, unsigned cap, ListShared& sh, T* held) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // a warp has 32 n columns in a row, a thread four of every 128, quads[32 i]
+  // a warp has 32 n columns in a row, a thread four of every 128
   const int n = p.per_segment / kThreads;
   const int col0 = segment * p.per_segment + warp * 32 * n;
-  float* mine = held + warp * 32 * n;
-  const float4* quads = reinterpret_cast<const float4*>(mine) + lane;
-  const int cols = max(0, min(32 * n, p.V - col0));
-  fetch(mine, static_cast<const T*>(p.logits) + row * p.ld + col0, cols, p.aligned, lane);
-  for (int c = cols + lane; c < 32 * n; c += 32) mine[c] = -INFINITY;
+  T* mine = held + warp * 32 * n;
+  auto quad = [&](int i) { return held_quad(mine + 4 * (32 * i + lane)); };
+  fetch(mine, static_cast<const T*>(p.logits) + row * p.ld + col0, max(0, min(32 * n, p.V - col0)), 32 * n, p.aligned, lane);
   sh.bins[tid] = 0;
   if (tid == 0) sh.listed = 0;
   fetched();
@@ -325,7 +319,7 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
   float part[kParts] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 8
   for (int i = 0; i < n / 4; ++i) {
-    const float4 q = quads[32 * i];
+    const float4 q = quad(i);
     part[0] = fmaxf(part[0], q.x);
     part[1] = fmaxf(part[1], q.y);
     part[2] = fmaxf(part[2], q.z);
@@ -372,8 +366,9 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
   float sum = 0.f;
   if (is_sharp(m, p.tau)) {
     for (int c = lane; c < 32 * n; c += 32) {
-      sum += mine[c] == m;
-      if (is_token(mine[c]) && mine[c] >= bound) push(mine[c], col0 + c);
+      const float z = held_logit(mine + c);
+      sum += z == m;
+      if (is_token(z) && z >= bound) push(z, col0 + c);
     }
   } else {
     // (z - m) / tau as one operation; what rounds off m / tau is the same for all, and made good in the end
@@ -381,7 +376,7 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
     float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < n / 4; ++i) {
-      const float4 q = quads[32 * i];
+      const float4 q = quad(i);
       const float z[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) s4[j] += exp2f_fast(fmaf(z[j], p.scale2, shift));
@@ -395,7 +390,7 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
     if (!(sum == sum)) {  // NaN among them, which is no token
       sum = 0.f;
       for (int i = 0; i < n / 4; ++i) {
-        const float4 q = quads[32 * i];
+        const float4 q = quad(i);
         const float z[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum += z[j] == z[j] ? exp2f_fast((z[j] - m) * p.scale2) : 0.f;
@@ -442,22 +437,19 @@ enum BinMode : int { kAll = 0, kMinP = 1, kTopP = 2 };
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params p) {
   __shared__ BinShared sh;
-  extern __shared__ __align__(16) float held[];
+  extern __shared__ __align__(16) uint8_t held_raw[];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / ctas;
-  // a warp has 32 n columns in a row, a thread four of every 128, quads[32 i]
+  // a warp has 32 n columns in a row, a thread four of every 128
   const int n = p.per_segment / kBinThreads;
   const int warp_col0 = rank * p.per_segment + warp * 32 * n;
-  const float4* quads = reinterpret_cast<const float4*>(held + warp * 32 * n) + lane;
+  T* mine = reinterpret_cast<T*>(held_raw) + warp * 32 * n;
+  auto quad = [&](int i) { return held_quad(mine + 4 * (32 * i + lane)); };
   launch_dependents();
   wait_previous();
-  {
-    const int cols = max(0, min(32 * n, p.V - warp_col0));
-    fetch(held + warp * 32 * n, static_cast<const T*>(p.logits) + row * p.ld + warp_col0, cols, p.aligned, lane);
-    for (int c = cols + lane; c < 32 * n; c += 32) held[warp * 32 * n + c] = -INFINITY;
-  }
+  fetch(mine, static_cast<const T*>(p.logits) + row * p.ld + warp_col0, max(0, min(32 * n, p.V - warp_col0)), 32 * n, p.aligned, lane);
   for (int i = tid; i < 3 * kWeightBins; i += kBinThreads) sh.bins[0][i] = 0;
   fill_exps(sh.exps);
   fetched();
@@ -465,7 +457,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   float m = -INFINITY;
 #pragma unroll 4
   for (int i = 0; i < n / 4; ++i) {
-    const float4 q = quads[32 * i];
+    const float4 q = quad(i);
     m = fmaxf(fmaxf(m, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
   }
   m = block_max(m, sh.fred);
@@ -482,7 +474,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   u64 own = 0, kept = 0, before;  // with top_p: what lies below all bins
 #pragma unroll 2
   for (int i = 0; i < n / 4; ++i) {
-    const float4 q = quads[32 * i];
+    const float4 q = quad(i);
     const float z[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -535,16 +527,16 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   const u64 above = block_scan<kBinThreads / 32>(tid < bin ? my_bin : 0ull, before, sh.red);
   if (tid == 0) p.weights[at] = above;
   auto column_of = [&](int k) { return 128 * (k / 4) + 4 * lane + k % 4; };  // of the warp's, the thread's k-th
-  auto mine_at = [&](int k) { return held[warp * 32 * n + column_of(k)]; };
+  auto mine_at = [&](int k) { return held_logit(mine + column_of(k)); };
   // between which the bin's logits lie
   const float least = __double2float_rd(w.m64 - kBinSteps * (bin + 1.0) / p.steps), most = __double2float_ru(w.m64 - (kBinSteps * bin - 1.0) / p.steps);
-  unsigned in_bin[kMostColumns / 32], mine = 0;  // bit 4 i + j: of the thread's i-th four the j-th
+  unsigned in_bin[kMostColumns / 32], count = 0;  // bit 4 i + j: of the thread's i-th four the j-th
 #pragma unroll
   for (int b = 0; b < kMostColumns / 32; ++b) {
     in_bin[b] = 0;
 #pragma unroll 4
     for (int i = 8 * b; i < min(n / 4, 8 * b + 8); ++i) {
-      const float4 q = quads[32 * i];
+      const float4 q = quad(i);
       const float z[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -555,10 +547,10 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
       const int k = __ffs(left) - 1;
       if (Weigher::bin_at(w.blunt_steps(mine_at(32 * b + k))) != bin) in_bin[b] &= ~(1u << k);
     }
-    mine += __popc(in_bin[b]);
+    count += __popc(in_bin[b]);
   }
   unsigned to;
-  const unsigned listed = block_scan<kBinThreads / 32>(mine, to, sh.red32);
+  const unsigned listed = block_scan<kBinThreads / 32>(count, to, sh.red32);
   if (tid == 0) p.counts[at] = static_cast<int>(min(listed, p.cap + 1u));
   u64* list = p.lists + at * p.cap;
 #pragma unroll
@@ -1059,7 +1051,8 @@ __global__ void __launch_bounds__(THREADS) finish_kernel(const Params p) {
 template <typename T, bool TOP, bool ALONE>
 __global__ void __launch_bounds__(kThreads) scan_list_kernel(const Params p) {
   __shared__ ListShared sh;
-  extern __shared__ __align__(16) float held[];
+  extern __shared__ __align__(16) uint8_t held_raw[];
+  T* held = reinterpret_cast<T*>(held_raw);
   launch_dependents();
   wait_previous();
   if constexpr (ALONE) {
@@ -1125,11 +1118,11 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
     p.cap = std::min(p.per_segment, 2 * p.rank + 64);
     torch::Tensor space;
     if (p.segments > 1) space = scan_space(p, logits);
-    const size_t held = sizeof(float) * p.per_segment;
+    const size_t held = sizeof(T) * p.per_segment;
     auto scan = p.segments == 1 ? rows::scan_list_kernel<T, TOP, true> : rows::scan_list_kernel<T, TOP, false>;
     static DeviceFlags configured[2];
     if (bool& done = configured[p.segments == 1].here(); !done) {
-      T1_CHECK_CUDA(cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(float) * rows::kStretch));
+      T1_CHECK_CUDA(cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(T) * rows::kStretch));
       done = true;
     }
     launch_after(what, scan, dim3(static_cast<unsigned>(p.rows) * p.segments), rows::kThreads, held, p);
@@ -1154,13 +1147,13 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
     static DeviceFlags configured[3];
     if (bool& done = configured[mode].here(); !done) {
       T1_CHECK_CUDA(cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         sizeof(float) * rows::kMostColumns * rows::kBinThreads));
+                                         sizeof(T) * rows::kMostColumns * rows::kBinThreads));
       done = true;
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * p.segments);
     cfg.blockDim = dim3(rows::kBinThreads);
-    cfg.dynamicSmemBytes = sizeof(float) * p.per_segment;
+    cfg.dynamicSmemBytes = sizeof(T) * p.per_segment;
     cfg.stream = stream();
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
