@@ -1172,8 +1172,8 @@ static void launch_rows(rows::Params& p, const torch::Tensor& logits) {
 
 template <bool TOP>
 static void run_rows(rows::Params& p, const torch::Tensor& logits, double temperature) {
-  TORCH_CHECK(logits.size(1) <= kMostVocab, "at most ", kMostVocab, " tokens, got ", logits.size(1));
-  TORCH_CHECK(logits.size(0) < (1ll << 24), "at most 2^24 rows, got ", logits.size(0));
+  TORCH_CHECK(logits.size(1) <= kMostVocab, "at most ", std::to_string(kMostVocab), " tokens, got ", std::to_string(logits.size(1)));
+  TORCH_CHECK(logits.size(0) < (1ll << 24), "at most 2^24 rows, got ", std::to_string(logits.size(0)));
   p.logits = logits.data_ptr();
   p.ld = logits.size(0) > 1 ? logits.stride(0) : 0;
   p.rows = static_cast<int>(logits.size(0));
@@ -1192,7 +1192,7 @@ static void run_rows(rows::Params& p, const torch::Tensor& logits, double temper
 std::vector<torch::Tensor> topk_logprobs(torch::Tensor logits, int64_t k, double temperature) {
   check_rows(logits, temperature);
   TORCH_CHECK(k >= 1 && k <= std::min<int64_t>(rows::kMostList, logits.size(1)), "k must lie in [1, min(V, ",
-              rows::kMostList, ")], got ", k);
+              std::to_string(rows::kMostList), ")], got ", std::to_string(k));
   const c10::cuda::CUDAGuard guard(logits.device());
   auto logp = torch::empty({logits.size(0), k}, logits.options().dtype(torch::kFloat32));
   auto ids = torch::empty({logits.size(0), k}, logits.options().dtype(torch::kInt64));
