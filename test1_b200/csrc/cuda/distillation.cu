@@ -31,7 +31,7 @@
 // one cluster of 8 CTAs has in one round waits for the others' counts and then
 // writes; a larger one is scaled by a second launch, out of L2.
 #include "arrivals.cuh"
-#include "common.cuh"
+#include "programmatic.cuh"
 
 #include <cooperative_groups.h>
 
@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
   constexpr int kRows = 32 / G;   // of a warp
   constexpr int kStep = VEC ? 4 : 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, of_row = lane % G;
+  if (ONE) tell_started();
   // entry j of the lane
   auto entry = [&](int j) { return VEC ? 4 * of_row + 4 * G * (j / 4) + j % 4 : of_row + G * j; };
   const int64_t t_step = static_cast<int64_t>(gridDim.x) * kWarps * kRows;
@@ -308,6 +309,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
   if (ONE) {
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned ctas = cluster.num_blocks();
+    wait_started();
     if (threadIdx.x < ctas) {
       cluster.map_shared_rank(of_cta, threadIdx.x)[cluster.block_rank()] = sum;
       cluster.map_shared_rank(live_of_cta, threadIdx.x)[cluster.block_rank()] = rows;

@@ -10,6 +10,11 @@ namespace t1 {
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// A CTA's shared memory is open to its cluster once the CTA has started: each
+// says so at its start, and waits for the others before the first access.
+__device__ __forceinline__ void tell_started() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void wait_started() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 // Every kernel launched so waits for the previous one before it touches memory.
 template <class... P, class... A>
 inline void launch_after(const char* what, void (*kern)(P...), dim3 grid, int threads, size_t smem, const A&... args) {

@@ -447,6 +447,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   const int warp_col0 = rank * p.per_segment + warp * 32 * n;
   T* mine = reinterpret_cast<T*>(held_raw) + warp * 32 * n;
   auto quad = [&](int i) { return held_quad(mine + 4 * (32 * i + lane)); };
+  if (ctas > 1) tell_started();
   launch_dependents();
   wait_previous();
   fetch(mine, static_cast<const T*>(p.logits) + row * p.ld + warp_col0, max(0, min(32 * n, p.V - warp_col0)), 32 * n, p.aligned, lane);
@@ -461,6 +462,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
     m = fmaxf(fmaxf(m, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
   }
   m = block_max(m, sh.fred);
+  if (ctas > 1) wait_started();
   tell_all(cluster, sh.max_of, m);
   for (int r = 0; r < ctas; ++r) m = fmaxf(m, sh.max_of[r]);
   const int64_t at = static_cast<int64_t>(row) * p.segments + rank;
