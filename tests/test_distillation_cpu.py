@@ -132,8 +132,11 @@ def test_refusals():
             ops.topk_logprobs(z, k)
     with pytest.raises(ValueError):
         ops.topk_logprobs(torch.zeros(2, 600), 513)
-    with pytest.raises(ValueError):
-        ops.topk_logprobs(z, 2, temperature=-1.0)
+    for tau in (-1.0, 1e30):  # 400 tau added to a logit has to stay finite
+        with pytest.raises(ValueError):
+            ops.topk_logprobs(z, 2, temperature=tau)
+        with pytest.raises(ValueError):
+            ops.sample_tokens(z, u, tau)
     ids = torch.zeros(2, 3, dtype=torch.int64)
     for bad in ((z, z[0], ids), (z, z, ids[:1]), (z, z, ids[:, :0]), (z, z, torch.zeros(2, 513, dtype=torch.int64))):
         with pytest.raises(ValueError):

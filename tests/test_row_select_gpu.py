@@ -133,6 +133,27 @@ def test_temperatures(tau, cuda_device):
     _check_logp(logp, want)
 
 
+@pytest.mark.parametrize("tau", [1e-37, 1e-6, 2.0 ** 64])
+def test_temperatures_and_logits_at_their_ends(tau, cuda_device):
+    """Rows of the type's lowest and largest values, alone and among others, and
+    numbers u outside [0, 1), which count as its ends (NaN as 0)."""
+    from test1_b200 import ops
+
+    z, _ = _logits(6, 4001, "plain", torch.float32, seed=8)
+    least, most = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
+    z[1], z[2], z[3, ::2], z[4, 7] = least, most, least, -INF
+    u = torch.tensor([1.0, float("nan"), -3.0, INF, -INF, 0.5], device="cuda")
+    for top_k, top_p, min_p in [(0, 1.0, 0.0), (7, 1.0, 0.0), (0, 0.5, 0.0), (0, 1.0, 0.3), (2000, 0.7, 0.1)]:
+        token, logp = ops.sample_tokens(z, u, tau, top_k, top_p, min_p)
+        at, want = oracle.sample(z, u, tau, top_k, top_p, min_p)
+        assert torch.equal(token.cpu(), at)
+        _check_logp(logp, want)
+    logp, ids = ops.topk_logprobs(z, 9, tau)
+    want, at = oracle.topk(z, 9, tau)
+    assert torch.equal(ids.cpu(), at)
+    _check_logp(logp, torch.where(want < least, -INF, want))  # fp32 has no such numbers
+
+
 def test_rows_apart_and_unaligned(cuda_device):
     from test1_b200 import ops
 
@@ -225,3 +246,5 @@ def test_refusals(cuda_device):
         native.topk_logprobs(z, 9)
     with pytest.raises(RuntimeError, match="top_p"):
         native.sample_tokens(z, z[:, 0].contiguous(), top_p=0.0)
+    with pytest.raises(RuntimeError, match="temperature"):
+        native.topk_logprobs(z, 2, 1e30)
