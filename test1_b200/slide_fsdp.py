@@ -929,7 +929,9 @@ class SlideFSDP(nn.Module):
         cache of keys and values: the pass streams every layer's weights from
         host memory, which for the Llama-3.1-8B architecture takes as long as
         the arithmetic of about 25 thousand tokens.  On several ranks every rank
-        generates its own batch, in as many passes as the longest."""
+        generates its own batch, in as many passes as the longest; passes are
+        collective, so ``max_new_tokens`` has to be the same on all, and
+        ``eos_token_id`` given on all or none."""
         self._check_ids(input_ids, None)
         ops.check_sampling(temperature, top_k, top_p, min_p)
         if input_ids.dim() != 2 or not input_ids.numel():
@@ -941,6 +943,12 @@ class SlideFSDP(nn.Module):
         lengths = torch.full((B,), S) if lengths is None else lengths.to("cpu", torch.int64)
         if lengths.shape != (B,) or int(lengths.min()) < 1 or int(lengths.max()) > S:
             raise ValueError(f"lengths must be [{B}] of 1 to {S} tokens")
+        if self.world_size > 1:
+            mine = torch.tensor([max_new_tokens, int(eos_token_id is None)], device=dev)
+            most = torch.cat([mine, -mine])
+            dist.all_reduce(most, op=dist.ReduceOp.MAX)
+            if not torch.equal(most[:2], -most[2:]):
+                raise ValueError("max_new_tokens must be the same on all ranks, eos_token_id given on all or none")
         longest, length = int(lengths.max()), lengths.to(dev)
         # the attention kernels take whole tiles; what lies behind a sequence's last token does not reach it
         tile = 256 if self.is_cuda else 1

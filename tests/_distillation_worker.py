@@ -38,6 +38,12 @@ def run(rank, world, port, mode, grad, eos, out_path):
         eng = SlideFSDP(LlamaForCausalLM(cfg), SlideFSDPConfig(dtype=torch.float32, device="cpu", lr=1e-3, weight_decay=0.01,
                                                                param_transfer_mode=mode, grad_sync_mode=grad))
         answers = eng.generate(prompts(cfg, rank), NEW, top_k=1, eos_token_id=eos)
+        refused = 0
+        for new, end in [(NEW + rank, eos), (NEW, eos if rank else None)]:
+            try:
+                eng.generate(prompts(cfg, rank), new, top_k=1, eos_token_id=end)
+            except ValueError:
+                refused += 1
         top = eng.top_logprobs(answers.input_ids, K)
         logps, ids = lists(cfg, rank, answers.input_ids.shape)
         losses = []
@@ -47,7 +53,7 @@ def run(rank, world, port, mode, grad, eos, out_path):
             losses.append(float(out.loss))
         eng.wait_for_updates()
         dist.barrier()
-        res = {"losses": losses, "answers": vars(answers), "top": top}
+        res = {"losses": losses, "answers": vars(answers), "top": top, "refused": refused}
         if rank == 0:
             res["master"] = {n: t.clone() for n, t in eng.named_master_tensors()}
         torch.save(res, out_path + f".{rank}")

@@ -50,6 +50,7 @@ def test_two_ranks(tmp_path, mode, grad):
     res = [torch.load(out + f".{r}") for r in range(world)]
     opt = torch.optim.AdamW(hf.parameters(), lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01)
     for r in range(world):
+        assert res[r]["refused"] == 2  # answers of other lengths than the other rank's
         a = res[r]["answers"]
         for b in range(2):
             answer = free[r][b, 7:].tolist()
