@@ -268,6 +268,26 @@ def test_two_streams_and_two_graphs_at_once(cuda_device):
         assert all(torch.equal(a, b) for (_, o), w in zip(graphs, want) for a, b in zip(o, w))
 
 
+def test_more_than_32_bits_of_logits(cuda_device):
+    """The rows behind 2^31 logits are what they are by themselves."""
+    from test1_b200 import ops
+
+    T, H, V = 17000, 64, 128257
+    x, w, _, _ = _inputs(T, H, V, 1, seed=11, masked=False)
+    u = torch.rand(T, device="cuda", generator=torch.Generator(device="cuda").manual_seed(11))
+    logits = ops.linear_logits(x, w)
+    assert logits.stride(0) * (T - 1) > 2 ** 31
+    last = slice(T - 200, T)
+    assert torch.equal(logits[last], ops.linear_logits(x[last], w))
+    alone = logits[last].clone()
+    for z, part in ((logits, alone), (logits.bfloat16(), alone.bfloat16())):
+        for all_rows, few in ((ops.topk_logprobs(z, 8), ops.topk_logprobs(part, 8)),
+                              (ops.sample_tokens(z, u, top_k=8), ops.sample_tokens(part, u[last], top_k=8)),
+                              (ops.sample_tokens(z, u, top_p=0.9), ops.sample_tokens(part, u[last], top_p=0.9)),
+                              (ops.sample_tokens(z, u, top_k=1500), ops.sample_tokens(part, u[last], top_k=1500))):
+            assert all(torch.equal(a[last], b) for a, b in zip(all_rows, few))
+
+
 def test_refusals(cuda_device):
     from test1_b200 import ops
 
