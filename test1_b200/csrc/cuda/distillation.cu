@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
   // exp(v) for v <= about 1
   auto exp64 = [&](float at) {
     constexpr float kRound = 12582912.f;  // 1.5 2^23: adding it leaves a whole number in the low bits
-    const float v = fmaxf(at, -600.f);
+    const float v = at < -600.f ? -600.f : at;  // NaN stays
     const float y = fmaf(v, 1.4426950408889634f * kExps, kRound);
     const int j = __float_as_int(y) - 0x4b400000;
     const float n = y - kRound;
@@ -215,16 +215,16 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
     if (!ONE) load();
     const int64_t t = t0 + lane / G;
     float a[PER], b[PER];
-    bool any = false;
+    unsigned kept = 0;  // bit j: entry j
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const bool keep = in_id[j] >= 0 && in_b[j] > -INFINITY;
       a[j] = keep ? in_a[j] : kNothing;
       b[j] = keep ? in_b[j] : kNothing;
-      any = any || keep;
+      kept |= static_cast<unsigned>(keep) << j;
     }
     t0 += t_step;
-    const unsigned lanes = __ballot_sync(0xffffffffu, any);
+    const unsigned lanes = __ballot_sync(0xffffffffu, kept != 0);
     const bool live = (G == 32 ? lanes : (lanes >> (lane & ~(G - 1))) & ((1u << (G & 31)) - 1)) != 0;
     float pk[PER], qk[PER];
     float loss = 0.f, rest = 0.f;  // rest: f'(p_r), without a tail sum p f'
@@ -241,10 +241,11 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
       }
       ps = 1.0 - lanes_sum<G>(ps);
       qs = 1.0 - lanes_sum<G>(qs);
-      const float pr = fmaxf(static_cast<float>(ps), kFloor), qr = fmaxf(static_cast<float>(qs), kFloor);
+      // a student's NaN is above no floor and below none
+      const float pr = ps <= kFloor ? kFloor : static_cast<float>(ps), qr = fmaxf(static_cast<float>(qs), kFloor);
       float fr, gr;
       divergence(p.kind, pr, qr, logf(__fdividef(qr, pr)), fr, gr);
-      rest = ps > kFloor ? __fdividef(gr, pr) : 0.f;
+      rest = ps <= kFloor ? 0.f : __fdividef(gr, pr);
       if (of_row == 0) loss = fr;
     } else {
       // scaled to sum to 1
@@ -276,16 +277,16 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      float f;
-      // of a student's -inf as much as there is
-      divergence(p.kind, pk[j], qk[j], fminf((b[j] - a[j]) - shift, 3e38f), f, g[j]);
+      float f, d = (b[j] - a[j]) - shift;
+      if (d > 3e38f) d = 3e38f;  // of a student's -inf as much as there is
+      divergence(p.kind, pk[j], qk[j], d, f, g[j]);
       loss += f;
       if (!TAIL) rest += g[j];
     }
     loss = lanes_sum<G>(loss);
     if (!TAIL) rest = lanes_sum<G>(rest);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) g[j] = fmaf(-pk[j], rest, g[j]);
+    for (int j = 0; j < PER; ++j) g[j] = kept >> j & 1 ? fmaf(-pk[j], rest, g[j]) : 0.f;
     if (of_row == 0) {
       if (t < p.T && !T1_OOB(t, p.T)) p.each[t] = loss;
       sum += loss;
