@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
       else p.dlogp[row + k] = g[j] * scale;
     }
   };
-  // An entry left out has the logarithm of no probability at all, in both, and so no part in anything below.
+  // An entry left out has the logarithm of no probability at all, in both, and so no part in the sums of a tail.  Without
+  // one only differences of logarithms count, which may all lie below this, and `kept` says what takes part.
   constexpr float kNothing = -1e4f;
   while (t0 < p.T) {
     if (!ONE) load();
@@ -249,24 +250,26 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
       if (of_row == 0) loss = fr;
     } else {
       // scaled to sum to 1
-      float am = a[0], bm = b[0], as = 0.f, bs = 0.f;
+      float am = -INFINITY, bm = -INFINITY, as = 0.f, bs = 0.f;
 #pragma unroll
-      for (int j = 1; j < PER; ++j) {
-        am = fmaxf(am, a[j]);
-        bm = fmaxf(bm, b[j]);
+      for (int j = 0; j < PER; ++j) {
+        const bool in = kept >> j & 1;
+        am = fmaxf(am, in ? a[j] : -INFINITY);
+        bm = fmaxf(bm, in ? b[j] : -INFINITY);
       }
       am = lanes_max<G>(am);
       bm = lanes_max<G>(bm);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        pk[j] = expf(a[j] - am);
-        qk[j] = expf(b[j] - bm);
+        const bool in = kept >> j & 1;
+        pk[j] = in ? expf(a[j] - am) : 0.f;
+        qk[j] = in ? expf(b[j] - bm) : 0.f;
         as += pk[j];
         bs += qk[j];
       }
       as = lanes_sum<G>(as);
       bs = lanes_sum<G>(bs);
-      shift = (bm - am) + logf(bs / as);
+      shift = live ? (bm - am) + logf(bs / as) : 0.f;
       as = live ? 1.f / as : 0.f;
       bs = live ? 1.f / bs : 0.f;
 #pragma unroll

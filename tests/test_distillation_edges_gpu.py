@@ -1,12 +1,15 @@
 """The distillation loss kernels at inputs that the other tests leave out: NaN
-in a student's log-probabilities."""
+in a student's log-probabilities, log-probabilities far below -1e4."""
 import math
 
 import pytest
 import torch
 
+import _lists_oracle as oracle
+
 pytestmark = pytest.mark.gpu
 KINDS = ["forward", "reverse", "jensen"]
+EPS = 2.0 ** -24
 
 
 def _lists(T, K, seed=0):
@@ -60,3 +63,31 @@ def test_nan_goes_on_to_the_output_layer(kind, cuda_device):
         assert bool(torch.isnan(logp[T // 2]).all()) and bool(torch.isnan(dlogp[T // 2]).all())
         assert math.isnan(float(loss))
         assert bool(torch.isnan(dx[T // 2]).all()) and bool(torch.isnan(dw).any())
+
+
+@pytest.mark.parametrize("T,K", [(2, 1), (3, 5), (4, 8), (6, 33), (5, 65), (1000, 5)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_far_below_without_a_tail(T, K, kind, cuda_device):
+    """Log-probabilities about -2e4, as a temperature of 1e-3 makes them, and
+    lists that leave lanes without an entry.
+
+    d = (b - a) - ((max b - max a) + log of the sums' ratio) has three roundings
+    at the size of the largest logarithm, A; a - max a is exact, p and q have the
+    relative error of K <= 65 additions and an exponential, below 128 roundings
+    with those of divisions and series; a gradient has p df/dp of its own entry and
+    of all.  (A left-out entry taken for one of -1e4 is off by about 1e4.)"""
+    from test1_b200 import ops
+
+    a, b, ids = _lists(T, K, seed=1)
+    a = a - 2e4
+    args = [t.cuda() for t in (a, b, ids)]
+    loss, dlogp, each = ops.distillation_loss_fwd_bwd(*args, kind=kind, tail=False)
+    want, grad, per, _ = oracle.distillation(a, b, ids, kind, False)
+    n, A, D = T, 2.0 ** 15, 16.0  # T rows; no logarithm above A, nor a difference of scaled ones above D
+    tol = 4 * A * EPS + 128 * EPS * (1 + D)
+    assert bool(((each.cpu().double() - per).abs() <= tol).all())
+    assert abs(float(loss) - float(want)) <= tol
+    assert bool(((dlogp.cpu().double() - grad).abs() <= 2 * tol / n).all())
+    # the same as from lists without the shift, whose logarithms are nearer: -2e4 rounds a to 2^-10
+    near, _, _ = ops.distillation_loss_fwd_bwd((a + 2e4).cuda(), *args[1:], kind=kind, tail=False)
+    assert abs(float(near) - float(loss)) <= 2 * tol
