@@ -105,7 +105,9 @@ class DistillationObjective:
     """Learning from a teacher's likeliest tokens.  Takes ``teacher_logps`` and
     ``teacher_ids`` [B, S, K] as ``SlideFSDP.top_logprobs`` of the teacher gives
     them (at this ``temperature``, of the same vocabulary); positions whose label
-    is -100 take no part, nor do entries of id -1.  The divergences and ``tail``
+    is -100 take no part, nor do entries of id -1 or, where the lists are on the
+    GPU, of an id beyond the student's vocabulary (in host memory it is refused).
+    The divergences and ``tail``
     are those of ``ops.distillation_loss_fwd_bwd``.  Results: ``divergence``
     [B, S], of every position; ``logps`` [B, S, K], of the teacher's tokens."""
 

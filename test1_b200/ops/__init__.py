@@ -242,7 +242,10 @@ def distillation_loss_fwd_bwd(logp, teacher_logp, ids, kind="forward", tail=True
     logp and teacher_logp [T, K] (fp32; the teacher's also bf16) are both
     models' log-probabilities of the tokens ids [T, K] (int64).  Entries of a
     negative id, or of a teacher's log-probability of -inf, are left out, and
-    rows without any entry take no part; a row's ids must differ.  With p the
+    rows without any entry take no part; a row's ids must differ and lie below
+    the vocabulary's size, which is not known here (``linear_topk_logprob_fwd``
+    gives other tokens a log-probability of 0, and that is probability 1: make
+    their ids negative for both).  With p the
     student's and q the teacher's probabilities of the listed tokens and, with
     ``tail``, of the rest of the vocabulary as one more outcome (at least
     2^-20: less is the rounding of what is listed), without it scaled to sum to

@@ -883,7 +883,7 @@ class SlideFSDP(nn.Module):
         if objective is not None:
             self._check_label_shape(input_ids, labels)
             if teacher_ids is not None:
-                self._check_teacher_ids(teacher_ids)
+                inputs["teacher_ids"] = self._known_ids(teacher_ids)
             step = ObjectiveStep.build(objective, *input_ids.shape, self.device, **inputs)
         loss = self._train_step(input_ids, labels, step)
         return CausalLMOutputWithPast(loss=loss, logits=None)
@@ -982,11 +982,18 @@ class SlideFSDP(nn.Module):
                     break
         return GeneratedAnswers(ids[:, :total], labels[:, :total], logps[:, :total], length)
 
-    def _check_teacher_ids(self, ids: torch.Tensor) -> None:
-        """As ``_check_ids``, for those in host memory."""
+    def _known_ids(self, ids: torch.Tensor) -> torch.Tensor:
+        """A teacher's ids, as ``_check_ids`` where they are in host memory.
+        Of those on the device, ids beyond this model's vocabulary (a teacher's
+        may be padded further) become -1, entries that take no part: the
+        log-probability 0 that the output layer gives such a token would be a
+        probability of 1 to the loss."""
         V = self.model_config.vocab_size
+        if ids.device.type != "cpu" and not ids.is_floating_point():
+            return torch.where(ids < V, ids.long(), -1)
         if ids.device.type == "cpu" and ids.numel() and int(ids.max()) >= V:
             raise ValueError(f"teacher_ids must lie below the vocabulary's {V}, got {int(ids.max())}")
+        return ids
 
     @staticmethod
     def _check_label_shape(input_ids: torch.Tensor, labels: torch.Tensor) -> None:

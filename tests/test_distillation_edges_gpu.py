@@ -1,11 +1,13 @@
 """The distillation loss kernels at inputs that the other tests leave out: NaN
-in a student's log-probabilities, log-probabilities far below -1e4."""
+in a student's log-probabilities, log-probabilities far below -1e4, tokens
+beyond the student's vocabulary."""
 import math
 
 import pytest
 import torch
 
 import _lists_oracle as oracle
+from test_distillation_gpu import _engine
 
 pytestmark = pytest.mark.gpu
 KINDS = ["forward", "reverse", "jensen"]
@@ -91,3 +93,30 @@ def test_far_below_without_a_tail(T, K, kind, cuda_device):
     # the same as from lists without the shift, whose logarithms are nearer: -2e4 rounds a to 2^-10
     near, _, _ = ops.distillation_loss_fwd_bwd((a + 2e4).cuda(), *args[1:], kind=kind, tail=False)
     assert abs(float(near) - float(loss)) <= 2 * tol
+
+
+@pytest.mark.parametrize("kind,tail", [("forward", True), ("reverse", True), ("jensen", False)])
+def test_teacher_of_a_larger_vocabulary(kind, tail, cuda_device):
+    """Ids on the GPU that the student's vocabulary does not have take no part,
+    as ids of -1 do not."""
+    from test1_b200 import DistillationObjective
+
+    eng, cfg = _engine(5, cuda_device, lr=0.0)
+    V = cfg.vocab_size
+    try:
+        ids = torch.randint(0, V, (2, 64), device=cuda_device)
+        g = torch.Generator(device="cuda").manual_seed(6)
+        logps, top = torch.log_softmax(torch.randn(2, 64, V + 500, device="cuda", generator=g), -1).topk(24, -1)
+        top[0, 0, 0], top[1, 1] = V, torch.arange(V, V + 24, device="cuda")
+        outs = []
+        for t in (top, torch.where(top < V, top, -1)):
+            out = eng(input_ids=ids, labels=ids, objective=DistillationObjective(kind=kind, tail=tail), teacher_logps=logps,
+                      teacher_ids=t)
+            outs.append((out.loss.clone(), eng.last_objective["divergence"].clone(), eng.last_objective["logps"].clone()))
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+        assert not bool(outs[0][1][1, 1].any()) and bool(torch.isfinite(outs[0][0]))
+        with pytest.raises(ValueError):
+            eng(input_ids=ids, labels=ids, objective=DistillationObjective(), teacher_logps=logps, teacher_ids=top.cpu())
+        eng.wait_for_updates()
+    finally:
+        eng.close()
