@@ -869,7 +869,7 @@ static void check_lists(const torch::Tensor& x, const torch::Tensor& w, const to
   TORCH_CHECK(ids.dim() == 2 && ids.size(0) == x.size(0), "ids must be [T, K]");
   TORCH_CHECK(ids.size(1) >= 1 && ids.size(1) <= 512, "a list has 1 to 512 tokens");
   TORCH_CHECK(ids.device() == x.device(), "operands must be on one device");
-  TORCH_CHECK(std::isfinite(temperature) && temperature > 0, "temperature must be positive");
+  TORCH_CHECK(std::isfinite(temperature) && temperature >= 0x1p-126, "temperature must be at least 2^-126 and finite");
 }
 
 // dlogp: null in the forward; logp and lse: null in the gradient.

@@ -1085,8 +1085,9 @@ static void check_rows(const torch::Tensor& logits, double temperature) {
   TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0, "logits must be [T, V]");
   TORCH_CHECK(logits.size(1) == 1 || logits.stride(1) == 1, "logits must be row-major");
   TORCH_CHECK(logits.size(0) < 2 || logits.stride(0) >= 0, "logits must not have a negative stride");
-  // the lowest logit less 400 temperatures (Weigher) has to be finite where it is not the lowest itself
-  TORCH_CHECK(temperature > 0 && temperature <= 0x1p64, "temperature must be positive, at most 2^64");
+  // log2(e) / temperature has to be finite (else a row of largest logit 0 has NaN where it meets 0), and the lowest logit
+  // less 400 temperatures (Weigher) where it is not the lowest itself
+  TORCH_CHECK(temperature >= 0x1p-126 && temperature <= 0x1p64, "temperature must lie in [2^-126, 2^64]");
 }
 
 constexpr int64_t kMostVocab = static_cast<int64_t>(rows::kMostCtas) * rows::kMostColumns * rows::kBinThreads;

@@ -29,8 +29,9 @@ from . import ops
 
 
 def check_temperature(temperature: float) -> None:
-    if not 0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    # below, fp32 has no inverse of it, and the log-probability of the likeliest token is NaN
+    if not ops.MIN_TEMPERATURE <= temperature < float("inf"):
+        raise ValueError(f"temperature must be at least 2^-126 and finite, got {temperature}")
 
 
 @dataclass

@@ -166,6 +166,7 @@ def policy_loss_fwd_bwd(logp, old_logp, ref_logp, advantages, targets, seq_len, 
 
 
 MAX_LIST = 512  # tokens of a row's list
+MIN_TEMPERATURE = 2.0 ** -126  # of rows and lists: fp32 has its inverse, and log2(e) times that
 MAX_TEMPERATURE = 2.0 ** 64  # of rows: 400 times as much, added to the lowest logit, stays finite
 
 
@@ -181,7 +182,7 @@ def topk_logprobs(logits, k, temperature=1.0):
     (logp [T, k] fp32, ids [T, k] int64), likeliest first, of equals the lowest
     index first.  Logits of -inf and NaN are no tokens; a row that has fewer
     than k ends with ids of -1 and log-probabilities of 0.  k is at most
-    MAX_LIST, V on the GPU 393216, a temperature 2^64."""
+    MAX_LIST, V on the GPU 393216; temperatures lie in [2^-126, 2^64]."""
     _check_logits(logits, temperature)
     if not 1 <= k <= min(MAX_LIST, logits.shape[1]):
         raise ValueError(f"k must lie in [1, {min(MAX_LIST, logits.shape[1])}], got {k}")
@@ -200,7 +201,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     the same inputs.  Returns (token [B] int64, logp [B] fp32), logp under the
     tempered distribution before the cuts, as ``linear_logprob_fwd`` gives it.
     Logits of -inf and NaN are no tokens; a row without any gives -1 and 0.  V
-    is at most 393216 on the GPU, a temperature 2^64."""
+    is at most 393216 on the GPU; temperatures lie in [2^-126, 2^64]."""
     _check_logits(logits, temperature)
     check_sampling(temperature, top_k, top_p, min_p)
     if u.dim() != 1 or u.shape[0] != logits.shape[0]:
@@ -216,7 +217,7 @@ def linear_topk_logprob_fwd(x, w, ids, temperature=1.0):
     x [T, H], w [V, H], ids [T, K] int64 (a teacher's likeliest tokens; K at
     most MAX_LIST) -> (logp [T, K], lse [T]) in fp32.  Entries outside the
     vocabulary give 0, and rows without any other give 0 in lse too: they take
-    no part."""
+    no part.  A temperature is at least 2^-126."""
     _check_lists(x, w, ids, temperature)
     return _impl(x).linear_topk_logprob_fwd(x, w, ids, float(temperature))
 
@@ -270,7 +271,7 @@ def check_distillation(kind):
 
 
 def check_sampling(temperature, top_k, top_p, min_p):
-    _check_row_temperature(temperature)
+    check_row_temperature(temperature)
     if top_k < 0 or top_k != int(top_k):
         raise ValueError(f"top_k must be a whole number, 0 for all tokens, got {top_k}")
     if not 0 < top_p <= 1:
@@ -284,12 +285,12 @@ def _check_logits(logits, temperature):
         raise ValueError(f"logits must be [T, V], got {tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits must be float32 or bfloat16, got {logits.dtype}")
-    _check_row_temperature(temperature)
+    check_row_temperature(temperature)
 
 
-def _check_row_temperature(temperature):
-    if not 0 < temperature <= MAX_TEMPERATURE:
-        raise ValueError(f"temperature must be positive, at most 2^64, got {temperature}")
+def check_row_temperature(temperature):
+    if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
+        raise ValueError(f"temperature must lie in [2^-126, 2^64], got {temperature}")
 
 
 def _check_lists(x, w, ids, temperature):
@@ -298,8 +299,8 @@ def _check_lists(x, w, ids, temperature):
                          f"{tuple(ids.shape)}")
     if not 1 <= ids.shape[1] <= MAX_LIST:
         raise ValueError(f"a list has 1 to {MAX_LIST} tokens, got {ids.shape[1]}")
-    if not 0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not MIN_TEMPERATURE <= temperature < float("inf"):
+        raise ValueError(f"temperature must be at least 2^-126 and finite, got {temperature}")
 
 
 def check_preference(beta, kind, label_smoothing):
