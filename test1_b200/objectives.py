@@ -24,6 +24,7 @@ from dataclasses import dataclass, field
 from typing import Dict, Optional
 
 import torch
+import torch.nn.functional as F
 
 from . import ops
 
@@ -145,13 +146,15 @@ class ObjectiveStep:
 
     objective: object
     inputs: Dict[str, Optional[torch.Tensor]]
+    seq_len: int  # of the caller's batch; the step's own may be longer
     results: Dict[str, torch.Tensor] = field(default_factory=dict)
 
     @classmethod
-    def build(cls, objective, batch: int, seq_len: int, device, **inputs) -> "ObjectiveStep":
+    def build(cls, objective, batch: int, seq_len: int, device, behind: int = 0, **inputs) -> "ObjectiveStep":
         """Checks the batch's inputs and moves them to ``device`` as flat fp32
         tensors.  Per-token inputs are [batch, seq_len] as ``token_logprobs``
-        returns them: entry [b, s] belongs to labels[b, s + 1]."""
+        returns them: entry [b, s] belongs to labels[b, s + 1].  ``behind``
+        positions without a label follow every sequence."""
         flat = {}
         lists = [t.shape for n, t in inputs.items() if n.startswith("teacher_") and t is not None]
         for name, t in inputs.items():
@@ -166,13 +169,15 @@ class ObjectiveStep:
                 if name == "teacher_ids" and t.is_floating_point():
                     raise ValueError(f"teacher_ids must be whole numbers, got {t.dtype}")
                 kept = torch.int64 if name == "teacher_ids" else t.dtype if t.dtype == torch.bfloat16 else torch.float32
-                flat[name] = t.to(device=device, dtype=kept, non_blocking=True).reshape(-1, t.shape[2])
+                t = F.pad(t.to(device=device, dtype=kept, non_blocking=True), (0, 0, 0, behind))
+                flat[name] = t.reshape(-1, t.shape[2])
                 continue
             if tuple(t.shape) != (batch, seq_len) and not (name == "advantages" and tuple(t.shape) == (batch,)):
                 raise ValueError(f"{name} must be [{batch}, {seq_len}], got {tuple(t.shape)}")
-            flat[name] = t.to(device=device, dtype=torch.float32, non_blocking=True).reshape(-1)
+            t = t.to(device=device, dtype=torch.float32, non_blocking=True)
+            flat[name] = (F.pad(t, (0, behind)) if t.dim() == 2 else t).reshape(-1)
         objective.check(flat, batch)  # before anything of the step has started
-        return cls(objective, flat)
+        return cls(objective, flat, seq_len)
 
     def token_lists(self, targets: torch.Tensor) -> Optional[torch.Tensor]:
         """[T, K] tokens whose log-probabilities the objective takes; None: the
@@ -182,7 +187,9 @@ class ObjectiveStep:
 
     def loss_and_grad(self, logp: torch.Tensor, targets: torch.Tensor, seq_len: int):
         loss, dlogp, results = self.objective.loss_and_grad(logp, targets, seq_len, self.inputs)
-        self.results = dict(results, logps=logp.view(-1, seq_len, *logp.shape[1:]))
+        results = dict(results, logps=logp.view(-1, seq_len, *logp.shape[1:]))
+        # those of positions are [B, S, ..]
+        self.results = {n: t[:, :self.seq_len].contiguous() if t.dim() > 1 else t for n, t in results.items()}
         return loss, dlogp
 
     @property

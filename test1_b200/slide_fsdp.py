@@ -47,6 +47,7 @@ from typing import Dict, List, Optional
 import torch
 import torch.distributed as dist
 import torch.nn as nn
+import torch.nn.functional as F
 
 from . import _native, ops
 from .config import SlideFSDPConfig
@@ -232,6 +233,8 @@ class SlideFSDP(nn.Module):
             raise NotImplementedError(
                 f"the sm_100a Llama kernels compute in bfloat16; dtype={self.dtype} runs on the "
                 f"generic layer path (other HF architectures) or with use_native_kernels=False")
+        # tokens of a sequence that the attention kernels take at a time
+        self._tile = 64 if self.is_cuda and not self.generic and config.use_native_kernels else 1
         self.base_model = model
         self.model_config = model.config
         self._split_model(model)
@@ -884,8 +887,8 @@ class SlideFSDP(nn.Module):
             self._check_label_shape(input_ids, labels)
             if teacher_ids is not None:
                 inputs["teacher_ids"] = self._known_ids(teacher_ids)
-            step = ObjectiveStep.build(objective, *input_ids.shape, self.device, **inputs)
-        loss = self._train_step(input_ids, labels, step)
+            step = ObjectiveStep.build(objective, *input_ids.shape, self.device, self._behind(input_ids), **inputs)
+        loss = self._train_step(*self._whole_tiles(input_ids, labels), step)
         return CausalLMOutputWithPast(loss=loss, logits=None)
 
     @torch.no_grad()
@@ -913,8 +916,10 @@ class SlideFSDP(nn.Module):
             raise ValueError(f"input_ids must be [B, S], got {tuple(input_ids.shape)}")
         if not 1 <= k <= most:
             raise ValueError(f"k must lie in [1, {most}], got {k}")
-        logp, ids = self._forward_only(input_ids, None, lambda layer, h, ctx: layer.top_logprobs(h, k, temperature))
-        return logp.view(*input_ids.shape, k), ids.view(*input_ids.shape, k)
+        B, S = input_ids.shape
+        tokens, _ = self._whole_tiles(input_ids)
+        logp, ids = self._forward_only(tokens, None, lambda layer, h, ctx: layer.top_logprobs(h, k, temperature))
+        return tuple(t.view(B, -1, k)[:, :S].contiguous() for t in (logp, ids))
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, lengths: Optional[torch.Tensor] = None, *,
@@ -1226,10 +1231,24 @@ class SlideFSDP(nn.Module):
         """Forward only; returns logits [B, S, V], or with labels their
         log-probabilities [B, S]."""
         B, T = input_ids.shape
+        ids, labels = self._whole_tiles(input_ids, labels)
         if labels is None:
-            return self._forward_only(input_ids, None, lambda layer, h, ctx: layer.logits(h)).view(B, T, -1)
-        return self._forward_only(input_ids, labels,
-                                  lambda layer, h, ctx: layer.logprobs(h, ctx.targets, temperature)).view(B, T)
+            return self._forward_only(ids, None, lambda layer, h, ctx: layer.logits(h)).view(*ids.shape, -1)[:, :T]
+        return self._forward_only(ids, labels, lambda layer, h, ctx: layer.logprobs(h, ctx.targets, temperature)) \
+            .view(B, -1)[:, :T].contiguous()
+
+    def _behind(self, input_ids: torch.Tensor) -> int:
+        """Tokens that a sequence lacks for whole tiles of the attention kernels."""
+        return -input_ids.shape[1] % self._tile if input_ids.dim() == 2 else 0
+
+    def _whole_tiles(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None):
+        """``input_ids`` and ``labels`` with these tokens behind them, of label
+        -100.  Attention is causal: they reach no token of the sequence, and no
+        gradient comes from them."""
+        more = self._behind(input_ids)
+        if not more:
+            return input_ids, labels
+        return F.pad(input_ids, (0, more)), None if labels is None else F.pad(labels, (0, more), value=-100)
 
     def _forward_only(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor], head):
         """All layers' forward pass; ``head(output_layer, h, ctx)`` makes the
