@@ -36,6 +36,7 @@ from __future__ import annotations
 
 import json
 import math
+import operator
 import os
 import time
 import uuid
@@ -936,24 +937,27 @@ class SlideFSDP(nn.Module):
         the arithmetic of about 25 thousand tokens.  On several ranks every rank
         generates its own batch, in as many passes as the longest; passes are
         collective, so ``max_new_tokens`` has to be the same on all, and
-        ``eos_token_id`` given on all or none."""
-        self._check_ids(input_ids, None)
-        ops.check_sampling(temperature, top_k, top_p, min_p)
-        if input_ids.dim() != 2 or not input_ids.numel():
-            raise ValueError(f"input_ids must be [B, S], got {tuple(input_ids.shape)}")
-        if max_new_tokens < 1:
-            raise ValueError(f"max_new_tokens must be positive, got {max_new_tokens}")
-        B, S = input_ids.shape
+        ``eos_token_id`` given on all or none.  Where one rank's arguments are
+        refused, all ranks raise."""
+        refused = None
+        try:
+            lengths = self._check_generate(input_ids, max_new_tokens, lengths, temperature, top_k, top_p, min_p)
+        except Exception as e:
+            refused = e
         dev = self.device
-        lengths = torch.full((B,), S) if lengths is None else lengths.to("cpu", torch.int64)
-        if lengths.shape != (B,) or int(lengths.min()) < 1 or int(lengths.max()) > S:
-            raise ValueError(f"lengths must be [{B}] of 1 to {S} tokens")
         if self.world_size > 1:
-            mine = torch.tensor([max_new_tokens, int(eos_token_id is None)], device=dev)
-            most = torch.cat([mine, -mine])
+            # a rank whose arguments are refused says so before it raises: the others must not wait for its passes
+            mine = [0, 0] if refused is not None else [max_new_tokens, int(eos_token_id is None)]
+            most = torch.tensor([int(refused is not None), *mine, *(-v for v in mine)], device=dev)
             dist.all_reduce(most, op=dist.ReduceOp.MAX)
-            if not torch.equal(most[:2], -most[2:]):
+            most = most.tolist()
+            if refused is None and most[0]:
+                raise ValueError("another rank's arguments of generate are refused")
+            if refused is None and most[1:3] != [-v for v in most[3:]]:
                 raise ValueError("max_new_tokens must be the same on all ranks, eos_token_id given on all or none")
+        if refused is not None:
+            raise refused
+        B, S = input_ids.shape
         longest, length = int(lengths.max()), lengths.to(dev)
         # the attention kernels take whole tiles; what lies behind a sequence's last token does not reach it
         tile = 256 if self.is_cuda else 1
@@ -986,6 +990,20 @@ class SlideFSDP(nn.Module):
                 if bool(ended):
                     break
         return GeneratedAnswers(ids[:, :total], labels[:, :total], logps[:, :total], length)
+
+    def _check_generate(self, input_ids, max_new_tokens, lengths, temperature, top_k, top_p, min_p) -> torch.Tensor:
+        """Refuses what ``generate`` does not take; the lengths in host memory."""
+        self._check_ids(input_ids, None)
+        ops.check_sampling(temperature, top_k, top_p, min_p)
+        if input_ids.dim() != 2 or not input_ids.numel():
+            raise ValueError(f"input_ids must be [B, S], got {tuple(input_ids.shape)}")
+        if operator.index(max_new_tokens) < 1:
+            raise ValueError(f"max_new_tokens must be positive, got {max_new_tokens}")
+        B, S = input_ids.shape
+        lengths = torch.full((B,), S) if lengths is None else lengths.to("cpu", torch.int64)
+        if lengths.shape != (B,) or int(lengths.min()) < 1 or int(lengths.max()) > S:
+            raise ValueError(f"lengths must be [{B}] of 1 to {S} tokens")
+        return lengths
 
     def _known_ids(self, ids: torch.Tensor) -> torch.Tensor:
         """A teacher's ids, as ``_check_ids`` where they are in host memory.
