@@ -908,10 +908,11 @@ class SlideFSDP(nn.Module):
     def top_logprobs(self, input_ids: torch.Tensor, k: int, temperature: float = 1.0):
         """The k likeliest next tokens at every position under the present
         weights, forward only: (log-probabilities [B, S, k] fp32, ids [B, S, k]
-        int64), likeliest first (``ops.topk_logprobs``).  Those of a teacher are
+        int64), likeliest first (``ops.topk_logprobs``, whose temperatures it
+        takes).  Those of a teacher are
         a ``DistillationObjective``'s ``teacher_logps`` and ``teacher_ids``."""
         self._check_ids(input_ids, None)
-        check_temperature(temperature)
+        ops.check_row_temperature(temperature)
         most = min(ops.MAX_LIST, self.model_config.vocab_size)
         if input_ids.dim() != 2 or not input_ids.numel():
             raise ValueError(f"input_ids must be [B, S], got {tuple(input_ids.shape)}")

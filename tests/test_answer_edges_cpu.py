@@ -108,3 +108,19 @@ def test_generated_answers_go_back_into_the_engine():
         eng.wait_for_updates()
     finally:
         eng.close()
+
+
+def test_scores_refuse_temperatures_before_the_layers_run():
+    eng, cfg = _engine(1)
+    ids = torch.zeros(1, 4, dtype=torch.int64)
+    ran = []
+    eng._forward_only = lambda *args: ran.append(args)
+    try:
+        for tau in (0.0, 1e-40, 2.0 ** 65, float("inf"), float("nan")):
+            with pytest.raises(ValueError):
+                eng.top_logprobs(ids, 3, temperature=tau)
+            with pytest.raises(ValueError):
+                eng.generate(ids, 3, temperature=tau)
+        assert not ran
+    finally:
+        eng.close()
