@@ -49,25 +49,27 @@ def test_what_lies_behind_changes_nothing(cuda_device):
         assert torch.equal(short, long[:, :69])
         for a, b in zip(eng.top_logprobs(ids[:, :69], 5), eng.top_logprobs(ids, 5)):
             assert torch.equal(a, b[:, :69])
-        short, long = (eng(input_ids=i, labels=t).loss.clone() for i, t in ((ids[:, :69], labels[:, :69]), (ids, labels)))
-        assert abs(float(short) - float(long)) <= 1e-5 * float(long)  # a sum of 128 tokens in any order
-        eng.wait_for_updates()
     finally:
         eng.close()
 
 
-def test_logits_of_odd_widths(cuda_device):
-    """bf16 logits take vocabularies of a multiple of 8."""
+def test_logits_and_loss_of_odd_widths(cuda_device):
+    """bf16 logits and the cross-entropy take vocabularies of a multiple of 8."""
     from test1_b200 import SlideFSDP, SlideFSDPConfig
     from test1_b200.models.llama import LlamaConfig, LlamaForCausalLM
 
     torch.manual_seed(13)
     cfg = LlamaConfig(vocab_size=4000, hidden_size=512, intermediate_size=1024, num_hidden_layers=2, num_attention_heads=4,
                       num_key_value_heads=2, initializer_range=0.1)
-    eng = SlideFSDP(LlamaForCausalLM(cfg, device="meta"), SlideFSDPConfig(dtype=torch.bfloat16, device=cuda_device))
+    eng = SlideFSDP(LlamaForCausalLM(cfg, device="meta"), SlideFSDPConfig(dtype=torch.bfloat16, device=cuda_device, lr=0.0))
     try:
         ids = torch.randint(0, 4000, (2, 128))
+        labels = torch.full_like(ids, -100)
+        labels[:, 5:69] = ids[:, 5:69]
         short, long = (eng(input_ids=i).logits for i in (ids[:, :69], ids))
         assert short.shape == (2, 69, 4000) and torch.equal(short, long[:, :69])
+        short, long = (eng(input_ids=i, labels=t).loss.clone() for i, t in ((ids[:, :69], labels[:, :69]), (ids, labels)))
+        assert abs(float(short) - float(long)) <= 1e-5 * float(long)  # a sum of 128 tokens in any order
+        eng.wait_for_updates()
     finally:
         eng.close()
