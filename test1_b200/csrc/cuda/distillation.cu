@@ -100,7 +100,7 @@ __device__ __forceinline__ float log_half_sum(float x) {
   return z * a;
 }
 
-// f(p, q) and p f'(p) of an outcome, d = log(q / p), finite: 0 times it is 0.
+// f(p, q) and p f'(p) of an outcome, d = log(q / p), finite where it is multiplied by 0.
 __device__ __forceinline__ void divergence(int kind, float p, float q, float d, float& f, float& g) {
   if (kind == kForward) {
     f = q * d;
@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       float f, d = (b[j] - a[j]) - shift;
-      if (d > 3e38f) d = 3e38f;  // of a student's -inf as much as there is
+      // of a student's -inf as much as there is where it has no weight; q times it is infinite
+      if (d > 3e38f && !(p.kind == kForward && qk[j] > 0.f)) d = 3e38f;
       divergence(p.kind, pk[j], qk[j], d, f, g[j]);
       loss += f;
       if (!TAIL) rest += g[j];

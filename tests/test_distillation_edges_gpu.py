@@ -95,6 +95,32 @@ def test_far_below_without_a_tail(T, K, kind, cuda_device):
     assert abs(float(near) - float(loss)) <= 2 * tol
 
 
+@pytest.mark.parametrize("T,K", [(3, 5), (4, 64), (3, 129), (2000, 7)])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tail", [True, False])
+def test_students_without_any_probability(T, K, kind, tail, cuda_device):
+    """A student's -inf: where the teacher has weight the forward divergence is
+    infinite, the others stay finite; where the teacher's weight is 0 in fp32 too,
+    none changes.
+
+    The divergences sum K + 1 <= 130 terms, of logarithms below 16, and their
+    factors have 128 roundings, as in the test above."""
+    from test1_b200 import ops
+    from test1_b200.ops import reference
+
+    a, b, ids = _lists(T, K, seed=2)
+    a[:, 0] = -math.inf
+    b[0, 0] = -1000.0  # no weight
+    loss, dlogp, each = (t.cpu() for t in ops.distillation_loss_fwd_bwd(a.cuda(), b.cuda(), ids.cuda(), kind=kind, tail=tail))
+    want, grad, per = reference.distillation_loss_fwd_bwd(a, b, ids, kind, tail)
+    assert torch.equal(torch.isinf(each), torch.isinf(per)) and bool(torch.isinf(each[1:]).all()) == (kind == "forward")
+    assert not bool(torch.isinf(each[0])) and bool(torch.isinf(loss)) == (kind == "forward")
+    finite = torch.isfinite(per)
+    tol = 256 * EPS * 17
+    assert bool(((each - per)[finite].abs() <= tol).all())
+    assert bool(((dlogp - grad).abs() <= 2 * tol / T).all())
+
+
 @pytest.mark.parametrize("kind,tail", [("forward", True), ("reverse", True), ("jensen", False)])
 def test_teacher_of_a_larger_vocabulary(kind, tail, cuda_device):
     """Ids on the GPU that the student's vocabulary does not have take no part,
