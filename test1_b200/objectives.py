@@ -189,7 +189,8 @@ class ObjectiveStep:
         loss, dlogp, results = self.objective.loss_and_grad(logp, targets, seq_len, self.inputs)
         results = dict(results, logps=logp.view(-1, seq_len, *logp.shape[1:]))
         # those of positions are [B, S, ..]
-        self.results = {n: t[:, :self.seq_len].contiguous() if t.dim() > 1 else t for n, t in results.items()}
+        self.results = {n: t[:, :self.seq_len].contiguous() if t.dim() > 1 and t.shape[1] == seq_len else t
+                        for n, t in results.items()}
         return loss, dlogp
 
     @property

@@ -110,6 +110,24 @@ def test_generated_answers_go_back_into_the_engine():
         eng.close()
 
 
+def test_results_of_no_positions_stay_whole():
+    """A caller's own objective may give results of other shapes."""
+    eng, cfg = _engine(8)
+
+    class Mine(PolicyObjective):
+        def loss_and_grad(self, logp, targets, seq_len, inputs):
+            loss, dlogp, results = super().loss_and_grad(logp, targets, seq_len, inputs)
+            return loss, dlogp, dict(results, table=torch.ones(3, 40))
+
+    ids = torch.zeros(2, 5, dtype=torch.int64)
+    try:
+        eng(input_ids=ids, labels=ids, objective=Mine(), old_logps=torch.zeros(2, 5), advantages=torch.ones(2))
+        assert eng.last_objective["table"].shape == (3, 40) and eng.last_objective["logps"].shape == (2, 5)
+        eng.wait_for_updates()
+    finally:
+        eng.close()
+
+
 def test_scores_refuse_temperatures_before_the_layers_run():
     eng, cfg = _engine(1)
     ids = torch.zeros(1, 4, dtype=torch.int64)
