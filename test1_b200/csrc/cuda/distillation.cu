@@ -61,6 +61,10 @@ struct Params {
   float* loss;
   float* dlogp;            // [T, K]
   float* each;             // [T]
+  // what was allocated, for the bounds-checked build
+  int64_t entries;         // of the inputs and dlogp
+  int64_t rows;            // of each
+  int blocks;              // of sums and counts
 };
 
 // Sums over G neighbouring lanes.
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
       if (VEC) {
         longlong2 i0 = make_longlong2(-1, -1), i1 = i0;
         float4 a4 = make_float4(0.f, 0.f, 0.f, 0.f), b4 = a4;
-        if (k < cols) {
+        if (k < cols && !T1_OOB(row + k + 3, p.entries)) {
           i0 = __ldcs(reinterpret_cast<const longlong2*>(p.ids + row + k));
           i1 = __ldcs(reinterpret_cast<const longlong2*>(p.ids + row + k) + 1);
           a4 = __ldcs(reinterpret_cast<const float4*>(p.logp + row + k));
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
         in_a[j] = a4.x, in_a[j + 1] = a4.y, in_a[j + 2] = a4.z, in_a[j + 3] = a4.w;
         in_b[j] = b4.x, in_b[j + 1] = b4.y, in_b[j + 2] = b4.z, in_b[j + 3] = b4.w;
       } else {
-        const bool in = k < cols;
+        const bool in = k < cols && !T1_OOB(row + k, p.entries);
         in_id[j] = in ? __ldcs(p.ids + row + k) : -1;
         in_a[j] = in ? __ldcs(p.logp + row + k) : 0.f;
         in_b[j] = !in              ? 0.f
@@ -204,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
 #pragma unroll
     for (int j = 0; j < PER; j += kStep) {
       const int k = entry(j);
-      if (k >= cols || T1_OOB(row + k + kStep - 1, p.T * p.K)) continue;
+      if (k >= cols || T1_OOB(row + k + kStep - 1, p.entries)) continue;
       if (VEC) *reinterpret_cast<float4*>(p.dlogp + row + k) = make_float4(g[j] * scale, g[j + 1] * scale, g[j + 2] * scale, g[j + 3] * scale);
       else p.dlogp[row + k] = g[j] * scale;
     }
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
 #pragma unroll
     for (int j = 0; j < PER; ++j) g[j] = kept >> j & 1 ? fmaf(-pk[j], rest, g[j]) : 0.f;
     if (of_row == 0) {
-      if (t < p.T && !T1_OOB(t, p.T)) p.each[t] = loss;
+      if (t < p.T && !T1_OOB(t, p.rows)) p.each[t] = loss;
       sum += loss;
       rows += live;
     }
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned ctas = cluster.num_blocks();
     wait_started();
-    if (threadIdx.x < ctas) {
+    if (threadIdx.x < ctas && !T1_OOB(ctas - 1, 8)) {
       cluster.map_shared_rank(of_cta, threadIdx.x)[cluster.block_rank()] = sum;
       cluster.map_shared_rank(live_of_cta, threadIdx.x)[cluster.block_rank()] = rows;
     }
@@ -333,8 +337,10 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
   }
   // the blocks' sums in their order, by the last one
   if (threadIdx.x == 0) {
-    __stcg(p.sums + blockIdx.x, sum);
-    __stcg(p.counts + blockIdx.x, rows);
+    if (!T1_OOB(blockIdx.x, p.blocks)) {
+      __stcg(p.sums + blockIdx.x, sum);
+      __stcg(p.counts + blockIdx.x, rows);
+    }
     __threadfence();
     last = atomicAdd(p.ticket.use, 1) == static_cast<int>(gridDim.x) - 1;
   }
@@ -344,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
   sum = 0.0;
   rows = 0;
   for (int i = lane; i < static_cast<int>(gridDim.x); i += 32) {
+    if (T1_OOB(i, p.blocks)) continue;
     sum += __ldcg(p.sums + i);
     rows += __ldcg(p.counts + i);
   }
@@ -357,16 +364,17 @@ __global__ void __launch_bounds__(kThreads, PER > 8 ? 1 : 4) loss_kernel(const P
 }
 
 // dlogp times the scale; dlogp is freshly allocated and so begins on 16 bytes.
-__global__ void __launch_bounds__(kThreads) scale_kernel(float* dlogp, int64_t n, const float* scale) {
+__global__ void __launch_bounds__(kThreads) scale_kernel(float* dlogp, int64_t n, int64_t entries, const float* scale) {
   const float s = *scale;
   const int64_t vecs = n / 4, step = static_cast<int64_t>(gridDim.x) * kThreads;
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   for (int64_t i = i0; i < vecs; i += step) {
+    if (T1_OOB(4 * i + 3, entries)) continue;
     float4 v = reinterpret_cast<float4*>(dlogp)[i];
     v = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
     reinterpret_cast<float4*>(dlogp)[i] = v;
   }
-  if (i0 < n - 4 * vecs) dlogp[4 * vecs + i0] *= s;
+  if (i0 < n - 4 * vecs && !T1_OOB(4 * vecs + i0, entries)) dlogp[4 * vecs + i0] *= s;
 }
 
 }  // namespace distil
@@ -398,6 +406,7 @@ static void launch_loss(distil::Params& p, bool tail) {
   auto ws = torch::empty({2 * blocks + 1}, torch::TensorOptions().dtype(torch::kFloat64).device(torch::kCUDA, at::cuda::current_device()));
   p.sums = ws.data_ptr<double>();
   p.counts = reinterpret_cast<int*>(p.sums + blocks);
+  p.blocks = blocks;
   p.scale = reinterpret_cast<float*>(p.sums + 2 * blocks);
   ArrivalCounters counters(1);
   p.ticket = counters.arrivals;
@@ -407,7 +416,7 @@ static void launch_loss(distil::Params& p, bool tail) {
   counters.launched();
   const int64_t n = p.T * p.K;
   distil::scale_kernel<<<static_cast<int>(std::min<int64_t>((n / 4 + distil::kThreads) / distil::kThreads, 8 * num_sms())),
-                         distil::kThreads, 0, stream()>>>(p.dlogp, n, p.scale);
+                         distil::kThreads, 0, stream()>>>(p.dlogp, n, p.entries, p.scale);
   check_launch("distillation_loss");
   count_launch(2);
 }
@@ -460,6 +469,8 @@ std::vector<torch::Tensor> distillation_loss(torch::Tensor logp, torch::Tensor t
   p.loss = loss.data_ptr<float>();
   p.dlogp = dlogp.data_ptr<float>();
   p.each = each.data_ptr<float>();
+  p.entries = dlogp.numel();
+  p.rows = each.numel();
   p.teacher_bf16 = te.scalar_type() == torch::kBFloat16;
   run_loss(p, tail);
   return {loss, dlogp, each};

@@ -112,8 +112,18 @@ struct Params {
   u64* lists;        // [rows][segments][cap]
   RowState* states;  // [rows] scan_bins
   u64* weights;      // [rows][segments] scan_bins: kept without top_p, above the bin with it
+  // what was allocated, for the bounds-checked build
+  int64_t elements;      // of the logits, from the first row's first to the last row's last
+  int64_t outputs;       // of ids and logp
+  int64_t all_segments;  // of part, counts and weights
+  int64_t list_slots;    // of lists
 };
 
+__device__ __forceinline__ unsigned held_bytes() {
+  unsigned n;
+  asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(n));
+  return n;
+}
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ float logit(const float* p) { return __ldg(p); }
@@ -130,11 +140,17 @@ __device__ __forceinline__ float4 held_quad(const bf16_t* p) {
                      __uint_as_float(q.y & 0xffff0000u));
 }
 
-// A warp's `cols` logits from `from` on to shared memory, and -inf up to `all`.
+// A warp's `all` logits of a row from column col0 on to shared memory, -inf behind the row's last.
 template <typename T>
-__device__ __forceinline__ void fetch(T* to, const T* from, int cols, int all, bool aligned, int lane) {
+__device__ __forceinline__ void fetch(const Params& p, T* held, int at, int row, int col0, int all, int lane) {
   constexpr int kVec = 16 / sizeof(T);
-  const int vecs = aligned ? cols / kVec : 0;
+  const int64_t first = row * p.ld + col0;
+  const T* from = static_cast<const T*>(p.logits) + first;
+  T* to = held + at;
+  int cols = max(0, min(all, p.V - col0));
+  if (T1_OOB((at + all) * sizeof(T) - 1, held_bytes())) return;
+  if (cols > 0 && T1_OOB(first + cols - 1, p.elements)) cols = 0;
+  const int vecs = p.aligned ? cols / kVec : 0;
   for (int i = lane; i < vecs; i += 32)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(to + kVec * i)), "l"(from + kVec * i) : "memory");
 #pragma unroll 8
@@ -276,6 +292,7 @@ template <int N>
 __device__ __forceinline__ void add_to(unsigned (&bins)[3][N], int b, u64 w) {
   const unsigned lo = static_cast<unsigned>(w) & 0xffffu, mid = static_cast<unsigned>(w >> 16) & 0xffffu,
                  hi = static_cast<unsigned>(w >> 32);
+  if (T1_OOB(b, N)) return;
   atomicAdd(&bins[0][b], lo);
   atomicAdd(&bins[1][b], mid);
   if (hi != 0) atomicAdd(&bins[2][b], hi);
@@ -302,15 +319,17 @@ struct Scan {
   unsigned listed;      // above the list's length: not all
 };
 
+// The list is `cap` of the `slots` of `lists`, from list0 on.
 template <typename T>
-__device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segment, u64* list, unsigned cap, ListShared& sh, T* held) {
+__device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segment, u64* lists, int64_t list0, int64_t slots,
+                                             unsigned cap, ListShared& sh, T* held) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // a warp has 32 n columns in a row, a thread four of every 128
   const int n = p.per_segment / kThreads;
   const int col0 = segment * p.per_segment + warp * 32 * n;
   T* mine = held + warp * 32 * n;
   auto quad = [&](int i) { return held_quad(mine + 4 * (32 * i + lane)); };
-  fetch(mine, static_cast<const T*>(p.logits) + row * p.ld + col0, max(0, min(32 * n, p.V - col0)), 32 * n, p.aligned, lane);
+  fetch(p, held, warp * 32 * n, row, col0, 32 * n, lane);
   sh.bins[tid] = 0;
   if (tid == 0) sh.listed = 0;
   fetched();
@@ -330,11 +349,11 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
   // few tokens need few parts
   if (p.rank <= kThreads / 4) {
     const float own = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    if (is_token(own)) atomicAdd(&sh.bins[step_of(m, own)], 1u);
+    if (is_token(own) && !T1_OOB(step_of(m, own), kBins)) atomicAdd(&sh.bins[step_of(m, own)], 1u);
   } else {
 #pragma unroll
     for (int j = 0; j < kParts; ++j)
-      if (is_token(part[j])) atomicAdd(&sh.bins[step_of(m, part[j])], 1u);
+      if (is_token(part[j]) && !T1_OOB(step_of(m, part[j]), kBins)) atomicAdd(&sh.bins[step_of(m, part[j])], 1u);
   }
   __syncthreads();
   if (warp == 0) {
@@ -361,7 +380,7 @@ __device__ __forceinline__ Scan scan_stretch(const Params& p, int row, int segme
   const float bound = sh.bin < 0 ? -INFINITY : sh.bin < kBins - 1 ? least_of(m, sh.bin) : INFINITY;
   auto push = [&](float z, int column) {
     const unsigned to = atomicAdd(&sh.listed, 1u);
-    if (to < cap) list[to] = place_of(z, column);
+    if (to < cap && !T1_OOB(list0 + to, slots)) lists[list0 + to] = place_of(z, column);
   };
   float sum = 0.f;
   if (is_sharp(m, p.tau)) {
@@ -427,7 +446,7 @@ __device__ __forceinline__ void sync_all(cg::cluster_group& cluster) {
 template <typename V>
 __device__ __forceinline__ void tell_all(cg::cluster_group& cluster, V* slots, V value) {
   const unsigned n = cluster.num_blocks();
-  if (threadIdx.x < n) cluster.map_shared_rank(slots, threadIdx.x)[cluster.block_rank()] = value;
+  if (threadIdx.x < n && !T1_OOB(cluster.block_rank(), kMostCtas)) cluster.map_shared_rank(slots, threadIdx.x)[cluster.block_rank()] = value;
   sync_all(cluster);
 }
 
@@ -450,7 +469,7 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   if (ctas > 1) tell_started();
   launch_dependents();
   wait_previous();
-  fetch(mine, static_cast<const T*>(p.logits) + row * p.ld + warp_col0, max(0, min(32 * n, p.V - warp_col0)), 32 * n, p.aligned, lane);
+  fetch(p, reinterpret_cast<T*>(held_raw), warp * 32 * n, row, warp_col0, 32 * n, lane);
   for (int i = tid; i < 3 * kWeightBins; i += kBinThreads) sh.bins[0][i] = 0;
   fill_exps(sh.exps);
   fetched();
@@ -466,6 +485,8 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   tell_all(cluster, sh.max_of, m);
   for (int r = 0; r < ctas; ++r) m = fmaxf(m, sh.max_of[r]);
   const int64_t at = static_cast<int64_t>(row) * p.segments + rank;
+  // the row's state and the segment's numbers are there (by the whole cluster: its barriers stay together)
+  if (T1_OOB(static_cast<int64_t>(row) * p.segments + ctas - 1, p.all_segments) || T1_OOB(row, p.rows) || T1_OOB(ctas - 1, kMostCtas)) return;
   const Weigher w(p, m, sh.exps);
   if (m == -INFINITY || w.sharp) {  // finish sees that
     if (rank == 0 && tid == 0) p.states[row] = {m, -1, 0, 0};
@@ -554,12 +575,11 @@ __global__ void __launch_bounds__(kBinThreads, 3) scan_bins_kernel(const Params 
   unsigned to;
   const unsigned listed = block_scan<kBinThreads / 32>(count, to, sh.red32);
   if (tid == 0) p.counts[at] = static_cast<int>(min(listed, p.cap + 1u));
-  u64* list = p.lists + at * p.cap;
 #pragma unroll
   for (int b = 0; b < kMostColumns / 32; ++b) {
     for (; in_bin[b] != 0; in_bin[b] &= in_bin[b] - 1, ++to) {
       const int k = 32 * b + __ffs(in_bin[b]) - 1;
-      if (to < p.cap) list[to] = place_of(mine_at(k), warp_col0 + column_of(k));
+      if (to < p.cap && !T1_OOB(at * p.cap + to, p.list_slots)) p.lists[at * p.cap + to] = place_of(mine_at(k), warp_col0 + column_of(k));
     }
   }
 }
@@ -617,12 +637,13 @@ __device__ __forceinline__ void order_list(u64* list, unsigned listed) {
       larger += __shfl_xor_sync(0xffffffffu, larger, 1);
     }
     __syncthreads();
-    if (i < listed && part == 0) list[larger] = mine;
+    if (i < listed && part == 0 && !T1_OOB(larger, kListSlots)) list[larger] = mine;
     __syncthreads();
     return;
   }
   unsigned slots = 1;
   while (slots < listed) slots *= 2;
+  if (T1_OOB(slots - 1, kListSlots)) return;  // the same for all threads
   for (unsigned i = listed + threadIdx.x; i < slots; i += THREADS) list[i] = 0;
   sort_list<THREADS>(list, slots);
 }
@@ -635,7 +656,8 @@ template <typename T, bool TOP, int THREADS, bool ALONE>
 __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShared& sh, const Scan& scan) {
   constexpr int kWarps = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* src = static_cast<const T*>(p.logits) + row * p.ld;
+  const int64_t row0 = row * p.ld;
+  const T* src = static_cast<const T*>(p.logits) + row0;
   const int64_t seg0 = static_cast<int64_t>(row) * p.segments;
   constexpr int kLowest = sizeof(T) == 2 ? 16 : 0;  // key bits below are the same in all of a type's values
   const unsigned first = p.first;
@@ -654,6 +676,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     complete = scan.listed <= kListSlots;
   } else if (p.by_list) {
     for (int s = tid; s < p.segments; s += THREADS) {
+      if (T1_OOB(seg0 + s, p.all_segments)) continue;
       const float4 of = p.part[seg0 + s];
       m = fmaxf(m, of.x);
       bound = fmaxf(bound, of.z);
@@ -662,19 +685,22 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     m = block_max(m, sh.fred);
     bound = block_max(bound, sh.fred);
     for (int s = tid; s < p.segments; s += THREADS) {
+      if (T1_OOB(seg0 + s, p.all_segments)) continue;
       const float4 of = p.part[seg0 + s];
       sum += of.x == m ? of.y : of.y * exp2f_fast((of.x - m) * p.scale2);
     }
     sum = block_sum(sum, sh.fred);
   } else {
-    m = p.states[row].m;
-    for (int s = tid; s < p.segments; s += THREADS) complete = complete && p.counts[seg0 + s] <= p.cap;
+    if (!T1_OOB(row, p.rows)) m = p.states[row].m;
+    for (int s = tid; s < p.segments; s += THREADS) complete = complete && !T1_OOB(seg0 + s, p.all_segments) && p.counts[seg0 + s] <= p.cap;
   }
   complete = __syncthreads_and(complete);
   if (m == -INFINITY) {
     for (int i = tid; i < (TOP ? p.first : 1); i += THREADS) {
-      p.ids[static_cast<int64_t>(row) * (TOP ? p.first : 1) + i] = -1;
-      p.logp[static_cast<int64_t>(row) * (TOP ? p.first : 1) + i] = 0.f;
+      const int64_t at = static_cast<int64_t>(row) * (TOP ? p.first : 1) + i;
+      if (T1_OOB(at, p.outputs)) continue;
+      p.ids[at] = -1;
+      p.logp[at] = 0.f;
     }
     return;
   }
@@ -685,13 +711,20 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     const unsigned to = atomicAdd(&sh.listed, 1u);
     if (to < kListSlots) sh.list[to] = place;
   };
+  auto write_draw = [&](int column, float z) {
+    if (T1_OOB(column, p.V) || T1_OOB(row, p.outputs)) return;
+    p.ids[row] = column;
+    p.logp[row] = log_p(z);
+  };
   // every token that the scan has listed
   const int warps_each = max(1, kWarps / p.segments);  // of a segment
   auto each_listed = [&](auto&& of) {
     for (int s = warp / warps_each; s < p.segments; s += kWarps / warps_each) {
+      if (T1_OOB(seg0 + s, p.all_segments)) continue;
       const int n = p.counts[seg0 + s];
-      const u64* list = p.lists + (seg0 + s) * p.cap;
-      for (int i = warp % warps_each * 32 + lane; i < n; i += 32 * warps_each) of(list[i]);
+      const int64_t list0 = (seg0 + s) * p.cap;
+      for (int i = warp % warps_each * 32 + lane; i < n; i += 32 * warps_each)
+        if (!T1_OOB(list0 + i, p.list_slots)) of(p.lists[list0 + i]);
     }
   };
   // the thread's bin in which `need` is reached (-1: in none), and in sh.before64 what comes before
@@ -711,7 +744,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     for (int i = tid; i < p.first; i += THREADS) {
       const bool in = i < static_cast<int>(n);
       const int64_t at = static_cast<int64_t>(row) * p.first + i;
-      if (T1_OOB(at, static_cast<int64_t>(p.rows) * p.first)) continue;
+      if (T1_OOB(at, p.outputs) || (in && (T1_OOB(i, kListSlots) || T1_OOB(column_at(sh.list[i]), p.V)))) continue;
       p.logp[at] = in ? log_p(logit_at(sh.list[i])) : 0.f;
       p.ids[at] = in ? column_at(sh.list[i]) : -1;
     }
@@ -724,7 +757,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     for (int c = c0 + lane; c - lane < c1; c += 16 * 32) {
       float z[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) z[j] = c + 32 * j < c1 ? logit(src + c + 32 * j) : -INFINITY;
+      for (int j = 0; j < 16; ++j) z[j] = c + 32 * j < c1 && !T1_OOB(row0 + c + 32 * j, p.elements) ? logit(src + c + 32 * j) : -INFINITY;
 #pragma unroll
       for (int j = 0; j < 16; ++j) of(z[j] == z[j] ? z[j] + 0.f : -INFINITY, c + 32 * j);
     }
@@ -733,7 +766,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   if (p.by_list && complete && !w.sharp) {
     bool enough = ALONE && bound > -INFINITY;  // not only all that there are
     if (!ALONE) {
-      each_listed([&](u64 e) { atomicAdd(&sh.bins[0][step_of(m, logit_at(e))], 1u); });
+      each_listed([&](u64 e) { if (!T1_OOB(step_of(m, logit_at(e)), kBins)) atomicAdd(&sh.bins[0][step_of(m, logit_at(e))], 1u); });
       __syncthreads();
       const int bin = reach(tid < kBins ? sh.bins[0][tid] : 0ull, first);
       enough = bin >= 0;
@@ -750,6 +783,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
         const float last = logit_at(sh.list[first - 1]);
         if (bound > last) {
           for (int s = 0; s < p.segments; ++s) {
+            if (T1_OOB(seg0 + s, p.all_segments)) continue;
             const float of = p.part[seg0 + s].z;
             if (of <= last) continue;
             each_column(s * p.per_segment, min(p.V, (s + 1) * p.per_segment), [&](float z, int c) {
@@ -800,10 +834,8 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
         const u64 target = target_of(p.u[row], block_scan<kWarps>(own, before, sh.red));
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-          if (before <= target && target < before + of[j]) {
-            p.ids[row] = static_cast<int>(~static_cast<unsigned>(e[j] >> 32));
-            p.logp[row] = log_p(logit_of(static_cast<unsigned>(e[j])));
-          }
+          if (before <= target && target < before + of[j])
+            write_draw(static_cast<int>(~static_cast<unsigned>(e[j] >> 32)), logit_of(static_cast<unsigned>(e[j])));
           before += of[j];
         }
         return;
@@ -832,7 +864,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
   auto batch = [&](int c, int c1, auto&& put) {
     float z[kBatch / 32];
 #pragma unroll
-    for (int j = 0; j < kBatch / 32; ++j) z[j] = c + 32 * j + lane < c1 ? logit(src + c + 32 * j + lane) : -INFINITY;
+    for (int j = 0; j < kBatch / 32; ++j) z[j] = c + 32 * j + lane < c1 && !T1_OOB(row0 + c + 32 * j + lane, p.elements) ? logit(src + c + 32 * j + lane) : -INFINITY;
     int n = 0;
 #pragma unroll
     for (int j = 0; j < kBatch / 32; ++j) {
@@ -849,7 +881,9 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     const int c0 = lo + warp * per, c1 = min(hi, c0 + per);
     u64 own = 0, before;
     for (int c = c0; c < c1; c += kBatch) {
-      const int n = batch(c, c1, [&](int i, float z, int) { sh.kept[warp][i] = z; });
+      const int n = batch(c, c1, [&](int i, float z, int) {
+        if (!T1_OOB(i, kBatch)) sh.kept[warp][i] = z;
+      });
       for (int i = lane; i < n; i += 32) own += w.weight(sh.kept[warp][i]);
       __syncwarp();
     }
@@ -860,16 +894,15 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     if (target < before || target >= before + of_warp) return;
     // this warp has it, and the list's place to itself
     for (int c = c0; c < c1; c += kBatch) {
-      const int n = batch(c, c1, [&](int i, float z, int column) { sh.list[i] = place_of(z, column); });
+      const int n = batch(c, c1, [&](int i, float z, int column) {
+        if (!T1_OOB(i, kListSlots)) sh.list[i] = place_of(z, column);
+      });
       for (int i = lane; i - lane < n; i += 32) {
         const u64 e = i < n ? sh.list[i] : 0ull;
         const u64 upto = before + warp_scan(i < n ? w.weight(logit_at(e)) : 0ull, lane);
         const unsigned past = __ballot_sync(0xffffffffu, target < upto);
         if (past != 0) {
-          if (lane == __ffs(past) - 1) {
-            p.ids[row] = column_at(e);
-            p.logp[row] = log_p(logit_at(e));
-          }
+          if (lane == __ffs(past) - 1) write_draw(column_at(e), logit_at(e));
           return;
         }
         before = __shfl_sync(0xffffffffu, upto, 31);
@@ -887,7 +920,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     u64 of_segments = 0, before_segment = 0;
     if (p.top_p == 1.0) {
       found = true;
-      if (tid < p.segments) sh.kept_of[tid] = p.weights[seg0 + tid];
+      if (tid < p.segments && !T1_OOB(seg0 + tid, p.all_segments) && !T1_OOB(tid, kMostCtas)) sh.kept_of[tid] = p.weights[seg0 + tid];
       __syncthreads();
       segment = 0;
     } else if (st.bin >= 0 && complete) {
@@ -933,7 +966,8 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
           kept = warp_sum64(kept);
           if (lane == 0) sh.border[warp] = kept;
           __syncthreads();
-          if (tid < p.segments) {
+          if (tid < p.segments && !T1_OOB(seg0 + tid, p.all_segments) && !T1_OOB((tid + 1) * warps_each - 1, kBinThreads / 32) &&
+              !T1_OOB(tid, kMostCtas)) {
             kept = p.weights[seg0 + tid];
             for (int v = 0; v < warps_each; ++v) kept += sh.border[tid * warps_each + v];
             sh.kept_of[tid] = kept;
@@ -946,7 +980,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int row, FinishShare
     if (segment == 0) {
       for (int s = 0; s < p.segments; ++s) of_segments += sh.kept_of[s];
       const u64 target = target_of(p.u[row], of_segments);
-      while (target >= before_segment + sh.kept_of[segment]) before_segment += sh.kept_of[segment++];
+      while (!T1_OOB(segment, p.segments) && target >= before_segment + sh.kept_of[segment]) before_segment += sh.kept_of[segment++];
       const int lo = segment * p.per_segment, hi = min(p.V, lo + p.per_segment);
       draw(lo, hi, true, target - before_segment);
       return;
@@ -1059,14 +1093,14 @@ __global__ void __launch_bounds__(kThreads) scan_list_kernel(const Params p) {
   wait_previous();
   if constexpr (ALONE) {
     __shared__ FinishShared rest;
-    const Scan scan = scan_stretch<T>(p, blockIdx.x, 0, rest.list, kListSlots, sh, held);
+    const Scan scan = scan_stretch<T>(p, blockIdx.x, 0, rest.list, 0, kListSlots, kListSlots, sh, held);
     __syncthreads();
     finish_row<T, TOP, kThreads, true>(p, blockIdx.x, rest, scan);
   } else {
     const int segment = blockIdx.x % p.segments;
-    const Scan scan = scan_stretch<T>(p, blockIdx.x / p.segments, segment, p.lists + static_cast<int64_t>(blockIdx.x) * p.cap,
-                                      p.cap, sh, held);
-    if (threadIdx.x == 0) {
+    const Scan scan = scan_stretch<T>(p, blockIdx.x / p.segments, segment, p.lists, static_cast<int64_t>(blockIdx.x) * p.cap,
+                                      p.list_slots, p.cap, sh, held);
+    if (threadIdx.x == 0 && !T1_OOB(blockIdx.x, p.all_segments)) {
       p.part[blockIdx.x] = make_float4(scan.m, scan.sum, scan.bound, 0.f);
       p.counts[blockIdx.x] = static_cast<int>(scan.listed);
     }
@@ -1105,6 +1139,8 @@ static torch::Tensor scan_space(rows::Params& p, const torch::Tensor& logits) {
   p.weights = reinterpret_cast<rows::u64*>(base + lists);
   p.states = reinterpret_cast<rows::RowState*>(base + lists + part);
   p.counts = reinterpret_cast<int*>(base + lists + part + states);
+  p.all_segments = segments;
+  p.list_slots = lists / 8;
   return buf;
 }
 
@@ -1181,6 +1217,7 @@ static void run_rows(rows::Params& p, const torch::Tensor& logits, double temper
   p.logits = logits.data_ptr();
   p.ld = logits.size(0) > 1 ? logits.stride(0) : 0;
   p.rows = static_cast<int>(logits.size(0));
+  p.elements = logits.size(0) > 0 ? (logits.size(0) - 1) * p.ld + logits.size(1) : 0;
   p.V = static_cast<int>(logits.size(1));
   p.aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * logits.element_size() % 16 == 0;
   p.tau = static_cast<float>(temperature);
@@ -1205,6 +1242,7 @@ std::vector<torch::Tensor> topk_logprobs(torch::Tensor logits, int64_t k, double
   p.by_list = true;
   p.logp = logp.data_ptr<float>();
   p.ids = ids.data_ptr<int64_t>();
+  p.outputs = ids.numel();
   run_rows<true>(p, logits, temperature);
   return {logp, ids};
 }
@@ -1226,6 +1264,7 @@ std::vector<torch::Tensor> sample_tokens(torch::Tensor logits, torch::Tensor u, 
   rows::Params p{};
   p.logp = logp.data_ptr<float>();
   p.ids = token.data_ptr<int64_t>();
+  p.outputs = token.numel();
   p.u = uc.data_ptr<float>();
   p.first = static_cast<int>(top_k >= logits.size(1) ? 0 : top_k);
   p.by_list = p.first != 0 && p.first <= rows::kMostFirst;
