@@ -1,5 +1,5 @@
-"""Rows of logits at inputs that the other tests leave out: the least
-temperature with a largest logit of 0."""
+"""Rows of logits at inputs that the other tests leave out: the least temperature
+with a largest logit of 0, masks that leave neighbouring tokens alone."""
 import math
 
 import pytest
@@ -33,6 +33,31 @@ def test_least_temperature_with_a_largest_logit_of_zero(V, dtype, cuda_device):
     for top_k, top_p, min_p in [(0, 1.0, 0.0), (3, 1.0, 0.0), (0, 0.5, 0.0), (0, 1.0, 0.3), (3, 0.7, 0.1)]:
         token, logp = ops.sample_tokens(z, u, LEAST, top_k, top_p, min_p)
         at, want = oracle.sample(z, u, LEAST, top_k, top_p, min_p)
+        assert torch.equal(token.cpu(), at)
+        _check_logp(logp, want)
+
+
+@pytest.mark.parametrize("B,V", [(2, 20011), (1, 128256)])
+@pytest.mark.parametrize("allowed", [26, 100, 1000, 9000])
+@pytest.mark.parametrize("lowest", [-math.inf, "min", -1e9])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_neighbouring_tokens_alone(B, V, allowed, lowest, dtype, cuda_device):
+    """Masks that leave some neighbours, as a grammar does: whole stretches are
+    empty, or equal to the type's lowest value."""
+    from test1_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(V + allowed)
+    z = 2 * torch.randn(B, V, device="cuda", generator=g)
+    z[:, :5000] = z[:, 5000 + allowed:] = torch.finfo(dtype).min if lowest == "min" else lowest
+    z = z.to(dtype)
+    u = torch.rand(B, device="cuda", generator=g)
+    logp, ids = ops.topk_logprobs(z, 64, 0.8)
+    want, at = oracle.topk(z, 64, 0.8)
+    assert torch.equal(ids.cpu(), at)
+    _check_logp(logp, torch.where(want < -3.4e38, -math.inf, want))
+    for top_k, top_p, min_p in [(50, 0.95, 0.0), (1000, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.05)]:
+        token, logp = ops.sample_tokens(z, u, 0.8, top_k, top_p, min_p)
+        at, want = oracle.sample(z, u, 0.8, top_k, top_p, min_p)
         assert torch.equal(token.cpu(), at)
         _check_logp(logp, want)
 
