@@ -24,9 +24,9 @@
 //
 // G lanes have a row, PER entries each; the inputs are read once.  (Asking for
 // them a round ahead takes the registers of half of the warps: 46 us for 65600
-// rows of 64 against 40.)  65600 rows of 64 take 35 us, 27 of them here: 11.6 M
-// warp instructions (forward; 18.4 M symmetric) at 1.5 to 1.8 a cycle bound it,
-// not its 84 MB.
+// rows of 64 against 40.)  65600 rows of 64 take 35 us (symmetric), 28 of them
+// here: instructions bound it (19.8 M of warps, 71 % of the issue slots; forward
+// 12.6 M, 61 %), not its 84 MB.
 // Every gradient is divided by the number of rows that take part.  A batch that
 // one cluster of 8 CTAs has in one round waits for the others' counts and then
 // writes; a larger one is scaled by a second launch, out of L2.

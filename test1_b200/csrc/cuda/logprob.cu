@@ -8,7 +8,7 @@
 //   dW[v, :]    = sum_t u[t, v] x[t, :]
 //
 // u is the one intermediate that is rounded: to bf16, for the tensor cores.
-// Its relative error of 2^-9 at most per element adds to the 2^-9 of the
+// Its relative error of 2^-8 at most per element adds to the 2^-8 of the
 // results' own rounding; all sums are fp32.  Before that rounding u is as good
 // as its formula in fp32: 1 - exp(logit - lse) of a target that is nearly sure
 // is off by what fp32 holds of lse (2^-24 of it), which logits summed in the

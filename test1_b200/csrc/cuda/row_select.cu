@@ -32,18 +32,22 @@
 //              vocabulary may fall into one).
 // Where a list is too long (many equal logits) or does not hold what is asked
 // for, finish finds the cut digit by digit, 8 bits at a time, of the
-// order-preserving integer of a logit, reading the row anew each time.
-// Measured: the likeliest 64 of 1024 rows of 128256 in 119 us (4.4 TB/s; 23
-// instructions a warp for 32 logits, at 2.8 of 4 a cycle); 256 draws with top_p
-// in 160 us, 137 of them scan_bins (45 instructions a logit for the exact weight
-// and its bin, at 57 % of the issue slots; the rest are barriers of the cluster);
-// one draw with top_k in 12 us, latencies of two launches.
+// order-preserving integer of a logit, reading the row anew each time.  Rows of
+// which only some hundred neighbouring tokens are not -inf, or whose masked
+// stretches hold a finite lowest value throughout, end there: a draw of 50 in
+// 410 to 530 us for one row of 128256, 16 unmasked.
+// Measured: the likeliest 64 of 1024 rows of 128256 in 119 to 133 us (4.4 to 4.0
+// TB/s; 21 instructions a warp for 32 logits in the scan, 75 % of its issue
+// slots); 256 draws with top_p in 162 us, 144 of them scan_bins (81 instructions
+// for 32 logits, at 57 % of the issue slots: 54 for the exact weight and its bin,
+// the rest behind the cluster's first barrier); one draw with top_k in 12 us,
+// latencies of two launches.
 //
 // Weights are 64-bit whole numbers, round(w 2^s) with V 2^s <= 2^62, from
 // exponentials in 64 bits: their sums do not depend on the order of the
 // additions, so a draw is the same every time, and where a border falls between
-// two tokens is off by less than V 2^-(s + 1) of the largest weight (4e-9 at
-// V = 128256 if all roundings went one way; 1e-11 in earnest).  In 32 bits one
+// two tokens is off by less than V 2^-(s + 1) of the largest weight (1.8e-9
+// at V = 128256, s = 45, if all roundings went one way; 1e-11 in earnest).  In 32 bits one
 // draw in a hundred from a flat distribution over 128256 tokens would take a
 // neighbour.
 #include "programmatic.cuh"
