@@ -1252,7 +1252,8 @@ class SlideFSDP(nn.Module):
         B, T = input_ids.shape
         ids, labels = self._whole_tiles(input_ids, labels)
         if labels is None:
-            return self._forward_only(ids, None, lambda layer, h, ctx: layer.logits(h)).view(*ids.shape, -1)[:, :T]
+            logits = self._forward_only(ids, None, lambda layer, h, ctx: layer.logits(h))
+            return logits.view(*ids.shape, -1)[:, :T].contiguous()
         return self._forward_only(ids, labels, lambda layer, h, ctx: layer.logprobs(h, ctx.targets, temperature)) \
             .view(B, -1)[:, :T].contiguous()
 
